@@ -1,0 +1,383 @@
+// Output projection fused with the softmax that follows it: logits = x [M, K] W [N, K]^T are formed on CTA pairs in 256 x 256
+// tiles (tcgen05 cta_group::2) and never leave tensor memory.
+//
+//   statistics: the epilogue reduces each row of a tile to (m, s, u, x[label]): largest logit, sums of softmax_stats.cuh
+//               relative to it, and the label's logit if it lies in the tile's columns; 16 bytes per row and tile go to
+//               stats[tile column][M] instead of 512 bytes of logits. token_log_probs_join combines the tiles.
+//   gradient:   the logits are formed again, and the epilogue writes d(logits) in bf16, the operand type of the two products
+//               that follow (d(x) = d(logits) W, dW = d(logits)^T x); the factor 1[label] - p is formed in fp32 from the fp32
+//               logits, so the one rounding is that of the stored operand.
+//
+// Same staging and synchronisation as the pair GEMM of gemm_bf16_2sm.cu (six 32 KB stages per CTA filled by TMA without
+// multicast, one issuing thread in the even CTA, two accumulators of 256 TMEM columns so that the epilogue of one tile runs
+// under the MMAs of the next). An epilogue thread owns one row, so the statistics need no exchange between threads.
+// Bound by the tensor cores: a tile takes 128 cycles per 16 of K, the epilogue about 2500 cycles (one exponential and
+// four to six FMA-pipe operations per logit on four warps), hidden behind the MMAs of the next tile from K = 512 on.
+#include <cuda.h>
+
+#include "../common/cta_pair.cuh"
+#include "../common/launch.h"
+#include "../common/ptx.cuh"
+#include "../common/tensor_map.h"
+#include "../ops/softmax_stats.cuh"
+#include "../ops/vocabulary.h"
+
+namespace b200 {
+
+namespace {
+
+constexpr int BM = 128;       // rows per CTA (256 per pair)
+constexpr int BN = kVocabTile;  // columns per pair
+constexpr int BN_HALF = 128;  // W rows staged per CTA
+constexpr int BK = 64;
+constexpr int STAGES = 6;
+constexpr int A_STAGE_BYTES = BM * BK * 2;
+constexpr int B_STAGE_BYTES = BN_HALF * BK * 2;
+constexpr int THREADS = 192;
+constexpr int TMEM_COLS = 512;
+constexpr int BOX_BYTES = 32 * 128;               // one epilogue box: 32 rows x 64 bf16
+constexpr int STAGING_BYTES = 4 * 2 * BOX_BYTES;  // two boxes for each of the four epilogue warps
+constexpr int SMEM_BYTES = STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + STAGING_BYTES + 1024 + 256;
+
+struct RowArgs {
+  const void* labels;
+  bool labels64;
+  float4* stats;  // statistics: [n tiles][M]
+  const float2* lse;
+  const float* entropy;
+  const float* d_log_probs;
+  long long d_log_probs_stride;
+  const float* d_entropy;
+  long long d_entropy_stride;
+  float logit_scale;
+  long long ignore_index;
+};
+
+enum class Mode : int { kStats, kGrad };
+
+template <Mode MODE, bool ENTROPY>
+__global__ void __launch_bounds__(THREADS, 1)
+    vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                          const __grid_constant__ CUtensorMap tmG, int M, int N, int K, int group, int* status, RowArgs rows) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + STAGES * A_STAGE_BYTES;
+  uint8_t* sStage = smem + STAGES * (A_STAGE_BYTES + B_STAGE_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sStage + STAGING_BYTES);
+  uint64_t* full = bars;
+  uint64_t* empty = bars + STAGES;
+  uint64_t* acc_full = bars + 2 * STAGES;
+  uint64_t* acc_empty = bars + 2 * STAGES + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t cta_rank = cluster_ctarank();  // 0 = leader
+  const bool leader = cta_rank == 0;
+  const int pair = blockIdx.x >> 1;
+  const int num_pairs = gridDim.x >> 1;
+  const int m_tiles = (M + 2 * BM - 1) / (2 * BM);
+  const int n_tiles = (N + BN - 1) / BN;
+  const int k_blocks = (K + BK - 1) / BK;
+  const int total = m_tiles * n_tiles;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8);
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tmem_alloc_2sm(tmem_slot, TMEM_COLS);
+    tmem_relinquish_2sm();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();  // both CTAs' barriers are initialised before anything remote touches them
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer (both CTAs)
+    if (lane == 0) {
+      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(&tmB);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int tile = pair; tile < total && ok; tile += num_pairs) {
+        const TileCoord tc = tile_coord(tile, m_tiles, n_tiles, group);
+        const int m0 = tc.mi * (2 * BM) + (int)cta_rank * BM;
+        const int n0 = tc.ni * BN + (int)cta_rank * BN_HALF;
+        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          if (!mbar_wait(&empty[s], ph ^ 1, abort_flag)) {
+            raise_status(status, kStatusWaitTimeoutProducer, abort_flag);
+            ok = false;
+            break;
+          }
+          const uint32_t full_leader = map_to_cta(smem_u32(&full[s]), 0);
+          if (leader) mbar_arrive_expect_tx(&full[s], 2 * (A_STAGE_BYTES + B_STAGE_BYTES));
+          tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA, full_leader, kb * BK, m0);
+          tma_load_2d_pair(sB + s * B_STAGE_BYTES, &tmB, full_leader, kb * BK, n0);
+        }
+      }
+      if (!ok) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);  // copies in flight land before the CTA may exit
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issuer (leader CTA only)
+    if (leader && lane == 0) {
+      constexpr uint32_t idesc = umma_idesc_bf16(2 * BM, BN, 0, 0);
+      uint32_t it = 0, tcount = 0;
+      bool ok = true;
+      for (int tile = pair; tile < total && ok; tile += num_pairs, ++tcount) {
+        const uint32_t buf = tcount & 1;
+        const uint32_t aph = (tcount >> 1) & 1;
+        if (!mbar_wait(&acc_empty[buf], aph ^ 1, abort_flag)) {
+          raise_status(status, kStatusWaitTimeoutMma, abort_flag);
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + buf * BN;
+        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
+          const uint32_t s = it % STAGES;
+          const uint32_t ph = (it / STAGES) & 1;
+          if (!mbar_wait(&full[s], ph, abort_flag)) {
+            raise_status(status, kStatusWaitTimeoutMma, abort_flag);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t a_base = smem_u32(sA + s * A_STAGE_BYTES);
+          const uint32_t b_base = smem_u32(sB + s * B_STAGE_BYTES);
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k) {
+            umma_f16_ss_2sm(d_tmem, umma_smem_desc_sw128(a_base + k * 32, 16, 1024), umma_smem_desc_sw128(b_base + k * 32, 16, 1024),
+                            idesc, (kb != 0 || k != 0) ? 1u : 0u);
+          }
+          const uint32_t e_local = smem_u32(&empty[s]);  // release the stage in both CTAs
+          umma_commit_2sm(map_to_cta(e_local, 0));
+          umma_commit_2sm(map_to_cta(e_local, 1));
+        }
+        if (ok) {
+          const uint32_t f_local = smem_u32(&acc_full[buf]);
+          umma_commit_2sm(map_to_cta(f_local, 0));
+          umma_commit_2sm(map_to_cta(f_local, 1));
+        }
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ epilogue: this CTA's 128 x 256 half
+    const int q = warp & 3;
+    uint8_t* stage0 = sStage + q * (2 * BOX_BYTES);
+    const float scale2 = rows.logit_scale * kLog2e;
+    uint32_t tcount = 0, nstore = 0;
+    for (int tile = pair; tile < total; tile += num_pairs, ++tcount) {
+      const TileCoord tc = tile_coord(tile, m_tiles, n_tiles, group);
+      const uint32_t buf = tcount & 1;
+      const uint32_t aph = (tcount >> 1) & 1;
+      const int row0 = tc.mi * (2 * BM) + (int)cta_rank * BM + q * 32;
+      const int row = row0 + lane;
+      const int tile_col0 = tc.ni * BN;
+      // the label's column relative to the tile; -1: not here
+      int label = -1;
+      bool ignored = true;
+      if (row < M) {
+        const long long l = load_label(rows.labels, rows.labels64, row);
+        ignored = l == rows.ignore_index || l < 0 || l >= N;
+        if (!ignored && l >= tile_col0 && l < tile_col0 + BN) label = (int)(l - tile_col0);
+      }
+      float2 L = make_float2(0.f, 0.f);
+      float gs = 0.f, hs = 0.f, H = 0.f;
+      bool zero = true;
+      if (MODE == Mode::kGrad && !ignored) {
+        L = rows.lse[row];
+        gs = rows.d_log_probs[row * rows.d_log_probs_stride] * rows.logit_scale;
+        if (ENTROPY) {
+          hs = rows.d_entropy[row * rows.d_entropy_stride] * rows.logit_scale;
+          H = rows.entropy[row];
+        }
+        zero = gs == 0.f && hs == 0.f;
+      }
+      if (!mbar_wait(&acc_full[buf], aph, abort_flag)) {
+        raise_status(status, kStatusWaitTimeoutEpilogue, abort_flag);
+        break;
+      }
+      tc_fence_after_sync();
+      const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + buf * BN;
+
+      if (MODE == Mode::kStats) {
+        Stats st = empty_stats();
+        float x_label = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          const int col0 = tile_col0 + c * 32;
+          if (col0 >= N) break;
+          uint32_t v[32];
+          B200_TMEM_LD_32(v, t_row + c * 32);
+          tmem_ld_wait();
+          if (c == BN / 32 - 1 || col0 + 32 >= N) {
+            // last read of this accumulator: hand the TMEM buffer back before the arithmetic
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+          }
+          float f[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[e]);
+          if (col0 + 32 > N) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (col0 + e >= N) f[e] = -INFINITY;
+          }
+          if ((label >> 5) == c) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if ((label & 31) == e) x_label = f[e];
+          }
+          accumulate<ENTROPY, 32>(st, f, scale2);
+        }
+        if (row < M) rows.stats[(long long)tc.ni * M + row] = make_float4(st.m, st.s, st.u, x_label);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN / 64; ++c) {
+          const int col0 = tile_col0 + c * 64;
+          if (col0 >= N) break;
+          uint8_t* box = stage0 + (nstore & 1) * BOX_BYTES;
+          if (lane == 0) tma_store_wait_read<1>();  // the store that used this box two boxes ago has read it
+          __syncwarp();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t v[32];
+            B200_TMEM_LD_32(v, t_row + c * 64 + half * 32);
+            tmem_ld_wait();
+            float f[32];
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const float d = score_gradient<ENTROPY>(log2_prob(__uint_as_float(v[e]), L, scale2), gs, hs, H);
+              f[e] = zero ? 0.f : d;
+            }
+            if ((label >> 5) == 2 * c + half) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if ((label & 31) == e) f[e] += gs;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              box_write(box, lane, half * 4 + j,
+                        make_uint4(pack_bf16x2(f[8 * j], f[8 * j + 1]), pack_bf16x2(f[8 * j + 2], f[8 * j + 3]),
+                                   pack_bf16x2(f[8 * j + 4], f[8 * j + 5]), pack_bf16x2(f[8 * j + 6], f[8 * j + 7])));
+          }
+          if (c == BN / 64 - 1 || col0 + 64 >= N) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && row0 < M) {
+            tma_store_2d(&tmG, box, col0, row0);
+            tma_store_commit();
+          }
+          ++nstore;
+        }
+      }
+    }
+    if (MODE == Mode::kGrad) {
+      // every bulk store of this warp has left shared memory and reached global memory before the CTA exits
+      if (lane == 0) tma_store_wait<0>();
+      __syncwarp();
+    }
+  }
+
+  // Neither CTA may free its TMEM or exit while the other can still reach into it.
+  tc_fence_before_sync();
+  __syncthreads();
+  cluster_sync_all();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_2sm(tmem_base, TMEM_COLS);
+  }
+}
+
+// Row panels of up to eight tiles: the pairs that run at a time share their A rows within a panel column and their W rows
+// across the panel (the raster of the plain pair GEMM).
+int panel(int m_tiles) { return m_tiles < 8 ? m_tiles : 8; }
+
+template <Mode MODE, bool ENTROPY>
+void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmG, int M, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
+  auto kernel = vocab_gemm_2sm_kernel<MODE, ENTROPY>;
+  check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "vocab gemm smem attr");
+  const int m_tiles = (M + 2 * BM - 1) / (2 * BM), n_tiles = (N + BN - 1) / BN;
+  int pairs = sm_count() / 2;
+  if ((long long)m_tiles * n_tiles < pairs) pairs = m_tiles * n_tiles;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * pairs, 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmG, M, N, K, panel(m_tiles), status, rows), "vocab gemm launch");
+  count_launch();
+}
+
+}  // namespace
+
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, int M, int N,
+                      int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream) {
+  if (M <= 0) return;
+  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, M, ldx, BK, BM);
+  const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
+  RowArgs rows = {};
+  rows.labels = labels;
+  rows.labels64 = labels64;
+  rows.stats = reinterpret_cast<float4*>(stats);
+  rows.logit_scale = logit_scale;
+  rows.ignore_index = -1;  // every label outside of [0, N) counts as none here
+  if (entropy) launch<Mode::kStats, true>(tmA, tmB, tmA, M, N, K, status, rows, stream);
+  else launch<Mode::kStats, false>(tmA, tmB, tmA, M, N, K, status, rows, stream);
+}
+
+void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labels64, const float2* lse, const float* entropy,
+                     const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
+                     void* grad, int M, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
+                     long long ignore_index, int* status, cudaStream_t stream) {
+  if (M <= 0) return;
+  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, M, ldx, BK, BM);
+  const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
+  const CUtensorMap tmG = make_tensor_map_2d_b16(grad, N, M, ldg, 64, 32);
+  RowArgs rows = {};
+  rows.labels = labels;
+  rows.labels64 = labels64;
+  rows.lse = lse;
+  rows.entropy = entropy;
+  rows.d_log_probs = d_log_probs;
+  rows.d_log_probs_stride = d_log_probs_stride;
+  rows.d_entropy = d_entropy;
+  rows.d_entropy_stride = d_entropy_stride;
+  rows.logit_scale = logit_scale;
+  rows.ignore_index = ignore_index;
+  if (d_entropy != nullptr) launch<Mode::kGrad, true>(tmA, tmB, tmG, M, N, K, status, rows, stream);
+  else launch<Mode::kGrad, false>(tmA, tmB, tmG, M, N, K, status, rows, stream);
+}
+
+}  // namespace b200

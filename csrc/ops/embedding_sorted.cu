@@ -1,0 +1,372 @@
+// Embedding lookup, out[t] = scale * W[id_t], and its gradient summed in sorted token order:
+//   dW[v] = scale * sum over t with id_t = v, in ascending t, of dout[t]
+//
+// The gradient sorts the pairs (id, t) as 64-bit keys, which are distinct, so the order is unique and every sum is taken in
+// the same order on every run; nothing is added atomically. Sorting: runs of 2048 keys in shared memory (bitonic), then
+// levels that merge 16 runs at a time by rank: a key's place is its place in its own run plus the number of smaller keys in
+// each of the 15 others (15 independent binary searches). Summing: a block takes 32 consecutive sorted tokens and a slab
+// of columns and reads each dout row once; a run of equal ids inside of the block's tokens goes straight to its row of dW, a run
+// that crosses the border to the next 32 leaves fp32 partial sums, which a last kernel joins in order. Sums are fp32 and are
+// rounded once, when a row of dW is written.
+//
+// Bound by HBM: dout is read once, the rows of dW are written once (read and written when they are accumulated into).
+#include <cuda_fp16.h>
+
+#include "../common/launch.h"
+#include "../common/ptx.cuh"
+#include "vocabulary.h"
+
+namespace b200 {
+
+namespace {
+
+constexpr int RUN = 2048;        // keys sorted by one block
+constexpr int FAN = 16;          // runs merged per level
+constexpr int TOKENS = 32;       // sorted tokens summed by one block
+constexpr int SUM_THREADS = 128;
+constexpr uint64_t kNoKey = ~0ull;
+constexpr uint32_t kNoId = 0x7fffffffu;  // ids outside of the table, sorted behind all others
+
+__device__ __forceinline__ uint32_t key_id(uint64_t key) { return (uint32_t)(key >> 32); }
+
+__device__ __forceinline__ long long load_id(const void* ids, bool ids64, long long t) {
+  return ids64 ? reinterpret_cast<const long long*>(ids)[t] : reinterpret_cast<const int*>(ids)[t];
+}
+
+// ------------------------------------------------------------------------- element types
+template <typename T, int N>
+struct Pack;
+template <typename T>
+struct Pack<T, 1> {
+  T v;
+};
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+template <typename T, int N>
+__device__ __forceinline__ Pack<T, N> load_pack(const T* p) {
+  return *reinterpret_cast<const Pack<T, N>*>(p);
+}
+template <typename T, int N>
+__device__ __forceinline__ float element(const Pack<T, N>& p, int i) {
+  if constexpr (N == 1) return to_float(p.v);
+  else return to_float(p.v[i]);
+}
+template <typename T, int N>
+__device__ __forceinline__ void set_element(Pack<T, N>& p, int i, float f) {
+  if constexpr (N == 1) p.v = from_float<T>(f);
+  else p.v[i] = from_float<T>(f);
+}
+
+// ------------------------------------------------------------------------- lookup
+constexpr int LOOKUP_ROWS = 4;
+constexpr int LOOKUP_THREADS = 128;
+
+template <typename T, int N>
+__global__ void __launch_bounds__(LOOKUP_THREADS)
+    embedding_lookup_kernel(const T* __restrict__ weight, const void* __restrict__ ids, bool ids64, T* __restrict__ out, long long tokens,
+                            long long V, int H, float scale, int* status) {
+  const long long t0 = (long long)blockIdx.x * LOOKUP_ROWS;
+  long long id[LOOKUP_ROWS];
+  bool live[LOOKUP_ROWS], good[LOOKUP_ROWS];
+#pragma unroll
+  for (int k = 0; k < LOOKUP_ROWS; ++k) {
+    live[k] = t0 + k < tokens;
+    id[k] = live[k] ? load_id(ids, ids64, t0 + k) : 0;
+    good[k] = live[k] && id[k] >= 0 && id[k] < V;
+    if (live[k] && !good[k] && threadIdx.x == 0 && blockIdx.y == 0 && status != nullptr) atomicCAS(status, 0, kStatusBadTokenId);
+  }
+  const int c = (blockIdx.y * LOOKUP_THREADS + threadIdx.x) * N;
+  if (c >= H) return;
+  Pack<T, N> v[LOOKUP_ROWS];
+#pragma unroll
+  for (int k = 0; k < LOOKUP_ROWS; ++k) {
+    if (good[k]) {
+      v[k] = load_pack<T, N>(weight + id[k] * H + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) set_element<T, N>(v[k], e, 0.f);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < LOOKUP_ROWS; ++k) {
+    if (!live[k]) break;
+    if (scale != 1.f) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) set_element<T, N>(v[k], e, element<T, N>(v[k], e) * scale);
+    }
+    *reinterpret_cast<Pack<T, N>*>(out + (t0 + k) * H + c) = v[k];
+  }
+}
+
+// ------------------------------------------------------------------------- sort
+// Each thread owns one pair of a compare-exchange step. Steps of distance <= 32 stay inside of the 64 keys of a warp.
+__global__ void __launch_bounds__(RUN / 2)
+    sort_runs_kernel(const void* __restrict__ ids, bool ids64, uint64_t* __restrict__ keys, long long T, long long V) {
+  __shared__ uint64_t s[RUN];
+  const long long base = (long long)blockIdx.x * RUN;
+  const int size = 2 * blockDim.x;  // power of two, >= 64
+  for (int i = threadIdx.x; i < size; i += blockDim.x) {
+    const long long t = base + i;
+    uint64_t key = kNoKey;
+    if (t < T) {
+      const long long id = load_id(ids, ids64, t);
+      key = (uint64_t)(id >= 0 && id < V ? (uint32_t)id : kNoId) << 32 | (uint32_t)t;
+    }
+    s[i] = key;
+  }
+  __syncthreads();
+  for (int k = 2; k <= size; k <<= 1) {
+    for (int j = k >> 1; j > 0; j >>= 1) {
+      const int low = threadIdx.x & (j - 1);
+      const int i = 2 * (threadIdx.x - low) + low;
+      const uint64_t a = s[i], b = s[i + j];
+      const bool up = (i & k) == 0;
+      if ((a > b) == up) {
+        s[i] = b;
+        s[i + j] = a;
+      }
+      // the next step's distance is j / 2, or k when this was the last of its stage
+      const int next = j > 1 ? j >> 1 : k;
+      if (j > 32 || next > 32) __syncthreads();
+      else __syncwarp();
+    }
+  }
+  for (int i = threadIdx.x; i < size; i += blockDim.x)
+    if (base + i < T) keys[base + i] = s[i];
+}
+
+// One level: groups of FAN sorted runs of `length` keys (a power of two; the last run may be short) become one sorted run each.
+__global__ void __launch_bounds__(256) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, long long T, long long length) {
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= T) return;
+  const uint64_t key = in[i];
+  const long long run = i / length, group = run / FAN;
+  const long long first = group * FAN;
+  long long below[FAN];
+#pragma unroll
+  for (int r = 0; r < FAN; ++r) below[r] = 0;
+  for (long long step = length; step > 0; step >>= 1) {
+#pragma unroll
+    for (int r = 0; r < FAN; ++r) {
+      const long long begin = (first + r) * length;
+      const long long n = min(length, T - begin);  // negative behind the last run
+      if (below[r] + step <= n && in[begin + below[r] + step - 1] < key) below[r] += step;
+    }
+  }
+  long long place = first * length;  // a run counts its own smaller keys the same way
+#pragma unroll
+  for (int r = 0; r < FAN; ++r) place += below[r];
+  out[place] = key;
+}
+
+// ------------------------------------------------------------------------- sums
+template <typename D, int N, bool ACC>
+__device__ __forceinline__ void write_row(D* dst, const float* acc, float scale) {
+  if constexpr (ACC) {
+    float* d = reinterpret_cast<float*>(dst);
+#pragma unroll
+    for (int e = 0; e < N; ++e) d[e] += acc[e] * scale;
+  } else {
+    Pack<D, N> v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) set_element<D, N>(v, e, acc[e] * scale);
+    *reinterpret_cast<Pack<D, N>*>(dst) = v;
+  }
+}
+
+// D: type of a dweight row (float when accumulating)
+template <typename T, typename D, int N, bool ACC>
+__global__ void __launch_bounds__(SUM_THREADS)
+    sum_tokens_kernel(const T* __restrict__ dout, const uint64_t* __restrict__ keys, D* __restrict__ dweight, float* __restrict__ partials,
+                      long long tokens, int H, float scale) {
+  __shared__ uint64_t s[TOKENS + 2];
+  const long long chunk = blockIdx.x, base = chunk * TOKENS;
+  if (threadIdx.x < TOKENS + 2) {
+    const long long i = base + (int)threadIdx.x - 1;
+    s[threadIdx.x] = i >= 0 && i < tokens ? keys[i] : kNoKey;  // kNoKey's id is no key's
+  }
+  __syncthreads();
+  const int c = (blockIdx.y * SUM_THREADS + threadIdx.x) * N;
+  if (c >= H) return;
+  const int count = (int)min((long long)TOKENS, tokens - base);
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  bool from_before = key_id(s[0]) == key_id(s[1]);
+  constexpr int UNROLL = 8;
+  for (int i0 = 0; i0 < count; i0 += UNROLL) {
+    Pack<T, N> v[UNROLL];
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const int i = i0 + k;
+      if (i < count && key_id(s[1 + i]) != kNoId) v[k] = load_pack<T, N>(dout + (long long)(uint32_t)s[1 + i] * H + c);
+    }
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const int i = i0 + k;
+      if (i >= count) break;
+      const uint32_t id = key_id(s[1 + i]);
+      if (id == kNoId) break;
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += element<T, N>(v[k], e);
+      const bool ends = key_id(s[2 + i]) != id;
+      if (ends || i == count - 1) {
+        if (ends && !from_before) {
+          write_row<D, N, ACC>(dweight + (long long)id * H + c, acc, scale);
+        } else {
+          // slot 0: the part of a run that began in an earlier chunk, slot 1: the head of a run that goes on
+          float* p = partials + (2 * chunk + (from_before ? 0 : 1)) * H + c;
+#pragma unroll
+          for (int e = 0; e < N; ++e) p[e] = acc[e];
+        }
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] = 0.f;
+        from_before = false;
+      }
+    }
+  }
+}
+
+// Joins the partial sums of runs that cross chunk borders: the block of the chunk in which the run begins adds its head and the
+// parts of the following chunks, eight strided sums per column that are added in order.
+constexpr int JOIN_LANES = 8;
+constexpr int JOIN_COLUMNS = 32;
+
+template <typename D, bool ACC>
+__global__ void __launch_bounds__(JOIN_LANES * JOIN_COLUMNS)
+    join_runs_kernel(const uint64_t* __restrict__ keys, D* __restrict__ dweight, const float* __restrict__ partials, long long tokens, int H, float scale) {
+  __shared__ float s[JOIN_LANES][JOIN_COLUMNS];
+  const long long chunks = (tokens + TOKENS - 1) / TOKENS;
+  const int column = threadIdx.x % JOIN_COLUMNS, lane = threadIdx.x / JOIN_COLUMNS;
+  const int c = blockIdx.y * JOIN_COLUMNS + column;
+  for (long long chunk = blockIdx.x; chunk + 1 < chunks; chunk += gridDim.x) {
+    const long long next = (chunk + 1) * TOKENS;
+    const uint32_t id = key_id(keys[next - 1]);
+    if (id == kNoId || key_id(keys[next]) != id) continue;           // no run crosses this border
+    const long long first = chunk * TOKENS;
+    if (key_id(keys[first]) == id && first > 0 && key_id(keys[first - 1]) == id) continue;  // it began earlier
+    // last chunk of the run: the last key with this id
+    long long lo = next, hi = tokens;  // keys[lo] has the id; keys[hi] has not
+    while (hi - lo > 1) {
+      const long long mid = (lo + hi) / 2;
+      if (key_id(keys[mid]) == id) lo = mid;
+      else hi = mid;
+    }
+    const long long parts = lo / TOKENS - chunk;
+    float acc = 0.f;
+    if (c < H) {
+      for (long long k = lane; k < parts; k += JOIN_LANES) acc += partials[2 * (chunk + 1 + k) * H + c];
+    }
+    s[lane][column] = acc;
+    __syncthreads();
+    if (lane == 0 && c < H) {
+      float total = partials[(2 * chunk + 1) * H + c];
+#pragma unroll
+      for (int l = 0; l < JOIN_LANES; ++l) total += s[l][column];
+      write_row<D, 1, ACC>(dweight + (long long)id * H + c, &total, scale);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T>
+bool wide_rows(int H, const void* a, const void* b) {
+  return (long long)H * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(b) % 16 == 0;
+}
+
+template <typename T>
+void lookup(const void* weight, const void* ids, bool ids64, void* out, long long tokens, long long V, int H, float scale, int* status, cudaStream_t stream) {
+  constexpr int N = 16 / sizeof(T);
+  const bool wide = wide_rows<T>(H, weight, out);
+  const int per_block = LOOKUP_THREADS * (wide ? N : 1);
+  const dim3 grid((unsigned)((tokens + LOOKUP_ROWS - 1) / LOOKUP_ROWS), (unsigned)((H + per_block - 1) / per_block));
+  if (wide)
+    embedding_lookup_kernel<T, N><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64, reinterpret_cast<T*>(out), tokens, V, H, scale, status);
+  else
+    embedding_lookup_kernel<T, 1><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64, reinterpret_cast<T*>(out), tokens, V, H, scale, status);
+}
+
+template <typename T, typename D, bool ACC>
+void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials, long long tokens, int H, float scale, cudaStream_t stream) {
+  constexpr int N = 16 / sizeof(T);
+  const bool wide = wide_rows<T>(H, dout, ACC ? dout : dweight);
+  const int per_block = SUM_THREADS * (wide ? N : 1);
+  const long long chunks = (tokens + TOKENS - 1) / TOKENS;
+  const dim3 grid((unsigned)chunks, (unsigned)((H + per_block - 1) / per_block));
+  if (wide)
+    sum_tokens_kernel<T, D, N, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys, reinterpret_cast<D*>(dweight), partials, tokens, H, scale);
+  else
+    sum_tokens_kernel<T, D, 1, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys, reinterpret_cast<D*>(dweight), partials, tokens, H, scale);
+  count_launch();
+  check_cuda(cudaGetLastError(), "embedding gradient sum launch");
+  if (chunks > 1) {
+    const dim3 join((unsigned)(chunks - 1 < 128 ? chunks - 1 : 128), (unsigned)((H + JOIN_COLUMNS - 1) / JOIN_COLUMNS));
+    join_runs_kernel<D, ACC><<<join, JOIN_LANES * JOIN_COLUMNS, 0, stream>>>(keys, reinterpret_cast<D*>(dweight), partials, tokens, H, scale);
+    count_launch();
+    check_cuda(cudaGetLastError(), "embedding gradient join launch");
+  }
+}
+
+template <typename T>
+void gradient(const void* dout, const uint64_t* keys, void* dweight, bool accumulate, float* partials, long long tokens, int H, float scale, cudaStream_t stream) {
+  if (accumulate) sums<T, float, true>(dout, keys, dweight, partials, tokens, H, scale, stream);
+  else sums<T, T, false>(dout, keys, dweight, partials, tokens, H, scale, stream);
+}
+
+long long key_bytes(long long T) { return (T * 8 + 255) / 256 * 256; }
+
+}  // namespace
+
+void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids64, void* out, long long T, long long V, int H,
+                      float scale, int* status, cudaStream_t stream) {
+  if (T == 0 || H == 0) return;
+  auto launch = type == Scalar::kBf16 ? lookup<__nv_bfloat16> : type == Scalar::kF16 ? lookup<__half> : lookup<float>;
+  launch(weight, ids, ids64, out, T, V, H, scale, status, stream);
+  count_launch();
+  check_cuda(cudaGetLastError(), "embedding lookup launch");
+}
+
+long long embedding_gradient_workspace(long long T, int H) {
+  const long long chunks = (T + TOKENS - 1) / TOKENS;
+  return 2 * key_bytes(T) + (chunks > 1 ? 2 * chunks * H * 4 : 0);
+}
+
+void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids64, void* dweight, bool accumulate, void* workspace,
+                        long long T, long long V, int H, float scale, cudaStream_t stream) {
+  if (T == 0 || H == 0) return;
+  uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
+  uint64_t* other = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(workspace) + key_bytes(T));
+  float* partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 2 * key_bytes(T));
+  int threads = 32;
+  while (threads < RUN / 2 && 2 * threads < T) threads *= 2;
+  sort_runs_kernel<<<(unsigned)((T + RUN - 1) / RUN), threads, 0, stream>>>(ids, ids64, keys, T, V);
+  count_launch();
+  check_cuda(cudaGetLastError(), "embedding gradient sort launch");
+  for (long long length = RUN; length < T; length *= FAN) {
+    merge_runs_kernel<<<(unsigned)((T + 255) / 256), 256, 0, stream>>>(keys, other, T, length);
+    count_launch();
+    check_cuda(cudaGetLastError(), "embedding gradient merge launch");
+    uint64_t* t = keys;
+    keys = other;
+    other = t;
+  }
+  auto launch = type == Scalar::kBf16 ? gradient<__nv_bfloat16> : type == Scalar::kF16 ? gradient<__half> : gradient<float>;
+  launch(dout, keys, dweight, accumulate, partials, T, H, scale, stream);
+}
+
+}  // namespace b200

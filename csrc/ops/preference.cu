@@ -1,0 +1,516 @@
+// Losses over per-token log-probabilities of packed answers, reduced per sequence.
+//
+// Preference loss: with d_t = lp_t - ref_t, s_i = sum (or mean) of d_t over sequence i and D = s_chosen - s_rejected,
+//   sigmoid: (1 - e) softplus(-b D) + e softplus(b D)      dD: -b ((1 - e) sigmoid(-b D) - e sigmoid(b D))
+//   hinge:   max(0, 1 - b D)                               dD: -b where b D < 1
+//   ipo:     (D - 1 / (2 b))^2                             dD: 2 (D - 1 / (2 b))
+// Policy loss: with r = exp(lp - old), k = ref - lp,
+//   l = max(-A r, -A clip(r, lo, hi)) + c (expm1(k) - k)    dlp: -A r where the clip does not bind, - c expm1(k)
+// optionally with a bound -dual A for A < 0 (no gradient where it binds).
+//
+// Both read 8 to 20 bytes a token once. The unit of work is a warp with 256 consecutive tokens, which walks the sequences
+// that overlap them; its partial sums of sequence i go to slot (256-token chunk + i), which no other (chunk, sequence) pair
+// shares, so that nothing is added atomically and results do not depend on the order in which blocks run. A second phase
+// adds a sequence's slots, one warp per sequence, in 64 bits. Up to kOneLaunch tokens both phases run in one launch of a
+// cluster of eight blocks (one launch latency, the phases separated by the cluster's barrier); above it the first phase
+// takes a grid of its own.
+#include <cmath>
+
+#include "../common/cta_pair.cuh"
+#include "../common/launch.h"
+#include "../common/ptx.cuh"
+#include "vocabulary.h"
+
+namespace b200 {
+
+namespace {
+
+constexpr int CHUNK = 256;                // tokens of one warp's unit of work
+constexpr int LANE_TOKENS = CHUNK / 32;
+constexpr int CLUSTER = 8;
+constexpr int CLUSTER_THREADS = 512;
+constexpr int WARPS_A = 8;                // warps per block of the wide first phase
+constexpr int WORDS = 4;                  // fp32 words per slot
+constexpr long long kOneLaunch = 65536;
+
+struct Span {
+  long long begin, end;
+};
+
+__device__ __forceinline__ Span sequence_span(const PackedTokens& p, int i) {
+  if (p.cu == nullptr) return {min(p.T, i * p.length), min(p.T, (i + 1) * p.length)};
+  const long long b = max(0LL, min(p.T, (long long)p.cu[i])), e = max(b, min(p.T, (long long)p.cu[i + 1]));
+  return {b, e};
+}
+
+// First sequence that ends behind token t (all lanes call it with the same t).
+__device__ __forceinline__ int first_sequence(const PackedTokens& p, long long t) {
+  if (p.cu == nullptr) return p.length > 0 ? (int)min((long long)p.sequences, t / p.length) : p.sequences;
+  int lo = 0, hi = p.sequences;  // answer in [lo, hi]
+  while (lo < hi) {
+    // 32 probes at a time
+    const int span = hi - lo;
+    const int probe = lo + (int)(((long long)span * (threadIdx.x & 31)) >> 5);
+    const bool ends_before = (long long)p.cu[probe + 1] <= t;
+    const unsigned votes = __ballot_sync(0xffffffffu, ends_before);
+    const int n = __popc(votes);  // ends are ordered: the first n probes lie before the answer
+    if (n == 0) {
+      hi = lo;
+    } else {
+      const int last = lo + (int)(((long long)span * (n - 1)) >> 5);
+      const int next = n < 32 ? lo + (int)(((long long)span * n) >> 5) : hi;
+      lo = last + 1;
+      hi = max(lo, next);
+    }
+  }
+  return lo;
+}
+
+// Value of `local` (a shared-memory word) in block `rank` of this cluster.
+__device__ __forceinline__ double cluster_read(const double* local, unsigned rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(map_to_cta(smem_u32(local), rank)) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ double warp_sum_f64(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sum of `v` over all threads of the cluster, in a fixed order, valid in thread 0 of block 0. scratch: 32 doubles of this block.
+__device__ __forceinline__ double cluster_sum(double v, double* scratch, double* block_total) {
+  v = warp_sum_f64(v);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double s = 0;
+    for (int w = 0; w < CLUSTER_THREADS / 32; ++w) s += scratch[w];
+    *block_total = s;
+  }
+  cluster_sync_all();
+  double total = 0;
+  if (cluster_ctarank() == 0 && threadIdx.x == 0)
+    for (int b = 0; b < CLUSTER; ++b) total += cluster_read(block_total, b);
+  cluster_sync_all();  // nobody leaves or reuses the words while block 0 reads them
+  return total;
+}
+
+// ------------------------------------------------------------------------- preference
+struct PreferenceIn {
+  const float* log_probs;
+  const float* reference;
+};
+
+// Partial (sum of lp - ref, number of tokens) of the sequences that overlap the warp's chunk.
+__device__ __forceinline__ void preference_chunk(const PreferenceIn& in, const PackedTokens& p, long long chunk, float* partials) {
+  const int lane = threadIdx.x & 31;
+  const long long base = chunk * CHUNK, limit = min(p.T, base + CHUNK);
+  for (int i = first_sequence(p, base); i < p.sequences; ++i) {
+    const Span s = sequence_span(p, i);
+    if (s.begin >= limit) break;
+    const long long b = max(s.begin, base), e = min(s.end, limit);
+    double d[LANE_TOKENS];  // differences of nearly equal numbers of both signs: kept exact, summed in 64 bits
+    int keep[LANE_TOKENS];
+#pragma unroll
+    for (int k = 0; k < LANE_TOKENS; ++k) {
+      const long long t = b + lane + 32 * k;
+      keep[k] = t < e && (p.mask == nullptr || p.mask[t] != 0);
+      d[k] = 0;
+      if (t < e) d[k] = (double)in.log_probs[t] - (in.reference != nullptr ? (double)in.reference[t] : 0.0);
+    }
+    double sum = 0;
+    int count = 0;
+#pragma unroll
+    for (int k = 0; k < LANE_TOKENS; ++k) {
+      if (keep[k]) {
+        sum += d[k];
+        ++count;
+      }
+    }
+    sum = warp_sum_f64(sum);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) *reinterpret_cast<double2*>(partials + (chunk + i) * WORDS) = make_double2(sum, (double)count);
+  }
+}
+
+// A sequence's log-ratio and token count from its slots (whole warp).
+__device__ __forceinline__ double2 preference_sequence(const PackedTokens& p, int i, const float* partials) {
+  const Span s = sequence_span(p, i);
+  double sum = 0, count = 0;
+  if (s.end > s.begin) {
+    const long long first = s.begin / CHUNK, last = (s.end - 1) / CHUNK;
+    for (long long c = first + (threadIdx.x & 31); c <= last; c += 32) {
+      const double2 v = __ldcg(reinterpret_cast<const double2*>(partials + (c + i) * WORDS));
+      sum += v.x;
+      count += v.y;
+    }
+  }
+  return make_double2(warp_sum_f64(sum), warp_sum_f64(count));
+}
+
+__device__ __forceinline__ double softplus(double x) { return fmax(x, 0.0) + log1p(exp(-fabs(x))); }
+__device__ __forceinline__ double sigmoid(double x) {
+  const double e = exp(-fabs(x));
+  return x >= 0 ? 1 / (1 + e) : e / (1 + e);
+}
+
+// Second phase: a warp of the cluster takes a pair at a time.
+__device__ __forceinline__ void preference_pairs(const PackedTokens& p, const PreferenceArgs& a, const float* partials, float* loss,
+                                                 float* rewards, float* slope, double* scratch, double* block_total) {
+  const int pairs = p.sequences / 2, lane = threadIdx.x & 31;
+  const double beta = a.beta, eps = a.label_smoothing;
+  const double scale = a.reduction == 2 ? 1.0 / pairs : 1.0;
+  double total = 0;
+  for (int i = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5); i < pairs; i += CLUSTER * (CLUSTER_THREADS / 32)) {
+    double2 w = preference_sequence(p, i, partials), l = preference_sequence(p, pairs + i, partials);
+    const double inv_w = a.average ? 1 / fmax(w.y, 1.0) : 1.0, inv_l = a.average ? 1 / fmax(l.y, 1.0) : 1.0;
+    if (lane == 0) {
+      const double sw = w.x * inv_w, sl = l.x * inv_l, diff = sw - sl, margin = beta * diff;
+      double value, d;
+      if (a.kind == PreferenceKind::kSigmoid) {
+        value = (1 - eps) * softplus(-margin);
+        if (eps != 0) value += eps * softplus(margin);
+        d = -beta * ((1 - eps) * sigmoid(-margin) - eps * sigmoid(margin));
+      } else if (a.kind == PreferenceKind::kHinge) {
+        value = margin != margin ? margin : fmax(0.0, 1 - margin);
+        d = margin < 1 ? -beta : margin != margin ? margin : 0.0;
+      } else {
+        const double off = diff - 0.5 / beta;
+        value = off * off;
+        d = 2 * off;
+      }
+      rewards[i] = (float)(beta * sw);
+      rewards[pairs + i] = (float)(beta * sl);
+      slope[i] = (float)(d * scale * inv_w);
+      slope[pairs + i] = (float)(-d * scale * inv_l);
+      if (a.reduction == 0) loss[i] = (float)value;
+      total += value;
+    }
+  }
+  if (a.reduction == 0) return;
+  total = cluster_sum(total, scratch, block_total);
+  if (cluster_ctarank() == 0 && threadIdx.x == 0) loss[0] = (float)(total * scale);
+}
+
+template <bool ONE_LAUNCH>
+__global__ void __launch_bounds__(CLUSTER_THREADS)
+    preference_cluster_kernel(PreferenceIn in, PackedTokens p, PreferenceArgs args, float* partials, float* loss, float* rewards, float* slope) {
+  __shared__ double scratch[CLUSTER_THREADS / 32];
+  __shared__ double block_total;
+  if (ONE_LAUNCH) {
+    const long long chunks = (p.T + CHUNK - 1) / CHUNK;
+    for (long long c = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5); c < chunks; c += CLUSTER * (CLUSTER_THREADS / 32))
+      preference_chunk(in, p, c, partials);
+    __threadfence();
+    cluster_sync_all();
+  }
+  preference_pairs(p, args, partials, loss, rewards, slope, scratch, &block_total);
+}
+
+__global__ void __launch_bounds__(WARPS_A * 32) preference_chunks_kernel(PreferenceIn in, PackedTokens p, float* partials) {
+  const long long c = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
+  if (c * CHUNK < p.T) preference_chunk(in, p, c, partials);
+}
+
+// Calls f(t, sequence or -1) for every token of the warp's chunk, sequence by sequence, tokens outside of all of them first.
+template <typename F>
+__device__ __forceinline__ void for_each_token(const PackedTokens& p, long long chunk, F f) {
+  const int lane = threadIdx.x & 31;
+  const long long base = chunk * CHUNK, limit = min(p.T, base + CHUNK);
+  long long done = base;
+  for (int i = first_sequence(p, base); i < p.sequences && done < limit; ++i) {
+    const Span s = sequence_span(p, i);
+    const long long b = max(min(s.begin, limit), done), e = max(min(s.end, limit), b);
+    for (long long t = done + lane; t < b; t += 32) f(t, -1);
+    for (long long t = b + lane; t < e; t += 32) f(t, i);
+    done = e;
+  }
+  for (long long t = done + lane; t < limit; t += 32) f(t, -1);
+}
+
+__global__ void __launch_bounds__(WARPS_A * 32)
+    preference_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ d_loss, long long d_loss_stride, PackedTokens p, float* __restrict__ grad) {
+  const long long c = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
+  if (c * CHUNK >= p.T) return;
+  const int pairs = p.sequences / 2;
+  for_each_token(p, c, [&](long long t, int i) {
+    float g = 0.f;
+    if (i >= 0 && (p.mask == nullptr || p.mask[t] != 0)) g = slope[i] * d_loss[(i < pairs ? i : i - pairs) * d_loss_stride];
+    grad[t] = g;
+  });
+}
+
+// ------------------------------------------------------------------------- policy
+struct PolicyIn {
+  const float* log_probs;
+  const float* old_log_probs;
+  const float* reference;
+  const float* advantages;
+};
+
+// expm1(k) - k without the cancellation of its first terms: the series k^2 (1/2 + k/6 + k^2/24 + ...) up to |k| = 1/4 (the
+// first term left out is below 2^-28 of the sum), the difference beyond, where at most three bits cancel.
+__device__ __forceinline__ float expm1_minus(float k) {
+  if (fabsf(k) > 0.25f) return expm1f(k) - k;
+  float q = 1.f / 362880.f;
+  q = fmaf(q, k, 1.f / 40320.f);
+  q = fmaf(q, k, 1.f / 5040.f);
+  q = fmaf(q, k, 1.f / 720.f);
+  q = fmaf(q, k, 1.f / 120.f);
+  q = fmaf(q, k, 1.f / 24.f);
+  q = fmaf(q, k, 1.f / 6.f);
+  q = fmaf(q, k, 0.5f);
+  return q * k * k;
+}
+
+struct TokenLoss {
+  float value, slope, kl;
+  int clipped;
+};
+
+__device__ __forceinline__ TokenLoss policy_token(float lp, float old, float ref, bool has_ref, float adv, const PolicyArgs& a) {
+  // the difference decides by which side of a border the token's gradient vanishes: formed and compared in 64 bits, where it
+  // is exact up to the borders' own rounding
+  const double delta = (double)lp - (double)old;
+  const float d_hi = (float)delta;
+  const float ratio = expf(d_hi);
+  TokenLoss out;
+  out.clipped = (adv > 0.f && delta > a.log_high) || (adv < 0.f && delta < a.log_low);
+  if (out.clipped) {
+    out.value = -adv * (adv > 0.f ? a.ratio_high : a.ratio_low);
+    out.slope = 0.f;
+  } else {
+    out.value = adv == 0.f ? 0.f : -adv * ratio;  // an infinite ratio of a token without advantage counts nothing
+    out.slope = out.value;
+  }
+  if (a.dual_clip != 0.f && adv < 0.f && out.value > -a.dual_clip * adv) {
+    out.value = -a.dual_clip * adv;
+    out.slope = 0.f;
+    out.clipped = 1;
+  }
+  out.kl = 0.f;
+  if (has_ref) {
+    const float k = ref - lp;
+    out.kl = expm1_minus(k);
+    if (a.kl_coef == 0.f) return out;  // reported only; an infinite estimate must not reach the loss as 0 * inf
+    out.value = fmaf(a.kl_coef, out.kl, out.value);
+    out.slope = fmaf(-a.kl_coef, expm1f(k), out.slope);
+  }
+  return out;
+}
+
+// Partial (loss, kl, clipped, tokens) of the warp's chunk: per sequence into slot (chunk + sequence) for the mean over
+// sequences, else all together into slot `chunk`. Writes the tokens' slopes.
+__device__ __forceinline__ void policy_chunk(const PolicyIn& in, const PackedTokens& p, const PolicyArgs& a, long long chunk, float* partials, float* slope) {
+  const int lane = threadIdx.x & 31;
+  const long long base = chunk * CHUNK, limit = min(p.T, base + CHUNK);
+  float loss = 0.f, kl = 0.f;
+  int clipped = 0, count = 0;
+  for (int i = first_sequence(p, base); i < p.sequences; ++i) {
+    const Span s = sequence_span(p, i);
+    if (s.begin >= limit) break;
+    const long long b = max(s.begin, base), e = min(s.end, limit);
+    const float seq_adv = a.per_token_advantage ? 0.f : in.advantages[i];
+    float lp[LANE_TOKENS], old[LANE_TOKENS], ref[LANE_TOKENS], adv[LANE_TOKENS];
+    bool keep[LANE_TOKENS];
+#pragma unroll
+    for (int k = 0; k < LANE_TOKENS; ++k) {
+      const long long t = b + lane + 32 * k;
+      keep[k] = t < e && (p.mask == nullptr || p.mask[t] != 0);
+      lp[k] = old[k] = ref[k] = 0.f;
+      adv[k] = seq_adv;
+      if (t < e) {
+        lp[k] = in.log_probs[t];
+        old[k] = in.old_log_probs[t];
+        if (in.reference != nullptr) ref[k] = in.reference[t];
+        if (a.per_token_advantage) adv[k] = in.advantages[t];
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < LANE_TOKENS; ++k) {
+      const long long t = b + lane + 32 * k;
+      if (!keep[k]) {
+        if (slope != nullptr && t < e) slope[t] = 0.f;
+        continue;
+      }
+      const TokenLoss v = policy_token(lp[k], old[k], ref[k], in.reference != nullptr, adv[k], a);
+      loss += v.value;
+      kl += v.kl;
+      clipped += v.clipped;
+      ++count;
+      if (slope != nullptr) slope[t] = v.slope;
+    }
+    if (a.reduction == 2) {
+      loss = warp_sum(loss);
+      kl = warp_sum(kl);
+      clipped = __reduce_add_sync(0xffffffffu, clipped);
+      count = __reduce_add_sync(0xffffffffu, count);
+      if (lane == 0) *reinterpret_cast<float4*>(partials + (chunk + i) * WORDS) = make_float4(loss, kl, (float)clipped, (float)count);
+      loss = kl = 0.f;
+      clipped = count = 0;
+    }
+  }
+  if (a.reduction != 2) {
+    loss = warp_sum(loss);
+    kl = warp_sum(kl);
+    clipped = __reduce_add_sync(0xffffffffu, clipped);
+    count = __reduce_add_sync(0xffffffffu, count);
+    if (lane == 0) *reinterpret_cast<float4*>(partials + chunk * WORDS) = make_float4(loss, kl, (float)clipped, (float)count);
+  }
+}
+
+__device__ __forceinline__ void policy_totals(const PackedTokens& p, const PolicyArgs& a, const float* partials, float* out, float* weight, double* scratch, double* block_total) {
+  const int lane = threadIdx.x & 31;
+  const int warp = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5);
+  constexpr int kWarps = CLUSTER * (CLUSTER_THREADS / 32);
+  double loss = 0, kl = 0, clipped = 0, count = 0, used = 0;
+  if (a.reduction == 2) {
+    for (int i = warp; i < p.sequences; i += kWarps) {
+      const Span s = sequence_span(p, i);
+      double l = 0, n = 0;
+      if (s.end > s.begin) {
+        const long long first = s.begin / CHUNK, last = (s.end - 1) / CHUNK;
+        for (long long c = first + lane; c <= last; c += 32) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(partials + (c + i) * WORDS));
+          l += v.x;
+          kl += v.y;
+          clipped += v.z;
+          n += v.w;
+        }
+      }
+      l = warp_sum_f64(l);
+      n = warp_sum_f64(n);
+      if (lane == 0) {
+        if (n > 0) {
+          loss += l / n;
+          count += n;
+          used += 1;
+        }
+        weight[i] = (float)(1.0 / fmax(n, 1.0));
+      }
+    }
+  } else {
+    const long long chunks = (p.T + CHUNK - 1) / CHUNK;
+    for (long long c = warp * 32 + lane; c < chunks; c += kWarps * 32) {
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(partials + c * WORDS));
+      loss += v.x;
+      kl += v.y;
+      clipped += v.z;
+      count += v.w;
+    }
+  }
+  loss = cluster_sum(loss, scratch, block_total);
+  kl = cluster_sum(kl, scratch, block_total);
+  clipped = cluster_sum(clipped, scratch, block_total);
+  count = cluster_sum(count, scratch, block_total);
+  if (a.reduction == 2) used = cluster_sum(used, scratch, block_total);
+  if (cluster_ctarank() == 0 && threadIdx.x == 0) {
+    const double tokens = fmax(count, 1.0);
+    const double divisor = a.reduction == 0 ? 1.0 : a.reduction == 1 ? tokens : fmax(used, 1.0);
+    out[0] = (float)(loss / divisor);
+    out[1] = (float)(kl / tokens);
+    out[2] = (float)(clipped / tokens);
+    out[3] = (float)(1.0 / divisor);
+  }
+}
+
+template <bool ONE_LAUNCH>
+__global__ void __launch_bounds__(CLUSTER_THREADS)
+    policy_cluster_kernel(PolicyIn in, PackedTokens p, PolicyArgs args, float* partials, float* out, float* slope, float* weight) {
+  __shared__ double scratch[CLUSTER_THREADS / 32];
+  __shared__ double block_total;
+  if (ONE_LAUNCH) {
+    const long long chunks = (p.T + CHUNK - 1) / CHUNK;
+    for (long long c = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5); c < chunks; c += CLUSTER * (CLUSTER_THREADS / 32))
+      policy_chunk(in, p, args, c, partials, slope);
+    __threadfence();
+    cluster_sync_all();
+  }
+  policy_totals(p, args, partials, out, weight, scratch, &block_total);
+}
+
+__global__ void __launch_bounds__(WARPS_A * 32) policy_chunks_kernel(PolicyIn in, PackedTokens p, PolicyArgs args, float* partials, float* slope) {
+  const long long c = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
+  if (c * CHUNK < p.T) policy_chunk(in, p, args, c, partials, slope);
+}
+
+__global__ void __launch_bounds__(WARPS_A * 32)
+    policy_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ out, const float* __restrict__ weight, const float* __restrict__ d_loss, PackedTokens p, int reduction,
+                      float* __restrict__ grad) {
+  const long long c = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
+  if (c * CHUNK >= p.T) return;
+  const float w = out[3] * d_loss[0];
+  for_each_token(p, c, [&](long long t, int i) {
+    float g = 0.f;
+    if (i >= 0 && (p.mask == nullptr || p.mask[t] != 0)) g = slope[t] * (reduction == 2 ? w * weight[i] : w);
+    grad[t] = g;
+  });
+}
+
+unsigned chunk_blocks(long long T) { return (unsigned)(((T + CHUNK - 1) / CHUNK + WARPS_A - 1) / WARPS_A); }
+
+template <typename Kernel, typename... Args>
+void launch_cluster(Kernel kernel, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(CLUSTER, 1, 1);
+  cfg.blockDim = dim3(CLUSTER_THREADS, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CLUSTER;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, args...), "loss cluster launch");
+  count_launch();
+}
+
+}  // namespace
+
+long long packed_partials(long long T, int sequences) { return ((T + CHUNK - 1) / CHUNK + sequences) * WORDS; }
+
+void preference_loss_fwd(const float* log_probs, const float* reference, PackedTokens tokens, PreferenceArgs args, float* partials,
+                         float* loss, float* rewards, float* slope, cudaStream_t stream) {
+  const PreferenceIn in = {log_probs, reference};
+  if (tokens.T <= kOneLaunch) {
+    launch_cluster(preference_cluster_kernel<true>, stream, in, tokens, args, partials, loss, rewards, slope);
+    return;
+  }
+  preference_chunks_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(in, tokens, partials);
+  count_launch();
+  check_cuda(cudaGetLastError(), "preference_loss launch");
+  launch_cluster(preference_cluster_kernel<false>, stream, in, tokens, args, partials, loss, rewards, slope);
+}
+
+void preference_loss_bwd(const float* slope, const float* d_loss, long long d_loss_stride, PackedTokens tokens, float* grad, cudaStream_t stream) {
+  if (tokens.T == 0) return;
+  preference_bwd_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(slope, d_loss, d_loss_stride, tokens, grad);
+  count_launch();
+  check_cuda(cudaGetLastError(), "preference_loss backward launch");
+}
+
+void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const float* reference, const float* advantages,
+                     PackedTokens tokens, PolicyArgs args, float* partials, float* out, float* slope, float* weight, cudaStream_t stream) {
+  const PolicyIn in = {log_probs, old_log_probs, reference, advantages};
+  if (tokens.T <= kOneLaunch) {
+    launch_cluster(policy_cluster_kernel<true>, stream, in, tokens, args, partials, out, slope, weight);
+    return;
+  }
+  policy_chunks_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(in, tokens, args, partials, slope);
+  count_launch();
+  check_cuda(cudaGetLastError(), "policy_loss launch");
+  launch_cluster(policy_cluster_kernel<false>, stream, in, tokens, args, partials, out, slope, weight);
+}
+
+void policy_loss_bwd(const float* slope, const float* out, const float* weight, const float* d_loss, PackedTokens tokens, int reduction,
+                     float* grad, cudaStream_t stream) {
+  if (tokens.T == 0) return;
+  policy_bwd_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(slope, out, weight, d_loss, tokens, reduction, grad);
+  count_launch();
+  check_cuda(cudaGetLastError(), "policy_loss backward launch");
+}
+
+}  // namespace b200

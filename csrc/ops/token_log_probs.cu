@@ -1,0 +1,352 @@
+// Log-probability of one given token per row of logits, and the row's entropy:
+//   z = logit_scale * logits,  L = logsumexp(z),  p = exp(z - L)
+//   log_prob = z[label] - L,   entropy = L - sum_j p_j z_j
+//   d logits_j = logit_scale * ( g (1[j = label] - p_j) - h p_j (z_j - L + entropy) )
+// with g, h the upstream gradients of the two outputs. Exponents are held in base 2, where the exponential is one
+// instruction; sums are fp32 and each value is rounded once, when it is stored.
+//
+// Forward: one pass with the running statistics of softmax_stats.cuh per thread, joined
+// over the CTA. Backward: one pass that reads the logits again and writes the gradient, since no gradient of a row is
+// known before its last logit has been read and a row (100 to 500 KB) does not stay on the SM until the upstream
+// gradient arrives. Both are bound by HBM.
+//
+// Rows may start at any element: a row that is not 16-byte aligned is read as aligned 16-byte words that are shifted
+// together (a row's shift is uniform), its first and last vectors element by element, so nothing outside of the row is
+// ever read. Ignored rows (label == ignore_index or outside of [0, V)) are not read at all: their outputs and gradients are 0,
+// whatever they hold.
+#include <cuda_fp16.h>
+
+#include "../common/launch.h"
+#include "../common/ptx.cuh"
+#include "softmax_stats.cuh"
+#include "vocabulary.h"
+
+namespace b200 {
+
+namespace {
+
+__device__ __forceinline__ long long row_offset(const RowMap& m, long long row) {
+  const long long o = row / m.inner;
+  return o * m.outer_stride + (row - o * m.inner) * m.row_stride;
+}
+
+template <typename T>
+struct Vec;
+template <>
+struct Vec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(uint4 v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = unpack_bf16x2(w[i]);
+      f[2 * i] = a.x;
+      f[2 * i + 1] = a.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  }
+  static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void store(__nv_bfloat16* p, float f) { *p = __float2bfloat16(f); }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int N = 8;
+  static __device__ __forceinline__ void unpack(uint4 v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = a.x;
+      f[2 * i + 1] = a.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+      w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
+  static __device__ __forceinline__ void store(__half* p, float f) { *p = __float2half_rn(f); }
+};
+template <>
+struct Vec<float> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ void unpack(uint4 v, float* f) {
+    f[0] = __uint_as_float(v.x);
+    f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z);
+    f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ float load(const float* p) { return *p; }
+  static __device__ __forceinline__ void store(float* p, float f) { *p = f; }
+};
+
+// The 16 bytes at `p + shift` of two aligned words, shift in bytes (1..15).
+__device__ __forceinline__ uint4 join_words(uint4 a, uint4 b, int shift) {
+  uint32_t w0, w1, w2, w3, w4;
+  switch (shift >> 2) {
+    case 0: w0 = a.x; w1 = a.y; w2 = a.z; w3 = a.w; w4 = b.x; break;
+    case 1: w0 = a.y; w1 = a.z; w2 = a.w; w3 = b.x; w4 = b.y; break;
+    case 2: w0 = a.z; w1 = a.w; w2 = b.x; w3 = b.y; w4 = b.z; break;
+    default: w0 = a.w; w1 = b.x; w2 = b.y; w3 = b.z; w4 = b.w; break;
+  }
+  const int bits = (shift & 3) * 8;
+  return make_uint4(__funnelshift_r(w0, w1, bits), __funnelshift_r(w1, w2, bits), __funnelshift_r(w2, w3, bits),
+                    __funnelshift_r(w3, w4, bits));
+}
+
+// A row cut into vectors of Vec<T>::N elements: vector i covers elements [i N, i N + N), the last one may be short.
+template <typename T>
+struct Row {
+  const T* p;
+  int V, vectors, shift;  // shift: bytes by which the row start lies above a 16-byte boundary
+
+  __device__ __forceinline__ Row(const T* start, int v)
+      : p(start), V(v), vectors((v + Vec<T>::N - 1) / Vec<T>::N), shift((int)(reinterpret_cast<uintptr_t>(start) & 15)) {}
+
+  // whole vectors whose 16-byte words all lie inside of the row
+  __device__ __forceinline__ bool wide(int i) const {
+    return shift == 0 ? (i + 1) * Vec<T>::N <= V : i > 0 && (i + 2) * Vec<T>::N <= V;
+  }
+  __device__ __forceinline__ uint4 load_wide(int i) const {
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(p + (long long)i * Vec<T>::N) & ~uintptr_t(15));
+    const uint4 a = __ldg(q);
+    if (shift == 0) return a;
+    return join_words(a, __ldg(q + 1), shift);
+  }
+  // elements past the row's end read as -inf (probability 0)
+  __device__ __forceinline__ void load_narrow(int i, float* f) const {
+#pragma unroll
+    for (int e = 0; e < Vec<T>::N; ++e) {
+      const int j = i * Vec<T>::N + e;
+      f[e] = j < V ? Vec<T>::load(p + j) : -INFINITY;
+    }
+  }
+};
+
+constexpr int FWD_THREADS = 512;
+
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(FWD_THREADS)
+    token_log_probs_fwd_kernel(const T* __restrict__ logits, const void* __restrict__ labels, bool labels64,
+                               float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, int V,
+                               RowMap map, float scale2, long long ignore_index) {
+  constexpr int N = Vec<T>::N;
+  __shared__ Stats red[FWD_THREADS / 32];
+  const long long row = blockIdx.x;
+  const long long label = load_label(labels, labels64, row);
+  if (label == ignore_index || label < 0 || label >= V) {
+    if (threadIdx.x == 0) {
+      log_probs[row] = 0.f;
+      lse[row] = make_float2(0.f, 0.f);
+      if (ENTROPY) entropy[row] = 0.f;
+    }
+    return;
+  }
+  const Row<T> r(logits + row_offset(map, row), V);
+  Stats st = empty_stats();
+  constexpr int UNROLL = 4;
+  for (int i0 = threadIdx.x; i0 < r.vectors; i0 += UNROLL * FWD_THREADS) {
+    uint4 v[UNROLL];
+    bool wide[UNROLL];
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const int i = i0 + k * FWD_THREADS;
+      wide[k] = i < r.vectors && r.wide(i);
+      if (wide[k]) v[k] = r.load_wide(i);
+    }
+#pragma unroll
+    for (int k = 0; k < UNROLL; ++k) {
+      const int i = i0 + k * FWD_THREADS;
+      if (i >= r.vectors) break;
+      float f[N];
+      if (wide[k]) Vec<T>::unpack(v[k], f);
+      else r.load_narrow(i, f);
+      accumulate<ENTROPY, N>(st, f, scale2);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats other;
+    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    other.u = ENTROPY ? __shfl_xor_sync(0xffffffffu, st.u, o) : 0.f;
+    st = merge<ENTROPY>(st, other, scale2);
+  }
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < FWD_THREADS / 32; ++w) st = merge<ENTROPY>(st, red[w], scale2);
+    const float log2_s = log2f(st.s);
+    lse[row] = make_float2(st.m, log2_s);
+    log_probs[row] = log2_prob(Vec<T>::load(r.p + label), make_float2(st.m, log2_s), scale2) * kLn2;
+    if (ENTROPY) entropy[row] = (log2_s - st.u / st.s) * kLn2;
+  }
+}
+
+constexpr int BWD_THREADS = 256;
+constexpr int BWD_UNROLL = 4;
+
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(BWD_THREADS)
+    token_log_probs_bwd_kernel(const T* __restrict__ logits, const void* __restrict__ labels, bool labels64,
+                               const float2* __restrict__ lse, const float* __restrict__ entropy,
+                               const float* __restrict__ d_log_probs, long long d_log_probs_stride,
+                               const float* __restrict__ d_entropy, long long d_entropy_stride, T* __restrict__ grad, int V,
+                               RowMap map, long long grad_stride, float logit_scale, float scale2,
+                               long long ignore_index) {
+  constexpr int N = Vec<T>::N;
+  const long long row = blockIdx.x;
+  const long long label = load_label(labels, labels64, row);
+  const bool ignored = label == ignore_index || label < 0 || label >= V;
+  const Row<T> r(logits + row_offset(map, row), V);
+  T* out = grad + row * grad_stride;
+  const float g = ignored ? 0.f : d_log_probs[row * d_log_probs_stride];
+  const float h = ignored || !ENTROPY ? 0.f : d_entropy[row * d_entropy_stride];
+  const int i0 = blockIdx.y * (BWD_THREADS * BWD_UNROLL) + threadIdx.x;
+  // rows without an upstream gradient get zeros and are not read
+  const bool zero = g == 0.f && h == 0.f;
+  const float2 L = lse[row];
+  const float H = ENTROPY ? entropy[row] : 0.f;
+  const float gs = g * logit_scale, hs = h * logit_scale;
+  uint4 v[BWD_UNROLL];
+  bool wide[BWD_UNROLL];
+#pragma unroll
+  for (int k = 0; k < BWD_UNROLL; ++k) {
+    const int i = i0 + k * BWD_THREADS;
+    wide[k] = i < r.vectors && r.wide(i);
+    v[k] = make_uint4(0, 0, 0, 0);
+    if (wide[k] && !zero) v[k] = r.load_wide(i);
+  }
+#pragma unroll
+  for (int k = 0; k < BWD_UNROLL; ++k) {
+    const int i = i0 + k * BWD_THREADS;
+    if (i >= r.vectors) return;
+    float f[N];
+    if (zero) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) f[e] = 0.f;
+    } else {
+      if (wide[k]) Vec<T>::unpack(v[k], f);
+      else r.load_narrow(i, f);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        f[e] = score_gradient<ENTROPY>(log2_prob(f[e], L, scale2), gs, hs, H);
+        if (i * N + e == label) f[e] += gs;
+      }
+    }
+    if ((i + 1) * N <= V) {
+      *reinterpret_cast<uint4*>(out + (long long)i * N) = Vec<T>::pack(f);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e)
+        if (i * N + e < V) Vec<T>::store(out + i * N + e, f[e]);
+    }
+  }
+}
+
+// One block: 32 rows (one per lane) x 32 warps that share the slices; the warps' statistics meet in shared memory.
+template <bool ENTROPY>
+__global__ void __launch_bounds__(1024)
+    token_log_probs_join_kernel(const float4* __restrict__ stats, int slices, int slice_width, const void* __restrict__ labels, bool labels64,
+                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, long long T, int V,
+                                float scale2, long long ignore_index) {
+  __shared__ Stats red[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = (long long)blockIdx.x * 32 + lane;
+  Stats st = empty_stats();
+  if (row < T) {
+    for (int i = warp; i < slices; i += 32) {
+      const float4 v = stats[(long long)i * T + row];
+      st = merge<ENTROPY>(st, Stats{v.x, v.y, v.z}, scale2);
+    }
+  }
+  red[warp][lane] = st;
+  __syncthreads();
+  if (warp != 0 || row >= T) return;
+  for (int w = 1; w < 32; ++w) st = merge<ENTROPY>(st, red[w][lane], scale2);
+  const long long label = load_label(labels, labels64, row);
+  if (label == ignore_index || label < 0 || label >= V) {
+    log_probs[row] = 0.f;
+    lse[row] = make_float2(0.f, 0.f);
+    if (ENTROPY) entropy[row] = 0.f;
+    return;
+  }
+  const float log2_s = log2f(st.s), x = stats[(long long)(label / slice_width) * T + row].w;
+  lse[row] = make_float2(st.m, log2_s);
+  log_probs[row] = log2_prob(x, make_float2(st.m, log2_s), scale2) * kLn2;
+  if (ENTROPY) entropy[row] = (log2_s - st.u / st.s) * kLn2;
+}
+
+template <typename T>
+void fwd(const void* logits, const void* labels, bool labels64, float* log_probs, float* entropy, float2* lse, long long rows,
+         int V, RowMap map, float scale2, long long ignore_index, cudaStream_t stream) {
+  const T* x = reinterpret_cast<const T*>(logits);
+  if (entropy != nullptr)
+    token_log_probs_fwd_kernel<T, true><<<(unsigned)rows, FWD_THREADS, 0, stream>>>(x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index);
+  else
+    token_log_probs_fwd_kernel<T, false><<<(unsigned)rows, FWD_THREADS, 0, stream>>>(x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index);
+}
+
+template <typename T>
+void bwd(const void* logits, const void* labels, bool labels64, const float2* lse, const float* entropy, const float* d_log_probs,
+         long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long rows, int V,
+         RowMap map, long long grad_stride, float logit_scale, long long ignore_index, cudaStream_t stream) {
+  const T* x = reinterpret_cast<const T*>(logits);
+  const int vectors = (V + Vec<T>::N - 1) / Vec<T>::N;
+  const dim3 grid((unsigned)rows, (unsigned)((vectors + BWD_THREADS * BWD_UNROLL - 1) / (BWD_THREADS * BWD_UNROLL)));
+  const float scale2 = logit_scale * kLog2e;
+  if (d_entropy != nullptr)
+    token_log_probs_bwd_kernel<T, true><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
+                                                                          reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index);
+  else
+    token_log_probs_bwd_kernel<T, false><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
+                                                                           reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index);
+}
+
+}  // namespace
+
+void token_log_probs_fwd(const void* logits, Scalar type, const void* labels, bool labels64, float* log_probs, float* entropy,
+                         float2* lse, long long T, int V, RowMap map, float logit_scale, long long ignore_index, cudaStream_t stream) {
+  if (T == 0) return;
+  auto launch = type == Scalar::kBf16 ? fwd<__nv_bfloat16> : type == Scalar::kF16 ? fwd<__half> : fwd<float>;
+  launch(logits, labels, labels64, log_probs, entropy, lse, T, V, map, logit_scale * kLog2e, ignore_index, stream);
+  count_launch();
+  check_cuda(cudaGetLastError(), "token_log_probs forward launch");
+}
+
+void token_log_probs_bwd(const void* logits, Scalar type, const void* labels, bool labels64, const float2* lse,
+                         const float* entropy, const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy,
+                         long long d_entropy_stride, void* grad, long long T, int V, RowMap map, long long grad_stride,
+                         float logit_scale, long long ignore_index, cudaStream_t stream) {
+  if (T == 0) return;
+  auto launch = type == Scalar::kBf16 ? bwd<__nv_bfloat16> : type == Scalar::kF16 ? bwd<__half> : bwd<float>;
+  launch(logits, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride, grad, T, V, map,
+         grad_stride, logit_scale, ignore_index, stream);
+  count_launch();
+  check_cuda(cudaGetLastError(), "token_log_probs backward launch");
+}
+
+void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
+                          float* entropy, float2* lse, long long T, int V, float logit_scale, long long ignore_index, cudaStream_t stream) {
+  if (T == 0) return;
+  const unsigned blocks = (unsigned)((T + 31) / 32);
+  const float4* st = reinterpret_cast<const float4*>(stats);
+  if (entropy != nullptr)
+    token_log_probs_join_kernel<true><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, T, V, logit_scale * kLog2e, ignore_index);
+  else
+    token_log_probs_join_kernel<false><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, T, V, logit_scale * kLog2e, ignore_index);
+  count_launch();
+  check_cuda(cudaGetLastError(), "token_log_probs join launch");
+}
+
+}  // namespace b200

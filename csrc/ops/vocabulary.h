@@ -1,0 +1,100 @@
+// Launch interface of the operators over the vocabulary (raw pointers and a stream, no tensor library types):
+// log-probabilities of given tokens, preference and policy losses, embedding gradient in sorted token order.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace b200 {
+
+enum class Scalar : int { kBf16 = 0, kF16 = 1, kF32 = 2 };
+
+// ---- ops/token_log_probs.cu
+// Where row r of a batch of logits [outer, inner, V] lies: (r / inner) * outer_stride + (r % inner) * row_stride elements from the base.
+struct RowMap {
+  long long inner, outer_stride, row_stride;
+};
+// T rows of V logits with a unit inner stride. log_probs: fp32 [T]; entropy: fp32 [T] or null; lse: [T] pairs (largest logit m,
+// log2 of sum 2^(logit_scale log2e (x - m))), the log-sum-exp as the backward pass takes it.
+void token_log_probs_fwd(const void* logits, Scalar type, const void* labels, bool labels64, float* log_probs, float* entropy,
+                         float2* lse, long long T, int V, RowMap map, float logit_scale, long long ignore_index, cudaStream_t stream);
+// d_log_probs / d_entropy: fp32 with strides (elements, 0 for a broadcast value); d_entropy may be null. grad: 16-byte
+// aligned rows, grad_stride elements apart.
+void token_log_probs_bwd(const void* logits, Scalar type, const void* labels, bool labels64, const float2* lse,
+                         const float* entropy, const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy,
+                         long long d_entropy_stride, void* grad, long long T, int V, RowMap map, long long grad_stride,
+                         float logit_scale, long long ignore_index, cudaStream_t stream);
+
+// Joins the statistics of `slices` column slices of the rows: stats[slice][T] = (m, s, u, the label's logit if it lies in the
+// slice), see softmax_stats.cuh. Ignored rows give 0.
+void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
+                          float* entropy, float2* lse, long long T, int V, float logit_scale, long long ignore_index, cudaStream_t stream);
+
+// ---- gemm/vocab_gemm_2sm.cu: logits = x [M, K] w [N, K]^T, bf16 operands with row strides that are multiples of 8 elements;
+// the logits stay in tensor memory.
+constexpr int kVocabTile = 256;  // columns per slice of the statistics
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, int M, int N,
+                      int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream);
+// grad[M, N] (bf16, row stride ldg, a multiple of 8): gradient of the logits, as token_log_probs_bwd defines it.
+void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labels64, const float2* lse, const float* entropy,
+                     const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
+                     void* grad, int M, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
+                     long long ignore_index, int* status, cudaStream_t stream);
+
+// ---- ops/preference.cu
+// A packed batch of `sequences` sequences of per-token values: sequence i is tokens [cu[i], cu[i + 1]), or, without cu,
+// [i * length, (i + 1) * length). mask (bytes, or null): tokens with 0 take no part and are not looked at. cu entries are
+// clamped to [0, T].
+struct PackedTokens {
+  long long T;
+  const int* cu;
+  long long length;
+  int sequences;
+  const unsigned char* mask;
+};
+long long packed_partials(long long T, int sequences);  // fp32 words of the workspace that both losses take
+
+enum class PreferenceKind : int { kSigmoid = 0, kHinge = 1, kIpo = 2 };
+struct PreferenceArgs {
+  PreferenceKind kind;
+  float beta, label_smoothing;
+  bool average;   // log-ratio of a sequence: mean over its tokens instead of the sum
+  int reduction;  // 0 = loss per pair, 1 = sum, 2 = mean
+};
+// sequences = 2 * pairs, chosen first. loss: [pairs] or [1]; rewards: [2 * pairs] = beta * log-ratio; slope: [2 * pairs] =
+// d(loss) / d(log-prob of a token of that sequence). reference may be null (0).
+void preference_loss_fwd(const float* log_probs, const float* reference, PackedTokens tokens, PreferenceArgs args, float* partials,
+                         float* loss, float* rewards, float* slope, cudaStream_t stream);
+// grad[t] = slope[sequence of t] * d_loss[pair * d_loss_stride], 0 for tokens that take no part.
+void preference_loss_bwd(const float* slope, const float* d_loss, long long d_loss_stride, PackedTokens tokens, float* grad,
+                         cudaStream_t stream);
+
+struct PolicyArgs {
+  double log_low, log_high;  // log(1 - clip_low), log(1 + clip_high): the clipping borders of log(ratio)
+  float ratio_low, ratio_high;
+  float dual_clip;           // 0: none
+  float kl_coef;
+  bool per_token_advantage;
+  int reduction;             // 0 = sum, 1 = mean over tokens, 2 = mean over sequences of their token means
+};
+// out: [4] = loss, mean KL estimate, fraction of clipped tokens, 1 / divisor of the reduction; slope (or null): [T] d(token's loss) /
+// d(log-prob); weight: [sequences] 1 / tokens of the sequence (reduction 2 only).
+void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const float* reference, const float* advantages,
+                     PackedTokens tokens, PolicyArgs args, float* partials, float* out, float* slope, float* weight, cudaStream_t stream);
+// grad[t] = slope[t] * out[3] (* weight[sequence of t]) * d_loss, 0 for tokens that take no part.
+void policy_loss_bwd(const float* slope, const float* out, const float* weight, const float* d_loss, PackedTokens tokens, int reduction, float* grad,
+                     cudaStream_t stream);
+
+// ---- ops/embedding_sorted.cu
+constexpr int kStatusBadTokenId = 7;  // an id outside of [0, V): its output row is 0, it takes no part in the gradient
+// out[t] = scale * weight[ids[t]]
+void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids64, void* out, long long T, long long V, int H,
+                      float scale, int* status, cudaStream_t stream);
+// Bytes of the workspace of the gradient.
+long long embedding_gradient_workspace(long long T, int H);
+// Rows of dweight that some id names: scale * sum of dout[t] over the tokens with that id, in the order of t; other rows are
+// not touched. accumulate: dweight is fp32 and is added to, else it has dout's type and is overwritten.
+void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids64, void* dweight, bool accumulate, void* workspace,
+                        long long T, long long V, int H, float scale, cudaStream_t stream);
+
+}  // namespace b200

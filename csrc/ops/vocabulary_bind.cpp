@@ -1,0 +1,334 @@
+// Python bindings of the vocabulary operators: argument checks, outputs and workspaces from the tensor allocator, launches on
+// the current stream of the operands' device.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "vocabulary.h"
+
+namespace b200 {
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
+
+Scalar scalar_of(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case torch::kBFloat16: return Scalar::kBf16;
+    case torch::kFloat16: return Scalar::kF16;
+    case torch::kFloat32: return Scalar::kF32;
+    default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32, got ", t.scalar_type());
+  }
+  return Scalar::kF32;
+}
+
+void check_device(const Tensor& t, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
+}
+
+void check_indices(const Tensor& t, const Tensor& like, const char* name) {
+  check_device(t, like, name);
+  TORCH_CHECK(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32, name, " must be int64 or int32, got ", t.scalar_type());
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+// fp32 values of `rows` rows as a pointer and a stride (0 for a broadcast value)
+const float* row_values(const Tensor& t, const Tensor& like, int64_t rows, const char* name, long long* stride) {
+  check_device(t, like, name);
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.dim() == 1 && t.size(0) == rows, name, " must be fp32 [", rows, "]");
+  *stride = t.stride(0);
+  return t.data_ptr<float>();
+}
+
+const float* contiguous_f32(const Tensor& t, const Tensor& like, int64_t count, const char* name) {
+  check_device(t, like, name);
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.numel() == count, name, " must be contiguous fp32 with ", count, " elements");
+  return t.data_ptr<float>();
+}
+
+Tensor empty_f32(int64_t n, const Tensor& like) { return torch::empty({n}, like.options().dtype(torch::kFloat32)); }
+
+Tensor empty_pairs(int64_t n, const Tensor& like) { return torch::empty({n, 2}, like.options().dtype(torch::kFloat32)); }
+float2* pairs(const Tensor& t) { return reinterpret_cast<float2*>(t.data_ptr<float>()); }
+const float2* checked_pairs(const Tensor& t, const Tensor& like, int64_t rows) {
+  return reinterpret_cast<const float2*>(contiguous_f32(t, like, 2 * rows, "lse"));
+}
+
+// logits: [outer, inner, V] with a unit inner stride
+RowMap row_map(const Tensor& logits) {
+  TORCH_CHECK(logits.dim() == 3, "logits must be [outer, inner, V]");
+  TORCH_CHECK(logits.stride(2) == 1 || logits.size(2) == 1, "logits must have a unit inner stride");
+  TORCH_CHECK(logits.size(2) > 0 && logits.size(2) <= (1 << 29), "the vocabulary size must be in [1, 2^29]");
+  TORCH_CHECK(logits.size(0) * logits.size(1) < (1LL << 31), "at most 2^31 - 1 rows of logits");
+  return {std::max<int64_t>(logits.size(1), 1), logits.stride(0), logits.stride(1)};
+}
+
+std::tuple<Tensor, Tensor, Tensor> log_probs_fwd(const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  const Scalar type = scalar_of(logits, "logits");
+  const RowMap map = row_map(logits);
+  const int64_t rows = logits.size(0) * logits.size(1);
+  check_indices(labels, logits, "labels");
+  TORCH_CHECK(labels.numel() == rows, "labels must have one entry per row of logits");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  Tensor log_probs = empty_f32(rows, logits), lse = empty_pairs(rows, logits), entropy = want_entropy ? empty_f32(rows, logits) : Tensor();
+  token_log_probs_fwd(logits.data_ptr(), type, labels.data_ptr(), labels.scalar_type() == torch::kInt64, log_probs.data_ptr<float>(),
+                      want_entropy ? entropy.data_ptr<float>() : nullptr, pairs(lse), rows, (int)logits.size(2), map, (float)logit_scale,
+                      ignore_index, stream_of(logits));
+  return {log_probs, entropy, lse};
+}
+
+// Gradient [outer, inner, V] in the logits' type; its rows start at multiples of 16 bytes (padded when V needs it).
+Tensor log_probs_bwd(const Tensor& logits, const Tensor& labels, const Tensor& lse, const OptTensor& entropy, const Tensor& d_log_probs,
+                     const OptTensor& d_entropy, double logit_scale, int64_t ignore_index) {
+  TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
+  const Scalar type = scalar_of(logits, "logits");
+  const RowMap map = row_map(logits);
+  const int64_t outer = logits.size(0), inner = logits.size(1), V = logits.size(2), rows = outer * inner;
+  check_indices(labels, logits, "labels");
+  TORCH_CHECK(labels.numel() == rows, "labels must have one entry per row of logits");
+  long long g_stride = 0, h_stride = 0;
+  const float* g = row_values(d_log_probs, logits, rows, "d_log_probs", &g_stride);
+  const float* h = d_entropy.has_value() ? row_values(*d_entropy, logits, rows, "d_entropy", &h_stride) : nullptr;
+  TORCH_CHECK(h == nullptr || entropy.has_value(), "the entropy gradient needs the entropy of the forward pass");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t per_16 = 16 / logits.element_size();
+  const int64_t pitch = (V + per_16 - 1) / per_16 * per_16;
+  Tensor grad = torch::empty({outer, inner, pitch}, logits.options()).narrow(2, 0, V);
+  token_log_probs_bwd(logits.data_ptr(), type, labels.data_ptr(), labels.scalar_type() == torch::kInt64, checked_pairs(lse, logits, rows),
+                      h != nullptr ? contiguous_f32(*entropy, logits, rows, "entropy") : nullptr, g, g_stride, h, h_stride, grad.data_ptr(), rows, (int)V,
+                      map, pitch, (float)logit_scale, ignore_index, stream_of(logits));
+  return grad;
+}
+
+void check_linear(const Tensor& x, const Tensor& w, const Tensor& labels) {
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == torch::kBFloat16 && w.scalar_type() == torch::kBFloat16, "hidden states and weight must be bf16 CUDA tensors");
+  check_device(w, x, "weight");
+  TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "hidden states must be [T, H] and the weight [V, H]");
+  TORCH_CHECK(x.stride(1) == 1 && w.stride(1) == 1, "hidden states and weight must have a unit inner stride");
+  TORCH_CHECK(x.size(1) > 0 && x.size(1) % 8 == 0 && x.stride(0) % 8 == 0 && w.stride(0) % 8 == 0, "H and the row strides must be multiples of 8");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(w.data_ptr())) % 16 == 0, "hidden states and weight must be 16-byte aligned");
+  TORCH_CHECK(w.size(0) > 0 && w.size(0) <= (1 << 29) && x.size(1) < (1 << 30) && x.size(0) < (1LL << 31), "sizes out of range");
+  check_indices(labels, x, "labels");
+  TORCH_CHECK(labels.numel() == x.size(0), "labels must have one entry per row of hidden states");
+}
+
+int* status_of(const Tensor& status, const Tensor& like) {
+  check_device(status, like, "status");
+  TORCH_CHECK(status.scalar_type() == torch::kInt32 && status.numel() >= 1, "status must be int32");
+  return status.data_ptr<int>();
+}
+
+const char* label_ptr(const Tensor& labels, int64_t row) { return reinterpret_cast<const char*>(labels.data_ptr()) + row * labels.element_size(); }
+
+// Rows that share one statistics buffer: 16 bytes per row and 256 columns stay below 512 MB.
+int64_t stats_rows(int64_t rows, int64_t slices) {
+  const int64_t most = std::max<int64_t>(256, ((512LL << 20) / (16 * slices)) / 256 * 256);
+  return std::min(rows, std::min<int64_t>(most, 1 << 20));
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy,
+                                                        const Tensor& status) {
+  check_linear(x, w, labels);
+  int* st = status_of(status, x);
+  const c10::cuda::CUDAGuard guard(x.device());
+  const int64_t rows = x.size(0), V = w.size(0), slices = (V + kVocabTile - 1) / kVocabTile;
+  const bool labels64 = labels.scalar_type() == torch::kInt64;
+  Tensor log_probs = empty_f32(rows, x), lse = empty_pairs(rows, x), entropy = want_entropy ? empty_f32(rows, x) : Tensor();
+  if (rows == 0) return {log_probs, entropy, lse};
+  const int64_t most = stats_rows(rows, slices);
+  Tensor stats = empty_f32(most * slices * 4, x);
+  const cudaStream_t stream = stream_of(x);
+  for (int64_t r = 0; r < rows; r += most) {
+    const int64_t n = std::min(most, rows - r);
+    const void* xr = reinterpret_cast<const char*>(x.data_ptr()) + r * x.stride(0) * 2;
+    vocab_gemm_stats(xr, w.data_ptr(), label_ptr(labels, r), labels64, stats.data_ptr<float>(), want_entropy, (int)n, (int)V, (int)x.size(1), x.stride(0), w.stride(0),
+                     (float)logit_scale, st, stream);
+    token_log_probs_join(stats.data_ptr<float>(), (int)slices, kVocabTile, label_ptr(labels, r), labels64, log_probs.data_ptr<float>() + r,
+                         want_entropy ? entropy.data_ptr<float>() + r : nullptr, pairs(lse) + r, n, (int)V, (float)logit_scale, ignore_index, stream);
+  }
+  return {log_probs, entropy, lse};
+}
+
+// grad[T, V] (bf16, row stride a multiple of 8) <- gradient of the logits
+void linear_log_probs_grad(const Tensor& x, const Tensor& w, const Tensor& labels, const Tensor& lse, const OptTensor& entropy, const Tensor& d_log_probs,
+                           const OptTensor& d_entropy, Tensor& grad, double logit_scale, int64_t ignore_index, const Tensor& status) {
+  check_linear(x, w, labels);
+  int* st = status_of(status, x);
+  const int64_t rows = x.size(0), V = w.size(0);
+  check_device(grad, x, "grad");
+  TORCH_CHECK(grad.scalar_type() == torch::kBFloat16 && grad.dim() == 2 && grad.size(0) == rows && grad.size(1) == V && grad.stride(1) == 1 && grad.stride(0) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0,
+              "grad must be bf16 [T, V] with 16-byte aligned rows");
+  long long g_stride = 0, h_stride = 0;
+  const float* g = row_values(d_log_probs, x, rows, "d_log_probs", &g_stride);
+  const float* h = d_entropy.has_value() ? row_values(*d_entropy, x, rows, "d_entropy", &h_stride) : nullptr;
+  TORCH_CHECK(h == nullptr || entropy.has_value(), "the entropy gradient needs the entropy of the forward pass");
+  const c10::cuda::CUDAGuard guard(x.device());
+  vocab_gemm_grad(x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.scalar_type() == torch::kInt64, checked_pairs(lse, x, rows),
+                  h != nullptr ? contiguous_f32(*entropy, x, rows, "entropy") : nullptr, g, g_stride, h, h_stride, grad.data_ptr(), (int)rows, (int)V, (int)x.size(1),
+                  x.stride(0), w.stride(0), grad.stride(0), (float)logit_scale, ignore_index, st, stream_of(x));
+}
+
+// ------------------------------------------------------------------------- losses over sequences
+PackedTokens packed_tokens(const Tensor& values, const OptTensor& cu, int64_t length, int64_t sequences, const OptTensor& mask) {
+  PackedTokens p = {};
+  p.T = values.numel();
+  TORCH_CHECK(p.T < (1LL << 31) && sequences >= 0 && sequences < (1LL << 31) - 1, "at most 2^31 - 1 tokens and sequences");
+  p.length = length;
+  p.sequences = (int)sequences;
+  if (cu.has_value()) {
+    check_device(*cu, values, "cu_seqlens");
+    TORCH_CHECK(cu->scalar_type() == torch::kInt32 && cu->is_contiguous() && cu->numel() == sequences + 1, "cu_seqlens must be contiguous int32 [sequences + 1]");
+    p.cu = cu->data_ptr<int>();
+  } else {
+    TORCH_CHECK(length * sequences == p.T, "sequences of one length must cover all tokens");
+  }
+  if (mask.has_value()) {
+    check_device(*mask, values, "mask");
+    TORCH_CHECK((mask->scalar_type() == torch::kBool || mask->scalar_type() == torch::kUInt8) && mask->is_contiguous() && mask->numel() == p.T,
+                "mask must be contiguous, boolean, one entry per token");
+    p.mask = reinterpret_cast<const unsigned char*>(mask->data_ptr());
+  }
+  return p;
+}
+
+// (loss, rewards [2 * pairs], slope [2 * pairs])
+std::tuple<Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu, int64_t length, int64_t sequences,
+                                                  const OptTensor& mask, int64_t kind, double beta, double label_smoothing, bool average, int64_t reduction) {
+  TORCH_CHECK(log_probs.is_cuda(), "log_probs must be a CUDA tensor");
+  TORCH_CHECK(sequences > 0 && sequences % 2 == 0, "an even number of sequences is needed: chosen, then rejected");
+  TORCH_CHECK(kind >= 0 && kind <= 2 && reduction >= 0 && reduction <= 2, "unknown loss type or reduction");
+  const PackedTokens p = packed_tokens(log_probs, cu, length, sequences, mask);
+  const float* lp = contiguous_f32(log_probs, log_probs, p.T, "log_probs");
+  const float* ref = reference.has_value() ? contiguous_f32(*reference, log_probs, p.T, "reference_log_probs") : nullptr;
+  const c10::cuda::CUDAGuard guard(log_probs.device());
+  Tensor loss = reduction == 0 ? empty_f32(sequences / 2, log_probs) : torch::empty({}, log_probs.options());
+  Tensor rewards = empty_f32(sequences, log_probs), slope = empty_f32(sequences, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
+  const PreferenceArgs args = {(PreferenceKind)kind, (float)beta, (float)label_smoothing, average, (int)reduction};
+  preference_loss_fwd(lp, ref, p, args, partials.data_ptr<float>(), loss.data_ptr<float>(), rewards.data_ptr<float>(), slope.data_ptr<float>(), stream_of(log_probs));
+  return {loss, rewards, slope};
+}
+
+Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& log_probs, const OptTensor& cu, int64_t length, const OptTensor& mask) {
+  const int64_t sequences = slope.numel();
+  const PackedTokens p = packed_tokens(log_probs, cu, length, sequences, mask);
+  contiguous_f32(slope, log_probs, sequences, "slope");
+  long long stride = 0;
+  const float* d = nullptr;
+  if (d_loss.dim() == 0) {
+    d = contiguous_f32(d_loss, log_probs, 1, "d_loss");
+  } else {
+    d = row_values(d_loss, log_probs, sequences / 2, "d_loss", &stride);
+  }
+  const c10::cuda::CUDAGuard guard(log_probs.device());
+  Tensor grad = torch::empty(log_probs.sizes(), log_probs.options());
+  preference_loss_bwd(slope.data_ptr<float>(), d, stride, p, grad.data_ptr<float>(), stream_of(log_probs));
+  return grad;
+}
+
+// (out [4], slope [T] or undefined, weight [sequences])
+std::tuple<Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Tensor& old_log_probs, const OptTensor& reference, const Tensor& advantages, bool per_token,
+                                              const OptTensor& cu, int64_t length, int64_t sequences, const OptTensor& mask, double clip_low, double clip_high,
+                                              double dual_clip, double kl_coef, int64_t reduction, bool want_slope) {
+  TORCH_CHECK(log_probs.is_cuda(), "log_probs must be a CUDA tensor");
+  TORCH_CHECK(reduction >= 0 && reduction <= 2, "unknown reduction");
+  const PackedTokens p = packed_tokens(log_probs, cu, length, sequences, mask);
+  const float* lp = contiguous_f32(log_probs, log_probs, p.T, "log_probs");
+  const float* old = contiguous_f32(old_log_probs, log_probs, p.T, "old_log_probs");
+  const float* ref = reference.has_value() ? contiguous_f32(*reference, log_probs, p.T, "reference_log_probs") : nullptr;
+  const float* adv = contiguous_f32(advantages, log_probs, per_token ? p.T : sequences, "advantages");
+  const c10::cuda::CUDAGuard guard(log_probs.device());
+  Tensor out = empty_f32(4, log_probs), slope = want_slope ? empty_f32(p.T, log_probs) : Tensor();
+  Tensor weight = empty_f32(reduction == 2 ? sequences : 0, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
+  PolicyArgs args = {};
+  args.log_low = std::log1p(-clip_low);
+  args.log_high = std::log1p(clip_high);
+  args.ratio_low = (float)(1.0 - clip_low);
+  args.ratio_high = (float)(1.0 + clip_high);
+  args.dual_clip = (float)dual_clip;
+  args.kl_coef = (float)kl_coef;
+  args.per_token_advantage = per_token;
+  args.reduction = (int)reduction;
+  policy_loss_fwd(lp, old, ref, adv, p, args, partials.data_ptr<float>(), out.data_ptr<float>(), want_slope ? slope.data_ptr<float>() : nullptr, weight.data_ptr<float>(),
+                  stream_of(log_probs));
+  return {out, slope, weight};
+}
+
+Tensor policy_bwd(const Tensor& slope, const Tensor& out, const Tensor& weight, const Tensor& d_loss, at::IntArrayRef shape, const OptTensor& cu, int64_t length,
+                  int64_t sequences, const OptTensor& mask, int64_t reduction) {
+  const PackedTokens p = packed_tokens(slope, cu, length, sequences, mask);
+  contiguous_f32(slope, slope, p.T, "slope");
+  contiguous_f32(out, slope, 4, "out");
+  contiguous_f32(weight, slope, reduction == 2 ? sequences : 0, "weight");
+  contiguous_f32(d_loss, slope, 1, "d_loss");
+  const c10::cuda::CUDAGuard guard(slope.device());
+  Tensor grad = torch::empty(shape, slope.options());
+  TORCH_CHECK(grad.numel() == p.T, "shape mismatch");
+  policy_loss_bwd(slope.data_ptr<float>(), out.data_ptr<float>(), weight.data_ptr<float>(), d_loss.data_ptr<float>(), p, (int)reduction, grad.data_ptr<float>(),
+                  stream_of(slope));
+  return grad;
+}
+
+// ------------------------------------------------------------------------- embedding
+Tensor embedding_lookup_(const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
+  TORCH_CHECK(weight.is_cuda() && weight.dim() == 2 && weight.is_contiguous(), "weight must be a contiguous [V, H] CUDA tensor");
+  const Scalar type = scalar_of(weight, "weight");
+  check_indices(ids, weight, "ids");
+  TORCH_CHECK(ids.numel() < (1LL << 31) && weight.size(1) < (1 << 30), "sizes out of range");
+  int* st = status_of(status, weight);
+  const c10::cuda::CUDAGuard guard(weight.device());
+  auto shape = ids.sizes().vec();
+  shape.push_back(weight.size(1));
+  Tensor out = torch::empty(shape, weight.options());
+  embedding_lookup(weight.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, out.data_ptr(), ids.numel(), weight.size(0), (int)weight.size(1), (float)scale, st,
+                   stream_of(weight));
+  return out;
+}
+
+// dweight (fp32, added to) or, without it, a new [V, H] gradient in dout's type.
+Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, const OptTensor& dweight, double scale) {
+  TORCH_CHECK(dout.is_cuda() && dout.is_contiguous() && dout.dim() >= 1, "dout must be a contiguous CUDA tensor");
+  const Scalar type = scalar_of(dout, "dout");
+  check_indices(ids, dout, "ids");
+  const int64_t T = ids.numel(), H = dout.size(-1);
+  TORCH_CHECK(dout.numel() == T * H && T < (1LL << 31) && H < (1 << 30) && V >= 0 && V < (1LL << 31) - 1, "dout must be [T, H] for T ids; at most 2^31 - 2 rows");
+  const c10::cuda::CUDAGuard guard(dout.device());
+  Tensor dw;
+  if (dweight.has_value()) {
+    dw = *dweight;
+    contiguous_f32(dw, dout, V * H, "dweight");
+  } else {
+    dw = torch::zeros({V, H}, dout.options());
+  }
+  Tensor workspace = torch::empty({embedding_gradient_workspace(T, (int)H)}, dout.options().dtype(torch::kUInt8));
+  embedding_gradient(dout.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, dw.data_ptr(), dweight.has_value(), workspace.data_ptr(), T, V, (int)H, (float)scale,
+                     stream_of(dout));
+  return dw;
+}
+
+}  // namespace
+
+void register_vocabulary(pybind11::module_& m) {
+  m.def("log_probs_fwd", &log_probs_fwd, "log-probabilities of given tokens, entropies and log-sum-exps of rows of logits");
+  m.def("log_probs_bwd", &log_probs_bwd);
+  m.def("linear_log_probs_fwd", &linear_log_probs_fwd, "the same from hidden states and the output weight");
+  m.def("linear_log_probs_grad", &linear_log_probs_grad);
+  m.def("preference_loss_fwd", &preference_fwd);
+  m.def("preference_loss_bwd", &preference_bwd);
+  m.def("policy_loss_fwd", &policy_fwd);
+  m.def("policy_loss_bwd", [](const Tensor& slope, const Tensor& out, const Tensor& weight, const Tensor& d_loss, std::vector<int64_t> shape, const OptTensor& cu, int64_t length,
+                              int64_t sequences, const OptTensor& mask, int64_t reduction) {
+    return policy_bwd(slope, out, weight, d_loss, shape, cu, length, sequences, mask, reduction);
+  });
+  m.def("embedding_lookup", &embedding_lookup_);
+  m.def("embedding_gradient", &embedding_gradient_, "embedding gradient summed in sorted token order");
+}
+
+}  // namespace b200

@@ -52,6 +52,7 @@ def status_word(device: torch.device | None = None) -> torch.Tensor:
 
 
 STATUS_GRAD_SCALE_MISMATCH = 6  # fused linear + cross entropy: upstream gradient differs from the promised scale
+STATUS_BAD_TOKEN_ID = 7  # embedding with a sorted gradient: an id outside of the table
 
 
 def check_status() -> None:
@@ -65,6 +66,8 @@ def check_status() -> None:
                 raise RuntimeError(f"cuda:{index}: the fused linear + cross entropy was promised a gradient scale "
                                    "(grad_scale_hint) that differs from the gradient it received; its weight and input "
                                    "gradients of the steps since the last check are wrong")
+            if code == STATUS_BAD_TOKEN_ID:
+                raise RuntimeError(f"cuda:{index}: an embedding was given a token id outside of its table")
             raise RuntimeError(f"a kernel on cuda:{index} gave up waiting (status {code})")
 
 
@@ -330,7 +333,11 @@ class _EmbeddingFn(torch.autograd.Function):
         return dw.to(weight.dtype), None, None
 
 
-def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, *, sorted_gradient: bool = False) -> torch.Tensor:
+    """``scale * weight[ids]``. ``sorted_gradient`` sums the weight gradient in sorted token order instead of with atomics:
+    see :func:`embedding_sorted`."""
+    if sorted_gradient:
+        return embedding_sorted(weight, ids, scale)
     if use_native(weight) and weight.dtype == torch.bfloat16 and ids.is_cuda and weight.shape[1] % 8 == 0:
         return _EmbeddingFn.apply(weight, ids.long(), float(scale))
     note_fallback("embedding", "hidden size is not a multiple of 8 or the ids are not on the device", weight)
@@ -438,3 +445,14 @@ def cross_entropy(logits: torch.Tensor, labels: torch.Tensor, *, ignore_index: i
     """fp32 cross entropy on materialised logits."""
     loss = F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1).long(), ignore_index=ignore_index, reduction=reduction)
     return loss
+
+
+from .vocabulary import (  # noqa: E402  (uses the helpers above)
+    PolicyLossOutput,
+    PreferenceLossOutput,
+    embedding_sorted,
+    fused_linear_token_log_probs,
+    policy_loss,
+    preference_loss,
+    token_log_probs,
+)

@@ -1,0 +1,478 @@
+"""Operators over the vocabulary for preference and reward tuning.
+
+* :func:`token_log_probs`: log-probabilities (and entropies) of given tokens under rows of logits
+* :func:`fused_linear_token_log_probs`: the same from hidden states and the output weight, logits never in memory
+* :func:`preference_loss`: loss over pairs of answers from their summed log-probability ratios
+* :func:`policy_loss`: clipped policy-gradient loss with a KL term
+* :func:`embedding_sorted`: embedding whose gradient is summed in sorted token order (``ops.embedding(sorted_gradient=True)``)
+
+Each runs the sm_100a kernels of ``csrc/ops`` and ``csrc/gemm`` on CUDA tensors and a plain PyTorch restatement elsewhere.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import NamedTuple
+
+import torch
+import torch.nn.functional as F
+
+from . import _flce_chunk_rows, _weight_grad_target, native, note_fallback, require_native, status_word
+from .timeline import site
+
+_LOGIT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _on_gpu(t: torch.Tensor, types: tuple[torch.dtype, ...]) -> bool:
+    if not t.is_cuda or t.dtype not in types:
+        return False
+    require_native()
+    return True
+
+
+def _check_labels(labels: torch.Tensor, rows: torch.Size, device: torch.device, name: str = "labels") -> None:
+    if labels.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"{name} must be int64 or int32, got {labels.dtype}")
+    if labels.shape != rows:
+        raise ValueError(f"{name} must have the shape {tuple(rows)}, got {tuple(labels.shape)}")
+    if labels.device != device:
+        raise ValueError(f"{name} must be on {device}, got {labels.device}")
+
+
+def _check_logit_scale(logit_scale: float) -> float:
+    logit_scale = float(logit_scale)
+    if not (math.isfinite(logit_scale) and logit_scale > 0):
+        raise ValueError(f"logit_scale must be positive and finite, got {logit_scale}")
+    return logit_scale
+
+
+# ----------------------------------------------------------------------------- token log-probabilities
+def _token_log_probs_torch(logits: torch.Tensor, labels: torch.Tensor, logit_scale: float, ignore_index: int, return_entropy: bool):
+    vocab = logits.shape[-1]
+    kept = (labels != ignore_index) & (labels >= 0) & (labels < vocab)
+    z = logits if logits.dtype == torch.float64 else logits.float()
+    z = torch.where(kept[..., None], z, 0.0) * logit_scale  # whatever an ignored row holds, it has no part and no gradient
+    logp = z.log_softmax(-1)
+    picked = logp.gather(-1, torch.where(kept, labels, 0).long()[..., None]).squeeze(-1)
+    picked = torch.where(kept, picked, 0.0)
+    if not return_entropy:
+        return picked
+    # a token of probability 0 contributes 0, also where its log-probability is -inf
+    entropy = -(logp.exp() * logp.clamp_min(torch.finfo(logp.dtype).min)).sum(-1)
+    return picked, torch.where(kept, entropy, 0.0)
+
+
+def _rows3(logits: torch.Tensor) -> torch.Tensor:
+    """``[outer, inner, V]`` view of a batch of logits (a shifted ``[B, S, V]`` slice stays a view), copied only where its layout has no such form."""
+    if logits.dim() == 1:
+        logits = logits[None, None]
+    elif logits.dim() == 2:
+        logits = logits[None]
+    elif logits.dim() > 3:
+        logits = logits.flatten(0, -3)
+    return logits if logits.stride(-1) == 1 or logits.shape[-1] == 1 else logits.contiguous()
+
+
+def _row_gradient(grad: torch.Tensor | None, rows: int, like: torch.Tensor) -> torch.Tensor:
+    if grad is None:
+        return torch.zeros((), dtype=torch.float32, device=like.device).expand(rows)
+    return grad.reshape(-1)
+
+
+class _TokenLogProbsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, logit_scale, ignore_index, return_entropy):
+        ctx.set_materialize_grads(False)
+        with site("token_log_probs.fwd"):
+            log_probs, entropy, lse = native().log_probs_fwd(_rows3(logits), labels.contiguous(), logit_scale, ignore_index, return_entropy)
+        ctx.save_for_backward(logits, labels, lse, entropy)
+        ctx.args = (logit_scale, ignore_index)
+        shape = labels.shape
+        return (log_probs.view(shape), entropy.view(shape)) if return_entropy else log_probs.view(shape)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_log_probs, d_entropy=None):
+        logits, labels, lse, entropy = ctx.saved_tensors
+        if d_log_probs is None and d_entropy is None:
+            return (None,) * 5
+        rows = labels.numel()
+        with site("token_log_probs.bwd"):
+            grad = native().log_probs_bwd(_rows3(logits), labels.contiguous(), lse, entropy, _row_gradient(d_log_probs, rows, lse),
+                                          None if d_entropy is None else d_entropy.reshape(-1), *ctx.args)
+        return grad.view(logits.shape), None, None, None, None
+
+
+def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0, ignore_index: int = -100,
+                    return_entropy: bool = False):
+    """Log-probability of ``labels[...]`` under ``softmax(logit_scale * logits[..., :])``, fp32, shaped like ``labels``; with
+    ``return_entropy`` also the entropy of each row's distribution (nats).
+
+    Rows whose label is ``ignore_index`` (or lies outside of the vocabulary) give 0 and no gradient, whatever they hold. Logits of
+    ``-inf`` are tokens of probability 0; a row of nothing but ``-inf`` has no distribution and gives NaN. ``logit_scale`` (1 /
+    temperature, 1 / ``m_width``) must be positive. bf16, fp16 and fp32 logits of any row stride run on the kernels."""
+    logit_scale = _check_logit_scale(logit_scale)
+    if logits.dim() < 1 or logits.shape[-1] == 0 or not logits.is_floating_point():
+        raise ValueError(f"logits must be floating point with a last dimension of at least 1, got {logits.dtype} {tuple(logits.shape)}")
+    _check_labels(labels, logits.shape[:-1], logits.device)
+    if not _on_gpu(logits, _LOGIT_TYPES):
+        return _token_log_probs_torch(logits, labels, logit_scale, ignore_index, return_entropy)
+    return _TokenLogProbsFn.apply(logits, labels, logit_scale, int(ignore_index), bool(return_entropy))
+
+
+# ----------------------------------------------------------------------------- from hidden states
+class _FusedLinearTokenLogProbsFn(torch.autograd.Function):
+    """Forward keeps 16 bytes per row and 256 columns of logits; backward forms the logits again, chunk of rows by chunk, as
+    their bf16 gradient, and multiplies that with the weight and the hidden states."""
+
+    @staticmethod
+    def forward(ctx, x, weight, labels, logit_scale, ignore_index, return_entropy):
+        ctx.set_materialize_grads(False)
+        with site("loss.lm_head.log_probs"):
+            log_probs, entropy, lse = native().linear_log_probs_fwd(x, weight, labels, logit_scale, ignore_index, return_entropy, status_word(x.device))
+        ctx.save_for_backward(x, weight, labels, lse, entropy)
+        ctx.args = (logit_scale, ignore_index)
+        return (log_probs, entropy) if return_entropy else log_probs
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_log_probs, d_entropy=None):
+        x, weight, labels, lse, entropy = ctx.saved_tensors
+        if d_log_probs is None and d_entropy is None:
+            return (None,) * 6
+        C, st = native(), status_word(x.device)
+        T, H = x.shape
+        V = weight.shape[0]
+        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
+        d_log_probs = _row_gradient(d_log_probs, T, lse)
+        rows = _flce_chunk_rows(T, V)
+        target = _weight_grad_target(weight) if need_dw else None
+        dx = torch.empty_like(x) if need_dx else None
+        dw = None
+        if need_dw:
+            # one chunk writes the weight's gradient in its own type; several add up in fp32
+            if target is not None:
+                dw = target.view(V, H)
+            elif rows == T and T > 0:
+                dw = torch.empty(V, H, device=x.device, dtype=weight.dtype)
+            else:
+                dw = torch.zeros(V, H, device=x.device, dtype=torch.float32)
+        pitch = (V + 7) // 8 * 8
+        dlogits = torch.empty(rows, pitch, device=x.device, dtype=torch.bfloat16)[:, :V]
+        for start in range(0, T, max(rows, 1)):
+            part = slice(start, min(start + rows, T))
+            dl, xc = dlogits[: part.stop - start], x[part]
+            with site("loss.lm_head.dlogits"):
+                C.linear_log_probs_grad(xc, weight, labels[part], lse[part], None if entropy is None else entropy[part], d_log_probs[part],
+                                        None if d_entropy is None else d_entropy[part], dl, *ctx.args, st)
+            if need_dx:
+                with site("loss.lm_head.dgrad"):
+                    C.gemm(dl, weight, dx[part], False, True, False, 1.0, st, 0)
+            if need_dw:
+                with site("loss.lm_head.wgrad"):
+                    C.gemm(dl, xc, dw, True, True, dw.dtype == torch.float32, 1.0, st, 0)
+        if target is not None:
+            dw = None
+        elif dw is not None:
+            dw = dw.to(weight.dtype)
+        return dx, dw, None, None, None, None
+
+
+def _gemm_rows(t: torch.Tensor) -> torch.Tensor:
+    """Rows that a tensor map can describe: unit inner stride, row stride and base multiples of 16 bytes."""
+    ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
+    return t if ok else t.contiguous()
+
+
+def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0,
+                                 ignore_index: int = -100, return_entropy: bool = False):
+    """:func:`token_log_probs` of ``logits = x @ weight.T`` without the logits: ``x [..., H]``, ``weight [V, H]``, ``labels [...]``.
+
+    The logits are formed in fp32 on the tensor cores and reduced where they are; the backward pass forms them a second time (8/6 of
+    the products of a path that keeps them) and needs a transient bf16 buffer of at most about 2.2 GB. bf16 operands with ``H`` a multiple
+    of 8 run on the kernels. Gradients of ``weight`` go to its ``main_grad`` when the engine provides one."""
+    logit_scale = _check_logit_scale(logit_scale)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise ValueError(f"hidden states [..., H] and a weight [V, H] are needed, got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if x.device != weight.device or x.dtype != weight.dtype or not x.is_floating_point():
+        raise ValueError(f"hidden states and weight must be floating point of one type on one device, got {x.dtype} on {x.device} and {weight.dtype} on {weight.device}")
+    _check_labels(labels, x.shape[:-1], x.device)
+    if not (_on_gpu(x, (torch.bfloat16,)) and x.shape[-1] % 8 == 0):
+        note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
+        return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
+    shape = labels.shape
+    out = _FusedLinearTokenLogProbsFn.apply(_gemm_rows(x.reshape(-1, x.shape[-1])), _gemm_rows(weight), labels.reshape(-1).contiguous(),
+                                            logit_scale, int(ignore_index), bool(return_entropy))
+    return tuple(o.view(shape) for o in out) if return_entropy else out.view(shape)
+
+
+# ----------------------------------------------------------------------------- losses over packed answers
+class PreferenceLossOutput(NamedTuple):
+    loss: torch.Tensor
+    chosen_rewards: torch.Tensor
+    rejected_rewards: torch.Tensor
+
+
+class PolicyLossOutput(NamedTuple):
+    loss: torch.Tensor
+    kl: torch.Tensor
+    clip_fraction: torch.Tensor
+
+
+_PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "ipo": 2}
+_PREFERENCE_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_POLICY_REDUCTIONS = {"sum": 0, "token_mean": 1, "sequence_mean": 2}
+
+
+def _check_like(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
+    if t.shape != like.shape or t.device != like.device or not t.is_floating_point():
+        raise ValueError(f"{name} must be floating point, shaped {tuple(like.shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    if t.requires_grad:
+        raise ValueError(f"{name} must not require a gradient (detach it): the loss is differentiated with respect to log_probs alone")
+    return t
+
+
+def _check_sequences(log_probs: torch.Tensor, cu_seqlens: torch.Tensor | None, mask: torch.Tensor | None) -> tuple[int, int]:
+    """``(number of sequences, their length when there is no cu_seqlens)``."""
+    if not log_probs.is_floating_point():
+        raise ValueError(f"log_probs must be floating point, got {log_probs.dtype}")
+    if mask is not None and (mask.shape != log_probs.shape or mask.device != log_probs.device or mask.is_floating_point()):
+        raise ValueError(f"mask must be boolean or integer, shaped {tuple(log_probs.shape)} on {log_probs.device}, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
+    if cu_seqlens is None:
+        if log_probs.dim() != 2:
+            raise ValueError(f"log_probs must be [sequences, length], or [tokens] with cu_seqlens, got {tuple(log_probs.shape)}")
+        return log_probs.shape[0], log_probs.shape[1]
+    if log_probs.dim() != 1:
+        raise ValueError(f"with cu_seqlens log_probs must be [tokens], got {tuple(log_probs.shape)}")
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64) or cu_seqlens.device != log_probs.device:
+        raise ValueError(f"cu_seqlens must be int32 or int64 [sequences + 1] on {log_probs.device}, got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)} on {cu_seqlens.device}")
+    return cu_seqlens.numel() - 1, 0
+
+
+def _sequence_ids(count: int, length: int, cu_seqlens: torch.Tensor | None, like: torch.Tensor) -> torch.Tensor:
+    """Sequence of each (flattened) token, ``count`` for tokens outside of all sequences."""
+    t = torch.arange(like.numel(), device=like.device)
+    if cu_seqlens is None:
+        return t // max(length, 1)
+    ids = torch.searchsorted(cu_seqlens[1:].long().contiguous(), t, right=True)
+    return torch.where(t < cu_seqlens[0], count, ids)
+
+
+def _fp32(t: torch.Tensor) -> torch.Tensor:
+    return t.float().contiguous()
+
+
+def _mask8(mask: torch.Tensor | None) -> torch.Tensor | None:
+    if mask is None:
+        return None
+    return (mask if mask.dtype == torch.bool else mask != 0).contiguous()
+
+
+class _PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_probs, reference, cu_seqlens, length, sequences, mask, *args):
+        with site("preference_loss.fwd"):
+            loss, rewards, slope = native().preference_loss_fwd(log_probs, reference, cu_seqlens, length, sequences, mask, *args)
+        ctx.save_for_backward(slope, log_probs, cu_seqlens, mask)
+        ctx.length = length
+        ctx.mark_non_differentiable(rewards)
+        return loss, rewards
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, _):
+        slope, log_probs, cu_seqlens, mask = ctx.saved_tensors
+        with site("preference_loss.bwd"):
+            grad = native().preference_loss_bwd(slope, d_loss, log_probs, cu_seqlens, ctx.length, mask)
+        return (grad,) + (None,) * 10
+
+
+def _preference_loss_torch(log_probs, reference, cu_seqlens, length, sequences, mask, kind, beta, label_smoothing, average, reduction):
+    lp = log_probs.reshape(-1)
+    d = lp if reference is None else lp - reference.reshape(-1)
+    ids = _sequence_ids(sequences, length, cu_seqlens, lp)
+    kept = ids < sequences if mask is None else (ids < sequences) & (mask.reshape(-1) != 0)
+    d = torch.where(kept, d, 0.0)
+    sums = torch.zeros(sequences + 1, dtype=d.dtype, device=d.device).index_add(0, ids, d)[:sequences]
+    if average:
+        tokens = torch.zeros(sequences + 1, dtype=d.dtype, device=d.device).index_add(0, ids, kept.to(d.dtype))[:sequences]
+        sums = sums / tokens.clamp_min(1)
+    chosen, rejected = sums.chunk(2)
+    margin = beta * (chosen - rejected)
+    if kind == 0:
+        loss = (1 - label_smoothing) * F.softplus(-margin) + (label_smoothing * F.softplus(margin) if label_smoothing else 0.0)
+    elif kind == 1:
+        loss = torch.relu(1 - margin)
+    else:
+        loss = (chosen - rejected - 0.5 / beta).square()
+    loss = loss if reduction == 0 else loss.sum() if reduction == 1 else loss.mean()
+    return loss, (beta * sums).detach()
+
+
+def preference_loss(log_probs: torch.Tensor, reference_log_probs: torch.Tensor | None, cu_seqlens: torch.Tensor | None = None, *,
+                    beta: float = 0.1, loss_type: str = "sigmoid", label_smoothing: float = 0.0, average_log_probs: bool = False,
+                    mask: torch.Tensor | None = None, reduction: str = "mean") -> PreferenceLossOutput:
+    """Loss over pairs of answers from per-token log-probabilities of the policy and of a frozen reference.
+
+    ``log_probs`` is packed ``[tokens]`` with ``cu_seqlens [2 * pairs + 1]`` or padded ``[2 * pairs, length]``: the chosen answers first,
+    then the rejected ones in the same order. With ``s`` an answer's sum (``average_log_probs``: mean) of ``log_probs - reference`` over the tokens
+    that ``mask`` keeps and ``D = s_chosen - s_rejected``: ``sigmoid`` is ``(1 - e) softplus(-beta D) + e softplus(beta D)`` with
+    ``e = label_smoothing``, ``hinge`` is ``max(0, 1 - beta D)``, ``ipo`` is ``(D - 1 / (2 beta))^2``. ``reference_log_probs=None`` leaves the reference out.
+
+    Returns the loss (reduced over pairs, or one per pair with ``reduction="none"``) and ``beta * s`` of the chosen and the rejected answers
+    (no gradient). An answer without tokens has ``s = 0``. Masked tokens, and tokens outside of all sequences, are not looked at and get a
+    gradient of 0."""
+    sequences, length = _check_sequences(log_probs, cu_seqlens, mask)
+    if sequences == 0 or sequences % 2:
+        raise ValueError(f"an even number of answers is needed (chosen, then rejected), got {sequences}")
+    if loss_type not in _PREFERENCE_KINDS or reduction not in _PREFERENCE_REDUCTIONS:
+        raise ValueError(f"unexpected loss_type ({loss_type}) or reduction ({reduction})")
+    beta, label_smoothing = float(beta), float(label_smoothing)
+    if not (math.isfinite(beta) and beta > 0):
+        raise ValueError(f"beta must be positive and finite, got {beta}")
+    if not 0 <= label_smoothing < 0.5 or (label_smoothing and loss_type != "sigmoid"):
+        raise ValueError(f"label_smoothing must be in [0, 0.5) and goes with loss_type='sigmoid', got {label_smoothing} for {loss_type}")
+    if reference_log_probs is not None:
+        _check_like(reference_log_probs, log_probs, "reference_log_probs")
+    args = (_PREFERENCE_KINDS[loss_type], beta, label_smoothing, bool(average_log_probs), _PREFERENCE_REDUCTIONS[reduction])
+    if _on_gpu(log_probs, (torch.float32, torch.bfloat16, torch.float16)):
+        cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
+        loss, rewards = _PreferenceLossFn.apply(_fp32(log_probs), None if reference_log_probs is None else _fp32(reference_log_probs), cu, length, sequences,
+                                                _mask8(mask), *args)
+    else:
+        wide = log_probs if log_probs.dtype == torch.float64 else log_probs.float()
+        loss, rewards = _preference_loss_torch(wide, None if reference_log_probs is None else reference_log_probs.to(wide.dtype), cu_seqlens, length, sequences, mask, *args)
+    pairs = sequences // 2
+    return PreferenceLossOutput(loss, rewards[:pairs], rewards[pairs:])
+
+
+class _PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction):
+        with site("policy_loss.fwd"):
+            out, slope, weight = native().policy_loss_fwd(log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high,
+                                                          dual_clip, kl_coef, reduction, ctx.needs_input_grad[0])
+        ctx.save_for_backward(slope, out, weight, cu_seqlens, mask)
+        ctx.args = (list(log_probs.shape), length, sequences, reduction)
+        loss = out[0].clone()  # a tensor of its own: `out` is needed again and must not be written through the loss
+        kl, clip_fraction = out[1], out[2]
+        ctx.mark_non_differentiable(kl, clip_fraction)
+        return loss, kl, clip_fraction
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_loss, *_):
+        slope, out, weight, cu_seqlens, mask = ctx.saved_tensors
+        shape, length, sequences, reduction = ctx.args
+        with site("policy_loss.bwd"):
+            grad = native().policy_loss_bwd(slope, out, weight, d_loss, shape, cu_seqlens, length, sequences, mask, reduction)
+        return (grad,) + (None,) * 13
+
+
+def _policy_loss_torch(log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction):
+    lp = log_probs.reshape(-1)
+    ids = _sequence_ids(sequences, length, cu_seqlens, lp)
+    kept = ids < sequences if mask is None else (ids < sequences) & (mask.reshape(-1) != 0)
+    # neither values nor gradients of tokens that take no part may reach a sum, also where they are not finite
+    own, old = torch.where(kept, lp, 0.0), torch.where(kept, old.reshape(-1), 0.0)
+    adv = advantages.reshape(-1) if per_token else torch.cat([advantages, advantages.new_zeros(1)])[ids]
+    adv = torch.where(kept, adv, 0.0)
+    delta = own.double() - old.double()
+    clipped = ((adv > 0) & (delta > math.log1p(clip_high))) | ((adv < 0) & (delta < (math.log1p(-clip_low) if clip_low < 1 else -math.inf)))
+    ratio = torch.where(clipped | (adv == 0), 0.0, delta).exp().to(own.dtype)
+    value = torch.where(clipped, -adv * torch.where(adv > 0, torch.full_like(adv, 1 + clip_high), 1 - clip_low), -adv * ratio)
+    if dual_clip:
+        bound = (adv < 0) & (value > -dual_clip * adv)
+        value, clipped = torch.where(bound, -dual_clip * adv, value), clipped | bound
+    kl = torch.zeros_like(value)
+    if reference is not None:
+        d = torch.where(kept, reference.reshape(-1), 0.0) - own
+        kl = torch.expm1(d) - d
+        if kl_coef:
+            value = value + kl_coef * kl
+    n = kept.sum().clamp_min(1)
+    if reduction == 2:
+        zeros = torch.zeros(sequences + 1, dtype=value.dtype, device=value.device)
+        tokens = zeros.index_add(0, ids, kept.to(value.dtype))[:sequences]
+        means = zeros.index_add(0, ids, value)[:sequences] / tokens.clamp_min(1)
+        loss = means.sum() / (tokens > 0).sum().clamp_min(1)
+    else:
+        loss = value.sum() if reduction == 0 else value.sum() / n
+    return loss, (kl.sum() / n).detach(), clipped.sum().to(value.dtype) / n
+
+
+def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor, *, reference_log_probs: torch.Tensor | None = None,
+                cu_seqlens: torch.Tensor | None = None, mask: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2,
+                dual_clip: float | None = None, kl_coef: float = 0.0, reduction: str = "token_mean") -> PolicyLossOutput:
+    """Clipped policy-gradient loss with a KL term, from per-token log-probabilities of sampled answers.
+
+    ``log_probs`` is packed ``[tokens]`` with ``cu_seqlens [sequences + 1]`` or padded ``[sequences, length]``; ``advantages`` has its shape, or
+    ``[sequences]`` for one value per answer. A token's loss is ``max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high))`` with
+    ``r = exp(log_probs - old_log_probs)``, bounded by ``-dual_clip A`` where ``A < 0``, plus ``kl_coef (exp(k) - 1 - k)`` with ``k = reference - log_probs``.
+    ``token_mean`` divides the sum by the number of tokens that ``mask`` keeps, ``sequence_mean`` averages the answers' token means over the answers
+    that keep a token, ``sum`` does neither.
+
+    Returns the loss, and over the kept tokens the mean of ``exp(k) - 1 - k`` (0 without a reference) and the share whose gradient was clipped (neither has
+    a gradient). Masked tokens, and tokens outside of all sequences, are not looked at and get a gradient of 0; nothing kept gives 0."""
+    sequences, length = _check_sequences(log_probs, cu_seqlens, mask)
+    _check_like(old_log_probs, log_probs, "old_log_probs")
+    if reference_log_probs is not None:
+        _check_like(reference_log_probs, log_probs, "reference_log_probs")
+    per_token = advantages.shape == log_probs.shape and not (cu_seqlens is not None and advantages.shape == (sequences,) and sequences == log_probs.numel())
+    _check_like(advantages, log_probs if per_token else log_probs.new_empty(()).expand(sequences), "advantages")
+    clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
+    if not (0 <= clip_low <= 1 and clip_high >= 0):
+        raise ValueError(f"clip_low must be in [0, 1] and clip_high at least 0, got {clip_low} and {clip_high}")
+    if not (math.isfinite(kl_coef) and kl_coef >= 0):
+        raise ValueError(f"kl_coef must be finite and at least 0, got {kl_coef}")
+    if kl_coef and reference_log_probs is None:
+        raise ValueError("kl_coef needs reference_log_probs")
+    if dual_clip is not None and not (math.isfinite(dual_clip) and dual_clip > 1):
+        raise ValueError(f"dual_clip must be finite and above 1, got {dual_clip}")
+    if reduction not in _POLICY_REDUCTIONS:
+        raise ValueError(f"unexpected reduction ({reduction})")
+    args = (clip_low, clip_high, float(dual_clip or 0.0), kl_coef, _POLICY_REDUCTIONS[reduction])
+    if _on_gpu(log_probs, (torch.float32, torch.bfloat16, torch.float16)):
+        cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
+        return PolicyLossOutput(*_PolicyLossFn.apply(_fp32(log_probs), _fp32(old_log_probs), None if reference_log_probs is None else _fp32(reference_log_probs),
+                                                     _fp32(advantages), per_token, cu, length, sequences, _mask8(mask), *args))
+    wide = log_probs if log_probs.dtype == torch.float64 else log_probs.float()
+    others = [None if t is None else t.to(wide.dtype) for t in (old_log_probs, reference_log_probs, advantages)]
+    return PolicyLossOutput(*_policy_loss_torch(wide, *others, per_token, cu_seqlens, length, sequences, mask, *args))
+
+
+# ----------------------------------------------------------------------------- embedding
+class _EmbeddingSortedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, ids, scale):
+        ctx.save_for_backward(ids)
+        ctx.weight, ctx.scale = weight, scale
+        with site("embedding.fwd"):
+            return native().embedding_lookup(weight, ids, scale, status_word(weight.device))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        (ids,) = ctx.saved_tensors
+        weight = ctx.weight
+        target = _weight_grad_target(weight)
+        with site("embedding.bwd"):
+            dw = native().embedding_gradient(dout.contiguous(), ids, weight.shape[0], None if target is None else target.view(weight.shape), ctx.scale)
+        return None if target is not None else dw, None, None
+
+
+def embedding_sorted(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[ids]`` whose weight gradient adds the rows of a token in ascending position: the same bits on every run, one rounding, no fp32
+    copy of the whole table (``ops.embedding(sorted_gradient=True)``). bf16, fp16 and fp32 tables of any width run on the kernels.
+
+    On the GPU an id outside of the table gives a row of zeros, takes no part in the gradient and raises the status word (``ops.check_status()``)."""
+    if weight.dim() != 2 or not weight.is_floating_point():
+        raise ValueError(f"the embedding table must be floating point [V, H], got {weight.dtype} {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
+    if ids.device != weight.device:
+        raise ValueError(f"ids must be on {weight.device}, got {ids.device}")
+    if not _on_gpu(weight, _LOGIT_TYPES):
+        out = F.embedding(ids, weight)
+        return out if scale == 1.0 else out * scale
+    return _EmbeddingSortedFn.apply(weight.contiguous(), ids.contiguous(), float(scale))
