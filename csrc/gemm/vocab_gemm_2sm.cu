@@ -55,6 +55,20 @@ struct RowArgs {
 
 enum class Mode : int { kStats, kGrad };
 
+// v[i] of 32 registers for a lane's own i: halved five times, so that the array stays in registers.
+__device__ __forceinline__ uint32_t select32_bits(const uint32_t (&v)[32], int i) {
+  uint32_t t[16];
+#pragma unroll
+  for (int k = 0; k < 16; ++k) t[k] = (i & 16) ? v[k + 16] : v[k];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) t[k] = (i & 8) ? t[k + 8] : t[k];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) t[k] = (i & 4) ? t[k + 4] : t[k];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) t[k] = (i & 2) ? t[k + 2] : t[k];
+  return (i & 1) ? t[1] : t[0];
+}
+
 template <Mode MODE, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 1)
     vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -235,20 +249,20 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
           }
-          float f[32];
-#pragma unroll
-          for (int e = 0; e < 32; ++e) f[e] = __uint_as_float(v[e]);
           if (col0 + 32 > N) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (col0 + e >= N) f[e] = -INFINITY;
+              if (col0 + e >= N) v[e] = __float_as_uint(-INFINITY);
           }
-          if ((label >> 5) == c) {
+          if ((label >> 5) == c) x_label = __uint_as_float(select32_bits(v, label & 31));
+          float top = __uint_as_float(v[0]);
+          F2 f[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if ((label & 31) == e) x_label = f[e];
+          for (int e = 0; e < 16; ++e) {
+            top = fmaxf(top, fmaxf(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])));
+            f[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
           }
-          accumulate<ENTROPY, 32>(st, f, scale2);
+          accumulate<ENTROPY, 32>(st, f, top, scale2);
         }
         if (row < M) rows.stats[(long long)tc.ni * M + row] = make_float4(st.m, st.s, st.u, x_label);
       } else {
@@ -264,22 +278,22 @@ __global__ void __launch_bounds__(THREADS, 1)
             uint32_t v[32];
             B200_TMEM_LD_32(v, t_row + c * 64 + half * 32);
             tmem_ld_wait();
-            float f[32];
+            uint32_t w[16];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const float d = score_gradient<ENTROPY>(log2_prob(__uint_as_float(v[e]), L, scale2), gs, hs, H);
-              f[e] = zero ? 0.f : d;
-            }
-            if ((label >> 5) == 2 * c + half) {
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if ((label & 31) == e) f[e] += gs;
+            for (int e = 0; e < 16; ++e) {
+              const float a = score_gradient<ENTROPY>(log2_prob(__uint_as_float(v[2 * e]), L, scale2), gs, hs, H);
+              const float b = score_gradient<ENTROPY>(log2_prob(__uint_as_float(v[2 * e + 1]), L, scale2), gs, hs, H);
+              w[e] = zero ? 0u : pack_bf16x2(a, b);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              box_write(box, lane, half * 4 + j,
-                        make_uint4(pack_bf16x2(f[8 * j], f[8 * j + 1]), pack_bf16x2(f[8 * j + 2], f[8 * j + 3]),
-                                   pack_bf16x2(f[8 * j + 4], f[8 * j + 5]), pack_bf16x2(f[8 * j + 6], f[8 * j + 7])));
+            for (int j = 0; j < 4; ++j) box_write(box, lane, half * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
+            if ((label >> 5) == 2 * c + half && !zero) {
+              // the label's own gradient, over the element of the row just written
+              const float d = log2_prob(__uint_as_float(select32_bits(v, label & 31)), L, scale2);
+              const int e = label & 63;
+              *reinterpret_cast<__nv_bfloat16*>(box + lane * 128 + (((e >> 3) ^ (lane & 7)) << 4) + (e & 7) * 2) =
+                  __float2bfloat16(gs + score_gradient<ENTROPY>(d, gs, hs, H));
+            }
           }
           if (c == BN / 64 - 1 || col0 + 64 >= N) {
             tc_fence_before_sync();

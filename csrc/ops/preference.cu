@@ -158,7 +158,7 @@ __device__ __forceinline__ double sigmoid(double x) {
 
 // Second phase: a warp of the cluster takes a pair at a time.
 __device__ __forceinline__ void preference_pairs(const PackedTokens& p, const PreferenceArgs& a, const float* partials, float* loss,
-                                                 float* rewards, float* slope, double* scratch, double* block_total) {
+                                                 float* chosen, float* rejected, float* slope, double* scratch, double* block_total) {
   const int pairs = p.sequences / 2, lane = threadIdx.x & 31;
   const double beta = a.beta, eps = a.label_smoothing;
   const double scale = a.reduction == 2 ? 1.0 / pairs : 1.0;
@@ -181,8 +181,8 @@ __device__ __forceinline__ void preference_pairs(const PackedTokens& p, const Pr
         value = off * off;
         d = 2 * off;
       }
-      rewards[i] = (float)(beta * sw);
-      rewards[pairs + i] = (float)(beta * sl);
+      chosen[i] = (float)(beta * sw);
+      rejected[i] = (float)(beta * sl);
       slope[i] = (float)(d * scale * inv_w);
       slope[pairs + i] = (float)(-d * scale * inv_l);
       if (a.reduction == 0) loss[i] = (float)value;
@@ -196,7 +196,7 @@ __device__ __forceinline__ void preference_pairs(const PackedTokens& p, const Pr
 
 template <bool ONE_LAUNCH>
 __global__ void __launch_bounds__(CLUSTER_THREADS)
-    preference_cluster_kernel(PreferenceIn in, PackedTokens p, PreferenceArgs args, float* partials, float* loss, float* rewards, float* slope) {
+    preference_cluster_kernel(PreferenceIn in, PackedTokens p, PreferenceArgs args, float* partials, float* loss, float* chosen, float* rejected, float* slope) {
   __shared__ double scratch[CLUSTER_THREADS / 32];
   __shared__ double block_total;
   if (ONE_LAUNCH) {
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(CLUSTER_THREADS)
     __threadfence();
     cluster_sync_all();
   }
-  preference_pairs(p, args, partials, loss, rewards, slope, scratch, &block_total);
+  preference_pairs(p, args, partials, loss, chosen, rejected, slope, scratch, &block_total);
 }
 
 __global__ void __launch_bounds__(WARPS_A * 32) preference_chunks_kernel(PreferenceIn in, PackedTokens p, float* partials) {
@@ -361,7 +361,7 @@ __device__ __forceinline__ void policy_chunk(const PolicyIn& in, const PackedTok
   }
 }
 
-__device__ __forceinline__ void policy_totals(const PackedTokens& p, const PolicyArgs& a, const float* partials, float* out, float* weight, double* scratch, double* block_total) {
+__device__ __forceinline__ void policy_totals(const PackedTokens& p, const PolicyArgs& a, const float* partials, const PolicyOut& out, float* weight, double* scratch, double* block_total) {
   const int lane = threadIdx.x & 31;
   const int warp = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5);
   constexpr int kWarps = CLUSTER * (CLUSTER_THREADS / 32);
@@ -409,16 +409,16 @@ __device__ __forceinline__ void policy_totals(const PackedTokens& p, const Polic
   if (cluster_ctarank() == 0 && threadIdx.x == 0) {
     const double tokens = fmax(count, 1.0);
     const double divisor = a.reduction == 0 ? 1.0 : a.reduction == 1 ? tokens : fmax(used, 1.0);
-    out[0] = (float)(loss / divisor);
-    out[1] = (float)(kl / tokens);
-    out[2] = (float)(clipped / tokens);
-    out[3] = (float)(1.0 / divisor);
+    *out.loss = (float)(loss / divisor);
+    *out.kl = (float)(kl / tokens);
+    *out.clipped = (float)(clipped / tokens);
+    *out.factor = (float)(1.0 / divisor);
   }
 }
 
 template <bool ONE_LAUNCH>
 __global__ void __launch_bounds__(CLUSTER_THREADS)
-    policy_cluster_kernel(PolicyIn in, PackedTokens p, PolicyArgs args, float* partials, float* out, float* slope, float* weight) {
+    policy_cluster_kernel(PolicyIn in, PackedTokens p, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight) {
   __shared__ double scratch[CLUSTER_THREADS / 32];
   __shared__ double block_total;
   if (ONE_LAUNCH) {
@@ -437,11 +437,11 @@ __global__ void __launch_bounds__(WARPS_A * 32) policy_chunks_kernel(PolicyIn in
 }
 
 __global__ void __launch_bounds__(WARPS_A * 32)
-    policy_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ out, const float* __restrict__ weight, const float* __restrict__ d_loss, PackedTokens p, int reduction,
+    policy_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ factor, const float* __restrict__ weight, const float* __restrict__ d_loss, PackedTokens p, int reduction,
                       float* __restrict__ grad) {
   const long long c = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
   if (c * CHUNK >= p.T) return;
-  const float w = out[3] * d_loss[0];
+  const float w = factor[0] * d_loss[0];
   for_each_token(p, c, [&](long long t, int i) {
     float g = 0.f;
     if (i >= 0 && (p.mask == nullptr || p.mask[t] != 0)) g = slope[t] * (reduction == 2 ? w * weight[i] : w);
@@ -473,16 +473,16 @@ void launch_cluster(Kernel kernel, cudaStream_t stream, Args... args) {
 long long packed_partials(long long T, int sequences) { return ((T + CHUNK - 1) / CHUNK + sequences) * WORDS; }
 
 void preference_loss_fwd(const float* log_probs, const float* reference, PackedTokens tokens, PreferenceArgs args, float* partials,
-                         float* loss, float* rewards, float* slope, cudaStream_t stream) {
+                         float* loss, float* chosen, float* rejected, float* slope, cudaStream_t stream) {
   const PreferenceIn in = {log_probs, reference};
   if (tokens.T <= kOneLaunch) {
-    launch_cluster(preference_cluster_kernel<true>, stream, in, tokens, args, partials, loss, rewards, slope);
+    launch_cluster(preference_cluster_kernel<true>, stream, in, tokens, args, partials, loss, chosen, rejected, slope);
     return;
   }
   preference_chunks_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(in, tokens, partials);
   count_launch();
   check_cuda(cudaGetLastError(), "preference_loss launch");
-  launch_cluster(preference_cluster_kernel<false>, stream, in, tokens, args, partials, loss, rewards, slope);
+  launch_cluster(preference_cluster_kernel<false>, stream, in, tokens, args, partials, loss, chosen, rejected, slope);
 }
 
 void preference_loss_bwd(const float* slope, const float* d_loss, long long d_loss_stride, PackedTokens tokens, float* grad, cudaStream_t stream) {
@@ -493,7 +493,7 @@ void preference_loss_bwd(const float* slope, const float* d_loss, long long d_lo
 }
 
 void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const float* reference, const float* advantages,
-                     PackedTokens tokens, PolicyArgs args, float* partials, float* out, float* slope, float* weight, cudaStream_t stream) {
+                     PackedTokens tokens, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight, cudaStream_t stream) {
   const PolicyIn in = {log_probs, old_log_probs, reference, advantages};
   if (tokens.T <= kOneLaunch) {
     launch_cluster(policy_cluster_kernel<true>, stream, in, tokens, args, partials, out, slope, weight);
@@ -505,10 +505,10 @@ void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const f
   launch_cluster(policy_cluster_kernel<false>, stream, in, tokens, args, partials, out, slope, weight);
 }
 
-void policy_loss_bwd(const float* slope, const float* out, const float* weight, const float* d_loss, PackedTokens tokens, int reduction,
+void policy_loss_bwd(const float* slope, const float* factor, const float* weight, const float* d_loss, PackedTokens tokens, int reduction,
                      float* grad, cudaStream_t stream) {
   if (tokens.T == 0) return;
-  policy_bwd_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(slope, out, weight, d_loss, tokens, reduction, grad);
+  policy_bwd_kernel<<<chunk_blocks(tokens.T), WARPS_A * 32, 0, stream>>>(slope, factor, weight, d_loss, tokens, reduction, grad);
   count_launch();
   check_cuda(cudaGetLastError(), "policy_loss backward launch");
 }

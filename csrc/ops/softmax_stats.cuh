@@ -45,18 +45,73 @@ __device__ __forceinline__ Stats merge(Stats a, Stats b, float c) {
   return {m, a.s + b.s, a.u + b.u};
 }
 
+// Two fp32 values in one register pair: one instruction for two FMAs, adds or products.
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+
+// Up to here the product m c can stand in for m: d = x c - m c is one FMA. Beyond (masks of the type's lowest value as the largest
+// logit, infinities) the difference is formed first. In the FMA form the rounding of m c is common to all elements of a row and cancels
+// between a logit and the sum.
+constexpr float kProductLimit = 1e30f;
+
+// N logits (an even number, in pairs) whose maximum is `top` enter the statistics.
 template <bool ENTROPY, int N>
-__device__ __forceinline__ void accumulate(Stats& a, const float* f, float c) {
-  float top = f[0];
-#pragma unroll
-  for (int e = 1; e < N; ++e) top = fmaxf(top, f[e]);
+__device__ __forceinline__ void accumulate(Stats& a, const F2 (&f)[N / 2], float top, float c) {
   if (top > a.m) rescale<ENTROPY>(a, top, c);
-  const float m = a.m == -INFINITY ? 0.f : a.m;
+  const float m = a.m == -INFINITY ? 0.f : a.m, mc = m * c;
+  F2 s0 = pack2(0.f, 0.f), s1 = s0, u0 = s0, u1 = s0;
+  const F2 c2 = pack2(c, c);
+  auto add = [&](F2 d2, int i) {
+    const float2 d = unpack2(d2);
+    const F2 x = pack2(fast_exp2(d.x), fast_exp2(d.y));
+    if (i & 1) s1 = add2(s1, x);
+    else s0 = add2(s0, x);
+    if (ENTROPY) {
+      const F2 e = pack2(fmaxf(d.x, kFloor2), fmaxf(d.y, kFloor2));
+      if (i & 1) u1 = fma2(x, e, u1);
+      else u0 = fma2(x, e, u0);
+    }
+  };
+  if (fabsf(mc) < kProductLimit) {
+    const F2 off = pack2(-mc, -mc);
 #pragma unroll
-  for (int e = 0; e < N; ++e) {
-    const float d = (f[e] - m) * c, x = fast_exp2(d);
-    a.s += x;
-    if (ENTROPY) a.u = fmaf(x, fmaxf(d, kFloor2), a.u);
+    for (int i = 0; i < N / 2; ++i) add(fma2(f[i], c2, off), i);
+  } else {
+    const F2 off = pack2(-m, -m);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) add(mul2(add2(f[i], off), c2), i);
+  }
+  const float2 s = unpack2(add2(s0, s1));
+  a.s += s.x + s.y;
+  if (ENTROPY) {
+    const float2 u = unpack2(add2(u0, u1));
+    a.u += u.x + u.y;
   }
 }
 

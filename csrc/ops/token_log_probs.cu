@@ -30,65 +30,80 @@ __device__ __forceinline__ long long row_offset(const RowMap& m, long long row) 
   return o * m.outer_stride + (row - o * m.inner) * m.row_stride;
 }
 
+// 16 bytes of logits: as fp32 pairs, their maximum, and back.
 template <typename T>
 struct Vec;
 template <>
 struct Vec<__nv_bfloat16> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(uint4 v, float* f) {
+  static __device__ __forceinline__ void unpack(uint4 v, F2* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 a = unpack_bf16x2(w[i]);
-      f[2 * i] = a.x;
-      f[2 * i + 1] = a.y;
-    }
+    for (int i = 0; i < 4; ++i) f[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 r = __hmax2(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
   }
+  static __device__ __forceinline__ float top(uint32_t w) { return fmaxf(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+  static __device__ __forceinline__ uint32_t pack(float2 f) { return pack_bf16x2(f.x, f.y); }
   static __device__ __forceinline__ float load(const __nv_bfloat16* p) { return __bfloat162float(*p); }
   static __device__ __forceinline__ void store(__nv_bfloat16* p, float f) { *p = __float2bfloat16(f); }
+  static __device__ __forceinline__ uint32_t bits(const __nv_bfloat16* p) { return *reinterpret_cast<const uint16_t*>(p); }
+  static constexpr uint32_t kNegInf = 0xff80u;
 };
 template <>
 struct Vec<__half> {
   static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(uint4 v, float* f) {
+  static __device__ __forceinline__ void unpack(uint4 v, F2* f) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-      f[2 * i] = a.x;
-      f[2 * i + 1] = a.y;
+      f[i] = pack2(a.x, a.y);
     }
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const __half2 h = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-      w[i] = *reinterpret_cast<const uint32_t*>(&h);
-    }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmax2(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+  static __device__ __forceinline__ float top(uint32_t w) {
+    const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return fmaxf(a.x, a.y);
+  }
+  static __device__ __forceinline__ uint32_t pack(float2 f) {
+    const __half2 h = __floats2half2_rn(f.x, f.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
   static __device__ __forceinline__ float load(const __half* p) { return __half2float(*p); }
   static __device__ __forceinline__ void store(__half* p, float f) { *p = __float2half_rn(f); }
+  static __device__ __forceinline__ uint32_t bits(const __half* p) { return *reinterpret_cast<const uint16_t*>(p); }
+  static constexpr uint32_t kNegInf = 0xfc00u;
 };
 template <>
 struct Vec<float> {
   static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(uint4 v, float* f) {
-    f[0] = __uint_as_float(v.x);
-    f[1] = __uint_as_float(v.y);
-    f[2] = __uint_as_float(v.z);
-    f[3] = __uint_as_float(v.w);
+  static __device__ __forceinline__ void unpack(uint4 v, F2* f) {
+    f[0] = pack2(__uint_as_float(v.x), __uint_as_float(v.y));
+    f[1] = pack2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  static __device__ __forceinline__ uint4 pack(const float* f) {
-    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+  static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ void store(float* p, float f) { *p = f; }
+  static __device__ __forceinline__ uint32_t bits(const float* p) { return __float_as_uint(*p); }
+  static constexpr uint32_t kNegInf = 0xff800000u;
 };
+
+template <typename T>
+__device__ __forceinline__ uint4 pack_vector(const F2* f) {
+  if constexpr (sizeof(T) == 4) {
+    const float2 a = unpack2(f[0]), b = unpack2(f[1]);
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+  } else {
+    return make_uint4(Vec<T>::pack(unpack2(f[0])), Vec<T>::pack(unpack2(f[1])), Vec<T>::pack(unpack2(f[2])), Vec<T>::pack(unpack2(f[3])));
+  }
+}
 
 // The 16 bytes at `p + shift` of two aligned words, shift in bytes (1..15).
 __device__ __forceinline__ uint4 join_words(uint4 a, uint4 b, int shift) {
@@ -123,13 +138,20 @@ struct Row {
     if (shift == 0) return a;
     return join_words(a, __ldg(q + 1), shift);
   }
-  // elements past the row's end read as -inf (probability 0)
-  __device__ __forceinline__ void load_narrow(int i, float* f) const {
+  // element by element; elements past the row's end read as -inf (probability 0)
+  __device__ __forceinline__ uint4 load_narrow(int i) const {
+    uint32_t w[4];
+    constexpr int kPerWord = 4 / (int)sizeof(T);
 #pragma unroll
-    for (int e = 0; e < Vec<T>::N; ++e) {
-      const int j = i * Vec<T>::N + e;
-      f[e] = j < V ? Vec<T>::load(p + j) : -INFINITY;
+    for (int k = 0; k < 4; ++k) {
+      w[k] = 0;
+#pragma unroll
+      for (int e = 0; e < kPerWord; ++e) {
+        const int j = i * Vec<T>::N + k * kPerWord + e;
+        w[k] |= (j < V ? Vec<T>::bits(p + j) : Vec<T>::kNegInf) << (16 * e);
+      }
     }
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 
@@ -154,25 +176,29 @@ __global__ void __launch_bounds__(FWD_THREADS)
   }
   const Row<T> r(logits + row_offset(map, row), V);
   Stats st = empty_stats();
+  // four vectors a thread at a time: their loads are in flight together, and one comparison of their common maximum with the
+  // running one decides about rescaling
   constexpr int UNROLL = 4;
+  constexpr uint32_t kNegInf = sizeof(T) == 2 ? Vec<T>::kNegInf * 0x10001u : Vec<T>::kNegInf;
   for (int i0 = threadIdx.x; i0 < r.vectors; i0 += UNROLL * FWD_THREADS) {
     uint4 v[UNROLL];
-    bool wide[UNROLL];
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       const int i = i0 + k * FWD_THREADS;
-      wide[k] = i < r.vectors && r.wide(i);
-      if (wide[k]) v[k] = r.load_wide(i);
+      v[k] = make_uint4(kNegInf, kNegInf, kNegInf, kNegInf);
+      if (i < r.vectors) {
+        if (r.wide(i)) v[k] = r.load_wide(i);
+        else v[k] = r.load_narrow(i);
+      }
     }
+    uint32_t top = kNegInf;
+    F2 f[UNROLL * N / 2];
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
-      const int i = i0 + k * FWD_THREADS;
-      if (i >= r.vectors) break;
-      float f[N];
-      if (wide[k]) Vec<T>::unpack(v[k], f);
-      else r.load_narrow(i, f);
-      accumulate<ENTROPY, N>(st, f, scale2);
+      top = Vec<T>::max2(top, Vec<T>::max2(Vec<T>::max2(v[k].x, v[k].y), Vec<T>::max2(v[k].z, v[k].w)));
+      Vec<T>::unpack(v[k], f + k * (N / 2));
     }
+    accumulate<ENTROPY, UNROLL * N>(st, f, Vec<T>::top(top), scale2);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -205,7 +231,8 @@ __global__ void __launch_bounds__(BWD_THREADS)
                                RowMap map, long long grad_stride, float logit_scale, float scale2,
                                long long ignore_index) {
   constexpr int N = Vec<T>::N;
-  const long long row = blockIdx.x;
+  // last row first: the logits that the forward pass (or the model) touched last are still in L2
+  const long long row = (long long)gridDim.x - 1 - blockIdx.x;
   const long long label = load_label(labels, labels64, row);
   const bool ignored = label == ignore_index || label < 0 || label >= V;
   const Row<T> r(logits + row_offset(map, row), V);
@@ -219,37 +246,56 @@ __global__ void __launch_bounds__(BWD_THREADS)
   const float H = ENTROPY ? entropy[row] : 0.f;
   const float gs = g * logit_scale, hs = h * logit_scale;
   uint4 v[BWD_UNROLL];
-  bool wide[BWD_UNROLL];
 #pragma unroll
   for (int k = 0; k < BWD_UNROLL; ++k) {
     const int i = i0 + k * BWD_THREADS;
-    wide[k] = i < r.vectors && r.wide(i);
     v[k] = make_uint4(0, 0, 0, 0);
-    if (wide[k] && !zero) v[k] = r.load_wide(i);
+    if (i < r.vectors && !zero) {
+      if (r.wide(i)) v[k] = r.load_wide(i);
+      else v[k] = r.load_narrow(i);
+    }
   }
+  const float mc = L.x * scale2;
+  const bool product = fabsf(mc) < kProductLimit;
+  const float off = product ? -mc - L.y : -L.x;
+  const F2 c2 = pack2(scale2, scale2), off2 = pack2(off, off), log2_s = pack2(-L.y, -L.y), gs2 = pack2(-gs, -gs);
+  const int label_vector = zero ? -1 : (int)(label / N);
 #pragma unroll
   for (int k = 0; k < BWD_UNROLL; ++k) {
     const int i = i0 + k * BWD_THREADS;
     if (i >= r.vectors) return;
-    float f[N];
-    if (zero) {
+    F2 f[N / 2];
+    Vec<T>::unpack(v[k], f);
 #pragma unroll
-      for (int e = 0; e < N; ++e) f[e] = 0.f;
-    } else {
-      if (wide[k]) Vec<T>::unpack(v[k], f);
-      else r.load_narrow(i, f);
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        f[e] = score_gradient<ENTROPY>(log2_prob(f[e], L, scale2), gs, hs, H);
-        if (i * N + e == label) f[e] += gs;
+    for (int j = 0; j < N / 2; ++j) {
+      if (zero) {
+        f[j] = pack2(0.f, 0.f);
+        continue;
+      }
+      const float2 d = unpack2(product ? fma2(f[j], c2, off2) : fma2(add2(f[j], off2), c2, log2_s));
+      const F2 p = pack2(fast_exp2(d.x), fast_exp2(d.y));
+      if (ENTROPY) {
+        const F2 w = pack2(-fmaf(hs, fmaf(fmaxf(d.x, kFloor2), kLn2, H), gs), -fmaf(hs, fmaf(fmaxf(d.y, kFloor2), kLn2, H), gs));
+        f[j] = mul2(p, w);
+      } else {
+        f[j] = mul2(p, gs2);
       }
     }
     if ((i + 1) * N <= V) {
-      *reinterpret_cast<uint4*>(out + (long long)i * N) = Vec<T>::pack(f);
+      *reinterpret_cast<uint4*>(out + (long long)i * N) = pack_vector<T>(f);
     } else {
 #pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (i * N + e < V) Vec<T>::store(out + i * N + e, f[e]);
+      for (int j = 0; j < N / 2; ++j) {
+        const float2 a = unpack2(f[j]);
+        if (i * N + 2 * j < V) Vec<T>::store(out + i * N + 2 * j, a.x);
+        if (i * N + 2 * j + 1 < V) Vec<T>::store(out + i * N + 2 * j + 1, a.y);
+      }
+    }
+    // the label's own gradient, over the vector just written by this thread
+    if (i == label_vector) {
+      const float x = Vec<T>::load(r.p + label);
+      const float d = product ? fmaf(x, scale2, off) : log2_prob(x, L, scale2);
+      Vec<T>::store(out + label, gs + score_gradient<ENTROPY>(d, gs, hs, H));
     }
   }
 }

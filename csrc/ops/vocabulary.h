@@ -61,10 +61,10 @@ struct PreferenceArgs {
   bool average;   // log-ratio of a sequence: mean over its tokens instead of the sum
   int reduction;  // 0 = loss per pair, 1 = sum, 2 = mean
 };
-// sequences = 2 * pairs, chosen first. loss: [pairs] or [1]; rewards: [2 * pairs] = beta * log-ratio; slope: [2 * pairs] =
+// sequences = 2 * pairs, chosen first. loss: [pairs] or [1]; chosen, rejected: [pairs] = beta * log-ratio; slope: [2 * pairs] =
 // d(loss) / d(log-prob of a token of that sequence). reference may be null (0).
 void preference_loss_fwd(const float* log_probs, const float* reference, PackedTokens tokens, PreferenceArgs args, float* partials,
-                         float* loss, float* rewards, float* slope, cudaStream_t stream);
+                         float* loss, float* chosen, float* rejected, float* slope, cudaStream_t stream);
 // grad[t] = slope[sequence of t] * d_loss[pair * d_loss_stride], 0 for tokens that take no part.
 void preference_loss_bwd(const float* slope, const float* d_loss, long long d_loss_stride, PackedTokens tokens, float* grad,
                          cudaStream_t stream);
@@ -77,12 +77,15 @@ struct PolicyArgs {
   bool per_token_advantage;
   int reduction;             // 0 = sum, 1 = mean over tokens, 2 = mean over sequences of their token means
 };
-// out: [4] = loss, mean KL estimate, fraction of clipped tokens, 1 / divisor of the reduction; slope (or null): [T] d(token's loss) /
+struct PolicyOut {
+  float *loss, *kl, *clipped, *factor;  // one value each; factor: 1 / divisor of the reduction
+};
+// kl: mean KL estimate, clipped: share of tokens whose gradient is clipped; slope (or null): [T] d(token's loss) /
 // d(log-prob); weight: [sequences] 1 / tokens of the sequence (reduction 2 only).
 void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const float* reference, const float* advantages,
-                     PackedTokens tokens, PolicyArgs args, float* partials, float* out, float* slope, float* weight, cudaStream_t stream);
-// grad[t] = slope[t] * out[3] (* weight[sequence of t]) * d_loss, 0 for tokens that take no part.
-void policy_loss_bwd(const float* slope, const float* out, const float* weight, const float* d_loss, PackedTokens tokens, int reduction, float* grad,
+                     PackedTokens tokens, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight, cudaStream_t stream);
+// grad[t] = slope[t] * factor (* weight[sequence of t]) * d_loss, 0 for tokens that take no part.
+void policy_loss_bwd(const float* slope, const float* factor, const float* weight, const float* d_loss, PackedTokens tokens, int reduction, float* grad,
                      cudaStream_t stream);
 
 // ---- ops/embedding_sorted.cu

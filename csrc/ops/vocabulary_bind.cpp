@@ -1,7 +1,11 @@
 // Python bindings of the vocabulary operators: argument checks, outputs and workspaces from the tensor allocator, launches on
-// the current stream of the operands' device.
+// the current stream of the operands' device. The operators whose kernels take a few microseconds are differentiable functions
+// here rather than in Python, where the bookkeeping of one call costs more than its kernels (preference loss of 4 pairs of 300 tokens, both
+// directions: 129 us with the function in Python).
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -16,6 +20,18 @@ namespace {
 using torch::Tensor;
 using OptTensor = c10::optional<Tensor>;
 
+// Parts of a message as strings: numbers are not put through the error macros' streams, since an extension that was linked with a C++ library
+// of its own formats them with facets that the library of torch does not share, which ends the process.
+std::string text(int64_t v) { return std::to_string(v); }
+std::string text(double v) { return std::to_string(v); }
+std::string text(torch::ScalarType t) { return c10::toString(t); }
+std::string text(const at::Device& d) { return d.str(); }
+std::string text(at::IntArrayRef sizes) {
+  std::string s = "[";
+  for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
+  return s + "]";
+}
+
 cudaStream_t stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 Scalar scalar_of(const Tensor& t, const char* name) {
@@ -23,32 +39,32 @@ Scalar scalar_of(const Tensor& t, const char* name) {
     case torch::kBFloat16: return Scalar::kBf16;
     case torch::kFloat16: return Scalar::kF16;
     case torch::kFloat32: return Scalar::kF32;
-    default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32, got ", t.scalar_type());
+    default: TORCH_CHECK(false, name, " must be bf16, fp16 or fp32, got ", text(t.scalar_type()));
   }
   return Scalar::kF32;
 }
 
 void check_device(const Tensor& t, const Tensor& like, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", text(like.device()), ", got ", text(t.device()));
 }
 
 void check_indices(const Tensor& t, const Tensor& like, const char* name) {
   check_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32, name, " must be int64 or int32, got ", t.scalar_type());
+  TORCH_CHECK(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32, name, " must be int64 or int32, got ", text(t.scalar_type()));
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
 
 // fp32 values of `rows` rows as a pointer and a stride (0 for a broadcast value)
 const float* row_values(const Tensor& t, const Tensor& like, int64_t rows, const char* name, long long* stride) {
   check_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.dim() == 1 && t.size(0) == rows, name, " must be fp32 [", rows, "]");
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.dim() == 1 && t.size(0) == rows, name, " must be fp32 [", text(rows), "]");
   *stride = t.stride(0);
   return t.data_ptr<float>();
 }
 
 const float* contiguous_f32(const Tensor& t, const Tensor& like, int64_t count, const char* name) {
   check_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.numel() == count, name, " must be contiguous fp32 with ", count, " elements");
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.numel() == count, name, " must be contiguous fp32 with ", text(count), " elements");
   return t.data_ptr<float>();
 }
 
@@ -77,7 +93,9 @@ std::tuple<Tensor, Tensor, Tensor> log_probs_fwd(const Tensor& logits, const Ten
   check_indices(labels, logits, "labels");
   TORCH_CHECK(labels.numel() == rows, "labels must have one entry per row of logits");
   const c10::cuda::CUDAGuard guard(logits.device());
-  Tensor log_probs = empty_f32(rows, logits), lse = empty_pairs(rows, logits), entropy = want_entropy ? empty_f32(rows, logits) : Tensor();
+  // outputs are tensors of their own, not views: a caller may change them in place
+  const auto f32 = logits.options().dtype(torch::kFloat32);
+  Tensor log_probs = torch::empty(labels.sizes(), f32), lse = empty_pairs(rows, logits), entropy = want_entropy ? torch::empty(labels.sizes(), f32) : Tensor();
   token_log_probs_fwd(logits.data_ptr(), type, labels.data_ptr(), labels.scalar_type() == torch::kInt64, log_probs.data_ptr<float>(),
                       want_entropy ? entropy.data_ptr<float>() : nullptr, pairs(lse), rows, (int)logits.size(2), map, (float)logit_scale,
                       ignore_index, stream_of(logits));
@@ -199,8 +217,8 @@ PackedTokens packed_tokens(const Tensor& values, const OptTensor& cu, int64_t le
   return p;
 }
 
-// (loss, rewards [2 * pairs], slope [2 * pairs])
-std::tuple<Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu, int64_t length, int64_t sequences,
+// (loss, chosen rewards, rejected rewards, slope [2 * pairs])
+std::tuple<Tensor, Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu, int64_t length, int64_t sequences,
                                                   const OptTensor& mask, int64_t kind, double beta, double label_smoothing, bool average, int64_t reduction) {
   TORCH_CHECK(log_probs.is_cuda(), "log_probs must be a CUDA tensor");
   TORCH_CHECK(sequences > 0 && sequences % 2 == 0, "an even number of sequences is needed: chosen, then rejected");
@@ -210,10 +228,10 @@ std::tuple<Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_probs, const
   const float* ref = reference.has_value() ? contiguous_f32(*reference, log_probs, p.T, "reference_log_probs") : nullptr;
   const c10::cuda::CUDAGuard guard(log_probs.device());
   Tensor loss = reduction == 0 ? empty_f32(sequences / 2, log_probs) : torch::empty({}, log_probs.options());
-  Tensor rewards = empty_f32(sequences, log_probs), slope = empty_f32(sequences, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
+  Tensor chosen = empty_f32(sequences / 2, log_probs), rejected = empty_f32(sequences / 2, log_probs), slope = empty_f32(sequences, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
   const PreferenceArgs args = {(PreferenceKind)kind, (float)beta, (float)label_smoothing, average, (int)reduction};
-  preference_loss_fwd(lp, ref, p, args, partials.data_ptr<float>(), loss.data_ptr<float>(), rewards.data_ptr<float>(), slope.data_ptr<float>(), stream_of(log_probs));
-  return {loss, rewards, slope};
+  preference_loss_fwd(lp, ref, p, args, partials.data_ptr<float>(), loss.data_ptr<float>(), chosen.data_ptr<float>(), rejected.data_ptr<float>(), slope.data_ptr<float>(), stream_of(log_probs));
+  return {loss, chosen, rejected, slope};
 }
 
 Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& log_probs, const OptTensor& cu, int64_t length, const OptTensor& mask) {
@@ -233,8 +251,8 @@ Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& l
   return grad;
 }
 
-// (out [4], slope [T] or undefined, weight [sequences])
-std::tuple<Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Tensor& old_log_probs, const OptTensor& reference, const Tensor& advantages, bool per_token,
+// (loss, kl, clipped share, factor [1], slope [T] or undefined, weight [sequences])
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Tensor& old_log_probs, const OptTensor& reference, const Tensor& advantages, bool per_token,
                                               const OptTensor& cu, int64_t length, int64_t sequences, const OptTensor& mask, double clip_low, double clip_high,
                                               double dual_clip, double kl_coef, int64_t reduction, bool want_slope) {
   TORCH_CHECK(log_probs.is_cuda(), "log_probs must be a CUDA tensor");
@@ -245,7 +263,7 @@ std::tuple<Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Ten
   const float* ref = reference.has_value() ? contiguous_f32(*reference, log_probs, p.T, "reference_log_probs") : nullptr;
   const float* adv = contiguous_f32(advantages, log_probs, per_token ? p.T : sequences, "advantages");
   const c10::cuda::CUDAGuard guard(log_probs.device());
-  Tensor out = empty_f32(4, log_probs), slope = want_slope ? empty_f32(p.T, log_probs) : Tensor();
+  Tensor loss = torch::empty({}, log_probs.options()), kl = torch::empty_like(loss), clipped = torch::empty_like(loss), factor = empty_f32(1, log_probs), slope = want_slope ? empty_f32(p.T, log_probs) : Tensor();
   Tensor weight = empty_f32(reduction == 2 ? sequences : 0, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
   PolicyArgs args = {};
   args.log_low = std::log1p(-clip_low);
@@ -256,22 +274,22 @@ std::tuple<Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Ten
   args.kl_coef = (float)kl_coef;
   args.per_token_advantage = per_token;
   args.reduction = (int)reduction;
-  policy_loss_fwd(lp, old, ref, adv, p, args, partials.data_ptr<float>(), out.data_ptr<float>(), want_slope ? slope.data_ptr<float>() : nullptr, weight.data_ptr<float>(),
+  policy_loss_fwd(lp, old, ref, adv, p, args, partials.data_ptr<float>(), {loss.data_ptr<float>(), kl.data_ptr<float>(), clipped.data_ptr<float>(), factor.data_ptr<float>()}, want_slope ? slope.data_ptr<float>() : nullptr, weight.data_ptr<float>(),
                   stream_of(log_probs));
-  return {out, slope, weight};
+  return {loss, kl, clipped, factor, slope, weight};
 }
 
-Tensor policy_bwd(const Tensor& slope, const Tensor& out, const Tensor& weight, const Tensor& d_loss, at::IntArrayRef shape, const OptTensor& cu, int64_t length,
+Tensor policy_bwd(const Tensor& slope, const Tensor& factor, const Tensor& weight, const Tensor& d_loss, at::IntArrayRef shape, const OptTensor& cu, int64_t length,
                   int64_t sequences, const OptTensor& mask, int64_t reduction) {
   const PackedTokens p = packed_tokens(slope, cu, length, sequences, mask);
   contiguous_f32(slope, slope, p.T, "slope");
-  contiguous_f32(out, slope, 4, "out");
+  contiguous_f32(factor, slope, 1, "factor");
   contiguous_f32(weight, slope, reduction == 2 ? sequences : 0, "weight");
   contiguous_f32(d_loss, slope, 1, "d_loss");
   const c10::cuda::CUDAGuard guard(slope.device());
   Tensor grad = torch::empty(shape, slope.options());
   TORCH_CHECK(grad.numel() == p.T, "shape mismatch");
-  policy_loss_bwd(slope.data_ptr<float>(), out.data_ptr<float>(), weight.data_ptr<float>(), d_loss.data_ptr<float>(), p, (int)reduction, grad.data_ptr<float>(),
+  policy_loss_bwd(slope.data_ptr<float>(), factor.data_ptr<float>(), weight.data_ptr<float>(), d_loss.data_ptr<float>(), p, (int)reduction, grad.data_ptr<float>(),
                   stream_of(slope));
   return grad;
 }
@@ -313,22 +331,220 @@ Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, con
   return dw;
 }
 
+// ------------------------------------------------------------------------- differentiable functions
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// The kernels' gradients have no derivative: with create_graph they are handed on with a node that says so when it is reached.
+Tensor once(const Tensor& grad, const char* name) {
+  if (!grad.defined() || !at::GradMode::is_enabled()) return grad;
+  Tensor leaf = grad.detach();
+  leaf.set_requires_grad(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " cannot be differentiated twice", 1);
+  return (*node)({leaf})[0];
+}
+
+// Upstream gradient of a per-row output as fp32 values with one stride; a missing one is zeros.
+Tensor row_gradient(const Tensor& grad, int64_t rows, const Tensor& like) {
+  if (!grad.defined()) return torch::zeros({}, like.options().dtype(torch::kFloat32)).expand({rows});
+  return grad.reshape({rows});
+}
+
+// [outer, inner, V] form of a batch of logits (a shifted [B, S, V] slice stays a view); a copy only where its layout has none.
+Tensor rows3(const Tensor& logits) {
+  Tensor t = logits.dim() == 1 ? logits.unsqueeze(0).unsqueeze(0) : logits.dim() == 2 ? logits.unsqueeze(0) : logits.dim() > 3 ? logits.flatten(0, -3) : logits;
+  return t.stride(2) == 1 || t.size(2) == 1 ? t : t.contiguous();
+}
+
+struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy) {
+    auto [log_probs, entropy, lse] = log_probs_fwd(rows3(logits), labels.contiguous(), logit_scale, ignore_index, want_entropy);
+    ctx->save_for_backward({logits, labels, lse, entropy});
+    ctx->saved_data["logit_scale"] = logit_scale;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->set_materialize_grads(false);
+    if (!want_entropy) return {log_probs};
+    return {log_probs, entropy};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &labels = saved[1], &lse = saved[2], &entropy = saved[3];
+    const bool has_h = grads.size() > 1 && grads[1].defined();
+    if (!grads[0].defined() && !has_h) return variable_list(5);
+    const int64_t rows = labels.numel();
+    Tensor grad = log_probs_bwd(rows3(logits), labels.contiguous(), lse, entropy.defined() ? OptTensor(entropy) : OptTensor(), row_gradient(grads[0], rows, lse),
+                                has_h ? OptTensor(row_gradient(grads[1], rows, lse)) : OptTensor(), ctx->saved_data["logit_scale"].toDouble(),
+                                ctx->saved_data["ignore_index"].toInt());
+    return {once(grad.view(logits.sizes()), "token_log_probs"), Tensor(), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+void check_logit_scale(double logit_scale) {
+  TORCH_CHECK_VALUE(std::isfinite(logit_scale) && logit_scale > 0, "logit_scale must be positive and finite, got ", text(logit_scale));
+}
+
+void check_label_shape(const Tensor& labels, at::IntArrayRef shape, const Tensor& like) {
+  TORCH_CHECK_VALUE(labels.scalar_type() == torch::kInt64 || labels.scalar_type() == torch::kInt32, "labels must be int64 or int32, got ", text(labels.scalar_type()));
+  TORCH_CHECK_VALUE(labels.sizes() == shape, "labels must have the shape ", text(shape), ", got ", text(labels.sizes()));
+  TORCH_CHECK_VALUE(labels.device() == like.device(), "labels must be on ", text(like.device()), ", got ", text(labels.device()));
+}
+
+variable_list token_log_probs(const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index, bool return_entropy) {
+  check_logit_scale(logit_scale);
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must have a last dimension of at least 1, got ", text(logits.sizes()));
+  check_label_shape(labels, logits.sizes().slice(0, logits.dim() - 1), logits);
+  return TokenLogProbs::apply(logits, labels, logit_scale, ignore_index, return_entropy);
+}
+
+// ---- losses: (log_probs as given, the same in fp32) so that the type conversion stays a differentiable step of its own
+struct Sequences {
+  int64_t count, length;
+  OptTensor cu, mask;
+};
+
+Sequences check_sequences(const Tensor& log_probs, const OptTensor& cu_seqlens, const OptTensor& mask) {
+  Sequences s = {};
+  TORCH_CHECK_VALUE(log_probs.is_floating_point(), "log_probs must be floating point, got ", text(log_probs.scalar_type()));
+  if (mask.has_value()) {
+    TORCH_CHECK_VALUE(mask->sizes() == log_probs.sizes() && mask->device() == log_probs.device() && !mask->is_floating_point(), "mask must be boolean or integer, shaped ",
+                      text(log_probs.sizes()), " on ", text(log_probs.device()), ", got ", text(mask->scalar_type()), " ", text(mask->sizes()), " on ", text(mask->device()));
+    s.mask = (mask->scalar_type() == torch::kBool ? *mask : mask->ne(0)).contiguous();
+  }
+  if (!cu_seqlens.has_value()) {
+    TORCH_CHECK_VALUE(log_probs.dim() == 2, "log_probs must be [sequences, length], or [tokens] with cu_seqlens, got ", text(log_probs.sizes()));
+    s.count = log_probs.size(0);
+    s.length = log_probs.size(1);
+    return s;
+  }
+  TORCH_CHECK_VALUE(log_probs.dim() == 1, "with cu_seqlens log_probs must be [tokens], got ", text(log_probs.sizes()));
+  const Tensor& cu = *cu_seqlens;
+  TORCH_CHECK_VALUE(cu.dim() == 1 && cu.numel() >= 1 && (cu.scalar_type() == torch::kInt32 || cu.scalar_type() == torch::kInt64) && cu.device() == log_probs.device(),
+                    "cu_seqlens must be int32 or int64 [sequences + 1] on ", text(log_probs.device()), ", got ", text(cu.scalar_type()), " ", text(cu.sizes()), " on ", text(cu.device()));
+  s.count = cu.numel() - 1;
+  s.cu = cu.to(torch::kInt32).contiguous();
+  return s;
+}
+
+Tensor check_values(const Tensor& t, at::IntArrayRef shape, const Tensor& like, const char* name) {
+  TORCH_CHECK_VALUE(t.sizes() == shape && t.device() == like.device() && t.is_floating_point(), name, " must be floating point, shaped ", text(shape), " on ", text(like.device()), ", got ",
+                    text(t.scalar_type()), " ", text(t.sizes()), " on ", text(t.device()));
+  TORCH_CHECK_VALUE(!t.requires_grad(), name, " must not require a gradient (detach it): the loss is differentiated with respect to log_probs alone");
+  return t.to(torch::kFloat32).contiguous();
+}
+
+OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu, const OptTensor& mask, int64_t length,
+                               int64_t sequences, int64_t kind, double beta, double label_smoothing, bool average, int64_t reduction) {
+    auto [loss, chosen, rejected, slope] = preference_fwd(log_probs, reference, cu, length, sequences, mask, kind, beta, label_smoothing, average, reduction);
+    ctx->save_for_backward({slope, log_probs, cu.value_or(Tensor()), mask.value_or(Tensor())});
+    ctx->saved_data["length"] = length;
+    ctx->mark_non_differentiable({chosen, rejected});
+    return {loss, chosen, rejected};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(11);
+    out[0] = once(preference_bwd(saved[0], grads[0], saved[1], optional(saved[2]), ctx->saved_data["length"].toInt(), optional(saved[3])), "preference_loss");
+    return out;
+  }
+};
+
+variable_list preference_loss(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu_seqlens, const OptTensor& mask, int64_t kind, double beta,
+                              double label_smoothing, bool average, int64_t reduction) {
+  const Sequences s = check_sequences(log_probs, cu_seqlens, mask);
+  TORCH_CHECK_VALUE(s.count > 0 && s.count % 2 == 0, "an even number of answers is needed (chosen, then rejected), got ", text(s.count));
+  TORCH_CHECK_VALUE(std::isfinite(beta) && beta > 0, "beta must be positive and finite, got ", text(beta));
+  TORCH_CHECK_VALUE(label_smoothing >= 0 && label_smoothing < 0.5 && (label_smoothing == 0 || kind == 0),
+                    "label_smoothing must be in [0, 0.5) and goes with loss_type='sigmoid', got ", text(label_smoothing));
+  OptTensor ref;
+  if (reference.has_value()) ref = check_values(*reference, log_probs.sizes(), log_probs, "reference_log_probs");
+  return PreferenceLoss::apply(log_probs.to(torch::kFloat32).contiguous(), ref, s.cu, s.mask, s.length, s.count, kind, beta, label_smoothing, average, reduction);
+}
+
+struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const Tensor& old, const OptTensor& reference, const Tensor& advantages, bool per_token,
+                               const OptTensor& cu, const OptTensor& mask, int64_t length, int64_t sequences, double clip_low, double clip_high, double dual_clip, double kl_coef,
+                               int64_t reduction, bool want_slope) {
+    auto [loss, kl, clipped, factor, slope, weight] = policy_fwd(log_probs, old, reference, advantages, per_token, cu, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction, want_slope);
+    ctx->save_for_backward({slope, factor, weight, cu.value_or(Tensor()), mask.value_or(Tensor())});
+    ctx->saved_data["shape"] = log_probs.sizes().vec();
+    ctx->saved_data["length"] = length;
+    ctx->saved_data["sequences"] = sequences;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->mark_non_differentiable({kl, clipped});
+    return {loss, kl, clipped};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    variable_list out(15);
+    out[0] = once(policy_bwd(saved[0], saved[1], saved[2], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[3]), ctx->saved_data["length"].toInt(),
+                             ctx->saved_data["sequences"].toInt(), optional(saved[4]), ctx->saved_data["reduction"].toInt()),
+                  "policy_loss");
+    return out;
+  }
+};
+
+variable_list policy_loss(const Tensor& log_probs, const Tensor& old, const Tensor& advantages, const OptTensor& reference, const OptTensor& cu_seqlens, const OptTensor& mask,
+                          double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t reduction) {
+  const Sequences s = check_sequences(log_probs, cu_seqlens, mask);
+  const Tensor o = check_values(old, log_probs.sizes(), log_probs, "old_log_probs");
+  OptTensor ref;
+  if (reference.has_value()) ref = check_values(*reference, log_probs.sizes(), log_probs, "reference_log_probs");
+  const bool per_sequence = advantages.dim() == 1 && advantages.size(0) == s.count;  // also where there are as many tokens
+  const bool per_token = !per_sequence && advantages.sizes() == log_probs.sizes();
+  const Tensor a = per_token ? check_values(advantages, log_probs.sizes(), log_probs, "advantages") : check_values(advantages, {s.count}, log_probs, "advantages");
+  TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low must be in [0, 1] and clip_high at least 0, got ", text(clip_low), " and ", text(clip_high));
+  TORCH_CHECK_VALUE(std::isfinite(kl_coef) && kl_coef >= 0, "kl_coef must be finite and at least 0, got ", text(kl_coef));
+  TORCH_CHECK_VALUE(kl_coef == 0 || reference.has_value(), "kl_coef needs reference_log_probs");
+  TORCH_CHECK_VALUE(dual_clip == 0 || (std::isfinite(dual_clip) && dual_clip > 1), "dual_clip must be finite and above 1, got ", text(dual_clip));
+  const Tensor lp = log_probs.to(torch::kFloat32).contiguous();
+  const bool want_slope = at::GradMode::is_enabled() && lp.requires_grad();
+  return PolicyLoss::apply(lp, o, ref, a, per_token, s.cu, s.mask, s.length, s.count, clip_low, clip_high, dual_clip, kl_coef, reduction, want_slope);
+}
+
+// The engine's fp32 gradient buffer of a parameter (its Python attribute main_grad), if it has one.
+OptTensor main_grad(const Tensor& weight) {
+  const py::gil_scoped_acquire gil;
+  const py::object p = py::cast(weight);
+  const py::object target = py::getattr(p, "main_grad", py::none());
+  if (target.is_none()) return OptTensor();
+  return py::cast<Tensor>(target).view(weight.sizes());
+}
+
+struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
+    Tensor out = embedding_lookup_(weight, ids, scale, status);
+    ctx->save_for_backward({weight, ids});
+    ctx->saved_data["scale"] = scale;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& weight = saved[0];
+    const OptTensor target = main_grad(weight);
+    Tensor dw = embedding_gradient_(grads[0].contiguous(), saved[1], weight.size(0), target, ctx->saved_data["scale"].toDouble());
+    return {target.has_value() ? Tensor() : once(dw, "embedding_sorted"), Tensor(), Tensor(), Tensor()};
+  }
+};
+
+Tensor embedding_sorted(const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
+  TORCH_CHECK_VALUE(weight.dim() == 2, "the embedding table must be [V, H], got ", text(weight.sizes()));
+  TORCH_CHECK_VALUE(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "ids must be int64 or int32, got ", text(ids.scalar_type()));
+  TORCH_CHECK_VALUE(ids.device() == weight.device(), "ids must be on ", text(weight.device()), ", got ", text(ids.device()));
+  return EmbeddingSorted::apply(weight.contiguous(), ids.contiguous(), scale, status);
+}
+
 }  // namespace
 
 void register_vocabulary(pybind11::module_& m) {
-  m.def("log_probs_fwd", &log_probs_fwd, "log-probabilities of given tokens, entropies and log-sum-exps of rows of logits");
-  m.def("log_probs_bwd", &log_probs_bwd);
-  m.def("linear_log_probs_fwd", &linear_log_probs_fwd, "the same from hidden states and the output weight");
-  m.def("linear_log_probs_grad", &linear_log_probs_grad);
-  m.def("preference_loss_fwd", &preference_fwd);
-  m.def("preference_loss_bwd", &preference_bwd);
-  m.def("policy_loss_fwd", &policy_fwd);
-  m.def("policy_loss_bwd", [](const Tensor& slope, const Tensor& out, const Tensor& weight, const Tensor& d_loss, std::vector<int64_t> shape, const OptTensor& cu, int64_t length,
-                              int64_t sequences, const OptTensor& mask, int64_t reduction) {
-    return policy_bwd(slope, out, weight, d_loss, shape, cu, length, sequences, mask, reduction);
-  });
-  m.def("embedding_lookup", &embedding_lookup_);
-  m.def("embedding_gradient", &embedding_gradient_, "embedding gradient summed in sorted token order");
+  m.def("token_log_probs", &token_log_probs, "log-probabilities of given tokens (and entropies) under rows of logits");
+  m.def("linear_log_probs_fwd", &linear_log_probs_fwd, "the same from hidden states and the output weight, with the rows' log-sum-exps");
+  m.def("linear_log_probs_grad", &linear_log_probs_grad, "gradient of the logits, formed again from hidden states and weight");
+  m.def("preference_loss", &preference_loss, "loss over pairs of answers: (loss, chosen rewards, rejected rewards)");
+  m.def("policy_loss", &policy_loss, "clipped policy loss with a KL term: (loss, KL estimate, clipped share)");
+  m.def("embedding_sorted", &embedding_sorted, "embedding whose gradient is summed in sorted token order");
 }
 
 }  // namespace b200

@@ -17,17 +17,15 @@ from typing import NamedTuple
 import torch
 import torch.nn.functional as F
 
-from . import _flce_chunk_rows, _weight_grad_target, native, note_fallback, require_native, status_word
+from . import _flce_chunk_rows, _weight_grad_target, native, note_fallback, status_word
 from .timeline import site
 
 _LOGIT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-def _on_gpu(t: torch.Tensor, types: tuple[torch.dtype, ...]) -> bool:
-    if not t.is_cuda or t.dtype not in types:
-        return False
-    require_native()
-    return True
+# CUDA tensors of the kernels' types go straight to the extension, which makes the same checks (as ValueErrors) as the Python
+# code makes for the other path: one call of the smallest cases costs a few microseconds there, tens of them here. `native()` raises where
+# the extension cannot be loaded.
 
 
 def _check_labels(labels: torch.Tensor, rows: torch.Size, device: torch.device, name: str = "labels") -> None:
@@ -62,45 +60,10 @@ def _token_log_probs_torch(logits: torch.Tensor, labels: torch.Tensor, logit_sca
     return picked, torch.where(kept, entropy, 0.0)
 
 
-def _rows3(logits: torch.Tensor) -> torch.Tensor:
-    """``[outer, inner, V]`` view of a batch of logits (a shifted ``[B, S, V]`` slice stays a view), copied only where its layout has no such form."""
-    if logits.dim() == 1:
-        logits = logits[None, None]
-    elif logits.dim() == 2:
-        logits = logits[None]
-    elif logits.dim() > 3:
-        logits = logits.flatten(0, -3)
-    return logits if logits.stride(-1) == 1 or logits.shape[-1] == 1 else logits.contiguous()
-
-
 def _row_gradient(grad: torch.Tensor | None, rows: int, like: torch.Tensor) -> torch.Tensor:
     if grad is None:
         return torch.zeros((), dtype=torch.float32, device=like.device).expand(rows)
     return grad.reshape(-1)
-
-
-class _TokenLogProbsFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, logit_scale, ignore_index, return_entropy):
-        ctx.set_materialize_grads(False)
-        with site("token_log_probs.fwd"):
-            log_probs, entropy, lse = native().log_probs_fwd(_rows3(logits), labels.contiguous(), logit_scale, ignore_index, return_entropy)
-        ctx.save_for_backward(logits, labels, lse, entropy)
-        ctx.args = (logit_scale, ignore_index)
-        shape = labels.shape
-        return (log_probs.view(shape), entropy.view(shape)) if return_entropy else log_probs.view(shape)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_log_probs, d_entropy=None):
-        logits, labels, lse, entropy = ctx.saved_tensors
-        if d_log_probs is None and d_entropy is None:
-            return (None,) * 5
-        rows = labels.numel()
-        with site("token_log_probs.bwd"):
-            grad = native().log_probs_bwd(_rows3(logits), labels.contiguous(), lse, entropy, _row_gradient(d_log_probs, rows, lse),
-                                          None if d_entropy is None else d_entropy.reshape(-1), *ctx.args)
-        return grad.view(logits.shape), None, None, None, None
 
 
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0, ignore_index: int = -100,
@@ -111,13 +74,15 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: 
     Rows whose label is ``ignore_index`` (or lies outside of the vocabulary) give 0 and no gradient, whatever they hold. Logits of
     ``-inf`` are tokens of probability 0; a row of nothing but ``-inf`` has no distribution and gives NaN. ``logit_scale`` (1 /
     temperature, 1 / ``m_width``) must be positive. bf16, fp16 and fp32 logits of any row stride run on the kernels."""
+    if logits.is_cuda and logits.dtype in _LOGIT_TYPES:
+        with site("token_log_probs"):
+            out = native().token_log_probs(logits, labels, logit_scale, ignore_index, return_entropy)
+        return tuple(out) if return_entropy else out[0]
     logit_scale = _check_logit_scale(logit_scale)
     if logits.dim() < 1 or logits.shape[-1] == 0 or not logits.is_floating_point():
         raise ValueError(f"logits must be floating point with a last dimension of at least 1, got {logits.dtype} {tuple(logits.shape)}")
     _check_labels(labels, logits.shape[:-1], logits.device)
-    if not _on_gpu(logits, _LOGIT_TYPES):
-        return _token_log_probs_torch(logits, labels, logit_scale, ignore_index, return_entropy)
-    return _TokenLogProbsFn.apply(logits, labels, logit_scale, int(ignore_index), bool(return_entropy))
+    return _token_log_probs_torch(logits, labels, logit_scale, ignore_index, return_entropy)
 
 
 # ----------------------------------------------------------------------------- from hidden states
@@ -197,7 +162,7 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
     if x.device != weight.device or x.dtype != weight.dtype or not x.is_floating_point():
         raise ValueError(f"hidden states and weight must be floating point of one type on one device, got {x.dtype} on {x.device} and {weight.dtype} on {weight.device}")
     _check_labels(labels, x.shape[:-1], x.device)
-    if not (_on_gpu(x, (torch.bfloat16,)) and x.shape[-1] % 8 == 0):
+    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0):
         note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
         return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
     shape = labels.shape
@@ -258,35 +223,6 @@ def _sequence_ids(count: int, length: int, cu_seqlens: torch.Tensor | None, like
     return torch.where(t < cu_seqlens[0], count, ids)
 
 
-def _fp32(t: torch.Tensor) -> torch.Tensor:
-    return t.float().contiguous()
-
-
-def _mask8(mask: torch.Tensor | None) -> torch.Tensor | None:
-    if mask is None:
-        return None
-    return (mask if mask.dtype == torch.bool else mask != 0).contiguous()
-
-
-class _PreferenceLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, log_probs, reference, cu_seqlens, length, sequences, mask, *args):
-        with site("preference_loss.fwd"):
-            loss, rewards, slope = native().preference_loss_fwd(log_probs, reference, cu_seqlens, length, sequences, mask, *args)
-        ctx.save_for_backward(slope, log_probs, cu_seqlens, mask)
-        ctx.length = length
-        ctx.mark_non_differentiable(rewards)
-        return loss, rewards
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_loss, _):
-        slope, log_probs, cu_seqlens, mask = ctx.saved_tensors
-        with site("preference_loss.bwd"):
-            grad = native().preference_loss_bwd(slope, d_loss, log_probs, cu_seqlens, ctx.length, mask)
-        return (grad,) + (None,) * 10
-
-
 def _preference_loss_torch(log_probs, reference, cu_seqlens, length, sequences, mask, kind, beta, label_smoothing, average, reduction):
     lp = log_probs.reshape(-1)
     d = lp if reference is None else lp - reference.reshape(-1)
@@ -322,11 +258,15 @@ def preference_loss(log_probs: torch.Tensor, reference_log_probs: torch.Tensor |
     Returns the loss (reduced over pairs, or one per pair with ``reduction="none"``) and ``beta * s`` of the chosen and the rejected answers
     (no gradient). An answer without tokens has ``s = 0``. Masked tokens, and tokens outside of all sequences, are not looked at and get a
     gradient of 0."""
+    if loss_type not in _PREFERENCE_KINDS or reduction not in _PREFERENCE_REDUCTIONS:
+        raise ValueError(f"unexpected loss_type ({loss_type}) or reduction ({reduction})")
+    if log_probs.is_cuda and log_probs.dtype in _LOGIT_TYPES:
+        with site("preference_loss"):
+            return PreferenceLossOutput(*native().preference_loss(log_probs, reference_log_probs, cu_seqlens, mask, _PREFERENCE_KINDS[loss_type], beta, label_smoothing,
+                                                                  average_log_probs, _PREFERENCE_REDUCTIONS[reduction]))
     sequences, length = _check_sequences(log_probs, cu_seqlens, mask)
     if sequences == 0 or sequences % 2:
         raise ValueError(f"an even number of answers is needed (chosen, then rejected), got {sequences}")
-    if loss_type not in _PREFERENCE_KINDS or reduction not in _PREFERENCE_REDUCTIONS:
-        raise ValueError(f"unexpected loss_type ({loss_type}) or reduction ({reduction})")
     beta, label_smoothing = float(beta), float(label_smoothing)
     if not (math.isfinite(beta) and beta > 0):
         raise ValueError(f"beta must be positive and finite, got {beta}")
@@ -335,38 +275,10 @@ def preference_loss(log_probs: torch.Tensor, reference_log_probs: torch.Tensor |
     if reference_log_probs is not None:
         _check_like(reference_log_probs, log_probs, "reference_log_probs")
     args = (_PREFERENCE_KINDS[loss_type], beta, label_smoothing, bool(average_log_probs), _PREFERENCE_REDUCTIONS[reduction])
-    if _on_gpu(log_probs, (torch.float32, torch.bfloat16, torch.float16)):
-        cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
-        loss, rewards = _PreferenceLossFn.apply(_fp32(log_probs), None if reference_log_probs is None else _fp32(reference_log_probs), cu, length, sequences,
-                                                _mask8(mask), *args)
-    else:
-        wide = log_probs if log_probs.dtype == torch.float64 else log_probs.float()
-        loss, rewards = _preference_loss_torch(wide, None if reference_log_probs is None else reference_log_probs.to(wide.dtype), cu_seqlens, length, sequences, mask, *args)
+    wide = log_probs if log_probs.dtype == torch.float64 else log_probs.float()
+    loss, rewards = _preference_loss_torch(wide, None if reference_log_probs is None else reference_log_probs.to(wide.dtype), cu_seqlens, length, sequences, mask, *args)
     pairs = sequences // 2
     return PreferenceLossOutput(loss, rewards[:pairs], rewards[pairs:])
-
-
-class _PolicyLossFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction):
-        with site("policy_loss.fwd"):
-            out, slope, weight = native().policy_loss_fwd(log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high,
-                                                          dual_clip, kl_coef, reduction, ctx.needs_input_grad[0])
-        ctx.save_for_backward(slope, out, weight, cu_seqlens, mask)
-        ctx.args = (list(log_probs.shape), length, sequences, reduction)
-        loss = out[0].clone()  # a tensor of its own: `out` is needed again and must not be written through the loss
-        kl, clip_fraction = out[1], out[2]
-        ctx.mark_non_differentiable(kl, clip_fraction)
-        return loss, kl, clip_fraction
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_loss, *_):
-        slope, out, weight, cu_seqlens, mask = ctx.saved_tensors
-        shape, length, sequences, reduction = ctx.args
-        with site("policy_loss.bwd"):
-            grad = native().policy_loss_bwd(slope, out, weight, d_loss, shape, cu_seqlens, length, sequences, mask, reduction)
-        return (grad,) + (None,) * 13
 
 
 def _policy_loss_torch(log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction):
@@ -406,19 +318,27 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
                 dual_clip: float | None = None, kl_coef: float = 0.0, reduction: str = "token_mean") -> PolicyLossOutput:
     """Clipped policy-gradient loss with a KL term, from per-token log-probabilities of sampled answers.
 
-    ``log_probs`` is packed ``[tokens]`` with ``cu_seqlens [sequences + 1]`` or padded ``[sequences, length]``; ``advantages`` has its shape, or
-    ``[sequences]`` for one value per answer. A token's loss is ``max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high))`` with
+    ``log_probs`` is packed ``[tokens]`` with ``cu_seqlens [sequences + 1]`` or padded ``[sequences, length]``; ``advantages`` is
+    ``[sequences]``, one value per answer, or else has the shape of ``log_probs``. A token's loss is ``max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high))`` with
     ``r = exp(log_probs - old_log_probs)``, bounded by ``-dual_clip A`` where ``A < 0``, plus ``kl_coef (exp(k) - 1 - k)`` with ``k = reference - log_probs``.
     ``token_mean`` divides the sum by the number of tokens that ``mask`` keeps, ``sequence_mean`` averages the answers' token means over the answers
     that keep a token, ``sum`` does neither.
 
     Returns the loss, and over the kept tokens the mean of ``exp(k) - 1 - k`` (0 without a reference) and the share whose gradient was clipped (neither has
     a gradient). Masked tokens, and tokens outside of all sequences, are not looked at and get a gradient of 0; nothing kept gives 0."""
+    if reduction not in _POLICY_REDUCTIONS:
+        raise ValueError(f"unexpected reduction ({reduction})")
+    if dual_clip is not None and not (math.isfinite(dual_clip) and dual_clip > 1):
+        raise ValueError(f"dual_clip must be finite and above 1, got {dual_clip}")
+    if log_probs.is_cuda and log_probs.dtype in _LOGIT_TYPES:
+        with site("policy_loss"):
+            return PolicyLossOutput(*native().policy_loss(log_probs, old_log_probs, advantages, reference_log_probs, cu_seqlens, mask, clip_low, clip_high, dual_clip or 0.0,
+                                                          kl_coef, _POLICY_REDUCTIONS[reduction]))
     sequences, length = _check_sequences(log_probs, cu_seqlens, mask)
     _check_like(old_log_probs, log_probs, "old_log_probs")
     if reference_log_probs is not None:
         _check_like(reference_log_probs, log_probs, "reference_log_probs")
-    per_token = advantages.shape == log_probs.shape and not (cu_seqlens is not None and advantages.shape == (sequences,) and sequences == log_probs.numel())
+    per_token = advantages.shape != (sequences,) and advantages.shape == log_probs.shape
     _check_like(advantages, log_probs if per_token else log_probs.new_empty(()).expand(sequences), "advantages")
     clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
     if not (0 <= clip_low <= 1 and clip_high >= 0):
@@ -427,52 +347,26 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
         raise ValueError(f"kl_coef must be finite and at least 0, got {kl_coef}")
     if kl_coef and reference_log_probs is None:
         raise ValueError("kl_coef needs reference_log_probs")
-    if dual_clip is not None and not (math.isfinite(dual_clip) and dual_clip > 1):
-        raise ValueError(f"dual_clip must be finite and above 1, got {dual_clip}")
-    if reduction not in _POLICY_REDUCTIONS:
-        raise ValueError(f"unexpected reduction ({reduction})")
     args = (clip_low, clip_high, float(dual_clip or 0.0), kl_coef, _POLICY_REDUCTIONS[reduction])
-    if _on_gpu(log_probs, (torch.float32, torch.bfloat16, torch.float16)):
-        cu = None if cu_seqlens is None else cu_seqlens.to(torch.int32).contiguous()
-        return PolicyLossOutput(*_PolicyLossFn.apply(_fp32(log_probs), _fp32(old_log_probs), None if reference_log_probs is None else _fp32(reference_log_probs),
-                                                     _fp32(advantages), per_token, cu, length, sequences, _mask8(mask), *args))
     wide = log_probs if log_probs.dtype == torch.float64 else log_probs.float()
     others = [None if t is None else t.to(wide.dtype) for t in (old_log_probs, reference_log_probs, advantages)]
     return PolicyLossOutput(*_policy_loss_torch(wide, *others, per_token, cu_seqlens, length, sequences, mask, *args))
 
 
 # ----------------------------------------------------------------------------- embedding
-class _EmbeddingSortedFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, ids, scale):
-        ctx.save_for_backward(ids)
-        ctx.weight, ctx.scale = weight, scale
-        with site("embedding.fwd"):
-            return native().embedding_lookup(weight, ids, scale, status_word(weight.device))
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dout):
-        (ids,) = ctx.saved_tensors
-        weight = ctx.weight
-        target = _weight_grad_target(weight)
-        with site("embedding.bwd"):
-            dw = native().embedding_gradient(dout.contiguous(), ids, weight.shape[0], None if target is None else target.view(weight.shape), ctx.scale)
-        return None if target is not None else dw, None, None
-
-
 def embedding_sorted(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
     """``scale * weight[ids]`` whose weight gradient adds the rows of a token in ascending position: the same bits on every run, one rounding, no fp32
     copy of the whole table (``ops.embedding(sorted_gradient=True)``). bf16, fp16 and fp32 tables of any width run on the kernels.
 
     On the GPU an id outside of the table gives a row of zeros, takes no part in the gradient and raises the status word (``ops.check_status()``)."""
+    if weight.is_cuda and weight.dtype in _LOGIT_TYPES:
+        with site("embedding"):
+            return native().embedding_sorted(weight, ids, scale, status_word(weight.device))
     if weight.dim() != 2 or not weight.is_floating_point():
         raise ValueError(f"the embedding table must be floating point [V, H], got {weight.dtype} {tuple(weight.shape)}")
     if ids.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"ids must be int64 or int32, got {ids.dtype}")
     if ids.device != weight.device:
         raise ValueError(f"ids must be on {weight.device}, got {ids.device}")
-    if not _on_gpu(weight, _LOGIT_TYPES):
-        out = F.embedding(ids, weight)
-        return out if scale == 1.0 else out * scale
-    return _EmbeddingSortedFn.apply(weight.contiguous(), ids.contiguous(), float(scale))
+    out = F.embedding(ids, weight)
+    return out if scale == 1.0 else out * scale

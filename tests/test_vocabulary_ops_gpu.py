@@ -441,3 +441,68 @@ def test_a_second_backward_pass_gives_the_same_gradients():
     loss = ops.policy_loss(lp[None], lp.detach()[None], torch.ones(1, device="cuda")).loss
     first = torch.autograd.grad(loss, logits, retain_graph=True)[0].clone()
     assert torch.equal(torch.autograd.grad(loss, logits)[0], first) and first.abs().max() > 0
+
+
+@pytest.mark.parametrize("call", [
+    lambda f, i: ops.token_log_probs(f(3, 5), f(3)),
+    lambda f, i: ops.token_log_probs(f(3, 5), i(4)),
+    lambda f, i: ops.token_log_probs(f(3, 5), i(3).cpu()),
+    lambda f, i: ops.token_log_probs(f(3, 0), i(3)),
+    lambda f, i: ops.token_log_probs(f(3, 5), i(3), logit_scale=0.0),
+    lambda f, i: ops.token_log_probs(f(3, 5), i(3), logit_scale=math.nan),
+    lambda f, i: ops.fused_linear_token_log_probs(f(3, 8).bfloat16(), f(5, 16).bfloat16(), i(3)),
+    lambda f, i: ops.fused_linear_token_log_probs(f(3, 8).bfloat16(), f(5, 8), i(3)),
+    lambda f, i: ops.fused_linear_token_log_probs(f(3, 8).bfloat16(), f(5, 8).bfloat16(), i(2)),
+    lambda f, i: ops.preference_loss(f(3, 3), None),
+    lambda f, i: ops.preference_loss(f(0, 3), None),
+    lambda f, i: ops.preference_loss(f(12), None),
+    lambda f, i: ops.preference_loss(f(4, 3), None, i(5)),
+    lambda f, i: ops.preference_loss(f(12), None, f(5)),
+    lambda f, i: ops.preference_loss(f(12), None, i(5).cpu()),
+    lambda f, i: ops.preference_loss(f(4, 3), f(4, 4)),
+    lambda f, i: ops.preference_loss(f(4, 3), f(4, 3).cpu()),
+    lambda f, i: ops.preference_loss(f(4, 3), f(4, 3).requires_grad_(True)),
+    lambda f, i: ops.preference_loss(f(4, 3), None, beta=0.0),
+    lambda f, i: ops.preference_loss(f(4, 3), None, loss_type="log"),
+    lambda f, i: ops.preference_loss(f(4, 3), None, reduction="batch"),
+    lambda f, i: ops.preference_loss(f(4, 3), None, label_smoothing=0.5),
+    lambda f, i: ops.preference_loss(f(4, 3), None, label_smoothing=0.1, loss_type="ipo"),
+    lambda f, i: ops.preference_loss(f(4, 3), None, mask=f(4, 3)),
+    lambda f, i: ops.preference_loss(f(4, 3), None, mask=i(4, 2)),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 2), f(4)),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3).requires_grad_(True), f(4)),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(3)),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4).requires_grad_(True)),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4), clip_low=1.5),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4), clip_high=-0.1),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4), dual_clip=1.0),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4), kl_coef=0.1),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4), reference_log_probs=f(4, 3), kl_coef=-0.1),
+    lambda f, i: ops.policy_loss(f(4, 3), f(4, 3), f(4), reduction="mean"),
+    lambda f, i: ops.embedding(f(5, 4), f(3), sorted_gradient=True),
+    lambda f, i: ops.embedding(f(5, 4), i(3).cpu(), sorted_gradient=True),
+    lambda f, i: ops.embedding(f(5), i(3), sorted_gradient=True),
+])
+def test_refusals(call):
+    with pytest.raises(ValueError):
+        call(lambda *s: torch.zeros(*s, device="cuda"), lambda *s: torch.zeros(*s, dtype=torch.long, device="cuda"))
+
+
+def test_outputs_may_be_changed_in_place_and_second_derivatives_are_refused():
+    logits = torch.randn(4, 50, device="cuda", requires_grad=True)
+    labels = torch.tensor([1, 2, -100, 4], device="cuda")
+    lp = ops.token_log_probs(logits, labels)
+    lp *= 2.0
+    out = ops.policy_loss(lp[None], lp.detach()[None], torch.ones(1, device="cuda"))
+    loss = out.loss
+    loss /= 4
+    out.kl.add_(1)
+    (grad,) = torch.autograd.grad(loss, logits, create_graph=True)
+    (want,) = torch.autograd.grad(-2.0 / 16 * torch.log_softmax(logits, -1)[[0, 1, 3], [1, 2, 4]].sum() * (4 / 4), logits)
+    assert (grad.detach() - want).abs().max() < 1e-6
+    with pytest.raises(RuntimeError, match="cannot be differentiated twice"):
+        grad.sum().backward()
+    pair = ops.preference_loss(torch.zeros(2, 3, device="cuda", requires_grad=True), None, reduction="none")
+    pair.loss.mul_(3.0)
+    pair.chosen_rewards.add_(1.0)
+    assert pair.loss.item() == pytest.approx(3 * math.log(2), rel=1e-6)
