@@ -3,16 +3,20 @@
 //
 //   statistics: the epilogue reduces each row of a tile to (m, s, u, x[label]): largest logit, sums of softmax_stats.cuh
 //               relative to it, and the label's logit if it lies in the tile's columns; 16 bytes per row and tile go to
-//               stats[tile column][M] instead of 512 bytes of logits. token_log_probs_join combines the tiles.
+//               stats[slice][row] for every 128 columns instead of 256 bytes of logits. token_log_probs_join combines them.
 //   gradient:   the logits are formed again, and the epilogue writes d(logits) in bf16, the operand type of the two products
 //               that follow (d(x) = d(logits) W, dW = d(logits)^T x); the factor 1[label] - p is formed in fp32 from the fp32
 //               logits, so the one rounding is that of the stored operand.
 //
 // Same staging and synchronisation as the pair GEMM of gemm_bf16_2sm.cu (six 32 KB stages per CTA filled by TMA without
 // multicast, one issuing thread in the even CTA, two accumulators of 256 TMEM columns so that the epilogue of one tile runs
-// under the MMAs of the next). An epilogue thread owns one row, so the statistics need no exchange between threads.
-// Bound by the tensor cores: a tile takes 128 cycles per 16 of K, the epilogue about 2500 cycles (one exponential and
-// four to six FMA-pipe operations per logit on four warps), hidden behind the MMAs of the next tile from K = 512 on.
+// under the MMAs of the next). An epilogue thread owns one row of 128 columns, so the statistics need no exchange between
+// threads. Eight epilogue warps, two per quarter of the tensor memory's lanes, each with half of the columns: with four, one per
+// scheduler and each instruction waiting for the one before, the epilogue of a tile with entropy took about 20000 cycles and
+// bounded the kernel up to K = 2048 (16384 cycles of MMAs a tile).
+//
+// Rows whose label does not count are left out of all products: the batch is compacted to its live rows beforehand, whose number only
+// the device knows (LiveRows), so the kernel takes its row count from memory and the grid is sized for the whole batch.
 #include <cuda.h>
 
 #include "../common/cta_pair.cuh"
@@ -27,22 +31,25 @@ namespace b200 {
 namespace {
 
 constexpr int BM = 128;       // rows per CTA (256 per pair)
-constexpr int BN = kVocabTile;  // columns per pair
+constexpr int BN = 256;       // columns per pair
+constexpr int SLICES = BN / kVocabSlice;
 constexpr int BN_HALF = 128;  // W rows staged per CTA
 constexpr int BK = 64;
 constexpr int STAGES = 6;
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int B_STAGE_BYTES = BN_HALF * BK * 2;
-constexpr int THREADS = 192;
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
 constexpr int TMEM_COLS = 512;
 constexpr int BOX_BYTES = 32 * 128;               // one epilogue box: 32 rows x 64 bf16
-constexpr int STAGING_BYTES = 4 * 2 * BOX_BYTES;  // two boxes for each of the four epilogue warps
+constexpr int STAGING_BYTES = EPI_WARPS * BOX_BYTES;
 constexpr int SMEM_BYTES = STAGES * (A_STAGE_BYTES + B_STAGE_BYTES) + STAGING_BYTES + 1024 + 256;
 
 struct RowArgs {
   const void* labels;
   bool labels64;
-  float4* stats;  // statistics: [n tiles][M]
+  float4* stats;  // statistics: [slices][live.rows]
+  LiveRows live;
   const float2* lse;
   const float* entropy;
   const float* d_log_probs;
@@ -72,7 +79,7 @@ __device__ __forceinline__ uint32_t select32_bits(const uint32_t (&v)[32], int i
 template <Mode MODE, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 1)
     vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                          const __grid_constant__ CUtensorMap tmG, int M, int N, int K, int group, int* status, RowArgs rows) {
+                          const __grid_constant__ CUtensorMap tmG, int N, int K, int* status, RowArgs rows) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -92,10 +99,15 @@ __global__ void __launch_bounds__(THREADS, 1)
   const bool leader = cta_rank == 0;
   const int pair = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
-  const int m_tiles = (M + 2 * BM - 1) / (2 * BM);
+  // rows of this launch that count; at least one tile is worked on, so that a batch without any leaves zeros behind
+  const int live = rows.live.count == nullptr ? rows.live.rows : max(0, min(rows.live.rows, *rows.live.count - rows.live.base));
+  const int m_tiles = max(1, (live + 2 * BM - 1) / (2 * BM));
   const int n_tiles = (N + BN - 1) / BN;
   const int k_blocks = (K + BK - 1) / BK;
   const int total = m_tiles * n_tiles;
+  // Row panels of up to eight tiles: the pairs that run at a time share their A rows within a panel column and their W rows
+  // across the panel (the raster of the plain pair GEMM).
+  const int group = min(m_tiles, 8);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -104,7 +116,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);
+      mbar_init(&acc_empty[b], 2 * EPI_WARPS);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -194,35 +206,38 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ epilogue: this CTA's 128 x 256 half
-    const int q = warp & 3;
-    uint8_t* stage0 = sStage + q * (2 * BOX_BYTES);
+    // ------------------------------------------------------------------ epilogue: 32 rows x 128 columns of this CTA's 128 x 256 half
+    const int q = warp & 3;             // the quarter of the lanes that this warp can read
+    const int half = (warp - 2) >> 2;   // its half of the columns
+    uint8_t* box = sStage + (warp - 2) * BOX_BYTES;
     const float scale2 = rows.logit_scale * kLog2e;
-    uint32_t tcount = 0, nstore = 0;
+    uint32_t tcount = 0;
     for (int tile = pair; tile < total; tile += num_pairs, ++tcount) {
       const TileCoord tc = tile_coord(tile, m_tiles, n_tiles, group);
       const uint32_t buf = tcount & 1;
       const uint32_t aph = (tcount >> 1) & 1;
       const int row0 = tc.mi * (2 * BM) + (int)cta_rank * BM + q * 32;
       const int row = row0 + lane;
-      const int tile_col0 = tc.ni * BN;
-      // the label's column relative to the tile; -1: not here
+      const int slice_col0 = tc.ni * BN + half * kVocabSlice;
+      // the label's column relative to the slice; -1: not here
       int label = -1;
       bool ignored = true;
-      if (row < M) {
-        const long long l = load_label(rows.labels, rows.labels64, row);
+      long long t = 0;  // the row's place in the batch
+      if (row < live) {
+        t = rows.live.index != nullptr ? rows.live.index[rows.live.base + row] : rows.live.base + row;
+        const long long l = load_label(rows.labels, rows.labels64, t);
         ignored = l == rows.ignore_index || l < 0 || l >= N;
-        if (!ignored && l >= tile_col0 && l < tile_col0 + BN) label = (int)(l - tile_col0);
+        if (!ignored && l >= slice_col0 && l < slice_col0 + kVocabSlice) label = (int)(l - slice_col0);
       }
       float2 L = make_float2(0.f, 0.f);
       float gs = 0.f, hs = 0.f, H = 0.f;
       bool zero = true;
       if (MODE == Mode::kGrad && !ignored) {
-        L = rows.lse[row];
-        gs = rows.d_log_probs[row * rows.d_log_probs_stride] * rows.logit_scale;
+        L = rows.lse[t];
+        gs = rows.d_log_probs[t * rows.d_log_probs_stride] * rows.logit_scale;
         if (ENTROPY) {
-          hs = rows.d_entropy[row * rows.d_entropy_stride] * rows.logit_scale;
-          H = rows.entropy[row];
+          hs = rows.d_entropy[t * rows.d_entropy_stride] * rows.logit_scale;
+          H = rows.entropy[t];
         }
         zero = gs == 0.f && hs == 0.f;
       }
@@ -231,19 +246,24 @@ __global__ void __launch_bounds__(THREADS, 1)
         break;
       }
       tc_fence_after_sync();
-      const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + buf * BN;
+      const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + half * kVocabSlice;
+      if (slice_col0 >= N) {  // nothing of the vocabulary here: the accumulator is handed back unread
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+        continue;
+      }
 
       if (MODE == Mode::kStats) {
         Stats st = empty_stats();
         float x_label = 0.f;
 #pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
-          const int col0 = tile_col0 + c * 32;
+        for (int c = 0; c < kVocabSlice / 32; ++c) {
+          const int col0 = slice_col0 + c * 32;
           if (col0 >= N) break;
           uint32_t v[32];
           B200_TMEM_LD_32(v, t_row + c * 32);
           tmem_ld_wait();
-          if (c == BN / 32 - 1 || col0 + 32 >= N) {
+          if (c == kVocabSlice / 32 - 1 || col0 + 32 >= N) {
             // last read of this accumulator: hand the TMEM buffer back before the arithmetic
             tc_fence_before_sync();
             __syncwarp();
@@ -264,19 +284,18 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
           accumulate<ENTROPY, 32>(st, f, top, scale2);
         }
-        if (row < M) rows.stats[(long long)tc.ni * M + row] = make_float4(st.m, st.s, st.u, x_label);
+        if (row < live) rows.stats[(long long)(tc.ni * SLICES + half) * rows.live.rows + row] = make_float4(st.m, st.s, st.u, x_label);
       } else {
 #pragma unroll 1
-        for (int c = 0; c < BN / 64; ++c) {
-          const int col0 = tile_col0 + c * 64;
+        for (int c = 0; c < kVocabSlice / 64; ++c) {
+          const int col0 = slice_col0 + c * 64;
           if (col0 >= N) break;
-          uint8_t* box = stage0 + (nstore & 1) * BOX_BYTES;
-          if (lane == 0) tma_store_wait_read<1>();  // the store that used this box two boxes ago has read it
+          if (lane == 0) tma_store_wait_read<0>();  // the store that used the box before has read it
           __syncwarp();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int part = 0; part < 2; ++part) {
             uint32_t v[32];
-            B200_TMEM_LD_32(v, t_row + c * 64 + half * 32);
+            B200_TMEM_LD_32(v, t_row + c * 64 + part * 32);
             tmem_ld_wait();
             uint32_t w[16];
 #pragma unroll
@@ -286,8 +305,8 @@ __global__ void __launch_bounds__(THREADS, 1)
               w[e] = zero ? 0u : pack_bf16x2(a, b);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) box_write(box, lane, half * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
-            if ((label >> 5) == 2 * c + half && !zero) {
+            for (int j = 0; j < 4; ++j) box_write(box, lane, part * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
+            if ((label >> 5) == 2 * c + part && !zero) {
               // the label's own gradient, over the element of the row just written
               const float d = log2_prob(__uint_as_float(select32_bits(v, label & 31)), L, scale2);
               const int e = label & 63;
@@ -295,18 +314,17 @@ __global__ void __launch_bounds__(THREADS, 1)
                   __float2bfloat16(gs + score_gradient<ENTROPY>(d, gs, hs, H));
             }
           }
-          if (c == BN / 64 - 1 || col0 + 64 >= N) {
+          if (c == kVocabSlice / 64 - 1 || col0 + 64 >= N) {
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0 && row0 < M) {
+          if (lane == 0 && row0 < rows.live.rows) {
             tma_store_2d(&tmG, box, col0, row0);
             tma_store_commit();
           }
-          ++nstore;
         }
       }
     }
@@ -327,15 +345,11 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// Row panels of up to eight tiles: the pairs that run at a time share their A rows within a panel column and their W rows
-// across the panel (the raster of the plain pair GEMM).
-int panel(int m_tiles) { return m_tiles < 8 ? m_tiles : 8; }
-
 template <Mode MODE, bool ENTROPY>
-void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmG, int M, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
+void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmG, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
   auto kernel = vocab_gemm_2sm_kernel<MODE, ENTROPY>;
   check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "vocab gemm smem attr");
-  const int m_tiles = (M + 2 * BM - 1) / (2 * BM), n_tiles = (N + BN - 1) / BN;
+  const int m_tiles = (rows.live.rows + 2 * BM - 1) / (2 * BM), n_tiles = (N + BN - 1) / BN;
   int pairs = sm_count() / 2;
   if ((long long)m_tiles * n_tiles < pairs) pairs = m_tiles * n_tiles;
   cudaLaunchConfig_t cfg = {};
@@ -350,36 +364,38 @@ void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& t
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmG, M, N, K, panel(m_tiles), status, rows), "vocab gemm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmG, N, K, status, rows), "vocab gemm launch");
   count_launch();
 }
 
 }  // namespace
 
-void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, int M, int N,
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, LiveRows live, int N,
                       int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream) {
-  if (M <= 0) return;
-  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, M, ldx, BK, BM);
+  if (live.rows <= 0) return;
+  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, live.rows, ldx, BK, BM);
   const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
   RowArgs rows = {};
+  rows.live = live;
   rows.labels = labels;
   rows.labels64 = labels64;
   rows.stats = reinterpret_cast<float4*>(stats);
   rows.logit_scale = logit_scale;
   rows.ignore_index = -1;  // every label outside of [0, N) counts as none here
-  if (entropy) launch<Mode::kStats, true>(tmA, tmB, tmA, M, N, K, status, rows, stream);
-  else launch<Mode::kStats, false>(tmA, tmB, tmA, M, N, K, status, rows, stream);
+  if (entropy) launch<Mode::kStats, true>(tmA, tmB, tmA, N, K, status, rows, stream);
+  else launch<Mode::kStats, false>(tmA, tmB, tmA, N, K, status, rows, stream);
 }
 
 void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labels64, const float2* lse, const float* entropy,
                      const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
-                     void* grad, int M, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
+                     void* grad, LiveRows live, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
                      long long ignore_index, int* status, cudaStream_t stream) {
-  if (M <= 0) return;
-  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, M, ldx, BK, BM);
+  if (live.rows <= 0) return;
+  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, live.rows, ldx, BK, BM);
   const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
-  const CUtensorMap tmG = make_tensor_map_2d_b16(grad, N, M, ldg, 64, 32);
+  const CUtensorMap tmG = make_tensor_map_2d_b16(grad, N, live.rows, ldg, 64, 32);
   RowArgs rows = {};
+  rows.live = live;
   rows.labels = labels;
   rows.labels64 = labels64;
   rows.lse = lse;
@@ -390,8 +406,8 @@ void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labe
   rows.d_entropy_stride = d_entropy_stride;
   rows.logit_scale = logit_scale;
   rows.ignore_index = ignore_index;
-  if (d_entropy != nullptr) launch<Mode::kGrad, true>(tmA, tmB, tmG, M, N, K, status, rows, stream);
-  else launch<Mode::kGrad, false>(tmA, tmB, tmG, M, N, K, status, rows, stream);
+  if (d_entropy != nullptr) launch<Mode::kGrad, true>(tmA, tmB, tmG, N, K, status, rows, stream);
+  else launch<Mode::kGrad, false>(tmA, tmB, tmG, N, K, status, rows, stream);
 }
 
 }  // namespace b200

@@ -304,22 +304,26 @@ __global__ void __launch_bounds__(BWD_THREADS)
 template <bool ENTROPY>
 __global__ void __launch_bounds__(1024)
     token_log_probs_join_kernel(const float4* __restrict__ stats, int slices, int slice_width, const void* __restrict__ labels, bool labels64,
-                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, long long T, int V,
+                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, LiveRows live, int V,
                                 float scale2, long long ignore_index) {
   __shared__ Stats red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const long long row = (long long)blockIdx.x * 32 + lane;
+  const int rows = live.count == nullptr ? live.rows : min(live.rows, *live.count - live.base);
+  if ((long long)blockIdx.x * 32 >= rows) return;
+  const int r = blockIdx.x * 32 + lane;
   Stats st = empty_stats();
-  if (row < T) {
+  if (r < rows) {
+#pragma unroll 4
     for (int i = warp; i < slices; i += 32) {
-      const float4 v = stats[(long long)i * T + row];
+      const float4 v = stats[(long long)i * live.rows + r];
       st = merge<ENTROPY>(st, Stats{v.x, v.y, v.z}, scale2);
     }
   }
   red[warp][lane] = st;
   __syncthreads();
-  if (warp != 0 || row >= T) return;
+  if (warp != 0 || r >= rows) return;
   for (int w = 1; w < 32; ++w) st = merge<ENTROPY>(st, red[w][lane], scale2);
+  const long long row = live.index != nullptr ? live.index[live.base + r] : live.base + r;
   const long long label = load_label(labels, labels64, row);
   if (label == ignore_index || label < 0 || label >= V) {
     log_probs[row] = 0.f;
@@ -327,7 +331,7 @@ __global__ void __launch_bounds__(1024)
     if (ENTROPY) entropy[row] = 0.f;
     return;
   }
-  const float log2_s = log2f(st.s), x = stats[(long long)(label / slice_width) * T + row].w;
+  const float log2_s = log2f(st.s), x = stats[(long long)(label / slice_width) * live.rows + r].w;
   lse[row] = make_float2(st.m, log2_s);
   log_probs[row] = log2_prob(x, make_float2(st.m, log2_s), scale2) * kLn2;
   if (ENTROPY) entropy[row] = (log2_s - st.u / st.s) * kLn2;
@@ -383,16 +387,95 @@ void token_log_probs_bwd(const void* logits, Scalar type, const void* labels, bo
 }
 
 void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
-                          float* entropy, float2* lse, long long T, int V, float logit_scale, long long ignore_index, cudaStream_t stream) {
-  if (T == 0) return;
-  const unsigned blocks = (unsigned)((T + 31) / 32);
+                          float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream) {
+  if (live.rows <= 0) return;
+  const unsigned blocks = (unsigned)((live.rows + 31) / 32);
   const float4* st = reinterpret_cast<const float4*>(stats);
   if (entropy != nullptr)
-    token_log_probs_join_kernel<true><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, T, V, logit_scale * kLog2e, ignore_index);
+    token_log_probs_join_kernel<true><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, live, V, logit_scale * kLog2e, ignore_index);
   else
-    token_log_probs_join_kernel<false><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, T, V, logit_scale * kLog2e, ignore_index);
+    token_log_probs_join_kernel<false><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, live, V, logit_scale * kLog2e, ignore_index);
   count_launch();
   check_cuda(cudaGetLastError(), "token_log_probs join launch");
+}
+
+// ------------------------------------------------------------------------- live rows of a batch
+namespace {
+
+// One block walks the labels 1024 at a time; a row's place is the number of live rows before it.
+__global__ void __launch_bounds__(1024)
+    live_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, int* __restrict__ index, int* __restrict__ slot, int* __restrict__ count,
+                     float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse) {
+  __shared__ int warp_sum[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int before = 0;
+  for (int t0 = 0; t0 < T; t0 += 1024) {
+    const int t = t0 + threadIdx.x;
+    bool live = false;
+    if (t < T) {
+      const long long l = load_label(labels, labels64, t);
+      live = l != ignore_index && l >= 0 && l < V;
+    }
+    const unsigned votes = __ballot_sync(0xffffffffu, live);
+    if (lane == 0) warp_sum[warp] = __popc(votes);
+    __syncthreads();
+    int lower = 0, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      const int n = warp_sum[w];
+      lower += w < warp ? n : 0;
+      all += n;
+    }
+    __syncthreads();
+    const int place = before + lower + __popc(votes & ((1u << lane) - 1));
+    if (t < T) {
+      slot[t] = live ? place : -1;
+      if (live) {
+        index[place] = t;
+      } else {
+        log_probs[t] = 0.f;
+        lse[t] = make_float2(0.f, 0.f);
+        if (entropy != nullptr) entropy[t] = 0.f;
+      }
+    }
+    before += all;
+  }
+  if (threadIdx.x == 0) *count = before;
+}
+
+__global__ void __launch_bounds__(128)
+    gather_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const int* __restrict__ index, const int* __restrict__ count, __nv_bfloat16* __restrict__ compact, int H) {
+  const int r = blockIdx.x, n = *count;
+  uint4* dst = reinterpret_cast<uint4*>(compact + (long long)r * H);
+  const uint4* src = r < n ? reinterpret_cast<const uint4*>(x + (long long)index[r] * ldx) : nullptr;
+  for (int i = threadIdx.x; i < H / 8; i += blockDim.x) dst[i] = src != nullptr ? src[i] : make_uint4(0, 0, 0, 0);
+}
+
+__global__ void __launch_bounds__(128) scatter_rows_kernel(const __nv_bfloat16* __restrict__ compact, const int* __restrict__ slot, __nv_bfloat16* __restrict__ out, int H) {
+  const int t = blockIdx.x, r = slot[t];
+  uint4* dst = reinterpret_cast<uint4*>(out + (long long)t * H);
+  const uint4* src = r >= 0 ? reinterpret_cast<const uint4*>(compact + (long long)r * H) : nullptr;
+  for (int i = threadIdx.x; i < H / 8; i += blockDim.x) dst[i] = src != nullptr ? src[i] : make_uint4(0, 0, 0, 0);
+}
+
+}  // namespace
+
+void vocab_live_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, int* index, int* slot, int* count, float* log_probs, float* entropy, float2* lse,
+                     cudaStream_t stream) {
+  live_rows_kernel<<<1, 1024, 0, stream>>>(labels, labels64, ignore_index, T, V, index, slot, count, log_probs, entropy, lse);
+  count_launch();
+  check_cuda(cudaGetLastError(), "live rows launch");
+}
+
+void vocab_gather_rows(const void* x, long long ldx, const int* index, const int* count, void* compact, int T, int H, cudaStream_t stream) {
+  gather_rows_kernel<<<T, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(x), ldx, index, count, reinterpret_cast<__nv_bfloat16*>(compact), H);
+  count_launch();
+  check_cuda(cudaGetLastError(), "gather rows launch");
+}
+
+void vocab_scatter_rows(const void* compact, const int* slot, void* out, int T, int H, cudaStream_t stream) {
+  scatter_rows_kernel<<<T, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(compact), slot, reinterpret_cast<__nv_bfloat16*>(out), H);
+  count_launch();
+  check_cuda(cudaGetLastError(), "scatter rows launch");
 }
 
 }  // namespace b200

@@ -25,21 +25,45 @@ void token_log_probs_bwd(const void* logits, Scalar type, const void* labels, bo
                          long long d_entropy_stride, void* grad, long long T, int V, RowMap map, long long grad_stride,
                          float logit_scale, long long ignore_index, cudaStream_t stream);
 
-// Joins the statistics of `slices` column slices of the rows: stats[slice][T] = (m, s, u, the label's logit if it lies in the
+// The rows of a batch that a product has to cover. index == null: rows base, base + 1, ... of the batch, `rows` of them. Else the
+// batch has been compacted to the rows whose label counts: compact row r is row index[r] of the batch, *count of them are live (known
+// on the device only), and this launch covers the live ones among compact rows [base, base + rows).
+struct LiveRows {
+  const int* index;
+  const int* count;
+  int base, rows;
+};
+// index[0 .. *count) <- rows with a label in [0, V) other than ignore_index, in order; slot[t] <- compact row of t or -1; outputs of the
+// other rows <- 0.
+void vocab_live_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, int* index, int* slot, int* count, float* log_probs, float* entropy, float2* lse,
+                     cudaStream_t stream);
+// compact[r] <- x[index[r]] (bf16 rows of H, a multiple of 8 elements), zeros from *count on
+void vocab_gather_rows(const void* x, long long ldx, const int* index, const int* count, void* compact, int T, int H, cudaStream_t stream);
+// out[t] <- compact[slot[t]], zeros where there is none
+void vocab_scatter_rows(const void* compact, const int* slot, void* out, int T, int H, cudaStream_t stream);
+
+// Joins the statistics of `slices` column slices of the rows: stats[slice][live.rows] = (m, s, u, the label's logit if it lies in the
 // slice), see softmax_stats.cuh. Ignored rows give 0.
 void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
-                          float* entropy, float2* lse, long long T, int V, float logit_scale, long long ignore_index, cudaStream_t stream);
+                          float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream);
 
 // ---- gemm/vocab_gemm_2sm.cu: logits = x [M, K] w [N, K]^T, bf16 operands with row strides that are multiples of 8 elements;
 // the logits stay in tensor memory.
-constexpr int kVocabTile = 256;  // columns per slice of the statistics
-void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, int M, int N,
+// x holds the rows of this launch; labels, lse and gradients are those of the whole batch.
+constexpr int kVocabSlice = 128;  // columns per slice of the statistics
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, LiveRows live, int N,
                       int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream);
-// grad[M, N] (bf16, row stride ldg, a multiple of 8): gradient of the logits, as token_log_probs_bwd defines it.
+// grad[live.rows, N] (bf16, row stride ldg, a multiple of 8): gradient of the logits, as token_log_probs_bwd defines it; rows behind
+// the live ones are 0 up to the next multiple of 256.
 void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labels64, const float2* lse, const float* entropy,
                      const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
-                     void* grad, int M, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
+                     void* grad, LiveRows live, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
                      long long ignore_index, int* status, cudaStream_t stream);
+
+// ---- gemm/gemm_bf16_2sm.cu: the pair GEMM over the live rows of a compacted batch only: M (limit_k false) or K (true) ends at
+// max(1, *count - base). Rows from there to the next multiple of 256 must be 0 in both operands (they may be multiplied).
+void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, bool a_mn, bool b_mn, bool f32_accumulate,
+                        const int* count, int base, bool limit_k, int* status, cudaStream_t stream);
 
 // ---- ops/preference.cu
 // A packed batch of `sequences` sequences of per-token values: sequence i is tokens [cu[i], cu[i + 1]), or, without cu,

@@ -143,55 +143,119 @@ int* status_of(const Tensor& status, const Tensor& like) {
   return status.data_ptr<int>();
 }
 
-const char* label_ptr(const Tensor& labels, int64_t row) { return reinterpret_cast<const char*>(labels.data_ptr()) + row * labels.element_size(); }
-
-// Rows that share one statistics buffer: 16 bytes per row and 256 columns stay below 512 MB.
+// Rows that share one statistics buffer: 16 bytes per row and slice stay below 512 MB.
 int64_t stats_rows(int64_t rows, int64_t slices) {
   const int64_t most = std::max<int64_t>(256, ((512LL << 20) / (16 * slices)) / 256 * 256);
   return std::min(rows, std::min<int64_t>(most, 1 << 20));
 }
 
-std::tuple<Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy,
-                                                        const Tensor& status) {
-  check_linear(x, w, labels);
-  int* st = status_of(status, x);
-  const c10::cuda::CUDAGuard guard(x.device());
-  const int64_t rows = x.size(0), V = w.size(0), slices = (V + kVocabTile - 1) / kVocabTile;
-  const bool labels64 = labels.scalar_type() == torch::kInt64;
-  Tensor log_probs = empty_f32(rows, x), lse = empty_pairs(rows, x), entropy = want_entropy ? empty_f32(rows, x) : Tensor();
-  if (rows == 0) return {log_probs, entropy, lse};
-  const int64_t most = stats_rows(rows, slices);
-  Tensor stats = empty_f32(most * slices * 4, x);
-  const cudaStream_t stream = stream_of(x);
-  for (int64_t r = 0; r < rows; r += most) {
-    const int64_t n = std::min(most, rows - r);
-    const void* xr = reinterpret_cast<const char*>(x.data_ptr()) + r * x.stride(0) * 2;
-    vocab_gemm_stats(xr, w.data_ptr(), label_ptr(labels, r), labels64, stats.data_ptr<float>(), want_entropy, (int)n, (int)V, (int)x.size(1), x.stride(0), w.stride(0),
-                     (float)logit_scale, st, stream);
-    token_log_probs_join(stats.data_ptr<float>(), (int)slices, kVocabTile, label_ptr(labels, r), labels64, log_probs.data_ptr<float>() + r,
-                         want_entropy ? entropy.data_ptr<float>() + r : nullptr, pairs(lse) + r, n, (int)V, (float)logit_scale, ignore_index, stream);
-  }
-  return {log_probs, entropy, lse};
+// A batch of more rows than one tile is compacted to its live rows first: a tile is computed whole, so a smaller batch gains nothing.
+constexpr int64_t kCompactAbove = 256;
+
+// map: int32 [2 T + 1] = index [T], slot [T], count, or empty where the batch is not compacted
+LiveRows live_rows(const Tensor& map, int64_t T, int64_t base, int64_t rows) {
+  LiveRows live = {nullptr, nullptr, (int)base, (int)rows};
+  if (map.numel() == 0) return live;
+  TORCH_CHECK(map.is_cuda() && map.scalar_type() == torch::kInt32 && map.is_contiguous() && map.numel() == 2 * T + 1, "the row map must be int32 [2 T + 1]");
+  live.index = map.data_ptr<int>();
+  live.count = map.data_ptr<int>() + 2 * T;
+  return live;
 }
 
-// grad[T, V] (bf16, row stride a multiple of 8) <- gradient of the logits
-void linear_log_probs_grad(const Tensor& x, const Tensor& w, const Tensor& labels, const Tensor& lse, const OptTensor& entropy, const Tensor& d_log_probs,
-                           const OptTensor& d_entropy, Tensor& grad, double logit_scale, int64_t ignore_index, const Tensor& status) {
+void* row_ptr(const Tensor& t, int64_t row) { return reinterpret_cast<char*>(t.data_ptr()) + row * t.stride(0) * t.element_size(); }
+
+// (log_probs, entropy, lse, the rows that were multiplied, row map)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
+                                                                        bool want_entropy, const Tensor& status) {
   check_linear(x, w, labels);
   int* st = status_of(status, x);
-  const int64_t rows = x.size(0), V = w.size(0);
-  check_device(grad, x, "grad");
-  TORCH_CHECK(grad.scalar_type() == torch::kBFloat16 && grad.dim() == 2 && grad.size(0) == rows && grad.size(1) == V && grad.stride(1) == 1 && grad.stride(0) % 8 == 0 &&
-                  reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0,
-              "grad must be bf16 [T, V] with 16-byte aligned rows");
-  long long g_stride = 0, h_stride = 0;
-  const float* g = row_values(d_log_probs, x, rows, "d_log_probs", &g_stride);
-  const float* h = d_entropy.has_value() ? row_values(*d_entropy, x, rows, "d_entropy", &h_stride) : nullptr;
-  TORCH_CHECK(h == nullptr || entropy.has_value(), "the entropy gradient needs the entropy of the forward pass");
   const c10::cuda::CUDAGuard guard(x.device());
-  vocab_gemm_grad(x.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.scalar_type() == torch::kInt64, checked_pairs(lse, x, rows),
-                  h != nullptr ? contiguous_f32(*entropy, x, rows, "entropy") : nullptr, g, g_stride, h, h_stride, grad.data_ptr(), (int)rows, (int)V, (int)x.size(1),
-                  x.stride(0), w.stride(0), grad.stride(0), (float)logit_scale, ignore_index, st, stream_of(x));
+  const int64_t rows = x.size(0), H = x.size(1), V = w.size(0), slices = (V + kVocabSlice - 1) / kVocabSlice;
+  const bool labels64 = labels.scalar_type() == torch::kInt64;
+  const cudaStream_t stream = stream_of(x);
+  Tensor log_probs = empty_f32(rows, x), lse = empty_pairs(rows, x), entropy = want_entropy ? empty_f32(rows, x) : Tensor();
+  float* ent = want_entropy ? entropy.data_ptr<float>() : nullptr;
+  const bool compact = rows > kCompactAbove;
+  Tensor map = torch::empty({compact ? 2 * rows + 1 : 0}, x.options().dtype(torch::kInt32)), xc = x;
+  if (rows == 0) return {log_probs, entropy, lse, xc, map};
+  if (compact) {
+    int* m = map.data_ptr<int>();
+    vocab_live_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, m, m + rows, m + 2 * rows, log_probs.data_ptr<float>(), ent, pairs(lse), stream);
+    xc = torch::empty({rows, H}, x.options());
+    vocab_gather_rows(x.data_ptr(), x.stride(0), m, m + 2 * rows, xc.data_ptr(), (int)rows, (int)H, stream);
+  }
+  const int64_t most = stats_rows(rows, slices);
+  Tensor stats = empty_f32(most * slices * 4, x);
+  for (int64_t r = 0; r < rows; r += most) {
+    const LiveRows live = live_rows(map, rows, r, std::min(most, rows - r));
+    vocab_gemm_stats(row_ptr(xc, r), w.data_ptr(), labels.data_ptr(), labels64, stats.data_ptr<float>(), want_entropy, live, (int)V, (int)H, xc.stride(0), w.stride(0),
+                     (float)logit_scale, st, stream);
+    token_log_probs_join(stats.data_ptr<float>(), (int)slices, kVocabSlice, labels.data_ptr(), labels64, log_probs.data_ptr<float>(), ent, pairs(lse), live, (int)V,
+                         (float)logit_scale, ignore_index, stream);
+  }
+  return {log_probs, entropy, lse, xc, map};
+}
+
+// grad[n, V] (bf16, row stride a multiple of 8) <- gradient of the logits of rows [base, base + n) of xc
+void linear_log_probs_grad(const Tensor& xc, const Tensor& w, const Tensor& labels, const Tensor& lse, const OptTensor& entropy, const Tensor& d_log_probs,
+                           const OptTensor& d_entropy, const Tensor& map, int64_t base, Tensor& grad, double logit_scale, int64_t ignore_index, const Tensor& status) {
+  check_linear(xc, w, labels);
+  int* st = status_of(status, xc);
+  const int64_t rows = xc.size(0), V = w.size(0), n = grad.size(0);
+  check_device(grad, xc, "grad");
+  TORCH_CHECK(grad.scalar_type() == torch::kBFloat16 && grad.dim() == 2 && grad.size(1) == V && grad.stride(1) == 1 && grad.stride(0) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0,
+              "grad must be bf16 [n, V] with 16-byte aligned rows");
+  TORCH_CHECK(base >= 0 && base + n <= rows, "rows out of range");
+  long long g_stride = 0, h_stride = 0;
+  const float* g = row_values(d_log_probs, xc, rows, "d_log_probs", &g_stride);
+  const float* h = d_entropy.has_value() ? row_values(*d_entropy, xc, rows, "d_entropy", &h_stride) : nullptr;
+  TORCH_CHECK(h == nullptr || entropy.has_value(), "the entropy gradient needs the entropy of the forward pass");
+  const c10::cuda::CUDAGuard guard(xc.device());
+  vocab_gemm_grad(row_ptr(xc, base), w.data_ptr(), labels.data_ptr(), labels.scalar_type() == torch::kInt64, checked_pairs(lse, xc, rows),
+                  h != nullptr ? contiguous_f32(*entropy, xc, rows, "entropy") : nullptr, g, g_stride, h, h_stride, grad.data_ptr(), live_rows(map, rows, base, n), (int)V,
+                  (int)xc.size(1), xc.stride(0), w.stride(0), grad.stride(0), (float)logit_scale, ignore_index, st, stream_of(xc));
+}
+
+// out = a b for the live rows of a compacted batch, which are a's rows (data gradient, bf16 out) ...
+void linear_log_probs_dgrad(const Tensor& dlogits, const Tensor& w, Tensor& out, const Tensor& map, int64_t base, const Tensor& status) {
+  const int64_t n = dlogits.size(0), V = w.size(0), H = w.size(1), T = (map.numel() - 1) / 2;
+  check_device(w, dlogits, "weight");
+  check_device(out, dlogits, "out");
+  TORCH_CHECK(dlogits.dim() == 2 && w.dim() == 2 && out.dim() == 2 && dlogits.size(1) == V && out.size(0) == n && out.size(1) == H && dlogits.stride(1) == 1 && w.stride(1) == 1 && out.stride(1) == 1,
+              "dgrad: shape mismatch");
+  TORCH_CHECK(dlogits.scalar_type() == torch::kBFloat16 && w.scalar_type() == torch::kBFloat16 && out.scalar_type() == torch::kBFloat16, "dgrad: bf16 operands are needed");
+  int* st = status_of(status, dlogits);
+  const c10::cuda::CUDAGuard guard(dlogits.device());
+  gemm_bf16_2sm_live(dlogits.data_ptr(), w.data_ptr(), out.data_ptr(), (int)n, (int)H, (int)V, dlogits.stride(0), w.stride(0), out.stride(0), false, true, false,
+                     live_rows(map, T, base, n).count, (int)base, false, st, stream_of(dlogits));
+}
+
+// ... or the rows both are contracted over (weight gradient; fp32 out is added to)
+void linear_log_probs_wgrad(const Tensor& dlogits, const Tensor& xc, Tensor& out, const Tensor& map, int64_t base, const Tensor& status) {
+  const int64_t n = dlogits.size(0), V = dlogits.size(1), H = xc.size(1), T = (map.numel() - 1) / 2;
+  check_device(xc, dlogits, "hidden states");
+  check_device(out, dlogits, "out");
+  TORCH_CHECK(dlogits.dim() == 2 && xc.dim() == 2 && out.dim() == 2 && xc.size(0) == n && out.size(0) == V && out.size(1) == H && dlogits.stride(1) == 1 && xc.stride(1) == 1 && out.stride(1) == 1,
+              "wgrad: shape mismatch");
+  TORCH_CHECK(dlogits.scalar_type() == torch::kBFloat16 && xc.scalar_type() == torch::kBFloat16 && (out.scalar_type() == torch::kBFloat16 || out.scalar_type() == torch::kFloat32),
+              "wgrad: bf16 operands and a bf16 or fp32 output are needed");
+  int* st = status_of(status, dlogits);
+  const c10::cuda::CUDAGuard guard(dlogits.device());
+  gemm_bf16_2sm_live(dlogits.data_ptr(), xc.data_ptr(), out.data_ptr(), (int)V, (int)H, (int)n, dlogits.stride(0), xc.stride(0), out.stride(0), true, true,
+                     out.scalar_type() == torch::kFloat32, live_rows(map, T, base, n).count, (int)base, true, st, stream_of(dlogits));
+}
+
+// dx[T, H] from the gradient of the compacted rows
+Tensor linear_log_probs_scatter(const Tensor& compact, const Tensor& map) {
+  const int64_t T = (map.numel() - 1) / 2;
+  TORCH_CHECK(compact.is_cuda() && compact.is_contiguous() && compact.scalar_type() == torch::kBFloat16 && compact.dim() == 2 && compact.size(0) == T && compact.size(1) % 8 == 0,
+              "the compacted gradient must be contiguous bf16 [T, H]");
+  check_device(map, compact, "row map");
+  const c10::cuda::CUDAGuard guard(compact.device());
+  Tensor out = torch::empty_like(compact);
+  vocab_scatter_rows(compact.data_ptr(), live_rows(map, T, 0, T).index + T, out.data_ptr(), (int)T, (int)compact.size(1), stream_of(compact));
+  return out;
 }
 
 // ------------------------------------------------------------------------- losses over sequences
@@ -441,11 +505,13 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     ctx->save_for_backward({slope, log_probs, cu.value_or(Tensor()), mask.value_or(Tensor())});
     ctx->saved_data["length"] = length;
     ctx->mark_non_differentiable({chosen, rejected});
+    ctx->set_materialize_grads(false);
     return {loss, chosen, rejected};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     variable_list out(11);
+    if (!grads[0].defined()) return out;
     out[0] = once(preference_bwd(saved[0], grads[0], saved[1], optional(saved[2]), ctx->saved_data["length"].toInt(), optional(saved[3])), "preference_loss");
     return out;
   }
@@ -474,11 +540,13 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     ctx->saved_data["sequences"] = sequences;
     ctx->saved_data["reduction"] = reduction;
     ctx->mark_non_differentiable({kl, clipped});
+    ctx->set_materialize_grads(false);
     return {loss, kl, clipped};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     variable_list out(15);
+    if (!grads[0].defined()) return out;
     out[0] = once(policy_bwd(saved[0], saved[1], saved[2], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[3]), ctx->saved_data["length"].toInt(),
                              ctx->saved_data["sequences"].toInt(), optional(saved[4]), ctx->saved_data["reduction"].toInt()),
                   "policy_loss");
@@ -518,11 +586,13 @@ struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
     Tensor out = embedding_lookup_(weight, ids, scale, status);
     ctx->save_for_backward({weight, ids});
     ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor& weight = saved[0];
+    if (!grads[0].defined()) return variable_list(4);
     const OptTensor target = main_grad(weight);
     Tensor dw = embedding_gradient_(grads[0].contiguous(), saved[1], weight.size(0), target, ctx->saved_data["scale"].toDouble());
     return {target.has_value() ? Tensor() : once(dw, "embedding_sorted"), Tensor(), Tensor(), Tensor()};
@@ -542,6 +612,9 @@ void register_vocabulary(pybind11::module_& m) {
   m.def("token_log_probs", &token_log_probs, "log-probabilities of given tokens (and entropies) under rows of logits");
   m.def("linear_log_probs_fwd", &linear_log_probs_fwd, "the same from hidden states and the output weight, with the rows' log-sum-exps");
   m.def("linear_log_probs_grad", &linear_log_probs_grad, "gradient of the logits, formed again from hidden states and weight");
+  m.def("linear_log_probs_dgrad", &linear_log_probs_dgrad);
+  m.def("linear_log_probs_wgrad", &linear_log_probs_wgrad);
+  m.def("linear_log_probs_scatter", &linear_log_probs_scatter);
   m.def("preference_loss", &preference_loss, "loss over pairs of answers: (loss, chosen rewards, rejected rewards)");
   m.def("policy_loss", &policy_loss, "clipped policy loss with a KL term: (loss, KL estimate, clipped share)");
   m.def("embedding_sorted", &embedding_sorted, "embedding whose gradient is summed in sorted token order");

@@ -87,55 +87,64 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: 
 
 # ----------------------------------------------------------------------------- from hidden states
 class _FusedLinearTokenLogProbsFn(torch.autograd.Function):
-    """Forward keeps 16 bytes per row and 256 columns of logits; backward forms the logits again, chunk of rows by chunk, as
-    their bf16 gradient, and multiplies that with the weight and the hidden states."""
+    """Forward keeps 16 bytes per row and 128 columns of logits; backward forms the logits again, chunk of rows by chunk, as
+    their bf16 gradient, and multiplies that with the weight and the hidden states. Batches of more than 256 rows are compacted to the rows whose
+    label counts; their number stays on the device (``row_map``), and all four products end at it."""
 
     @staticmethod
     def forward(ctx, x, weight, labels, logit_scale, ignore_index, return_entropy):
         ctx.set_materialize_grads(False)
         with site("loss.lm_head.log_probs"):
-            log_probs, entropy, lse = native().linear_log_probs_fwd(x, weight, labels, logit_scale, ignore_index, return_entropy, status_word(x.device))
-        ctx.save_for_backward(x, weight, labels, lse, entropy)
+            log_probs, entropy, lse, xc, row_map = native().linear_log_probs_fwd(x, weight, labels, logit_scale, ignore_index, return_entropy, status_word(x.device))
+        ctx.save_for_backward(xc, weight, labels, lse, entropy, row_map)
         ctx.args = (logit_scale, ignore_index)
         return (log_probs, entropy) if return_entropy else log_probs
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_log_probs, d_entropy=None):
-        x, weight, labels, lse, entropy = ctx.saved_tensors
+        xc, weight, labels, lse, entropy, row_map = ctx.saved_tensors
         if d_log_probs is None and d_entropy is None:
             return (None,) * 6
-        C, st = native(), status_word(x.device)
-        T, H = x.shape
+        C, st = native(), status_word(xc.device)
+        T, H = xc.shape
         V = weight.shape[0]
+        compact = row_map.numel() > 0
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         d_log_probs = _row_gradient(d_log_probs, T, lse)
-        rows = _flce_chunk_rows(T, V)
+        rows = max(_flce_chunk_rows(T, V), 1)
         target = _weight_grad_target(weight) if need_dw else None
-        dx = torch.empty_like(x) if need_dx else None
+        dx = torch.empty(T, H, device=xc.device, dtype=xc.dtype) if need_dx else None
         dw = None
         if need_dw:
             # one chunk writes the weight's gradient in its own type; several add up in fp32
             if target is not None:
                 dw = target.view(V, H)
-            elif rows == T and T > 0:
-                dw = torch.empty(V, H, device=x.device, dtype=weight.dtype)
+            elif rows == T:
+                dw = torch.empty(V, H, device=xc.device, dtype=weight.dtype)
             else:
-                dw = torch.zeros(V, H, device=x.device, dtype=torch.float32)
+                dw = torch.zeros(V, H, device=xc.device, dtype=torch.float32)
         pitch = (V + 7) // 8 * 8
-        dlogits = torch.empty(rows, pitch, device=x.device, dtype=torch.bfloat16)[:, :V]
-        for start in range(0, T, max(rows, 1)):
+        dlogits = torch.empty(min(rows, T), pitch, device=xc.device, dtype=torch.bfloat16)[:, :V]
+        for start in range(0, T, rows):
             part = slice(start, min(start + rows, T))
-            dl, xc = dlogits[: part.stop - start], x[part]
+            dl = dlogits[: part.stop - start]
             with site("loss.lm_head.dlogits"):
-                C.linear_log_probs_grad(xc, weight, labels[part], lse[part], None if entropy is None else entropy[part], d_log_probs[part],
-                                        None if d_entropy is None else d_entropy[part], dl, *ctx.args, st)
+                C.linear_log_probs_grad(xc, weight, labels, lse, entropy, d_log_probs, d_entropy, row_map, start, dl, *ctx.args, st)
             if need_dx:
                 with site("loss.lm_head.dgrad"):
-                    C.gemm(dl, weight, dx[part], False, True, False, 1.0, st, 0)
+                    if compact:
+                        C.linear_log_probs_dgrad(dl, weight, dx[part], row_map, start, st)
+                    else:
+                        C.gemm(dl, weight, dx[part], False, True, False, 1.0, st, 0)
             if need_dw:
                 with site("loss.lm_head.wgrad"):
-                    C.gemm(dl, xc, dw, True, True, dw.dtype == torch.float32, 1.0, st, 0)
+                    if compact:
+                        C.linear_log_probs_wgrad(dl, xc[part], dw, row_map, start, st)
+                    else:
+                        C.gemm(dl, xc[part], dw, True, True, dw.dtype == torch.float32, 1.0, st, 0)
+        if need_dx and compact:
+            dx = C.linear_log_probs_scatter(dx, row_map)
         if target is not None:
             dw = None
         elif dw is not None:

@@ -213,6 +213,27 @@ def test_fused_linear_token_log_probs_in_chunks_and_into_main_grad(monkeypatch):
     _check_linear(x, w, labels, g, zero, lp.detach(), None, x.grad, w.main_grad - 2.0)
 
 
+@pytest.mark.parametrize("kept", [0.0, 0.01, 0.5])
+@pytest.mark.parametrize("chunk", [128, 384, 4096])
+def test_fused_linear_token_log_probs_leaves_ignored_rows_out(kept, chunk, monkeypatch):
+    import lm_engine.ops.vocabulary as vocabulary
+
+    monkeypatch.setattr(vocabulary, "_flce_chunk_rows", lambda T, V: min(T, chunk))
+    x, w, labels, g, h = _linear_case(1000, 64, 333, 8)
+    labels[torch.rand(1000, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) >= kept] = -100
+    x[labels == -100] = math.nan  # not looked at
+    junk = torch.full((64 << 20,), math.nan, device="cuda")  # what the allocator hands out next holds NaN
+    del junk
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    lp, ent = ops.fused_linear_token_log_probs(x, w, labels, return_entropy=True)
+    dx, dw = torch.autograd.grad((lp, ent), (x, w), (g, h))
+    assert (lp[labels == -100] == 0).all() and (ent[labels == -100] == 0).all() and (dx[labels == -100] == 0).all()
+    with torch.no_grad():
+        x[labels == -100] = 0
+    _check_linear(x, w, labels, g, h, lp, ent, dx, dw)
+
+
 def test_fused_linear_token_log_probs_strided_operands_and_shapes():
     x, w, labels, g, h = _linear_case(24, 64, 300, 6)
     wide = torch.zeros(24, 96, device="cuda", dtype=torch.bfloat16)
