@@ -2,12 +2,12 @@
 //   dW[v] = scale * sum over t with id_t = v, in ascending t, of dout[t]
 //
 // The gradient sorts the pairs (id, t) as 64-bit keys, which are distinct, so the order is unique and every sum is taken in
-// the same order on every run; nothing is added atomically. Sorting: runs of 2048 keys in shared memory (bitonic), then
+// the same order on every run; nothing is added atomically. Sorting: runs of 512 keys in shared memory (bitonic), then
 // levels that merge 16 runs at a time by rank: a key's place is its place in its own run plus the number of smaller keys in
-// each of the 15 others (15 independent binary searches). Summing: a block takes 32 consecutive sorted tokens and a slab
-// of columns and reads each dout row once; a run of equal ids inside of the block's tokens goes straight to its row of dW, a run
-// that crosses the border to the next 32 leaves fp32 partial sums, which a last kernel joins in order. Sums are fp32 and are
-// rounded once, when a row of dW is written.
+// each of the 15 others (independent binary searches, 16 loads in flight). Summing: a block takes 8 to 128 consecutive sorted
+// tokens (a chunk) and a slab of columns and reads each dout row once; a run of equal ids inside of the chunk goes straight to its row of
+// dW, a run that crosses the border to the next chunk leaves fp32 partial sums, which a last kernel joins in order. Sums
+// are fp32 and are rounded once, when a row of dW is written.
 //
 // Bound by HBM: dout is read once, the rows of dW are written once (read and written when they are accumulated into).
 #include <cuda_fp16.h>
@@ -20,9 +20,9 @@ namespace b200 {
 
 namespace {
 
-constexpr int RUN = 2048;        // keys sorted by one block
-constexpr int FAN = 16;          // runs merged per level
-constexpr int TOKENS = 32;       // sorted tokens summed by one block
+constexpr int LOG_RUN = 9, RUN = 1 << LOG_RUN;  // keys sorted by one block
+constexpr int LOG_FAN = 4, FAN = 1 << LOG_FAN;  // runs merged per level
+constexpr int MAX_CHUNK = 128;   // sorted tokens summed by one block, at most
 constexpr int SUM_THREADS = 128;
 constexpr uint64_t kNoKey = ~0ull;
 constexpr uint32_t kNoId = 0x7fffffffu;  // ids outside of the table, sorted behind all others
@@ -151,26 +151,29 @@ __global__ void __launch_bounds__(RUN / 2)
 }
 
 // One level: groups of FAN sorted runs of `length` keys (a power of two; the last run may be short) become one sorted run each.
-__global__ void __launch_bounds__(256) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, long long T, long long length) {
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+__global__ void __launch_bounds__(128) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int T, int log_length) {
+  const int i = blockIdx.x * 128 + threadIdx.x;
   if (i >= T) return;
   const uint64_t key = in[i];
-  const long long run = i / length, group = run / FAN;
-  const long long first = group * FAN;
-  long long below[FAN];
+  const int first = (i >> log_length) / FAN * FAN;          // first run of the group
+  const int begin = first << log_length;
+  int pos[FAN], end[FAN];                                  // pos: keys before it, in its run, are smaller
 #pragma unroll
-  for (int r = 0; r < FAN; ++r) below[r] = 0;
-  for (long long step = length; step > 0; step >>= 1) {
-#pragma unroll
-    for (int r = 0; r < FAN; ++r) {
-      const long long begin = (first + r) * length;
-      const long long n = min(length, T - begin);  // negative behind the last run
-      if (below[r] + step <= n && in[begin + below[r] + step - 1] < key) below[r] += step;
-    }
+  for (int r = 0; r < FAN; ++r) {
+    const long long b = ((long long)(first + r)) << log_length;
+    pos[r] = (int)min((long long)T, b);
+    end[r] = (int)min((long long)T, b + (1LL << log_length));
   }
-  long long place = first * length;  // a run counts its own smaller keys the same way
+  int place = begin;
 #pragma unroll
-  for (int r = 0; r < FAN; ++r) place += below[r];
+  for (int r = 0; r < FAN; ++r) place -= pos[r];
+  for (int step = 1 << log_length; step > 0; step >>= 1) {
+#pragma unroll
+    for (int r = 0; r < FAN; ++r)
+      if (step <= end[r] - pos[r] && in[pos[r] + step - 1] < key) pos[r] += step;
+  }
+#pragma unroll
+  for (int r = 0; r < FAN; ++r) place += pos[r];
   out[place] = key;
 }
 
@@ -178,9 +181,15 @@ __global__ void __launch_bounds__(256) merge_runs_kernel(const uint64_t* __restr
 template <typename D, int N, bool ACC>
 __device__ __forceinline__ void write_row(D* dst, const float* acc, float scale) {
   if constexpr (ACC) {
+    constexpr int W = N >= 4 ? 4 : 1;
     float* d = reinterpret_cast<float*>(dst);
 #pragma unroll
-    for (int e = 0; e < N; ++e) d[e] += acc[e] * scale;
+    for (int e = 0; e < N; e += W) {
+      Pack<float, W> v = load_pack<float, W>(d + e);
+#pragma unroll
+      for (int k = 0; k < W; ++k) set_element<float, W>(v, k, element<float, W>(v, k) + acc[e + k] * scale);
+      *reinterpret_cast<Pack<float, W>*>(d + e) = v;
+    }
   } else {
     Pack<D, N> v;
 #pragma unroll
@@ -193,17 +202,17 @@ __device__ __forceinline__ void write_row(D* dst, const float* acc, float scale)
 template <typename T, typename D, int N, bool ACC>
 __global__ void __launch_bounds__(SUM_THREADS)
     sum_tokens_kernel(const T* __restrict__ dout, const uint64_t* __restrict__ keys, D* __restrict__ dweight, float* __restrict__ partials,
-                      long long tokens, int H, float scale) {
-  __shared__ uint64_t s[TOKENS + 2];
-  const long long chunk = blockIdx.x, base = chunk * TOKENS;
-  if (threadIdx.x < TOKENS + 2) {
-    const long long i = base + (int)threadIdx.x - 1;
-    s[threadIdx.x] = i >= 0 && i < tokens ? keys[i] : kNoKey;  // kNoKey's id is no key's
+                      long long tokens, int chunk_tokens, int H, float scale) {
+  __shared__ uint64_t s[MAX_CHUNK + 2];
+  const long long chunk = blockIdx.x, base = chunk * chunk_tokens;
+  for (int k = threadIdx.x; k < chunk_tokens + 2; k += SUM_THREADS) {
+    const long long i = base + k - 1;
+    s[k] = i >= 0 && i < tokens ? keys[i] : kNoKey;  // kNoKey's id is no key's
   }
   __syncthreads();
   const int c = (blockIdx.y * SUM_THREADS + threadIdx.x) * N;
   if (c >= H) return;
-  const int count = (int)min((long long)TOKENS, tokens - base);
+  const int count = (int)min((long long)chunk_tokens, tokens - base);
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
@@ -243,45 +252,68 @@ __global__ void __launch_bounds__(SUM_THREADS)
 }
 
 // Joins the partial sums of runs that cross chunk borders: the block of the chunk in which the run begins adds its head and the
-// parts of the following chunks, eight strided sums per column that are added in order.
-constexpr int JOIN_LANES = 8;
-constexpr int JOIN_COLUMNS = 32;
+// parts of the following chunks. Two threads share a column's parts, every other one each, and their sums are added in order.
+constexpr int JOIN_LANES = 2;
+constexpr int JOIN_COLUMNS = 128;
+constexpr int JOIN_THREADS = JOIN_LANES * JOIN_COLUMNS;
 
-template <typename D, bool ACC>
-__global__ void __launch_bounds__(JOIN_LANES * JOIN_COLUMNS)
-    join_runs_kernel(const uint64_t* __restrict__ keys, D* __restrict__ dweight, const float* __restrict__ partials, long long tokens, int H, float scale) {
-  __shared__ float s[JOIN_LANES][JOIN_COLUMNS];
-  const long long chunks = (tokens + TOKENS - 1) / TOKENS;
-  const int column = threadIdx.x % JOIN_COLUMNS, lane = threadIdx.x / JOIN_COLUMNS;
-  const int c = blockIdx.y * JOIN_COLUMNS + column;
-  for (long long chunk = blockIdx.x; chunk + 1 < chunks; chunk += gridDim.x) {
-    const long long next = (chunk + 1) * TOKENS;
-    const uint32_t id = key_id(keys[next - 1]);
-    if (id == kNoId || key_id(keys[next]) != id) continue;           // no run crosses this border
-    const long long first = chunk * TOKENS;
-    if (key_id(keys[first]) == id && first > 0 && key_id(keys[first - 1]) == id) continue;  // it began earlier
-    // last chunk of the run: the last key with this id
-    long long lo = next, hi = tokens;  // keys[lo] has the id; keys[hi] has not
-    while (hi - lo > 1) {
-      const long long mid = (lo + hi) / 2;
-      if (key_id(keys[mid]) == id) lo = mid;
-      else hi = mid;
-    }
-    const long long parts = lo / TOKENS - chunk;
-    float acc = 0.f;
-    if (c < H) {
-      for (long long k = lane; k < parts; k += JOIN_LANES) acc += partials[2 * (chunk + 1 + k) * H + c];
-    }
-    s[lane][column] = acc;
-    __syncthreads();
-    if (lane == 0 && c < H) {
-      float total = partials[(2 * chunk + 1) * H + c];
-#pragma unroll
-      for (int l = 0; l < JOIN_LANES; ++l) total += s[l][column];
-      write_row<D, 1, ACC>(dweight + (long long)id * H + c, &total, scale);
-    }
-    __syncthreads();
+template <typename D, int N, bool ACC>
+__global__ void __launch_bounds__(JOIN_THREADS)
+    join_runs_kernel(const uint64_t* __restrict__ keys, D* __restrict__ dweight, const float* __restrict__ partials, int tokens, int chunk_tokens, int H, float scale) {
+  __shared__ Pack<float, N> s[JOIN_COLUMNS];
+  const int chunks = (tokens + chunk_tokens - 1) / chunk_tokens, chunk = blockIdx.x;
+  const int first = chunk * chunk_tokens, next = first + chunk_tokens;  // next < tokens: the last chunk has no block
+  const uint32_t id = key_id(keys[next - 1]), after = key_id(keys[next]), here = key_id(keys[first]), before = first > 0 ? key_id(keys[first - 1]) : ~0u;
+  if (id == kNoId || after != id) return;          // no run crosses this border
+  if (here == id && before == id) return;          // it began in an earlier chunk
+  // chunks behind this one that the run fills to their last token, and one more in which it ends
+  int parts = 0;
+  for (;;) {
+    const long long c = (long long)chunk + 1 + parts + threadIdx.x;
+    const long long last = (c + 1) * chunk_tokens - 1;
+    const bool through = c < chunks && last + 1 < tokens && key_id(keys[last]) == id && key_id(keys[last + 1]) == id;
+    // runs are contiguous: the threads that see it pass through are the first ones
+    const int n = __syncthreads_count(through);
+    parts += n;
+    if (n < JOIN_THREADS) break;
   }
+  ++parts;
+  const int column = threadIdx.x % JOIN_COLUMNS, lane = threadIdx.x / JOIN_COLUMNS;
+  const int c = (blockIdx.y * JOIN_COLUMNS + column) * N;
+  float acc[N];
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = 0.f;
+  if (c < H) {
+    if (lane == 0) {
+      const Pack<float, N> v = load_pack<float, N>(partials + (2LL * chunk + 1) * H + c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] = element<float, N>(v, e);
+    }
+#pragma unroll 8
+    for (int k = lane; k < parts; k += JOIN_LANES) {
+      const Pack<float, N> v = load_pack<float, N>(partials + 2LL * (chunk + 1 + k) * H + c);
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += element<float, N>(v, e);
+    }
+  }
+  if (lane == 1) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) set_element<float, N>(s[column], e, acc[e]);
+  }
+  __syncthreads();
+  if (lane == 0 && c < H) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] += element<float, N>(s[column], e);
+    write_row<D, N, ACC>(dweight + (long long)id * H + c, acc, scale);
+  }
+}
+
+__global__ void __launch_bounds__(256) fill_zero_kernel(uint4* __restrict__ p, long long n, int tail) {
+  if (blockIdx.x == 0 && threadIdx.x < tail) reinterpret_cast<unsigned char*>(p + n)[threadIdx.x] = 0;
+  const long long base = (long long)blockIdx.x * 1024 + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (base + k * 256 < n) p[base + k * 256] = make_uint4(0, 0, 0, 0);
 }
 
 template <typename T>
@@ -301,22 +333,27 @@ void lookup(const void* weight, const void* ids, bool ids64, void* out, long lon
     embedding_lookup_kernel<T, 1><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64, reinterpret_cast<T*>(out), tokens, V, H, scale, status);
 }
 
-template <typename T, typename D, bool ACC>
+// Tokens of one chunk: as many as leave about four blocks per SM, at most 128 (fewer and longer chunks mean fewer partial sums; with
+// fewer blocks the chains of loads of a chunk are not covered). A rule on the sizes alone, so the order of additions is, too.
+int chunk_tokens(long long T, int H, int columns) {
+  const long long slabs = (H + columns - 1) / columns;
+  int n = 8;
+  while (n < MAX_CHUNK && (T + 2 * n - 1) / (2 * n) * slabs >= 592) n *= 2;
+  return n;
+}
+
+template <typename T, typename D, int N, bool ACC>
 void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials, long long tokens, int H, float scale, cudaStream_t stream) {
-  constexpr int N = 16 / sizeof(T);
-  const bool wide = wide_rows<T>(H, dout, ACC ? dout : dweight);
-  const int per_block = SUM_THREADS * (wide ? N : 1);
-  const long long chunks = (tokens + TOKENS - 1) / TOKENS;
-  const dim3 grid((unsigned)chunks, (unsigned)((H + per_block - 1) / per_block));
-  if (wide)
-    sum_tokens_kernel<T, D, N, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys, reinterpret_cast<D*>(dweight), partials, tokens, H, scale);
-  else
-    sum_tokens_kernel<T, D, 1, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys, reinterpret_cast<D*>(dweight), partials, tokens, H, scale);
+  const int columns = SUM_THREADS * N, n = chunk_tokens(tokens, H, columns);
+  const long long chunks = (tokens + n - 1) / n;
+  const dim3 grid((unsigned)chunks, (unsigned)((H + columns - 1) / columns));
+  sum_tokens_kernel<T, D, N, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys, reinterpret_cast<D*>(dweight), partials, tokens, n, H, scale);
   count_launch();
   check_cuda(cudaGetLastError(), "embedding gradient sum launch");
   if (chunks > 1) {
-    const dim3 join((unsigned)(chunks - 1 < 128 ? chunks - 1 : 128), (unsigned)((H + JOIN_COLUMNS - 1) / JOIN_COLUMNS));
-    join_runs_kernel<D, ACC><<<join, JOIN_LANES * JOIN_COLUMNS, 0, stream>>>(keys, reinterpret_cast<D*>(dweight), partials, tokens, H, scale);
+    constexpr int J = N == 1 ? 1 : 4;  // partial sums are fp32: 16 bytes are four columns
+    const dim3 join((unsigned)(chunks - 1), (unsigned)((H + J * JOIN_COLUMNS - 1) / (J * JOIN_COLUMNS)));
+    join_runs_kernel<D, J, ACC><<<join, JOIN_THREADS, 0, stream>>>(keys, reinterpret_cast<D*>(dweight), partials, (int)tokens, n, H, scale);
     count_launch();
     check_cuda(cudaGetLastError(), "embedding gradient join launch");
   }
@@ -324,8 +361,15 @@ void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials
 
 template <typename T>
 void gradient(const void* dout, const uint64_t* keys, void* dweight, bool accumulate, float* partials, long long tokens, int H, float scale, cudaStream_t stream) {
-  if (accumulate) sums<T, float, true>(dout, keys, dweight, partials, tokens, H, scale, stream);
-  else sums<T, T, false>(dout, keys, dweight, partials, tokens, H, scale, stream);
+  constexpr int N = 16 / sizeof(T);
+  const bool wide = wide_rows<T>(H, dout, dweight);
+  if (accumulate) {
+    if (wide) sums<T, float, N, true>(dout, keys, dweight, partials, tokens, H, scale, stream);
+    else sums<T, float, 1, true>(dout, keys, dweight, partials, tokens, H, scale, stream);
+  } else {
+    if (wide) sums<T, T, N, false>(dout, keys, dweight, partials, tokens, H, scale, stream);
+    else sums<T, T, 1, false>(dout, keys, dweight, partials, tokens, H, scale, stream);
+  }
 }
 
 long long key_bytes(long long T) { return (T * 8 + 255) / 256 * 256; }
@@ -341,8 +385,18 @@ void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids
   check_cuda(cudaGetLastError(), "embedding lookup launch");
 }
 
-long long embedding_gradient_workspace(long long T, int H) {
-  const long long chunks = (T + TOKENS - 1) / TOKENS;
+void embedding_zero(void* p, long long bytes, cudaStream_t stream) {
+  if (bytes == 0) return;
+  const long long n = bytes / 16;
+  fill_zero_kernel<<<(unsigned)(n / 1024 + 1), 256, 0, stream>>>(reinterpret_cast<uint4*>(p), n, (int)(bytes % 16));
+  count_launch();
+  check_cuda(cudaGetLastError(), "embedding gradient fill launch");
+}
+
+long long embedding_gradient_workspace(long long T, int H, Scalar type) {
+  const int columns = SUM_THREADS * (type == Scalar::kF32 ? 4 : 8);  // narrower slabs never make more chunks
+  const int n = chunk_tokens(T, H, columns);
+  const long long chunks = (T + n - 1) / n;
   return 2 * key_bytes(T) + (chunks > 1 ? 2 * chunks * H * 4 : 0);
 }
 
@@ -357,8 +411,8 @@ void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids
   sort_runs_kernel<<<(unsigned)((T + RUN - 1) / RUN), threads, 0, stream>>>(ids, ids64, keys, T, V);
   count_launch();
   check_cuda(cudaGetLastError(), "embedding gradient sort launch");
-  for (long long length = RUN; length < T; length *= FAN) {
-    merge_runs_kernel<<<(unsigned)((T + 255) / 256), 256, 0, stream>>>(keys, other, T, length);
+  for (int log_length = LOG_RUN; (1LL << log_length) < T; log_length += LOG_FAN) {
+    merge_runs_kernel<<<(unsigned)((T + 127) / 128), 128, 0, stream>>>(keys, other, (int)T, log_length);
     count_launch();
     check_cuda(cudaGetLastError(), "embedding gradient merge launch");
     uint64_t* t = keys;

@@ -363,7 +363,7 @@ Tensor embedding_lookup_(const Tensor& weight, const Tensor& ids, double scale, 
   TORCH_CHECK(weight.is_cuda() && weight.dim() == 2 && weight.is_contiguous(), "weight must be a contiguous [V, H] CUDA tensor");
   const Scalar type = scalar_of(weight, "weight");
   check_indices(ids, weight, "ids");
-  TORCH_CHECK(ids.numel() < (1LL << 31) && weight.size(1) < (1 << 30), "sizes out of range");
+  TORCH_CHECK(ids.numel() <= (1LL << 30) && weight.size(1) < (1 << 30), "sizes out of range");
   int* st = status_of(status, weight);
   const c10::cuda::CUDAGuard guard(weight.device());
   auto shape = ids.sizes().vec();
@@ -380,16 +380,17 @@ Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, con
   const Scalar type = scalar_of(dout, "dout");
   check_indices(ids, dout, "ids");
   const int64_t T = ids.numel(), H = dout.size(-1);
-  TORCH_CHECK(dout.numel() == T * H && T < (1LL << 31) && H < (1 << 30) && V >= 0 && V < (1LL << 31) - 1, "dout must be [T, H] for T ids; at most 2^31 - 2 rows");
+  TORCH_CHECK(dout.numel() == T * H && T <= (1LL << 30) && H < (1 << 30) && V >= 0 && V < (1LL << 31) - 1, "dout must be [T, H] for T ids; at most 2^30 tokens and 2^31 - 2 rows");
   const c10::cuda::CUDAGuard guard(dout.device());
   Tensor dw;
   if (dweight.has_value()) {
     dw = *dweight;
     contiguous_f32(dw, dout, V * H, "dweight");
   } else {
-    dw = torch::zeros({V, H}, dout.options());
+    dw = torch::empty({V, H}, dout.options());
+    embedding_zero(dw.data_ptr(), V * H * dw.element_size(), stream_of(dout));
   }
-  Tensor workspace = torch::empty({embedding_gradient_workspace(T, (int)H)}, dout.options().dtype(torch::kUInt8));
+  Tensor workspace = torch::empty({embedding_gradient_workspace(T, (int)H, type)}, dout.options().dtype(torch::kUInt8));
   embedding_gradient(dout.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, dw.data_ptr(), dweight.has_value(), workspace.data_ptr(), T, V, (int)H, (float)scale,
                      stream_of(dout));
   return dw;
