@@ -203,11 +203,14 @@ template <typename T, typename D, int N, bool ACC>
 __global__ void __launch_bounds__(SUM_THREADS)
     sum_tokens_kernel(const T* __restrict__ dout, const uint64_t* __restrict__ keys, D* __restrict__ dweight, float* __restrict__ partials,
                       long long tokens, int chunk_tokens, int H, float scale) {
-  __shared__ uint64_t s[MAX_CHUNK + 2];
+  __shared__ uint32_t ids[MAX_CHUNK + 2], rows[MAX_CHUNK];
   const long long chunk = blockIdx.x, base = chunk * chunk_tokens;
   for (int k = threadIdx.x; k < chunk_tokens + 2; k += SUM_THREADS) {
     const long long i = base + k - 1;
-    s[k] = i >= 0 && i < tokens ? keys[i] : kNoKey;  // kNoKey's id is no key's
+    const uint64_t key = i >= 0 && i < tokens ? keys[i] : kNoKey;  // kNoKey's id is no key's
+    ids[k] = key_id(key);
+    // places without a token read row 0, so that a batch of loads has no condition in it and stays in flight together
+    if (k > 0 && k <= chunk_tokens) rows[k - 1] = key == kNoKey ? 0u : (uint32_t)key;
   }
   __syncthreads();
   const int c = (blockIdx.y * SUM_THREADS + threadIdx.x) * N;
@@ -216,24 +219,20 @@ __global__ void __launch_bounds__(SUM_THREADS)
   float acc[N];
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = 0.f;
-  bool from_before = key_id(s[0]) == key_id(s[1]);
-  constexpr int UNROLL = 8;
+  bool from_before = ids[0] == ids[1];
+  constexpr int UNROLL = 8;  // divides every chunk size
   for (int i0 = 0; i0 < count; i0 += UNROLL) {
     Pack<T, N> v[UNROLL];
 #pragma unroll
-    for (int k = 0; k < UNROLL; ++k) {
-      const int i = i0 + k;
-      if (i < count && key_id(s[1 + i]) != kNoId) v[k] = load_pack<T, N>(dout + (long long)(uint32_t)s[1 + i] * H + c);
-    }
+    for (int k = 0; k < UNROLL; ++k) v[k] = load_pack<T, N>(dout + (long long)rows[i0 + k] * H + c);
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       const int i = i0 + k;
-      if (i >= count) break;
-      const uint32_t id = key_id(s[1 + i]);
-      if (id == kNoId) break;
+      const uint32_t id = ids[1 + i];
+      if (i >= count || id == kNoId) break;
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[e] += element<T, N>(v[k], e);
-      const bool ends = key_id(s[2 + i]) != id;
+      const bool ends = ids[2 + i] != id;
       if (ends || i == count - 1) {
         if (ends && !from_before) {
           write_row<D, N, ACC>(dweight + (long long)id * H + c, acc, scale);
@@ -252,15 +251,15 @@ __global__ void __launch_bounds__(SUM_THREADS)
 }
 
 // Joins the partial sums of runs that cross chunk borders: the block of the chunk in which the run begins adds its head and the
-// parts of the following chunks. Two threads share a column's parts, every other one each, and their sums are added in order.
-constexpr int JOIN_LANES = 2;
-constexpr int JOIN_COLUMNS = 128;
+// parts of the following chunks. Four threads share a column's parts, every fourth one each, and their sums are added in order.
+constexpr int JOIN_LANES = 4;
+constexpr int JOIN_COLUMNS = 64;
 constexpr int JOIN_THREADS = JOIN_LANES * JOIN_COLUMNS;
 
 template <typename D, int N, bool ACC>
 __global__ void __launch_bounds__(JOIN_THREADS)
     join_runs_kernel(const uint64_t* __restrict__ keys, D* __restrict__ dweight, const float* __restrict__ partials, int tokens, int chunk_tokens, int H, float scale) {
-  __shared__ Pack<float, N> s[JOIN_COLUMNS];
+  __shared__ Pack<float, N> s[JOIN_LANES][JOIN_COLUMNS];
   const int chunks = (tokens + chunk_tokens - 1) / chunk_tokens, chunk = blockIdx.x;
   const int first = chunk * chunk_tokens, next = first + chunk_tokens;  // next < tokens: the last chunk has no block
   const uint32_t id = key_id(keys[next - 1]), after = key_id(keys[next]), here = key_id(keys[first]), before = first > 0 ? key_id(keys[first - 1]) : ~0u;
@@ -296,14 +295,14 @@ __global__ void __launch_bounds__(JOIN_THREADS)
       for (int e = 0; e < N; ++e) acc[e] += element<float, N>(v, e);
     }
   }
-  if (lane == 1) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) set_element<float, N>(s[column], e, acc[e]);
-  }
+  for (int e = 0; e < N; ++e) set_element<float, N>(s[lane][column], e, acc[e]);
   __syncthreads();
   if (lane == 0 && c < H) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) acc[e] += element<float, N>(s[column], e);
+    for (int l = 1; l < JOIN_LANES; ++l)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += element<float, N>(s[l][column], e);
     write_row<D, N, ACC>(dweight + (long long)id * H + c, acc, scale);
   }
 }
