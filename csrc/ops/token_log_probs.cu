@@ -16,6 +16,7 @@
 // whatever they hold.
 #include <cuda_fp16.h>
 
+#include "../common/cta_pair.cuh"
 #include "../common/launch.h"
 #include "../common/ptx.cuh"
 #include "softmax_stats.cuh"
@@ -158,7 +159,7 @@ struct Row {
   }
 };
 
-constexpr int FWD_THREADS = 512;
+constexpr int FWD_THREADS = 256;  // four blocks on an SM: 174 -> 159 us at 4096 x 128256 bf16 against two blocks of 512
 constexpr int FWD_UNROLL = 4;
 
 // COUNT vectors of a thread at once; one comparison of their common maximum with the running one decides about rescaling.
@@ -178,9 +179,8 @@ __device__ __forceinline__ void accumulate_vectors(Stats& st, const uint4 (&v)[C
 // The wide vectors of a row in groups of four per thread whose loads have no condition between them (the compiler keeps loads
 // behind a branch in order, one in flight: 222 instead of 150 us at 4096 x 128256 bf16).
 template <typename T, bool ENTROPY, bool ALIGNED>
-__device__ __forceinline__ void accumulate_wide(Stats& st, const Row<T>& r, float scale2) {
-  const int end = r.end_wide();
-  int i = r.first_wide() + threadIdx.x;
+__device__ __forceinline__ void accumulate_wide(Stats& st, const Row<T>& r, int first, int end, float scale2) {
+  int i = first + threadIdx.x;
   for (; i + (FWD_UNROLL - 1) * FWD_THREADS < end; i += FWD_UNROLL * FWD_THREADS) {
     uint4 v[FWD_UNROLL];
 #pragma unroll
@@ -193,16 +193,19 @@ __device__ __forceinline__ void accumulate_wide(Stats& st, const Row<T>& r, floa
   }
 }
 
-template <typename T, bool ENTROPY>
-__global__ void __launch_bounds__(FWD_THREADS)
+// CLUSTER blocks share a row.
+template <typename T, bool ENTROPY, int CLUSTER>
+__global__ void __launch_bounds__(FWD_THREADS, 1024 / FWD_THREADS)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, const void* __restrict__ labels, bool labels64,
                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, int V,
                                RowMap map, float scale2, long long ignore_index) {
   __shared__ Stats red[FWD_THREADS / 32];
-  const long long row = blockIdx.x;
+  __shared__ Stats block_stats;
+  const long long row = blockIdx.x / CLUSTER;
+  const int rank = blockIdx.x % CLUSTER;
   const long long label = load_label(labels, labels64, row);
-  if (label == ignore_index || label < 0 || label >= V) {
-    if (threadIdx.x == 0) {
+  if (label == ignore_index || label < 0 || label >= V) {  // all blocks of the row leave
+    if (threadIdx.x == 0 && rank == 0) {
       log_probs[row] = 0.f;
       lse[row] = make_float2(0.f, 0.f);
       if (ENTROPY) entropy[row] = 0.f;
@@ -211,13 +214,15 @@ __global__ void __launch_bounds__(FWD_THREADS)
   }
   const Row<T> r(logits + row_offset(map, row), V);
   Stats st = empty_stats();
-  if (r.shift == 0) accumulate_wide<T, ENTROPY, true>(st, r, scale2);
-  else accumulate_wide<T, ENTROPY, false>(st, r, scale2);
+  const int before = r.first_wide(), behind = max(r.end_wide(), before);
+  const int share = (behind - before + CLUSTER - 1) / CLUSTER;
+  const int first = before + rank * share, end = min(behind, first + share);
+  if (r.shift == 0) accumulate_wide<T, ENTROPY, true>(st, r, first, end, scale2);
+  else accumulate_wide<T, ENTROPY, false>(st, r, first, end, scale2);
   // the (at most three) vectors at the ends of the row that are not wide, one thread each
-  const int before = r.first_wide(), narrow = before + max(0, r.vectors - max(r.end_wide(), before));
-  if (threadIdx.x < narrow) {
-    const int i = threadIdx.x < before ? threadIdx.x : max(r.end_wide(), before) + threadIdx.x - before;
-    const uint4 v[1] = {r.load_narrow(i)};
+  const int narrow = before + r.vectors - behind;
+  if (rank == 0 && threadIdx.x < narrow) {
+    const uint4 v[1] = {r.load_narrow(threadIdx.x < before ? threadIdx.x : behind + threadIdx.x - before)};
     accumulate_vectors<T, ENTROPY, 1>(st, v, scale2);
   }
 #pragma unroll
@@ -231,7 +236,26 @@ __global__ void __launch_bounds__(FWD_THREADS)
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = st;
   __syncthreads();
   if (threadIdx.x == 0) {
+#pragma unroll
     for (int w = 1; w < FWD_THREADS / 32; ++w) st = merge<ENTROPY>(st, red[w], scale2);
+    block_stats = st;
+  }
+  if (CLUSTER > 1) {
+    cluster_sync_all();
+    if (rank == 0 && threadIdx.x == 0) {
+#pragma unroll
+      for (int b = 1; b < CLUSTER; ++b) {
+        Stats other;
+        const uint32_t at = map_to_cta(smem_u32(&block_stats), b);
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.m) : "r"(at) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.s) : "r"(at + 4) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(other.u) : "r"(at + 8) : "memory");
+        st = merge<ENTROPY>(st, other, scale2);
+      }
+    }
+    cluster_sync_all();  // nobody leaves while its statistics are read
+  }
+  if (threadIdx.x == 0 && rank == 0) {
     const float log2_s = log2f(st.s);
     lse[row] = make_float2(st.m, log2_s);
     log_probs[row] = log2_prob(Vec<T>::load(r.p + label), make_float2(st.m, log2_s), scale2) * kLn2;
@@ -249,31 +273,33 @@ __global__ void __launch_bounds__(BWD_THREADS)
                                const float* __restrict__ d_log_probs, long long d_log_probs_stride,
                                const float* __restrict__ d_entropy, long long d_entropy_stride, T* __restrict__ grad, int V,
                                RowMap map, long long grad_stride, float logit_scale, float scale2,
-                               long long ignore_index) {
+                               long long ignore_index, unsigned chunks) {
   constexpr int N = Vec<T>::N;
   // last row first: the logits that the forward pass (or the model) touched last are still in L2
-  const long long row = (long long)gridDim.x - 1 - blockIdx.x;
+  // and the blocks of a row are consecutive: 4096 x 128256 354 -> 333 us (2.0 GB)
+  const unsigned chunk = blockIdx.x % chunks;
+  const long long row = gridDim.x / chunks - 1 - blockIdx.x / chunks;
   const long long label = load_label(labels, labels64, row);
   const bool ignored = label == ignore_index || label < 0 || label >= V;
   const Row<T> r(logits + row_offset(map, row), V);
   T* out = grad + row * grad_stride;
   const float g = ignored ? 0.f : d_log_probs[row * d_log_probs_stride];
   const float h = ignored || !ENTROPY ? 0.f : d_entropy[row * d_entropy_stride];
-  const int i0 = blockIdx.y * (BWD_THREADS * BWD_UNROLL) + threadIdx.x;
+  const int i0 = chunk * (BWD_THREADS * BWD_UNROLL) + threadIdx.x;
   // rows without an upstream gradient get zeros and are not read
   const bool zero = g == 0.f && h == 0.f;
   const float2 L = lse[row];
   const float H = ENTROPY ? entropy[row] : 0.f;
   const float gs = g * logit_scale, hs = h * logit_scale;
   uint4 v[BWD_UNROLL];
-  const int last = blockIdx.y * (BWD_THREADS * BWD_UNROLL) + BWD_THREADS * BWD_UNROLL;
+  const int last = chunk * (BWD_THREADS * BWD_UNROLL) + BWD_THREADS * BWD_UNROLL;
   if (zero) {
 #pragma unroll
     for (int k = 0; k < BWD_UNROLL; ++k) v[k] = make_uint4(0, 0, 0, 0);
   } else if (r.shift == 0 && last <= r.end_wide()) {
 #pragma unroll
     for (int k = 0; k < BWD_UNROLL; ++k) v[k] = r.template load_wide<true>(i0 + k * BWD_THREADS);
-  } else if (blockIdx.y > 0 && last <= r.end_wide()) {
+  } else if (chunk > 0 && last <= r.end_wide()) {
 #pragma unroll
     for (int k = 0; k < BWD_UNROLL; ++k) v[k] = r.template load_wide<false>(i0 + k * BWD_THREADS);
   } else {
@@ -370,10 +396,33 @@ template <typename T>
 void fwd(const void* logits, const void* labels, bool labels64, float* log_probs, float* entropy, float2* lse, long long rows,
          int V, RowMap map, float scale2, long long ignore_index, cudaStream_t stream) {
   const T* x = reinterpret_cast<const T*>(logits);
-  if (entropy != nullptr)
-    token_log_probs_fwd_kernel<T, true><<<(unsigned)rows, FWD_THREADS, 0, stream>>>(x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index);
-  else
-    token_log_probs_fwd_kernel<T, false><<<(unsigned)rows, FWD_THREADS, 0, stream>>>(x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index);
+  auto launch = [&](auto kernel, int cluster) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster), 1, 1);
+    cfg.blockDim = dim3(FWD_THREADS, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 1 : 0;
+    check_cuda(cudaLaunchKernelEx(&cfg, kernel, x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index), "token_log_probs forward launch");
+  };
+  // Blocks per row: more than one only while all of them run at once, four per SM, and each has a vector per thread. Few long rows
+  // gain (32 x 49152 bf16: 7.8 us with one block of 1024 threads, 6.6 with eight of 256); with more blocks than run at a time the
+  // two cluster barriers of a row cost more than the shorter last wave saves (1531 x 50001 fp32: 54 us with one, 61 with two).
+  const int vectors = V / Vec<T>::N;
+  int cluster = 1;
+  while (cluster < 8 && 2 * rows * cluster <= 4LL * sm_count() && vectors / (2 * cluster) >= FWD_THREADS) cluster *= 2;
+  const bool e = entropy != nullptr;
+  switch (cluster) {
+    case 1: e ? launch(token_log_probs_fwd_kernel<T, true, 1>, 1) : launch(token_log_probs_fwd_kernel<T, false, 1>, 1); break;
+    case 2: e ? launch(token_log_probs_fwd_kernel<T, true, 2>, 2) : launch(token_log_probs_fwd_kernel<T, false, 2>, 2); break;
+    case 4: e ? launch(token_log_probs_fwd_kernel<T, true, 4>, 4) : launch(token_log_probs_fwd_kernel<T, false, 4>, 4); break;
+    default: e ? launch(token_log_probs_fwd_kernel<T, true, 8>, 8) : launch(token_log_probs_fwd_kernel<T, false, 8>, 8); break;
+  }
 }
 
 template <typename T>
@@ -382,14 +431,15 @@ void bwd(const void* logits, const void* labels, bool labels64, const float2* ls
          RowMap map, long long grad_stride, float logit_scale, long long ignore_index, cudaStream_t stream) {
   const T* x = reinterpret_cast<const T*>(logits);
   const int vectors = (V + Vec<T>::N - 1) / Vec<T>::N;
-  const dim3 grid((unsigned)rows, (unsigned)((vectors + BWD_THREADS * BWD_UNROLL - 1) / (BWD_THREADS * BWD_UNROLL)));
+  const unsigned chunks = (unsigned)((vectors + BWD_THREADS * BWD_UNROLL - 1) / (BWD_THREADS * BWD_UNROLL));
+  const unsigned grid = (unsigned)rows * chunks;
   const float scale2 = logit_scale * kLog2e;
   if (d_entropy != nullptr)
     token_log_probs_bwd_kernel<T, true><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
-                                                                          reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index);
+                                                                          reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index, chunks);
   else
     token_log_probs_bwd_kernel<T, false><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
-                                                                           reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index);
+                                                                           reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index, chunks);
 }
 
 }  // namespace
