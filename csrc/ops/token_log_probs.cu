@@ -355,7 +355,8 @@ __global__ void __launch_bounds__(BWD_THREADS)
   }
 }
 
-// One block: 32 rows (one per lane) x 32 warps that share the slices; the warps' statistics meet in shared memory.
+// One block: 32 rows (one per lane) x 32 warps that share the slices, eight loads in flight each; then every warp takes one row
+// and its lanes join the 32 warps' statistics pairwise.
 template <bool ENTROPY>
 __global__ void __launch_bounds__(1024)
     token_log_probs_join_kernel(const float4* __restrict__ stats, int slices, int slice_width, const void* __restrict__ labels, bool labels64,
@@ -364,20 +365,33 @@ __global__ void __launch_bounds__(1024)
   __shared__ Stats red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = live.count == nullptr ? live.rows : min(live.rows, *live.count - live.base);
-  if ((long long)blockIdx.x * 32 >= rows) return;
-  const int r = blockIdx.x * 32 + lane;
+  const int r0 = blockIdx.x * 32;
+  if (r0 >= rows) return;
   Stats st = empty_stats();
-  if (r < rows) {
-#pragma unroll 4
-    for (int i = warp; i < slices; i += 32) {
-      const float4 v = stats[(long long)i * live.rows + r];
-      st = merge<ENTROPY>(st, Stats{v.x, v.y, v.z}, scale2);
-    }
+  const float4* column = stats + min(r0 + lane, rows - 1);  // lanes behind the last row repeat it
+  constexpr int BATCH = 8;
+  for (int i0 = warp; i0 < slices; i0 += 32 * BATCH) {
+    float4 v[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) v[k] = column[(long long)min(i0 + 32 * k, slices - 1) * live.rows];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k)
+      if (i0 + 32 * k < slices) st = merge<ENTROPY>(st, Stats{v[k].x, v[k].y, v[k].z}, scale2);
   }
   red[warp][lane] = st;
   __syncthreads();
-  if (warp != 0 || r >= rows) return;
-  for (int w = 1; w < 32; ++w) st = merge<ENTROPY>(st, red[w][lane], scale2);
+  const int r = r0 + warp;
+  if (r >= rows) return;
+  st = red[lane][warp];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats other;
+    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    other.u = ENTROPY ? __shfl_xor_sync(0xffffffffu, st.u, o) : 0.f;
+    st = merge<ENTROPY>(st, other, scale2);
+  }
+  if (lane != 0) return;
   const long long row = live.index != nullptr ? live.index[live.base + r] : live.base + r;
   const long long label = load_label(labels, labels64, row);
   if (label == ignore_index || label < 0 || label >= V) {
@@ -481,52 +495,64 @@ void token_log_probs_join(const float* stats, int slices, int slice_width, const
 // ------------------------------------------------------------------------- live rows of a batch
 namespace {
 
-// One block walks the labels 1024 at a time; a row's place is the number of live rows before it.
-__global__ void __launch_bounds__(1024)
-    live_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, int* __restrict__ index, int* __restrict__ slot, int* __restrict__ count,
-                     float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse) {
-  __shared__ int warp_sum[32];
+// A block takes 32 rows of the batch: it counts the live rows before them (all of the earlier labels, 8 bytes each, from L2), which gives
+// its rows their places, and copies the live ones there. The d-th row that does not count clears compact row T - 1 - d, so that
+// all rows behind the live ones are zeros.
+constexpr int COMPACT_ROWS = 32;
+constexpr int COMPACT_THREADS = 256;
+
+__global__ void __launch_bounds__(COMPACT_THREADS)
+    compact_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, const __nv_bfloat16* __restrict__ x, long long ldx, int H, int* __restrict__ index,
+                        int* __restrict__ slot, int* __restrict__ count, __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs, float* __restrict__ entropy,
+                        float2* __restrict__ lse) {
+  __shared__ int warp_count[COMPACT_THREADS / 32], place[COMPACT_ROWS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int before = 0;
-  for (int t0 = 0; t0 < T; t0 += 1024) {
-    const int t = t0 + threadIdx.x;
-    bool live = false;
-    if (t < T) {
-      const long long l = load_label(labels, labels64, t);
-      live = l != ignore_index && l >= 0 && l < V;
-    }
+  const int t0 = blockIdx.x * COMPACT_ROWS;
+  auto is_live = [&](int t) {
+    const long long l = load_label(labels, labels64, t);
+    return l != ignore_index && l >= 0 && l < V;
+  };
+  int n = 0;
+#pragma unroll 4
+  for (int t = threadIdx.x; t < t0; t += COMPACT_THREADS) n += is_live(t) ? 1 : 0;
+  n = __reduce_add_sync(0xffffffffu, n);
+  if (lane == 0) warp_count[warp] = n;
+  __syncthreads();
+  if (warp == 0) {
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < COMPACT_THREADS / 32; ++w) before += warp_count[w];
+    const int t = t0 + lane;
+    const bool live = t < T && is_live(t);
     const unsigned votes = __ballot_sync(0xffffffffu, live);
-    if (lane == 0) warp_sum[warp] = __popc(votes);
-    __syncthreads();
-    int lower = 0, all = 0;
-    for (int w = 0; w < 32; ++w) {
-      const int n = warp_sum[w];
-      lower += w < warp ? n : 0;
-      all += n;
-    }
-    __syncthreads();
-    const int place = before + lower + __popc(votes & ((1u << lane) - 1));
+    const int p = before + __popc(votes & ((1u << lane) - 1));  // live rows before t
     if (t < T) {
-      slot[t] = live ? place : -1;
+      slot[t] = live ? p : -1;
       if (live) {
-        index[place] = t;
+        index[p] = t;
       } else {
         log_probs[t] = 0.f;
         lse[t] = make_float2(0.f, 0.f);
         if (entropy != nullptr) entropy[t] = 0.f;
       }
+      if (t == T - 1) *count = p + (live ? 1 : 0);
     }
-    before += all;
+    place[lane] = live ? p : t < T ? -(T - 1 - (t - p)) - 1 : 0;
   }
-  if (threadIdx.x == 0) *count = before;
-}
-
-__global__ void __launch_bounds__(128)
-    gather_rows_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, const int* __restrict__ index, const int* __restrict__ count, __nv_bfloat16* __restrict__ compact, int H) {
-  const int r = blockIdx.x, n = *count;
-  uint4* dst = reinterpret_cast<uint4*>(compact + (long long)r * H);
-  const uint4* src = r < n ? reinterpret_cast<const uint4*>(x + (long long)index[r] * ldx) : nullptr;
-  for (int i = threadIdx.x; i < H / 8; i += blockDim.x) dst[i] = src != nullptr ? src[i] : make_uint4(0, 0, 0, 0);
+  __syncthreads();
+  // eight warps, a row each at a time
+  for (int k = warp; k < COMPACT_ROWS && t0 + k < T; k += COMPACT_THREADS / 32) {
+    const int p = place[k];
+    const bool live = p >= 0;
+    uint4* dst = reinterpret_cast<uint4*>(compact + (long long)(live ? p : -p - 1) * H);
+    const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(t0 + k) * ldx);
+    if (live) {
+#pragma unroll 4
+      for (int i = lane; i < H / 8; i += 32) dst[i] = src[i];
+    } else {
+      for (int i = lane; i < H / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
 }
 
 __global__ void __launch_bounds__(128) scatter_rows_kernel(const __nv_bfloat16* __restrict__ compact, const int* __restrict__ slot, __nv_bfloat16* __restrict__ out, int H) {
@@ -538,17 +564,12 @@ __global__ void __launch_bounds__(128) scatter_rows_kernel(const __nv_bfloat16* 
 
 }  // namespace
 
-void vocab_live_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, int* index, int* slot, int* count, float* log_probs, float* entropy, float2* lse,
-                     cudaStream_t stream) {
-  live_rows_kernel<<<1, 1024, 0, stream>>>(labels, labels64, ignore_index, T, V, index, slot, count, log_probs, entropy, lse);
+void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* slot, int* count, void* compact,
+                        float* log_probs, float* entropy, float2* lse, cudaStream_t stream) {
+  compact_rows_kernel<<<(T + COMPACT_ROWS - 1) / COMPACT_ROWS, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V, reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, index, slot,
+                                                                                             count, reinterpret_cast<__nv_bfloat16*>(compact), log_probs, entropy, lse);
   count_launch();
-  check_cuda(cudaGetLastError(), "live rows launch");
-}
-
-void vocab_gather_rows(const void* x, long long ldx, const int* index, const int* count, void* compact, int T, int H, cudaStream_t stream) {
-  gather_rows_kernel<<<T, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(x), ldx, index, count, reinterpret_cast<__nv_bfloat16*>(compact), H);
-  count_launch();
-  check_cuda(cudaGetLastError(), "gather rows launch");
+  check_cuda(cudaGetLastError(), "compact rows launch");
 }
 
 void vocab_scatter_rows(const void* compact, const int* slot, void* out, int T, int H, cudaStream_t stream) {

@@ -33,12 +33,10 @@ struct LiveRows {
   const int* count;
   int base, rows;
 };
-// index[0 .. *count) <- rows with a label in [0, V) other than ignore_index, in order; slot[t] <- compact row of t or -1; outputs of the
-// other rows <- 0.
-void vocab_live_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, int* index, int* slot, int* count, float* log_probs, float* entropy, float2* lse,
-                     cudaStream_t stream);
-// compact[r] <- x[index[r]] (bf16 rows of H, a multiple of 8 elements), zeros from *count on
-void vocab_gather_rows(const void* x, long long ldx, const int* index, const int* count, void* compact, int T, int H, cudaStream_t stream);
+// index[0 .. *count) <- rows with a label in [0, V) other than ignore_index, in order; slot[t] <- compact row of t or -1; compact[r] <-
+// x[index[r]] (bf16 rows of H, a multiple of 8 elements), zeros from *count on; outputs of the rows that do not count <- 0.
+void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* slot, int* count, void* compact,
+                        float* log_probs, float* entropy, float2* lse, cudaStream_t stream);
 // out[t] <- compact[slot[t]], zeros where there is none
 void vocab_scatter_rows(const void* compact, const int* slot, void* out, int T, int H, cudaStream_t stream);
 

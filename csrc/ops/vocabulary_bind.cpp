@@ -180,9 +180,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Te
   if (rows == 0) return {log_probs, entropy, lse, xc, map};
   if (compact) {
     int* m = map.data_ptr<int>();
-    vocab_live_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, m, m + rows, m + 2 * rows, log_probs.data_ptr<float>(), ent, pairs(lse), stream);
     xc = torch::empty({rows, H}, x.options());
-    vocab_gather_rows(x.data_ptr(), x.stride(0), m, m + 2 * rows, xc.data_ptr(), (int)rows, (int)H, stream);
+    vocab_compact_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, x.data_ptr(), x.stride(0), (int)H, m, m + rows, m + 2 * rows, xc.data_ptr(),
+                       log_probs.data_ptr<float>(), ent, pairs(lse), stream);
   }
   const int64_t most = stats_rows(rows, slices);
   Tensor stats = empty_f32(most * slices * 4, x);
