@@ -495,63 +495,64 @@ void token_log_probs_join(const float* stats, int slices, int slice_width, const
 // ------------------------------------------------------------------------- live rows of a batch
 namespace {
 
-// A block takes 32 rows of the batch: it counts the live rows before them (all of the earlier labels, 8 bytes each, from L2), which gives
-// its rows their places, and copies the live ones there. The d-th row that does not count clears compact row T - 1 - d, so that
-// all rows behind the live ones are zeros.
-constexpr int COMPACT_ROWS = 32;
+// A block takes `share` consecutive rows of the batch: it counts the live rows before them (all of the earlier labels, from L2), which
+// gives its rows their places, and copies the live ones there, a warp per row. The d-th row that does not count clears compact row
+// T - 1 - d, so that all rows behind the live ones are zeros.
 constexpr int COMPACT_THREADS = 256;
 
 __global__ void __launch_bounds__(COMPACT_THREADS)
-    compact_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, const __nv_bfloat16* __restrict__ x, long long ldx, int H, int* __restrict__ index,
-                        int* __restrict__ slot, int* __restrict__ count, __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs, float* __restrict__ entropy,
-                        float2* __restrict__ lse) {
-  __shared__ int warp_count[COMPACT_THREADS / 32], place[COMPACT_ROWS];
+    compact_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, const __nv_bfloat16* __restrict__ x, long long ldx, int H, int share,
+                        int* __restrict__ index, int* __restrict__ slot, int* __restrict__ count, __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs,
+                        float* __restrict__ entropy, float2* __restrict__ lse) {
+  __shared__ int warp_count[COMPACT_THREADS / 32], place[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int t0 = blockIdx.x * COMPACT_ROWS;
+  const int first = blockIdx.x * share, end = min(T, first + share);
   auto is_live = [&](int t) {
     const long long l = load_label(labels, labels64, t);
     return l != ignore_index && l >= 0 && l < V;
   };
   int n = 0;
 #pragma unroll 4
-  for (int t = threadIdx.x; t < t0; t += COMPACT_THREADS) n += is_live(t) ? 1 : 0;
+  for (int t = threadIdx.x; t < first; t += COMPACT_THREADS) n += is_live(t) ? 1 : 0;
   n = __reduce_add_sync(0xffffffffu, n);
   if (lane == 0) warp_count[warp] = n;
   __syncthreads();
-  if (warp == 0) {
-    int before = 0;
+  int before = 0;
 #pragma unroll
-    for (int w = 0; w < COMPACT_THREADS / 32; ++w) before += warp_count[w];
-    const int t = t0 + lane;
-    const bool live = t < T && is_live(t);
-    const unsigned votes = __ballot_sync(0xffffffffu, live);
-    const int p = before + __popc(votes & ((1u << lane) - 1));  // live rows before t
-    if (t < T) {
-      slot[t] = live ? p : -1;
-      if (live) {
-        index[p] = t;
-      } else {
-        log_probs[t] = 0.f;
-        lse[t] = make_float2(0.f, 0.f);
-        if (entropy != nullptr) entropy[t] = 0.f;
+  for (int w = 0; w < COMPACT_THREADS / 32; ++w) before += warp_count[w];
+  for (int t0 = first; t0 < end; t0 += 32) {
+    if (warp == 0) {
+      const int t = t0 + lane;
+      const bool live = t < end && is_live(t);
+      const unsigned votes = __ballot_sync(0xffffffffu, live);
+      const int p = before + __popc(votes & ((1u << lane) - 1));  // live rows before t
+      before += __popc(votes);
+      if (t < end) {
+        slot[t] = live ? p : -1;
+        if (live) {
+          index[p] = t;
+        } else {
+          log_probs[t] = 0.f;
+          lse[t] = make_float2(0.f, 0.f);
+          if (entropy != nullptr) entropy[t] = 0.f;
+        }
+        if (t == T - 1) *count = p + (live ? 1 : 0);
+        place[lane] = live ? p : -(T - 1 - (t - p)) - 1;
       }
-      if (t == T - 1) *count = p + (live ? 1 : 0);
     }
-    place[lane] = live ? p : t < T ? -(T - 1 - (t - p)) - 1 : 0;
-  }
-  __syncthreads();
-  // eight warps, a row each at a time
-  for (int k = warp; k < COMPACT_ROWS && t0 + k < T; k += COMPACT_THREADS / 32) {
-    const int p = place[k];
-    const bool live = p >= 0;
-    uint4* dst = reinterpret_cast<uint4*>(compact + (long long)(live ? p : -p - 1) * H);
-    const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(t0 + k) * ldx);
-    if (live) {
-#pragma unroll 4
-      for (int i = lane; i < H / 8; i += 32) dst[i] = src[i];
-    } else {
-      for (int i = lane; i < H / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    for (int k = warp; k < 32 && t0 + k < end; k += COMPACT_THREADS / 32) {
+      const int p = place[k];
+      uint4* dst = reinterpret_cast<uint4*>(compact + (long long)(p >= 0 ? p : -p - 1) * H);
+      const uint4* src = reinterpret_cast<const uint4*>(x + (long long)(t0 + k) * ldx);
+      if (p >= 0) {
+#pragma unroll 8
+        for (int i = lane; i < H / 8; i += 32) dst[i] = src[i];
+      } else {
+        for (int i = lane; i < H / 8; i += 32) dst[i] = make_uint4(0, 0, 0, 0);
+      }
     }
+    __syncthreads();
   }
 }
 
@@ -566,8 +567,11 @@ __global__ void __launch_bounds__(128) scatter_rows_kernel(const __nv_bfloat16* 
 
 void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* slot, int* count, void* compact,
                         float* log_probs, float* entropy, float2* lse, cudaStream_t stream) {
-  compact_rows_kernel<<<(T + COMPACT_ROWS - 1) / COMPACT_ROWS, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V, reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, index, slot,
-                                                                                             count, reinterpret_cast<__nv_bfloat16*>(compact), log_probs, entropy, lse);
+  // a row per warp as long as that makes at most 1024 blocks (each of them reads all labels before its rows)
+  int share = 8;
+  while ((T + share - 1) / share > 1024) share *= 2;
+  compact_rows_kernel<<<(T + share - 1) / share, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V, reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, share, index, slot, count,
+                                                                               reinterpret_cast<__nv_bfloat16*>(compact), log_probs, entropy, lse);
   count_launch();
   check_cuda(cudaGetLastError(), "compact rows launch");
 }

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "ops.h"
 #include "vocabulary.h"
 
 namespace b200 {
@@ -196,66 +197,15 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Te
   return {log_probs, entropy, lse, xc, map};
 }
 
-// grad[n, V] (bf16, row stride a multiple of 8) <- gradient of the logits of rows [base, base + n) of xc
-void linear_log_probs_grad(const Tensor& xc, const Tensor& w, const Tensor& labels, const Tensor& lse, const OptTensor& entropy, const Tensor& d_log_probs,
-                           const OptTensor& d_entropy, const Tensor& map, int64_t base, Tensor& grad, double logit_scale, int64_t ignore_index, const Tensor& status) {
-  check_linear(xc, w, labels);
-  int* st = status_of(status, xc);
-  const int64_t rows = xc.size(0), V = w.size(0), n = grad.size(0);
-  check_device(grad, xc, "grad");
-  TORCH_CHECK(grad.scalar_type() == torch::kBFloat16 && grad.dim() == 2 && grad.size(1) == V && grad.stride(1) == 1 && grad.stride(0) % 8 == 0 &&
-                  reinterpret_cast<uintptr_t>(grad.data_ptr()) % 16 == 0,
-              "grad must be bf16 [n, V] with 16-byte aligned rows");
-  TORCH_CHECK(base >= 0 && base + n <= rows, "rows out of range");
-  long long g_stride = 0, h_stride = 0;
-  const float* g = row_values(d_log_probs, xc, rows, "d_log_probs", &g_stride);
-  const float* h = d_entropy.has_value() ? row_values(*d_entropy, xc, rows, "d_entropy", &h_stride) : nullptr;
-  TORCH_CHECK(h == nullptr || entropy.has_value(), "the entropy gradient needs the entropy of the forward pass");
-  const c10::cuda::CUDAGuard guard(xc.device());
-  vocab_gemm_grad(row_ptr(xc, base), w.data_ptr(), labels.data_ptr(), labels.scalar_type() == torch::kInt64, checked_pairs(lse, xc, rows),
-                  h != nullptr ? contiguous_f32(*entropy, xc, rows, "entropy") : nullptr, g, g_stride, h, h_stride, grad.data_ptr(), live_rows(map, rows, base, n), (int)V,
-                  (int)xc.size(1), xc.stride(0), w.stride(0), grad.stride(0), (float)logit_scale, ignore_index, st, stream_of(xc));
-}
-
-// out = a b for the live rows of a compacted batch, which are a's rows (data gradient, bf16 out) ...
-void linear_log_probs_dgrad(const Tensor& dlogits, const Tensor& w, Tensor& out, const Tensor& map, int64_t base, const Tensor& status) {
-  const int64_t n = dlogits.size(0), V = w.size(0), H = w.size(1), T = (map.numel() - 1) / 2;
-  check_device(w, dlogits, "weight");
-  check_device(out, dlogits, "out");
-  TORCH_CHECK(dlogits.dim() == 2 && w.dim() == 2 && out.dim() == 2 && dlogits.size(1) == V && out.size(0) == n && out.size(1) == H && dlogits.stride(1) == 1 && w.stride(1) == 1 && out.stride(1) == 1,
-              "dgrad: shape mismatch");
-  TORCH_CHECK(dlogits.scalar_type() == torch::kBFloat16 && w.scalar_type() == torch::kBFloat16 && out.scalar_type() == torch::kBFloat16, "dgrad: bf16 operands are needed");
-  int* st = status_of(status, dlogits);
-  const c10::cuda::CUDAGuard guard(dlogits.device());
-  gemm_bf16_2sm_live(dlogits.data_ptr(), w.data_ptr(), out.data_ptr(), (int)n, (int)H, (int)V, dlogits.stride(0), w.stride(0), out.stride(0), false, true, false,
-                     live_rows(map, T, base, n).count, (int)base, false, st, stream_of(dlogits));
-}
-
-// ... or the rows both are contracted over (weight gradient; fp32 out is added to)
-void linear_log_probs_wgrad(const Tensor& dlogits, const Tensor& xc, Tensor& out, const Tensor& map, int64_t base, const Tensor& status) {
-  const int64_t n = dlogits.size(0), V = dlogits.size(1), H = xc.size(1), T = (map.numel() - 1) / 2;
-  check_device(xc, dlogits, "hidden states");
-  check_device(out, dlogits, "out");
-  TORCH_CHECK(dlogits.dim() == 2 && xc.dim() == 2 && out.dim() == 2 && xc.size(0) == n && out.size(0) == V && out.size(1) == H && dlogits.stride(1) == 1 && xc.stride(1) == 1 && out.stride(1) == 1,
-              "wgrad: shape mismatch");
-  TORCH_CHECK(dlogits.scalar_type() == torch::kBFloat16 && xc.scalar_type() == torch::kBFloat16 && (out.scalar_type() == torch::kBFloat16 || out.scalar_type() == torch::kFloat32),
-              "wgrad: bf16 operands and a bf16 or fp32 output are needed");
-  int* st = status_of(status, dlogits);
-  const c10::cuda::CUDAGuard guard(dlogits.device());
-  gemm_bf16_2sm_live(dlogits.data_ptr(), xc.data_ptr(), out.data_ptr(), (int)V, (int)H, (int)n, dlogits.stride(0), xc.stride(0), out.stride(0), true, true,
-                     out.scalar_type() == torch::kFloat32, live_rows(map, T, base, n).count, (int)base, true, st, stream_of(dlogits));
-}
-
-// dx[T, H] from the gradient of the compacted rows
-Tensor linear_log_probs_scatter(const Tensor& compact, const Tensor& map) {
-  const int64_t T = (map.numel() - 1) / 2;
-  TORCH_CHECK(compact.is_cuda() && compact.is_contiguous() && compact.scalar_type() == torch::kBFloat16 && compact.dim() == 2 && compact.size(0) == T && compact.size(1) % 8 == 0,
-              "the compacted gradient must be contiguous bf16 [T, H]");
-  check_device(map, compact, "row map");
-  const c10::cuda::CUDAGuard guard(compact.device());
-  Tensor out = torch::empty_like(compact);
-  vocab_scatter_rows(compact.data_ptr(), live_rows(map, T, 0, T).index + T, out.data_ptr(), (int)T, (int)compact.size(1), stream_of(compact));
-  return out;
+// out (+)= a b of the products that follow: rows of the batch (or of its live rows) are the rows of a, or what both are contracted over.
+void product(const Tensor& a, const Tensor& b, Tensor& out, bool contract_rows, const LiveRows& live, int* status, cudaStream_t stream) {
+  const int M = (int)out.size(0), N = (int)out.size(1), K = (int)(contract_rows ? a.size(0) : a.size(1));
+  const bool f32 = out.scalar_type() == torch::kFloat32;  // fp32 outputs are added to
+  if (live.count != nullptr)
+    gemm_bf16_2sm_live(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, a.stride(0), b.stride(0), out.stride(0), contract_rows, true, f32, live.count, live.base, contract_rows, status,
+                       stream);
+  else
+    (M >= 256 ? gemm_bf16_2sm : gemm_bf16)(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, a.stride(0), b.stride(0), out.stride(0), contract_rows, true, f32 ? 2 : 0, 1.f, status, 0, stream);
 }
 
 // ------------------------------------------------------------------------- losses over sequences
@@ -444,6 +394,83 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   }
 };
 
+// The engine's fp32 gradient buffer of a parameter (its Python attribute main_grad), if it has one.
+OptTensor main_grad(const Tensor& weight) {
+  const py::gil_scoped_acquire gil;
+  const py::object p = py::cast(weight);
+  const py::object target = py::getattr(p, "main_grad", py::none());
+  if (target.is_none()) return OptTensor();
+  Tensor t = py::cast<Tensor>(target).view(weight.sizes());
+  TORCH_CHECK(t.is_cuda() && t.device() == weight.device() && t.scalar_type() == torch::kFloat32 && t.is_contiguous(), "main_grad must be a contiguous fp32 tensor on the weight's device");
+  return t;
+}
+
+// Forward keeps 16 bytes per row and 128 columns of logits; backward forms the logits again, chunk of rows by chunk, as their bf16
+// gradient, and multiplies that with the weight and the hidden states. Batches of more than 256 rows are compacted to the rows whose
+// label counts, and all four products end there.
+struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy, int64_t chunk,
+                               const Tensor& status) {
+    auto [log_probs, entropy, lse, xc, map] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy, status);
+    ctx->save_for_backward({xc, w, labels, lse, entropy, map, status});
+    ctx->saved_data["logit_scale"] = logit_scale;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["chunk"] = chunk;
+    ctx->set_materialize_grads(false);
+    if (!want_entropy) return {log_probs};
+    return {log_probs, entropy};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5];
+    const bool has_h = grads.size() > 1 && grads[1].defined();
+    if (!grads[0].defined() && !has_h) return variable_list(8);
+    const int64_t T = xc.size(0), H = xc.size(1), V = w.size(0);
+    const int64_t chunk = std::max<int64_t>(std::min(ctx->saved_data["chunk"].toInt(), T), 1);
+    const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
+    const Tensor g = row_gradient(grads[0], T, lse), h = has_h ? row_gradient(grads[1], T, lse) : Tensor();
+    long long g_stride = 0, h_stride = 0;
+    const float* gp = row_values(g, xc, T, "d_log_probs", &g_stride);
+    const float* hp = has_h ? row_values(h, xc, T, "d_entropy", &h_stride) : nullptr;
+    int* st = status_of(saved[6], xc);
+    const c10::cuda::CUDAGuard guard(xc.device());
+    const cudaStream_t stream = stream_of(xc);
+    Tensor dx, dw;
+    if (need_dx) dx = torch::empty({T, H}, xc.options());
+    OptTensor target;
+    if (need_dw) {
+      target = main_grad(w);
+      // one chunk writes the weight's gradient in its own type; several add up in fp32
+      if (target.has_value()) dw = *target;
+      else if (chunk == T) dw = torch::empty({V, H}, w.options());
+      else dw = torch::zeros({V, H}, w.options().dtype(torch::kFloat32));
+    }
+    Tensor dlogits = torch::empty({std::min(chunk, T), (V + 7) / 8 * 8}, xc.options()).narrow(1, 0, V);
+    for (int64_t r = 0; r < T; r += chunk) {
+      const int64_t n = std::min(chunk, T - r);
+      const LiveRows live = live_rows(map, T, r, n);
+      const Tensor dl = dlogits.narrow(0, 0, n), xr = xc.narrow(0, r, n);
+      vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.scalar_type() == torch::kInt64, pairs(lse), has_h ? entropy.data_ptr<float>() : nullptr, gp, g_stride, hp,
+                      h_stride, dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0), dl.stride(0), (float)ctx->saved_data["logit_scale"].toDouble(),
+                      ctx->saved_data["ignore_index"].toInt(), st, stream);
+      if (need_dx) {
+        Tensor out = dx.narrow(0, r, n);
+        product(dl, w, out, false, live, st, stream);
+      }
+      if (need_dw) product(dl, xr, dw, true, live, st, stream);
+    }
+    if (need_dx && map.numel() > 0) {
+      Tensor scattered = torch::empty_like(dx);
+      vocab_scatter_rows(dx.data_ptr(), live_rows(map, T, 0, T).index + T, scattered.data_ptr(), (int)T, (int)H, stream);
+      dx = scattered;
+    }
+    variable_list out(8);
+    if (need_dx) out[0] = once(dx, "fused_linear_token_log_probs");
+    if (need_dw && !target.has_value()) out[1] = once(dw.to(w.scalar_type()), "fused_linear_token_log_probs");
+    return out;
+  }
+};
+
 void check_logit_scale(double logit_scale) {
   TORCH_CHECK_VALUE(std::isfinite(logit_scale) && logit_scale > 0, "logit_scale must be positive and finite, got ", text(logit_scale));
 }
@@ -459,6 +486,27 @@ variable_list token_log_probs(const Tensor& logits, const Tensor& labels, double
   TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must have a last dimension of at least 1, got ", text(logits.sizes()));
   check_label_shape(labels, logits.sizes().slice(0, logits.dim() - 1), logits);
   return TokenLogProbs::apply(logits, labels, logit_scale, ignore_index, return_entropy);
+}
+
+// Rows that a tensor map can describe: unit inner stride, row stride and base multiples of 16 bytes.
+Tensor mapped_rows(const Tensor& t) {
+  const bool ok = t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.contiguous();
+}
+
+variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool return_entropy, int64_t chunk, const Tensor& status) {
+  check_logit_scale(logit_scale);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(0) > 0 && w.size(1) > 0, "hidden states [..., H] and a weight [V, H] are needed, got ", text(x.sizes()), " and ",
+                    text(w.sizes()));
+  TORCH_CHECK_VALUE(x.device() == w.device() && x.scalar_type() == w.scalar_type(), "hidden states and weight must be of one type on one device, got ", text(x.scalar_type()), " on ",
+                    text(x.device()), " and ", text(w.scalar_type()), " on ", text(w.device()));
+  const auto shape = x.sizes().slice(0, x.dim() - 1);
+  check_label_shape(labels, shape, x);
+  variable_list out = LinearTokenLogProbs::apply(mapped_rows(x.reshape({labels.numel(), x.size(-1)})), mapped_rows(w), labels.reshape({labels.numel()}).contiguous(), logit_scale, ignore_index,
+                                                 return_entropy, chunk, status);
+  if (x.dim() != 2)
+    for (auto& t : out) t = t.view(shape);
+  return out;
 }
 
 // ---- losses: (log_probs as given, the same in fp32) so that the type conversion stays a differentiable step of its own
@@ -573,15 +621,6 @@ variable_list policy_loss(const Tensor& log_probs, const Tensor& old, const Tens
   return PolicyLoss::apply(lp, o, ref, a, per_token, s.cu, s.mask, s.length, s.count, clip_low, clip_high, dual_clip, kl_coef, reduction, want_slope);
 }
 
-// The engine's fp32 gradient buffer of a parameter (its Python attribute main_grad), if it has one.
-OptTensor main_grad(const Tensor& weight) {
-  const py::gil_scoped_acquire gil;
-  const py::object p = py::cast(weight);
-  const py::object target = py::getattr(p, "main_grad", py::none());
-  if (target.is_none()) return OptTensor();
-  return py::cast<Tensor>(target).view(weight.sizes());
-}
-
 struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
     Tensor out = embedding_lookup_(weight, ids, scale, status);
@@ -611,11 +650,7 @@ Tensor embedding_sorted(const Tensor& weight, const Tensor& ids, double scale, c
 
 void register_vocabulary(pybind11::module_& m) {
   m.def("token_log_probs", &token_log_probs, "log-probabilities of given tokens (and entropies) under rows of logits");
-  m.def("linear_log_probs_fwd", &linear_log_probs_fwd, "the same from hidden states and the output weight, with the rows' log-sum-exps");
-  m.def("linear_log_probs_grad", &linear_log_probs_grad, "gradient of the logits, formed again from hidden states and weight");
-  m.def("linear_log_probs_dgrad", &linear_log_probs_dgrad);
-  m.def("linear_log_probs_wgrad", &linear_log_probs_wgrad);
-  m.def("linear_log_probs_scatter", &linear_log_probs_scatter);
+  m.def("linear_token_log_probs", &linear_token_log_probs, "the same from hidden states and the output weight");
   m.def("preference_loss", &preference_loss, "loss over pairs of answers: (loss, chosen rewards, rejected rewards)");
   m.def("policy_loss", &policy_loss, "clipped policy loss with a KL term: (loss, KL estimate, clipped share)");
   m.def("embedding_sorted", &embedding_sorted, "embedding whose gradient is summed in sorted token order");

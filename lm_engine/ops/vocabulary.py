@@ -17,7 +17,7 @@ from typing import NamedTuple
 import torch
 import torch.nn.functional as F
 
-from . import _flce_chunk_rows, _weight_grad_target, native, note_fallback, status_word
+from . import _flce_chunk_rows, native, note_fallback, status_word
 from .timeline import site
 
 _LOGIT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -60,12 +60,6 @@ def _token_log_probs_torch(logits: torch.Tensor, labels: torch.Tensor, logit_sca
     return picked, torch.where(kept, entropy, 0.0)
 
 
-def _row_gradient(grad: torch.Tensor | None, rows: int, like: torch.Tensor) -> torch.Tensor:
-    if grad is None:
-        return torch.zeros((), dtype=torch.float32, device=like.device).expand(rows)
-    return grad.reshape(-1)
-
-
 def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0, ignore_index: int = -100,
                     return_entropy: bool = False):
     """Log-probability of ``labels[...]`` under ``softmax(logit_scale * logits[..., :])``, fp32, shaped like ``labels``; with
@@ -86,78 +80,6 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: 
 
 
 # ----------------------------------------------------------------------------- from hidden states
-class _FusedLinearTokenLogProbsFn(torch.autograd.Function):
-    """Forward keeps 16 bytes per row and 128 columns of logits; backward forms the logits again, chunk of rows by chunk, as
-    their bf16 gradient, and multiplies that with the weight and the hidden states. Batches of more than 256 rows are compacted to the rows whose
-    label counts; their number stays on the device (``row_map``), and all four products end at it."""
-
-    @staticmethod
-    def forward(ctx, x, weight, labels, logit_scale, ignore_index, return_entropy):
-        ctx.set_materialize_grads(False)
-        with site("loss.lm_head.log_probs"):
-            log_probs, entropy, lse, xc, row_map = native().linear_log_probs_fwd(x, weight, labels, logit_scale, ignore_index, return_entropy, status_word(x.device))
-        ctx.save_for_backward(xc, weight, labels, lse, entropy, row_map)
-        ctx.args = (logit_scale, ignore_index)
-        return (log_probs, entropy) if return_entropy else log_probs
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_log_probs, d_entropy=None):
-        xc, weight, labels, lse, entropy, row_map = ctx.saved_tensors
-        if d_log_probs is None and d_entropy is None:
-            return (None,) * 6
-        C, st = native(), status_word(xc.device)
-        T, H = xc.shape
-        V = weight.shape[0]
-        compact = row_map.numel() > 0
-        need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        d_log_probs = _row_gradient(d_log_probs, T, lse)
-        rows = max(_flce_chunk_rows(T, V), 1)
-        target = _weight_grad_target(weight) if need_dw else None
-        dx = torch.empty(T, H, device=xc.device, dtype=xc.dtype) if need_dx else None
-        dw = None
-        if need_dw:
-            # one chunk writes the weight's gradient in its own type; several add up in fp32
-            if target is not None:
-                dw = target.view(V, H)
-            elif rows == T:
-                dw = torch.empty(V, H, device=xc.device, dtype=weight.dtype)
-            else:
-                dw = torch.zeros(V, H, device=xc.device, dtype=torch.float32)
-        pitch = (V + 7) // 8 * 8
-        dlogits = torch.empty(min(rows, T), pitch, device=xc.device, dtype=torch.bfloat16)[:, :V]
-        for start in range(0, T, rows):
-            part = slice(start, min(start + rows, T))
-            dl = dlogits[: part.stop - start]
-            with site("loss.lm_head.dlogits"):
-                C.linear_log_probs_grad(xc, weight, labels, lse, entropy, d_log_probs, d_entropy, row_map, start, dl, *ctx.args, st)
-            if need_dx:
-                with site("loss.lm_head.dgrad"):
-                    if compact:
-                        C.linear_log_probs_dgrad(dl, weight, dx[part], row_map, start, st)
-                    else:
-                        C.gemm(dl, weight, dx[part], False, True, False, 1.0, st, 0)
-            if need_dw:
-                with site("loss.lm_head.wgrad"):
-                    if compact:
-                        C.linear_log_probs_wgrad(dl, xc[part], dw, row_map, start, st)
-                    else:
-                        C.gemm(dl, xc[part], dw, True, True, dw.dtype == torch.float32, 1.0, st, 0)
-        if need_dx and compact:
-            dx = C.linear_log_probs_scatter(dx, row_map)
-        if target is not None:
-            dw = None
-        elif dw is not None:
-            dw = dw.to(weight.dtype)
-        return dx, dw, None, None, None, None
-
-
-def _gemm_rows(t: torch.Tensor) -> torch.Tensor:
-    """Rows that a tensor map can describe: unit inner stride, row stride and base multiples of 16 bytes."""
-    ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1] and t.data_ptr() % 16 == 0
-    return t if ok else t.contiguous()
-
-
 def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0,
                                  ignore_index: int = -100, return_entropy: bool = False):
     """:func:`token_log_probs` of ``logits = x @ weight.T`` without the logits: ``x [..., H]``, ``weight [V, H]``, ``labels [...]``.
@@ -165,19 +87,18 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
     The logits are formed in fp32 on the tensor cores and reduced where they are; the backward pass forms them a second time (8/6 of
     the products of a path that keeps them) and needs a transient bf16 buffer of at most about 2.2 GB. bf16 operands with ``H`` a multiple
     of 8 run on the kernels. Gradients of ``weight`` go to its ``main_grad`` when the engine provides one."""
+    if x.is_cuda and x.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0:
+        with site("loss.lm_head.log_probs"):
+            out = native().linear_token_log_probs(x, weight, labels, logit_scale, ignore_index, return_entropy, _flce_chunk_rows(labels.numel(), weight.shape[0]), status_word(x.device))
+        return tuple(out) if return_entropy else out[0]
     logit_scale = _check_logit_scale(logit_scale)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"hidden states [..., H] and a weight [V, H] are needed, got {tuple(x.shape)} and {tuple(weight.shape)}")
     if x.device != weight.device or x.dtype != weight.dtype or not x.is_floating_point():
         raise ValueError(f"hidden states and weight must be floating point of one type on one device, got {x.dtype} on {x.device} and {weight.dtype} on {weight.device}")
     _check_labels(labels, x.shape[:-1], x.device)
-    if not (x.is_cuda and x.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0):
-        note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
-        return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
-    shape = labels.shape
-    out = _FusedLinearTokenLogProbsFn.apply(_gemm_rows(x.reshape(-1, x.shape[-1])), _gemm_rows(weight), labels.reshape(-1).contiguous(),
-                                            logit_scale, int(ignore_index), bool(return_entropy))
-    return tuple(o.view(shape) for o in out) if return_entropy else out.view(shape)
+    note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
+    return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
 
 
 # ----------------------------------------------------------------------------- losses over packed answers
