@@ -15,6 +15,7 @@ from .loss import (
     clear_aux_loss,
     get_autoregressive_language_modeling_loss,
     get_aux_loss,
+    get_token_log_probs,
     is_aux_loss_zero,
 )
 from .modeling import (

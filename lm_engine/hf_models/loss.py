@@ -118,3 +118,36 @@ def get_autoregressive_language_modeling_loss(
     if logit_scale != 1.0:
         x = x * logit_scale
     return ops.cross_entropy(x, labels, reduction=reduction)
+
+
+def get_token_log_probs(
+    lm_logits: torch.Tensor | None,
+    labels: torch.Tensor,
+    hidden_states: torch.Tensor | None = None,
+    vocab_weight: torch.Tensor | None = None,
+    cu_seqlens: torch.Tensor | None = None,
+    use_padding_free_transformer: bool = False,
+    shift_logits_and_labels: bool = True,
+    tensor_parallel_enabled: bool = False,
+    logit_scale: float = 1.0,
+    return_entropy: bool = False,
+) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """Per-token log-probabilities of the labels, the input of ``ops.preference_loss`` and ``ops.policy_loss``, with the conventions of
+    :func:`get_autoregressive_language_modeling_loss` (ignored label = -100; ``lm_logits``, or ``hidden_states`` and ``vocab_weight`` for the
+    fused path). The result (fp32, with ``return_entropy`` also the entropies) is shaped like ``labels``: when labels are shifted, position ``t``
+    holds the log-probability of token ``t + 1`` and the last position of every document or row holds 0."""
+    fused = lm_logits is None
+    if tensor_parallel_enabled:
+        raise ValueError("token log-probabilities need the whole vocabulary on one rank; they cannot be combined with tensor parallelism")
+    if shift_logits_and_labels:
+        # the labels move, not the logits: a shifted slice of the logits would be copied
+        shifted = torch.full_like(labels, -100)
+        shifted[..., :-1] = labels[..., 1:]
+        if use_padding_free_transformer:
+            if cu_seqlens is None:
+                raise ValueError("cu_seqlens is needed to shift labels of packed documents")
+            shifted[cu_seqlens[1:].long() - 1] = -100
+        labels = shifted
+    if fused:
+        return ops.fused_linear_token_log_probs(hidden_states, vocab_weight, labels, logit_scale=logit_scale, return_entropy=return_entropy)
+    return ops.token_log_probs(lm_logits, labels, logit_scale=logit_scale, return_entropy=return_entropy)

@@ -333,10 +333,10 @@ class _EmbeddingFn(torch.autograd.Function):
         return dw.to(weight.dtype), None, None
 
 
-def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, *, sorted_gradient: bool = False) -> torch.Tensor:
-    """``scale * weight[ids]``. ``sorted_gradient`` sums the weight gradient in sorted token order instead of with atomics:
-    see :func:`embedding_sorted`."""
-    if sorted_gradient:
+def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, *, sorted_gradient: bool | None = None) -> torch.Tensor:
+    """``scale * weight[ids]``. ``sorted_gradient`` sums the weight gradient in sorted token order instead of with atomics, whose
+    order differs from run to run (see :func:`embedding_sorted`); by default it follows ``torch.use_deterministic_algorithms``."""
+    if torch.are_deterministic_algorithms_enabled() if sorted_gradient is None else sorted_gradient:
         return embedding_sorted(weight, ids, scale)
     if use_native(weight) and weight.dtype == torch.bfloat16 and ids.is_cuda and weight.shape[1] % 8 == 0:
         return _EmbeddingFn.apply(weight, ids.long(), float(scale))

@@ -155,6 +155,52 @@ def test_sorted_embedding_on_the_cpu_is_the_plain_one():
     assert torch.autograd.gradcheck(lambda a: ops.embedding(a, ids, 2.0, sorted_gradient=True), (w,))
 
 
+def test_token_log_probs_of_a_model_shift_like_the_language_modelling_loss():
+    """Summed log-probabilities are minus the summed loss, padded and packed, from logits and from hidden states, and drive both losses."""
+    from lm_engine.hf_models import get_autoregressive_language_modeling_loss, get_token_log_probs
+
+    gen = torch.Generator().manual_seed(5)
+    hidden, weight = torch.randn(2, 6, 8, generator=gen), torch.randn(13, 8, generator=gen)
+    labels = torch.randint(0, 13, (2, 6), generator=gen)
+    labels[0, :3] = -100
+    logits = hidden @ weight.t()
+    want = get_autoregressive_language_modeling_loss(logits, labels, reduction="sum", logit_scale=0.5)
+    lp = get_token_log_probs(logits, labels, logit_scale=0.5)
+    assert lp.shape == labels.shape and torch.allclose(lp.sum(), -want, rtol=1e-5) and (lp[:, -1] == 0).all() and (lp[0, :2] == 0).all()
+    assert torch.allclose(get_token_log_probs(None, labels, hidden, weight, logit_scale=0.5), lp, atol=1e-5)
+    unshifted = get_token_log_probs(logits, labels, logit_scale=0.5, shift_logits_and_labels=False)
+    assert torch.allclose(unshifted.sum(), -get_autoregressive_language_modeling_loss(logits, labels, reduction="sum", logit_scale=0.5, shift_logits_and_labels=False), rtol=1e-5)
+    cu = torch.tensor([0, 4, 4, 9, 12], dtype=torch.int32)
+    flat, packed = logits.reshape(12, 13), labels.reshape(12)
+    want = get_autoregressive_language_modeling_loss(flat, packed.clone(), cu_seqlens=cu, use_padding_free_transformer=True, reduction="sum")
+    lp, entropy = get_token_log_probs(flat, packed, cu_seqlens=cu, use_padding_free_transformer=True, return_entropy=True)
+    assert torch.allclose(lp.sum(), -want, rtol=1e-5) and (lp[[3, 8, 11]] == 0).all() and (entropy >= 0).all()
+    leaf = lp.detach().requires_grad_(True)
+    (grad,) = torch.autograd.grad(ops.preference_loss(leaf, lp.detach() - 0.1, cu).loss, leaf)
+    assert torch.isfinite(grad).all() and grad.abs().max() > 0
+    with pytest.raises(ValueError):
+        get_token_log_probs(logits, labels, tensor_parallel_enabled=True)
+    with pytest.raises(ValueError):
+        get_token_log_probs(flat, packed, use_padding_free_transformer=True)
+
+
+def test_embedding_layer_follows_the_deterministic_switch(monkeypatch):
+    from lm_engine.hf_models.layers.basic import ParameterizedEmbedding
+
+    layer = ParameterizedEmbedding(5, 4, std=0.1)
+    ids = torch.tensor([1, 4, 1])
+    called = []
+    monkeypatch.setattr(ops, "embedding_sorted", lambda w, i, s: called.append(s) or torch.nn.functional.embedding(i, w))
+    plain = layer(ids)
+    assert not called
+    torch.use_deterministic_algorithms(True)
+    try:
+        assert torch.equal(layer(ids), plain) and called == [1.0]
+        assert torch.equal(ops.embedding(layer.weight, ids, sorted_gradient=False), plain) and called == [1.0]
+    finally:
+        torch.use_deterministic_algorithms(False)
+
+
 LP = torch.zeros(4, 3)
 CU = torch.tensor([0, 3, 6, 9, 12])
 
@@ -203,3 +249,37 @@ CU = torch.tensor([0, 3, 6, 9, 12])
 def test_refusals(call):
     with pytest.raises(ValueError):
         call()
+
+
+F32, I64 = (lambda *s: torch.zeros(*s)), (lambda *s: torch.zeros(*s, dtype=torch.long))
+LOSS = dict(zip(("kind", "beta", "smoothing", "average", "reduction"), (0, 0.1, 0.0, False, 2)))
+POLICY = (0.2, 0.2, 0.0, 0.0, 1)
+
+
+@pytest.mark.parametrize("call", [
+    lambda C: C.token_log_probs(F32(3, 5), F32(3), 1.0, -100, False),
+    lambda C: C.token_log_probs(F32(3, 5), I64(4), 1.0, -100, False),
+    lambda C: C.token_log_probs(F32(3, 0), I64(3), 1.0, -100, False),
+    lambda C: C.token_log_probs(F32(3, 5), I64(3), -0.5, -100, False),
+    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 9), I64(3), 1.0, -100, False, 256, F32(1)),
+    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 8).half(), I64(3), 1.0, -100, False, 256, F32(1)),
+    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 8), I64(3), math.inf, -100, False, 256, F32(1)),
+    lambda C: C.preference_loss(F32(3, 3), None, None, None, *LOSS.values()),
+    lambda C: C.preference_loss(F32(12), None, None, None, *LOSS.values()),
+    lambda C: C.preference_loss(F32(12), None, F32(5), None, *LOSS.values()),
+    lambda C: C.preference_loss(F32(4, 3), F32(4, 4), None, None, *LOSS.values()),
+    lambda C: C.preference_loss(F32(4, 3), None, None, F32(4, 3), *LOSS.values()),
+    lambda C: C.preference_loss(F32(4, 3), None, None, None, *(LOSS | dict(beta=0.0)).values()),
+    lambda C: C.preference_loss(F32(4, 3), None, None, None, *(LOSS | dict(kind=2, smoothing=0.1)).values()),
+    lambda C: C.policy_loss(F32(4, 3), F32(4, 3), F32(3), None, None, None, *POLICY),
+    lambda C: C.policy_loss(F32(4, 3), F32(4, 3).requires_grad_(True), F32(4), None, None, None, *POLICY),
+    lambda C: C.policy_loss(F32(4, 3), F32(4, 3), F32(4), None, None, None, 1.2, *POLICY[1:]),
+    lambda C: C.policy_loss(F32(4, 3), F32(4, 3), F32(4), None, None, None, 0.2, 0.2, 0.0, 0.1, 1),
+    lambda C: C.policy_loss(F32(4, 3), F32(4, 3), F32(4), None, None, None, 0.2, 0.2, 0.5, 0.0, 1),
+    lambda C: C.embedding_sorted(F32(5, 4), F32(3), 1.0, F32(1)),
+    lambda C: C.embedding_sorted(F32(5), I64(3), 1.0, F32(1)),
+])
+def test_the_extension_refuses_the_same_calls(call):
+    """Its checks come before anything that needs a device, so their errors (numbers in them included) are raised here as they are on a GPU."""
+    with pytest.raises(ValueError):
+        call(ops.native())
