@@ -159,8 +159,12 @@ struct Row {
   }
 };
 
-constexpr int FWD_THREADS = 256;  // four blocks on an SM: 174 -> 159 us at 4096 x 128256 bf16 against two blocks of 512
-constexpr int FWD_UNROLL = 4;
+// Measured at 4096 x 128256 bf16, one row in eight ignored (0.92 GB): two blocks of 512 threads on an SM with four vectors a thread in flight
+// 174 us, four of 256 158, five of 256 with three vectors 156 (5.9 TB/s); fetching the next vectors before the present ones are
+// worked on gains 2 us more at the cost of the registers of one block, and is left out.
+constexpr int FWD_THREADS = 256;
+constexpr int FWD_UNROLL = 3;
+constexpr int FWD_BLOCKS = 5;
 
 // COUNT vectors of a thread at once; one comparison of their common maximum with the running one decides about rescaling.
 template <typename T, bool ENTROPY, int COUNT>
@@ -176,7 +180,7 @@ __device__ __forceinline__ void accumulate_vectors(Stats& st, const uint4 (&v)[C
   accumulate<ENTROPY, COUNT * N>(st, f, Vec<T>::top(top), scale2);
 }
 
-// The wide vectors of a row in groups of four per thread whose loads have no condition between them (the compiler keeps loads
+// The wide vectors of a row in groups of three per thread whose loads have no condition between them (the compiler keeps loads
 // behind a branch in order, one in flight: 222 instead of 150 us at 4096 x 128256 bf16).
 template <typename T, bool ENTROPY, bool ALIGNED>
 __device__ __forceinline__ void accumulate_wide(Stats& st, const Row<T>& r, int first, int end, float scale2) {
@@ -195,7 +199,7 @@ __device__ __forceinline__ void accumulate_wide(Stats& st, const Row<T>& r, int 
 
 // CLUSTER blocks share a row.
 template <typename T, bool ENTROPY, int CLUSTER>
-__global__ void __launch_bounds__(FWD_THREADS, 1024 / FWD_THREADS)
+__global__ void __launch_bounds__(FWD_THREADS, FWD_BLOCKS)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, const void* __restrict__ labels, bool labels64,
                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, int V,
                                RowMap map, float scale2, long long ignore_index) {
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 1024 / FWD_THREADS)
 }
 
 constexpr int BWD_THREADS = 256;
-constexpr int BWD_UNROLL = 4;
+constexpr int BWD_UNROLL = 8;  // 32 KB of a row per block; with 16 KB 335 us, with 64 KB 350
 
 template <typename T, bool ENTROPY>
 __global__ void __launch_bounds__(BWD_THREADS)
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(BWD_THREADS)
                                long long ignore_index, unsigned chunks) {
   constexpr int N = Vec<T>::N;
   // last row first: the logits that the forward pass (or the model) touched last are still in L2
-  // and the blocks of a row are consecutive: 4096 x 128256 354 -> 333 us (2.0 GB)
+  // and the blocks of a row are consecutive: 4096 x 128256 354 -> 333 us with 16 KB a block, 301 us (6.5 TB/s of 2.0 GB) with 32 KB
   const unsigned chunk = blockIdx.x % chunks;
   const long long row = gridDim.x / chunks - 1 - blockIdx.x / chunks;
   const long long label = load_label(labels, labels64, row);
