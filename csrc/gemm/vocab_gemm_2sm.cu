@@ -4,6 +4,9 @@
 //   statistics: the epilogue reduces each row of a tile to (m, s, u, x[label]): largest logit, sums of softmax_stats.cuh
 //               relative to it, and the label's logit if it lies in the tile's columns; 16 bytes per row and tile go to
 //               stats[slice][row] for every 128 columns instead of 256 bytes of logits. token_log_probs_join combines them.
+//   statistics, logits kept: the same, and the fp32 logits leave through shared memory and bulk tensor stores, for a backward
+//               pass that has the memory for them: 2.1 GB of stores hide under 2.6 ms of MMAs (4096 x 4096 x 128256), and what
+//               the gradient mode would take, 2.7 ms, becomes a pass over memory.
 //   gradient:   the logits are formed again, and the epilogue writes d(logits) in bf16, the operand type of the two products
 //               that follow (d(x) = d(logits) W, dW = d(logits)^T x); the factor 1[label] - p is formed in fp32 from the fp32
 //               logits, so the one rounding is that of the stored operand.
@@ -60,7 +63,7 @@ struct RowArgs {
   long long ignore_index;
 };
 
-enum class Mode : int { kStats, kGrad };
+enum class Mode : int { kStats, kStatsKeep, kGrad };
 
 // v[i] of 32 registers for a lane's own i: halved five times, so that the array stays in registers.
 __device__ __forceinline__ uint32_t select32_bits(const uint32_t (&v)[32], int i) {
@@ -79,7 +82,7 @@ __device__ __forceinline__ uint32_t select32_bits(const uint32_t (&v)[32], int i
 template <Mode MODE, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 1)
     vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                          const __grid_constant__ CUtensorMap tmG, int N, int K, int* status, RowArgs rows) {
+                          const __grid_constant__ CUtensorMap tmOut, int N, int K, int* status, RowArgs rows) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -253,7 +256,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         continue;
       }
 
-      if (MODE == Mode::kStats) {
+      if (MODE != Mode::kGrad) {
         Stats st = empty_stats();
         float x_label = 0.f;
 #pragma unroll 1
@@ -268,6 +271,18 @@ __global__ void __launch_bounds__(THREADS, 1)
             tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
+          }
+          if (MODE == Mode::kStatsKeep) {
+            if (lane == 0) tma_store_wait_read<0>();  // the store that used the box before has read it
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j) box_write(box, lane, j, make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0 && row0 < live) {
+              tma_store_2d(&tmOut, box, col0, row0);
+              tma_store_commit();
+            }
           }
           if (col0 + 32 > N) {
 #pragma unroll
@@ -322,13 +337,13 @@ __global__ void __launch_bounds__(THREADS, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && row0 < rows.live.rows) {
-            tma_store_2d(&tmG, box, col0, row0);
+            tma_store_2d(&tmOut, box, col0, row0);
             tma_store_commit();
           }
         }
       }
     }
-    if (MODE == Mode::kGrad) {
+    if (MODE != Mode::kStats) {
       // every bulk store of this warp has left shared memory and reached global memory before the CTA exits
       if (lane == 0) tma_store_wait<0>();
       __syncwarp();
@@ -346,7 +361,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 template <Mode MODE, bool ENTROPY>
-void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmG, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
+void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
   auto kernel = vocab_gemm_2sm_kernel<MODE, ENTROPY>;
   check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "vocab gemm smem attr");
   const int m_tiles = (rows.live.rows + 2 * BM - 1) / (2 * BM), n_tiles = (N + BN - 1) / BN;
@@ -364,13 +379,13 @@ void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& t
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmG, N, K, status, rows), "vocab gemm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmOut, N, K, status, rows), "vocab gemm launch");
   count_launch();
 }
 
 }  // namespace
 
-void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, LiveRows live, int N,
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl, bool entropy, LiveRows live, int N,
                       int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
   const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, live.rows, ldx, BK, BM);
@@ -382,8 +397,15 @@ void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool lab
   rows.stats = reinterpret_cast<float4*>(stats);
   rows.logit_scale = logit_scale;
   rows.ignore_index = -1;  // every label outside of [0, N) counts as none here
-  if (entropy) launch<Mode::kStats, true>(tmA, tmB, tmA, N, K, status, rows, stream);
-  else launch<Mode::kStats, false>(tmA, tmB, tmA, N, K, status, rows, stream);
+  if (logits != nullptr) {
+    const CUtensorMap tmL = make_tensor_map_2d_f32(logits, N, live.rows, ldl, 32, 32);
+    if (entropy) launch<Mode::kStatsKeep, true>(tmA, tmB, tmL, N, K, status, rows, stream);
+    else launch<Mode::kStatsKeep, false>(tmA, tmB, tmL, N, K, status, rows, stream);
+  } else if (entropy) {
+    launch<Mode::kStats, true>(tmA, tmB, tmA, N, K, status, rows, stream);
+  } else {
+    launch<Mode::kStats, false>(tmA, tmB, tmA, N, K, status, rows, stream);
+  }
 }
 
 void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labels64, const float2* lse, const float* entropy,

@@ -496,6 +496,112 @@ void token_log_probs_join(const float* stats, int slices, int slice_width, const
   check_cuda(cudaGetLastError(), "token_log_probs join launch");
 }
 
+// ------------------------------------------------------------------------- gradient of kept logits
+namespace {
+
+constexpr int GRAD_THREADS = 256;
+constexpr int GRAD_UNROLL = 4;  // vectors of eight columns per thread: 32 KB of a row per block
+
+// fp32 rows in, bf16 rows out; the blocks of a row are consecutive. Rows from the live ones to the next multiple of 256 are cleared, those
+// behind are left alone.
+template <bool ENTROPY>
+__global__ void __launch_bounds__(GRAD_THREADS)
+    grad_rows_kernel(const float* __restrict__ logits, long long ldl, const void* __restrict__ labels, bool labels64, const float2* __restrict__ lse, const float* __restrict__ entropy,
+                     const float* __restrict__ d_log_probs, long long d_log_probs_stride, const float* __restrict__ d_entropy, long long d_entropy_stride,
+                     __nv_bfloat16* __restrict__ grad, long long ldg, LiveRows live, int V, float logit_scale, float scale2, long long ignore_index, unsigned chunks) {
+  const unsigned chunk = blockIdx.x % chunks;
+  const int r = blockIdx.x / chunks;
+  const int rows = live.count == nullptr ? live.rows : max(0, min(live.rows, *live.count - live.base));
+  if (r >= rows && (live.count == nullptr || r >= max(256, (rows + 255) / 256 * 256))) return;
+  float gs = 0.f, hs = 0.f, H = 0.f;
+  float2 L = make_float2(0.f, 0.f);
+  long long label = -1;
+  if (r < rows) {
+    const long long t = live.index != nullptr ? live.index[live.base + r] : live.base + r;
+    label = load_label(labels, labels64, t);
+    if (label != ignore_index && label >= 0 && label < V) {
+      L = lse[t];
+      gs = d_log_probs[t * d_log_probs_stride] * logit_scale;
+      if (ENTROPY) {
+        hs = d_entropy[t * d_entropy_stride] * logit_scale;
+        H = entropy[t];
+      }
+    }
+  }
+  const bool zero = gs == 0.f && hs == 0.f;
+  const float* x = logits + (long long)r * ldl;
+  __nv_bfloat16* out = grad + (long long)r * ldg;
+  const int i0 = chunk * (GRAD_THREADS * GRAD_UNROLL) + threadIdx.x;
+  uint4 v[GRAD_UNROLL][2];
+  const bool whole = ((int)chunk + 1) * (GRAD_THREADS * GRAD_UNROLL * 8) <= V;
+  if (whole && !zero) {
+#pragma unroll
+    for (int k = 0; k < GRAD_UNROLL; ++k) {
+      const uint4* q = reinterpret_cast<const uint4*>(x + (long long)(i0 + k * GRAD_THREADS) * 8);
+      v[k][0] = __ldg(q);
+      v[k][1] = __ldg(q + 1);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < GRAD_UNROLL; ++k) {
+      uint32_t w[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = (i0 + k * GRAD_THREADS) * 8 + e;
+        w[e] = !zero && j < V ? __float_as_uint(x[j]) : 0u;
+      }
+      v[k][0] = make_uint4(w[0], w[1], w[2], w[3]);
+      v[k][1] = make_uint4(w[4], w[5], w[6], w[7]);
+    }
+  }
+  const float mc = L.x * scale2;
+  const bool product = fabsf(mc) < kProductLimit;
+  const float off = product ? -mc - L.y : -L.x;
+  const F2 c2 = pack2(scale2, scale2), off2 = pack2(off, off), log2_s = pack2(-L.y, -L.y), gs2 = pack2(-gs, -gs);
+#pragma unroll
+  for (int k = 0; k < GRAD_UNROLL; ++k) {
+    const int i = i0 + k * GRAD_THREADS;
+    if (i * 8 >= V) return;
+    F2 f[4];
+    Vec<float>::unpack(v[k][0], f);
+    Vec<float>::unpack(v[k][1], f + 2);
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 d = unpack2(product ? fma2(f[j], c2, off2) : fma2(add2(f[j], off2), c2, log2_s));
+      const F2 p = pack2(fast_exp2(d.x), fast_exp2(d.y));
+      float2 y;
+      if (ENTROPY) y = unpack2(mul2(p, pack2(-fmaf(hs, fmaf(fmaxf(d.x, kFloor2), kLn2, H), gs), -fmaf(hs, fmaf(fmaxf(d.y, kFloor2), kLn2, H), gs))));
+      else y = unpack2(mul2(p, gs2));
+      w[j] = zero ? 0u : pack_bf16x2(y.x, y.y);
+    }
+    if ((i + 1) * 8 <= V) {
+      *reinterpret_cast<uint4*>(out + (long long)i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (i * 8 + e < V) reinterpret_cast<uint16_t*>(out)[i * 8 + e] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+    }
+    // the label's own gradient, over the vector just written by this thread
+    if (!zero && label >> 3 == i) out[label] = __float2bfloat16(gs + score_gradient<ENTROPY>(log2_prob(x[label], L, scale2), gs, hs, H));
+  }
+}
+
+}  // namespace
+
+void token_log_probs_grad_rows(const float* logits, long long ldl, const void* labels, bool labels64, const float2* lse, const float* entropy, const float* d_log_probs,
+                               long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long ldg, LiveRows live, int N, float logit_scale,
+                               long long ignore_index, cudaStream_t stream) {
+  if (live.rows <= 0) return;
+  constexpr int kColumns = GRAD_THREADS * GRAD_UNROLL * 8;
+  const unsigned chunks = (unsigned)((N + kColumns - 1) / kColumns);
+  auto kernel = d_entropy != nullptr ? grad_rows_kernel<true> : grad_rows_kernel<false>;
+  kernel<<<(unsigned)live.rows * chunks, GRAD_THREADS, 0, stream>>>(logits, ldl, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
+                                                                    reinterpret_cast<__nv_bfloat16*>(grad), ldg, live, N, logit_scale, logit_scale * kLog2e, ignore_index, chunks);
+  count_launch();
+  check_cuda(cudaGetLastError(), "kept logits gradient launch");
+}
+
 // ------------------------------------------------------------------------- live rows of a batch
 namespace {
 

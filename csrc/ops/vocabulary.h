@@ -49,7 +49,8 @@ void token_log_probs_join(const float* stats, int slices, int slice_width, const
 // the logits stay in tensor memory.
 // x holds the rows of this launch; labels, lse and gradients are those of the whole batch.
 constexpr int kVocabSlice = 128;  // columns per slice of the statistics
-void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, bool entropy, LiveRows live, int N,
+// logits: null, or fp32 [live.rows, N] with a row stride ldl that is a multiple of 4, which keeps the live rows' logits.
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl, bool entropy, LiveRows live, int N,
                       int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream);
 // grad[live.rows, N] (bf16, row stride ldg, a multiple of 8): gradient of the logits, as token_log_probs_bwd defines it; rows behind
 // the live ones are 0 up to the next multiple of 256.
@@ -57,6 +58,11 @@ void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labe
                      const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
                      void* grad, LiveRows live, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
                      long long ignore_index, int* status, cudaStream_t stream);
+
+// The same from kept logits (fp32, row stride ldl), without a product.
+void token_log_probs_grad_rows(const float* logits, long long ldl, const void* labels, bool labels64, const float2* lse, const float* entropy, const float* d_log_probs,
+                               long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long ldg, LiveRows live, int N, float logit_scale,
+                               long long ignore_index, cudaStream_t stream);
 
 // ---- gemm/gemm_bf16_2sm.cu: the pair GEMM over the live rows of a compacted batch only: M (limit_k false) or K (true) ends at
 // max(1, *count - base). Rows from there to the next multiple of 256 must be 0 in both operands (they may be multiplied).

@@ -165,9 +165,9 @@ LiveRows live_rows(const Tensor& map, int64_t T, int64_t base, int64_t rows) {
 
 void* row_ptr(const Tensor& t, int64_t row) { return reinterpret_cast<char*>(t.data_ptr()) + row * t.stride(0) * t.element_size(); }
 
-// (log_probs, entropy, lse, the rows that were multiplied, row map)
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
-                                                                        bool want_entropy, const Tensor& status) {
+// (log_probs, entropy, lse, the rows that were multiplied, row map, their logits if they are kept)
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
+                                                                        bool want_entropy, bool keep_logits, const Tensor& status) {
   check_linear(x, w, labels);
   int* st = status_of(status, x);
   const c10::cuda::CUDAGuard guard(x.device());
@@ -178,7 +178,9 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Te
   float* ent = want_entropy ? entropy.data_ptr<float>() : nullptr;
   const bool compact = rows > kCompactAbove;
   Tensor map = torch::empty({compact ? 2 * rows + 1 : 0}, x.options().dtype(torch::kInt32)), xc = x;
-  if (rows == 0) return {log_probs, entropy, lse, xc, map};
+  Tensor logits;
+  if (keep_logits) logits = empty_f32(rows * ((V + 3) / 4 * 4), x).view({rows, (V + 3) / 4 * 4});
+  if (rows == 0) return {log_probs, entropy, lse, xc, map, logits};
   if (compact) {
     int* m = map.data_ptr<int>();
     xc = torch::empty({rows, H}, x.options());
@@ -189,12 +191,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Te
   Tensor stats = empty_f32(most * slices * 4, x);
   for (int64_t r = 0; r < rows; r += most) {
     const LiveRows live = live_rows(map, rows, r, std::min(most, rows - r));
-    vocab_gemm_stats(row_ptr(xc, r), w.data_ptr(), labels.data_ptr(), labels64, stats.data_ptr<float>(), want_entropy, live, (int)V, (int)H, xc.stride(0), w.stride(0),
+    vocab_gemm_stats(row_ptr(xc, r), w.data_ptr(), labels.data_ptr(), labels64, stats.data_ptr<float>(), keep_logits ? reinterpret_cast<float*>(row_ptr(logits, r)) : nullptr,
+                     keep_logits ? logits.stride(0) : 0, want_entropy, live, (int)V, (int)H, xc.stride(0), w.stride(0),
                      (float)logit_scale, st, stream);
     token_log_probs_join(stats.data_ptr<float>(), (int)slices, kVocabSlice, labels.data_ptr(), labels64, log_probs.data_ptr<float>(), ent, pairs(lse), live, (int)V,
                          (float)logit_scale, ignore_index, stream);
   }
-  return {log_probs, entropy, lse, xc, map};
+  return {log_probs, entropy, lse, xc, map, logits};
 }
 
 // out (+)= a b of the products that follow: rows of the batch (or of its live rows) are the rows of a, or what both are contracted over.
@@ -405,14 +408,15 @@ OptTensor main_grad(const Tensor& weight) {
   return t;
 }
 
-// Forward keeps 16 bytes per row and 128 columns of logits; backward forms the logits again, chunk of rows by chunk, as their bf16
-// gradient, and multiplies that with the weight and the hidden states. Batches of more than 256 rows are compacted to the rows whose
-// label counts, and all four products end there.
+// Forward reduces the logits to 16 bytes per row and 128 columns. Backward needs them again: kept in fp32 where `keep_logits` says so, else
+// formed a second time; either way they become, chunk of rows by chunk, their bf16 gradient, which is multiplied with the weight and
+// the hidden states. Both ways see the same fp32 logits. Batches of more than 256 rows are compacted to the
+// rows whose label counts, and all products end there.
 struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy, int64_t chunk,
-                               const Tensor& status) {
-    auto [log_probs, entropy, lse, xc, map] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy, status);
-    ctx->save_for_backward({xc, w, labels, lse, entropy, map, status});
+                               bool keep_logits, const Tensor& status) {
+    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy, keep_logits, status);
+    ctx->save_for_backward({xc, w, labels, lse, entropy, map, status, logits});
     ctx->saved_data["logit_scale"] = logit_scale;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["chunk"] = chunk;
@@ -422,9 +426,9 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5];
+    const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5], &logits = saved[7];
     const bool has_h = grads.size() > 1 && grads[1].defined();
-    if (!grads[0].defined() && !has_h) return variable_list(8);
+    if (!grads[0].defined() && !has_h) return variable_list(9);
     const int64_t T = xc.size(0), H = xc.size(1), V = w.size(0);
     const int64_t chunk = std::max<int64_t>(std::min(ctx->saved_data["chunk"].toInt(), T), 1);
     const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
@@ -450,9 +454,16 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
       const int64_t n = std::min(chunk, T - r);
       const LiveRows live = live_rows(map, T, r, n);
       const Tensor dl = dlogits.narrow(0, 0, n), xr = xc.narrow(0, r, n);
-      vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels.scalar_type() == torch::kInt64, pairs(lse), has_h ? entropy.data_ptr<float>() : nullptr, gp, g_stride, hp,
-                      h_stride, dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0), dl.stride(0), (float)ctx->saved_data["logit_scale"].toDouble(),
-                      ctx->saved_data["ignore_index"].toInt(), st, stream);
+      const bool labels64 = labels.scalar_type() == torch::kInt64;
+      const float logit_scale = (float)ctx->saved_data["logit_scale"].toDouble();
+      const int64_t ignore_index = ctx->saved_data["ignore_index"].toInt();
+      const float* ent = has_h ? entropy.data_ptr<float>() : nullptr;
+      if (logits.defined())
+        token_log_probs_grad_rows(reinterpret_cast<const float*>(row_ptr(logits, r)), logits.stride(0), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(),
+                                  dl.stride(0), live, (int)V, logit_scale, ignore_index, stream);
+      else
+        vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0),
+                        dl.stride(0), logit_scale, ignore_index, st, stream);
       if (need_dx) {
         Tensor out = dx.narrow(0, r, n);
         product(dl, w, out, false, live, st, stream);
@@ -464,7 +475,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
       vocab_scatter_rows(dx.data_ptr(), live_rows(map, T, 0, T).index + T, scattered.data_ptr(), (int)T, (int)H, stream);
       dx = scattered;
     }
-    variable_list out(8);
+    variable_list out(9);
     if (need_dx) out[0] = once(dx, "fused_linear_token_log_probs");
     if (need_dw && !target.has_value()) out[1] = once(dw.to(w.scalar_type()), "fused_linear_token_log_probs");
     return out;
@@ -494,7 +505,8 @@ Tensor mapped_rows(const Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
-variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool return_entropy, int64_t chunk, const Tensor& status) {
+variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool return_entropy, int64_t chunk, int64_t keep_bytes,
+                                     const Tensor& status) {
   check_logit_scale(logit_scale);
   TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(0) > 0 && w.size(1) > 0, "hidden states [..., H] and a weight [V, H] are needed, got ", text(x.sizes()), " and ",
                     text(w.sizes()));
@@ -502,8 +514,9 @@ variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Ten
                     text(x.device()), " and ", text(w.scalar_type()), " on ", text(w.device()));
   const auto shape = x.sizes().slice(0, x.dim() - 1);
   check_label_shape(labels, shape, x);
+  const bool keep = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()) && 4.0 * (double)labels.numel() * (double)w.size(0) <= (double)keep_bytes;
   variable_list out = LinearTokenLogProbs::apply(mapped_rows(x.reshape({labels.numel(), x.size(-1)})), mapped_rows(w), labels.reshape({labels.numel()}).contiguous(), logit_scale, ignore_index,
-                                                 return_entropy, chunk, status);
+                                                 return_entropy, chunk, keep, status);
   if (x.dim() != 2)
     for (auto& t : out) t = t.view(shape);
   return out;

@@ -261,9 +261,9 @@ POLICY = (0.2, 0.2, 0.0, 0.0, 1)
     lambda C: C.token_log_probs(F32(3, 5), I64(4), 1.0, -100, False),
     lambda C: C.token_log_probs(F32(3, 0), I64(3), 1.0, -100, False),
     lambda C: C.token_log_probs(F32(3, 5), I64(3), -0.5, -100, False),
-    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 9), I64(3), 1.0, -100, False, 256, F32(1)),
-    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 8).half(), I64(3), 1.0, -100, False, 256, F32(1)),
-    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 8), I64(3), math.inf, -100, False, 256, F32(1)),
+    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 9), I64(3), 1.0, -100, False, 256, 0, F32(1)),
+    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 8).half(), I64(3), 1.0, -100, False, 256, 0, F32(1)),
+    lambda C: C.linear_token_log_probs(F32(3, 8), F32(5, 8), I64(3), math.inf, -100, False, 256, 0, F32(1)),
     lambda C: C.preference_loss(F32(3, 3), None, None, None, *LOSS.values()),
     lambda C: C.preference_loss(F32(12), None, None, None, *LOSS.values()),
     lambda C: C.preference_loss(F32(12), None, F32(5), None, *LOSS.values()),

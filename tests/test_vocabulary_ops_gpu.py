@@ -177,7 +177,11 @@ def _check_linear(x, w, labels, g, h, lp, ent, dx, dw, scale=1.0, ignore_index=-
 
 @pytest.mark.parametrize("tokens,hidden,vocab", [(1, 8, 1), (3, 64, 40), (130, 72, 257), (256, 128, 1024), (300, 256, 1003), (777, 512, 5000)])
 @pytest.mark.parametrize("entropy", [False, True])
-def test_fused_linear_token_log_probs(tokens, hidden, vocab, entropy):
+@pytest.mark.parametrize("keep", [0, 4 << 30])
+def test_fused_linear_token_log_probs(tokens, hidden, vocab, entropy, keep, monkeypatch):
+    import lm_engine.ops.vocabulary as vocabulary
+
+    monkeypatch.setattr(vocabulary, "_KEEP_LOGITS_BYTES", keep)
     x, w, labels, g, h = _linear_case(tokens, hidden, vocab, tokens)
     if tokens > 2:
         labels[0], labels[2] = -100, -7
@@ -213,11 +217,35 @@ def test_fused_linear_token_log_probs_in_chunks_and_into_main_grad(monkeypatch):
     _check_linear(x, w, labels, g, zero, lp.detach(), None, x.grad, w.main_grad - 2.0)
 
 
-@pytest.mark.parametrize("kept", [0.0, 0.01, 0.5])
-@pytest.mark.parametrize("chunk", [128, 384, 4096])
-def test_fused_linear_token_log_probs_leaves_ignored_rows_out(kept, chunk, monkeypatch):
+@pytest.mark.parametrize("tokens,hidden,vocab", [(1, 8, 1), (130, 72, 257), (300, 256, 1003), (1000, 64, 5000)])
+@pytest.mark.parametrize("entropy", [False, True])
+def test_fused_linear_token_log_probs_kept_or_formed_twice_are_the_same(tokens, hidden, vocab, entropy, monkeypatch):
     import lm_engine.ops.vocabulary as vocabulary
 
+    x, w, labels, g, h = _linear_case(tokens, hidden, vocab, tokens)
+    labels[::3] = -100
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    results = []
+    for keep in (0, 1 << 30):
+        monkeypatch.setattr(vocabulary, "_KEEP_LOGITS_BYTES", keep)
+        out = ops.fused_linear_token_log_probs(x, w, labels, logit_scale=1.25, return_entropy=entropy)
+        outs = out if entropy else (out,)
+        results.append((*outs, *torch.autograd.grad(outs, (x, w), [g, h][: len(outs)])))
+    for i, (a, b) in enumerate(zip(*results)):
+        if i < len(outs):
+            assert torch.equal(a, b)
+        else:  # the exponents' last rounding differs: (x - m) c - log2 s against x c - (m c + log2 s)
+            assert (a.float() - b.float()).norm() <= 2.0**-10 * b.float().norm()
+
+
+@pytest.mark.parametrize("keep", [0, 4 << 30])
+@pytest.mark.parametrize("kept", [0.0, 0.01, 0.5])
+@pytest.mark.parametrize("chunk", [128, 384, 4096])
+def test_fused_linear_token_log_probs_leaves_ignored_rows_out(kept, chunk, keep, monkeypatch):
+    import lm_engine.ops.vocabulary as vocabulary
+
+    monkeypatch.setattr(vocabulary, "_KEEP_LOGITS_BYTES", keep)
     monkeypatch.setattr(vocabulary, "_flce_chunk_rows", lambda T, V: min(T, chunk))
     x, w, labels, g, h = _linear_case(1000, 64, 333, 8)
     labels[torch.rand(1000, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) >= kept] = -100
