@@ -69,8 +69,8 @@ struct KernelOpts {
   const __nv_bfloat16* fc;  // EPI_SWIGLU_BWD: the saved projection [M, 2 I] = [up | gate]
   long long ldfc;   // its row stride in elements
   int split_k;      // >= 1; > 1 only with the bulk-reduction epilogues: each tile is computed as that many partial sums over K
-  const int* live;  // null, or the device's count of live rows: M (limit_k 0) or K (1) ends at max(1, *live - live_base)
-  int live_base, limit_k;
+  const int* live;  // null, or the device's count of live rows: K ends at max(1, *live - live_base)
+  int live_base;
   long long* trace; // TRACE builds: TRACE_WORDS cycle counters per CTA
 };
 
@@ -100,11 +100,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   const bool leader = cta_rank == 0;
   const int pair = blockIdx.x >> 1;
   const int num_pairs = gridDim.x >> 1;
-  if (opts.live != nullptr) {
-    const int rows = max(1, *opts.live - opts.live_base);
-    if (opts.limit_k) K = min(K, rows);
-    else M = min(M, rows);
-  }
+  if (opts.live != nullptr) K = min(K, max(1, *opts.live - opts.live_base));
   const int m_tiles = (M + 2 * BM - 1) / (2 * BM);
   const int n_tiles = (N + BN - 1) / BN;
   const int k_blocks = (K + BK - 1) / BK;
@@ -659,7 +655,7 @@ PairGemmTuning& pair_gemm_tuning() { return g_tuning; }
 namespace {
 
 void pair_gemm(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
-               bool a_mn, bool b_mn, int epi, float alpha, const int* live, int live_base, bool limit_k, int* status, int max_ctas, cudaStream_t stream) {
+               bool a_mn, bool b_mn, int epi, float alpha, const int* live, int live_base, int* status, int max_ctas, cudaStream_t stream) {
   if (M <= 0 || N <= 0 || K <= 0) return;
   if ((lda & 7) || (ldb & 7)) throw std::runtime_error("gemm_bf16_2sm: leading dimensions of A and B must be multiples of 8");
   LaunchArgs a;
@@ -681,7 +677,6 @@ void pair_gemm(const void* A, const void* B, void* C, int M, int N, int K, long 
   a.opts.split_k = 1;
   a.opts.live = live;
   a.opts.live_base = live_base;
-  a.opts.limit_k = limit_k ? 1 : 0;
   // (a K that only the device knows is not split: a part could come out empty)
   if (c_ok && (epi == EPI_F32_ACC || epi == EPI_BF16_ACC) && max_ctas <= 0 && live == nullptr)
     a.opts.split_k = g_tuning.split_k > 0 ? g_tuning.split_k : default_split(M, N, K, sm_count() / 2);
@@ -704,12 +699,12 @@ void pair_gemm(const void* A, const void* B, void* C, int M, int N, int K, long 
 // Same contract as gemm_bf16 (see gemm_bf16.cu).
 void gemm_bf16_2sm(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
                    bool a_mn, bool b_mn, int epi, float alpha, int* status, int max_ctas, cudaStream_t stream) {
-  pair_gemm(A, B, C, M, N, K, lda, ldb, ldc, a_mn, b_mn, epi, alpha, nullptr, 0, false, status, max_ctas, stream);
+  pair_gemm(A, B, C, M, N, K, lda, ldb, ldc, a_mn, b_mn, epi, alpha, nullptr, 0, status, max_ctas, stream);
 }
 
-void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, bool a_mn, bool b_mn, bool f32_accumulate,
-                        const int* count, int base, bool limit_k, int* status, cudaStream_t stream) {
-  pair_gemm(A, B, C, M, N, K, lda, ldb, ldc, a_mn, b_mn, f32_accumulate ? EPI_F32_ACC : EPI_BF16, 1.f, count, base, limit_k, status, 0, stream);
+void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, bool f32_accumulate, LiveRows live, int* status,
+                        cudaStream_t stream) {
+  pair_gemm(A, B, C, M, N, K, lda, ldb, ldc, true, true, f32_accumulate ? EPI_F32_ACC : EPI_BF16, 1.f, live.count, live.base, status, 0, stream);
 }
 
 // fc[M, 2I] = A[M, K] W[2I, K]^T (both halves stored) and act[M, I] = fc[:, :I] * silu(fc[:, I:]) in one kernel.
@@ -731,7 +726,7 @@ void gemm_bf16_swiglu(const void* A, const void* W, void* fc, void* act, int M, 
   a.opts.fc = nullptr;
   a.opts.ldfc = 0;
   a.opts.live = nullptr;
-  a.opts.live_base = a.opts.limit_k = 0;
+  a.opts.live_base = 0;
   a.opts.split_k = 1;
   a.opts.trace = nullptr;
   launch_variant<0, 0, EPI_SWIGLU, false>(a);
@@ -758,7 +753,7 @@ void gemm_bf16_swiglu_bwd(const void* dy, const void* W, const void* fc, void* d
   a.opts.fc = reinterpret_cast<const __nv_bfloat16*>(fc);
   a.opts.ldfc = ldfc;
   a.opts.live = nullptr;
-  a.opts.live_base = a.opts.limit_k = 0;
+  a.opts.live_base = 0;
   a.opts.split_k = 1;
   a.opts.trace = g_tuning.trace;
   if (a.opts.trace != nullptr) launch_variant<0, 1, EPI_SWIGLU_BWD, true>(a);

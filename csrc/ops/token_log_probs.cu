@@ -612,7 +612,7 @@ constexpr int COMPACT_THREADS = 256;
 
 __global__ void __launch_bounds__(COMPACT_THREADS)
     compact_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, const __nv_bfloat16* __restrict__ x, long long ldx, int H, int share,
-                        int* __restrict__ index, int* __restrict__ slot, int* __restrict__ count, __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs,
+                        int* __restrict__ index, int* __restrict__ count, __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs,
                         float* __restrict__ entropy, float2* __restrict__ lse) {
   __shared__ int warp_count[COMPACT_THREADS / 32], place[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -638,7 +638,6 @@ __global__ void __launch_bounds__(COMPACT_THREADS)
       const int p = before + __popc(votes & ((1u << lane) - 1));  // live rows before t
       before += __popc(votes);
       if (t < end) {
-        slot[t] = live ? p : -1;
         if (live) {
           index[p] = t;
         } else {
@@ -666,30 +665,17 @@ __global__ void __launch_bounds__(COMPACT_THREADS)
   }
 }
 
-__global__ void __launch_bounds__(128) scatter_rows_kernel(const __nv_bfloat16* __restrict__ compact, const int* __restrict__ slot, __nv_bfloat16* __restrict__ out, int H) {
-  const int t = blockIdx.x, r = slot[t];
-  uint4* dst = reinterpret_cast<uint4*>(out + (long long)t * H);
-  const uint4* src = r >= 0 ? reinterpret_cast<const uint4*>(compact + (long long)r * H) : nullptr;
-  for (int i = threadIdx.x; i < H / 8; i += blockDim.x) dst[i] = src != nullptr ? src[i] : make_uint4(0, 0, 0, 0);
-}
-
 }  // namespace
 
-void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* slot, int* count, void* compact,
+void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* count, void* compact,
                         float* log_probs, float* entropy, float2* lse, cudaStream_t stream) {
   // a row per warp as long as that makes at most 1024 blocks (each of them reads all labels before its rows)
   int share = 8;
   while ((T + share - 1) / share > 1024) share *= 2;
-  compact_rows_kernel<<<(T + share - 1) / share, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V, reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, share, index, slot, count,
+  compact_rows_kernel<<<(T + share - 1) / share, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V, reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, share, index, count,
                                                                                reinterpret_cast<__nv_bfloat16*>(compact), log_probs, entropy, lse);
   count_launch();
   check_cuda(cudaGetLastError(), "compact rows launch");
-}
-
-void vocab_scatter_rows(const void* compact, const int* slot, void* out, int T, int H, cudaStream_t stream) {
-  scatter_rows_kernel<<<T, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(compact), slot, reinterpret_cast<__nv_bfloat16*>(out), H);
-  count_launch();
-  check_cuda(cudaGetLastError(), "scatter rows launch");
 }
 
 }  // namespace b200

@@ -33,13 +33,10 @@ struct LiveRows {
   const int* count;
   int base, rows;
 };
-// index[0 .. *count) <- rows with a label in [0, V) other than ignore_index, in order; slot[t] <- compact row of t or -1; compact[r] <-
+// index[0 .. *count) <- rows with a label in [0, V) other than ignore_index, in order; compact[r] <-
 // x[index[r]] (bf16 rows of H, a multiple of 8 elements), zeros from *count on; outputs of the rows that do not count <- 0.
-void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* slot, int* count, void* compact,
+void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* count, void* compact,
                         float* log_probs, float* entropy, float2* lse, cudaStream_t stream);
-// out[t] <- compact[slot[t]], zeros where there is none
-void vocab_scatter_rows(const void* compact, const int* slot, void* out, int T, int H, cudaStream_t stream);
-
 // Joins the statistics of `slices` column slices of the rows: stats[slice][live.rows] = (m, s, u, the label's logit if it lies in the
 // slice), see softmax_stats.cuh. Ignored rows give 0.
 void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
@@ -64,10 +61,17 @@ void token_log_probs_grad_rows(const float* logits, long long ldl, const void* l
                                long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long ldg, LiveRows live, int N, float logit_scale,
                                long long ignore_index, cudaStream_t stream);
 
-// ---- gemm/gemm_bf16_2sm.cu: the pair GEMM over the live rows of a compacted batch only: M (limit_k false) or K (true) ends at
-// max(1, *count - base). Rows from there to the next multiple of 256 must be 0 in both operands (they may be multiplied).
-void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, bool a_mn, bool b_mn, bool f32_accumulate,
-                        const int* count, int base, bool limit_k, int* status, cudaStream_t stream);
+// ---- gemm/streamk_gemm_2sm.cu: C [live.rows, N] = A [live.rows, K] B [K, N], bf16, for few tiles and a long K. Tiles that several CTA
+// pairs share leave fp32 partial tiles in `partials` (streamk_partials() words); streamk_rows puts the result together and writes live
+// row r to row t of `out`, its place in the batch. lda, ldb and N: multiples of 8; C and out: rows of N.
+long long streamk_partials();
+void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream);
+void streamk_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream);
+
+// ---- gemm/gemm_bf16_2sm.cu: C [M, N] (+)= A [K, M]^T B [K, N] on CTA pairs, where the K rows are those of a compacted batch: the
+// contraction ends at max(1, *count - base). Rows from there to the next multiple of 64 must be 0 in both operands.
+void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, bool f32_accumulate, LiveRows live, int* status,
+                        cudaStream_t stream);
 
 // ---- ops/preference.cu
 // A packed batch of `sequences` sequences of per-token values: sequence i is tokens [cu[i], cu[i + 1]), or, without cu,

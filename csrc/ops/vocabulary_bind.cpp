@@ -153,13 +153,13 @@ int64_t stats_rows(int64_t rows, int64_t slices) {
 // A batch of more rows than one tile is compacted to its live rows first: a tile is computed whole, so a smaller batch gains nothing.
 constexpr int64_t kCompactAbove = 256;
 
-// map: int32 [2 T + 1] = index [T], slot [T], count, or empty where the batch is not compacted
+// map: int32 [T + 1] = index [T], count, or empty where the batch is not compacted
 LiveRows live_rows(const Tensor& map, int64_t T, int64_t base, int64_t rows) {
   LiveRows live = {nullptr, nullptr, (int)base, (int)rows};
   if (map.numel() == 0) return live;
-  TORCH_CHECK(map.is_cuda() && map.scalar_type() == torch::kInt32 && map.is_contiguous() && map.numel() == 2 * T + 1, "the row map must be int32 [2 T + 1]");
+  TORCH_CHECK(map.is_cuda() && map.scalar_type() == torch::kInt32 && map.is_contiguous() && map.numel() == T + 1, "the row map must be int32 [T + 1]");
   live.index = map.data_ptr<int>();
-  live.count = map.data_ptr<int>() + 2 * T;
+  live.count = map.data_ptr<int>() + T;
   return live;
 }
 
@@ -177,14 +177,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(
   Tensor log_probs = empty_f32(rows, x), lse = empty_pairs(rows, x), entropy = want_entropy ? empty_f32(rows, x) : Tensor();
   float* ent = want_entropy ? entropy.data_ptr<float>() : nullptr;
   const bool compact = rows > kCompactAbove;
-  Tensor map = torch::empty({compact ? 2 * rows + 1 : 0}, x.options().dtype(torch::kInt32)), xc = x;
+  Tensor map = torch::empty({compact ? rows + 1 : 0}, x.options().dtype(torch::kInt32)), xc = x;
   Tensor logits;
   if (keep_logits) logits = empty_f32(rows * ((V + 3) / 4 * 4), x).view({rows, (V + 3) / 4 * 4});
   if (rows == 0) return {log_probs, entropy, lse, xc, map, logits};
   if (compact) {
     int* m = map.data_ptr<int>();
     xc = torch::empty({rows, H}, x.options());
-    vocab_compact_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, x.data_ptr(), x.stride(0), (int)H, m, m + rows, m + 2 * rows, xc.data_ptr(),
+    vocab_compact_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, x.data_ptr(), x.stride(0), (int)H, m, m + rows, xc.data_ptr(),
                        log_probs.data_ptr<float>(), ent, pairs(lse), stream);
   }
   const int64_t most = stats_rows(rows, slices);
@@ -198,17 +198,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(
                          (float)logit_scale, ignore_index, stream);
   }
   return {log_probs, entropy, lse, xc, map, logits};
-}
-
-// out (+)= a b of the products that follow: rows of the batch (or of its live rows) are the rows of a, or what both are contracted over.
-void product(const Tensor& a, const Tensor& b, Tensor& out, bool contract_rows, const LiveRows& live, int* status, cudaStream_t stream) {
-  const int M = (int)out.size(0), N = (int)out.size(1), K = (int)(contract_rows ? a.size(0) : a.size(1));
-  const bool f32 = out.scalar_type() == torch::kFloat32;  // fp32 outputs are added to
-  if (live.count != nullptr)
-    gemm_bf16_2sm_live(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, a.stride(0), b.stride(0), out.stride(0), contract_rows, true, f32, live.count, live.base, contract_rows, status,
-                       stream);
-  else
-    (M >= 256 ? gemm_bf16_2sm : gemm_bf16)(a.data_ptr(), b.data_ptr(), out.data_ptr(), M, N, K, a.stride(0), b.stride(0), out.stride(0), contract_rows, true, f32 ? 2 : 0, 1.f, status, 0, stream);
 }
 
 // ------------------------------------------------------------------------- losses over sequences
@@ -439,8 +428,13 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     int* st = status_of(saved[6], xc);
     const c10::cuda::CUDAGuard guard(xc.device());
     const cudaStream_t stream = stream_of(xc);
-    Tensor dx, dw;
-    if (need_dx) dx = torch::empty({T, H}, xc.options());
+    Tensor dx, dw, dxc, partials;
+    if (need_dx) {
+      dx = torch::empty({T, H}, xc.options());
+      if (map.numel() > 0) embedding_zero(dx.data_ptr(), T * H * 2, stream);  // rows that take no part
+      dxc = torch::empty({std::min(chunk, T), H}, xc.options());
+      partials = empty_f32(streamk_partials(), xc);
+    }
     OptTensor target;
     if (need_dw) {
       target = main_grad(w);
@@ -465,15 +459,17 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
         vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0),
                         dl.stride(0), logit_scale, ignore_index, st, stream);
       if (need_dx) {
-        Tensor out = dx.narrow(0, r, n);
-        product(dl, w, out, false, live, st, stream);
+        streamk_gemm(dl.data_ptr(), w.data_ptr(), dxc.data_ptr(), partials.data_ptr<float>(), live, (int)H, (int)V, dl.stride(0), w.stride(0), st, stream);
+        streamk_rows(dxc.data_ptr(), partials.data_ptr<float>(), live, dx.data_ptr(), (int)H, (int)V, stream);
       }
-      if (need_dw) product(dl, xr, dw, true, live, st, stream);
-    }
-    if (need_dx && map.numel() > 0) {
-      Tensor scattered = torch::empty_like(dx);
-      vocab_scatter_rows(dx.data_ptr(), live_rows(map, T, 0, T).index + T, scattered.data_ptr(), (int)T, (int)H, stream);
-      dx = scattered;
+      if (need_dw) {
+        const bool f32 = dw.scalar_type() == torch::kFloat32;
+        if (live.count != nullptr)
+          gemm_bf16_2sm_live(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0), dw.stride(0), f32, live, st, stream);
+        else
+          (V >= 256 ? gemm_bf16_2sm : gemm_bf16)(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0), dw.stride(0), true, true, f32 ? 2 : 0, 1.f,
+                                                 st, 0, stream);
+      }
     }
     variable_list out(9);
     if (need_dx) out[0] = once(dx, "fused_linear_token_log_probs");
