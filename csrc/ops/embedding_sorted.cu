@@ -113,11 +113,36 @@ __global__ void __launch_bounds__(LOOKUP_THREADS)
   }
 }
 
+// ------------------------------------------------------------------------- zeros
+// A share of the zero fill of a new gradient, carried by the blocks of a kernel behind those that do its own work: sorting is a chain of
+// latencies on few SMs, filling is all bandwidth, and together they take the longer of the two (32768 x 4096 of 128256:
+// 141 us of fill and 27 of sorting become 148).
+struct Fill {
+  uint4* p;
+  long long n;  // 16-byte words
+  int tail;     // bytes behind them
+};
+constexpr int FILL_WORDS = 8;  // per thread
+
+__device__ __forceinline__ void fill_zero(const Fill& f, long long block) {
+  if (block == 0 && threadIdx.x < f.tail) reinterpret_cast<unsigned char*>(f.p + f.n)[threadIdx.x] = 0;
+  const long long base = block * (FILL_WORDS * blockDim.x) + threadIdx.x;
+#pragma unroll
+  for (int k = 0; k < FILL_WORDS; ++k) {
+    const long long i = base + k * blockDim.x;
+    if (i < f.n) f.p[i] = make_uint4(0, 0, 0, 0);
+  }
+}
+
 // ------------------------------------------------------------------------- sort
 // Each thread owns one pair of a compare-exchange step. Steps of distance <= 32 stay inside of the 64 keys of a warp.
 __global__ void __launch_bounds__(RUN / 2)
-    sort_runs_kernel(const void* __restrict__ ids, bool ids64, uint64_t* __restrict__ keys, long long T, long long V) {
+    sort_runs_kernel(const void* __restrict__ ids, bool ids64, uint64_t* __restrict__ keys, long long T, long long V, int runs, Fill fill) {
   __shared__ uint64_t s[RUN];
+  if (blockIdx.x >= runs) {
+    fill_zero(fill, blockIdx.x - runs);
+    return;
+  }
   const long long base = (long long)blockIdx.x * RUN;
   const int size = 2 * blockDim.x;  // power of two, >= 64
   for (int i = threadIdx.x; i < size; i += blockDim.x) {
@@ -151,7 +176,11 @@ __global__ void __launch_bounds__(RUN / 2)
 }
 
 // One level: groups of FAN sorted runs of `length` keys (a power of two; the last run may be short) become one sorted run each.
-__global__ void __launch_bounds__(128) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int T, int log_length) {
+__global__ void __launch_bounds__(128) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int T, int log_length, int blocks, Fill fill) {
+  if (blockIdx.x >= blocks) {
+    fill_zero(fill, blockIdx.x - blocks);
+    return;
+  }
   const int i = blockIdx.x * 128 + threadIdx.x;
   if (i >= T) return;
   const uint64_t key = in[i];
@@ -307,14 +336,6 @@ __global__ void __launch_bounds__(JOIN_THREADS)
   }
 }
 
-__global__ void __launch_bounds__(256) fill_zero_kernel(uint4* __restrict__ p, long long n, int tail) {
-  if (blockIdx.x == 0 && threadIdx.x < tail) reinterpret_cast<unsigned char*>(p + n)[threadIdx.x] = 0;
-  const long long base = (long long)blockIdx.x * 1024 + threadIdx.x;
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (base + k * 256 < n) p[base + k * 256] = make_uint4(0, 0, 0, 0);
-}
-
 template <typename T>
 bool wide_rows(int H, const void* a, const void* b) {
   return (long long)H * sizeof(T) % 16 == 0 && reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(b) % 16 == 0;
@@ -384,14 +405,6 @@ void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids
   check_cuda(cudaGetLastError(), "embedding lookup launch");
 }
 
-void embedding_zero(void* p, long long bytes, cudaStream_t stream) {
-  if (bytes == 0) return;
-  const long long n = bytes / 16;
-  fill_zero_kernel<<<(unsigned)(n / 1024 + 1), 256, 0, stream>>>(reinterpret_cast<uint4*>(p), n, (int)(bytes % 16));
-  count_launch();
-  check_cuda(cudaGetLastError(), "embedding gradient fill launch");
-}
-
 long long embedding_gradient_workspace(long long T, int H, Scalar type) {
   const int columns = SUM_THREADS * (type == Scalar::kF32 ? 4 : 8);  // narrower slabs never make more chunks
   const int n = chunk_tokens(T, H, columns);
@@ -401,17 +414,30 @@ long long embedding_gradient_workspace(long long T, int H, Scalar type) {
 
 void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids64, void* dweight, bool accumulate, void* workspace,
                         long long T, long long V, int H, float scale, cudaStream_t stream) {
-  if (T == 0 || H == 0) return;
+  if (H == 0 || (T == 0 && accumulate)) return;
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
   uint64_t* other = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(workspace) + key_bytes(T));
   float* partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 2 * key_bytes(T));
   int threads = 32;
   while (threads < RUN / 2 && 2 * threads < T) threads *= 2;
-  sort_runs_kernel<<<(unsigned)((T + RUN - 1) / RUN), threads, 0, stream>>>(ids, ids64, keys, T, V);
+  int kernels = 1;
+  for (int log_length = LOG_RUN; (1LL << log_length) < T; log_length += LOG_FAN) ++kernels;
+  // every kernel of the sort carries the same share of the zeros of a new gradient
+  const long long size = type == Scalar::kF32 ? 4 : 2, bytes = accumulate ? 0 : V * H * size, words = bytes / 16;
+  auto share = [&](int k) {
+    const long long begin = words * k / kernels, end = words * (k + 1) / kernels;
+    return Fill{reinterpret_cast<uint4*>(dweight) + begin, end - begin, k + 1 == kernels ? (int)(bytes % 16) : 0};
+  };
+  auto fill_blocks = [](const Fill& f, int block) { return (unsigned)((f.n + FILL_WORDS * block - 1) / (FILL_WORDS * block) + (f.n == 0 && f.tail > 0 ? 1 : 0)); };
+  const unsigned runs = (unsigned)((T + RUN - 1) / RUN), blocks = (unsigned)((T + 127) / 128);
+  Fill fill = share(0);
+  sort_runs_kernel<<<runs + fill_blocks(fill, threads), threads, 0, stream>>>(ids, ids64, keys, T, V, (int)runs, fill);
   count_launch();
   check_cuda(cudaGetLastError(), "embedding gradient sort launch");
-  for (int log_length = LOG_RUN; (1LL << log_length) < T; log_length += LOG_FAN) {
-    merge_runs_kernel<<<(unsigned)((T + 127) / 128), 128, 0, stream>>>(keys, other, (int)T, log_length);
+  int k = 1;
+  for (int log_length = LOG_RUN; (1LL << log_length) < T; log_length += LOG_FAN, ++k) {
+    fill = share(k);
+    merge_runs_kernel<<<blocks + fill_blocks(fill, 128), 128, 0, stream>>>(keys, other, (int)T, log_length, (int)blocks, fill);
     count_launch();
     check_cuda(cudaGetLastError(), "embedding gradient merge launch");
     uint64_t* t = keys;
@@ -419,7 +445,7 @@ void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids
     other = t;
   }
   auto launch = type == Scalar::kBf16 ? gradient<__nv_bfloat16> : type == Scalar::kF16 ? gradient<__half> : gradient<float>;
-  launch(dout, keys, dweight, accumulate, partials, T, H, scale, stream);
+  if (T > 0) launch(dout, keys, dweight, accumulate, partials, T, H, scale, stream);
 }
 
 }  // namespace b200

@@ -125,12 +125,10 @@ constexpr int kStatusBadTokenId = 7;  // an id outside of [0, V): its output row
 // out[t] = scale * weight[ids[t]]
 void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids64, void* out, long long T, long long V, int H,
                       float scale, int* status, cudaStream_t stream);
-// Zeros over `bytes` bytes from a 16-byte aligned address.
-void embedding_zero(void* p, long long bytes, cudaStream_t stream);
 // Bytes of the workspace of the gradient (256-byte aligned).
 long long embedding_gradient_workspace(long long T, int H, Scalar type);
-// Rows of dweight that some id names: scale * sum of dout[t] over the tokens with that id, in the order of t; other rows are
-// not touched. accumulate: dweight is fp32 and is added to, else it has dout's type and is overwritten.
+// dweight[v] = scale * sum of dout[t] over the tokens with id v, in the order of t. accumulate: dweight is fp32, is added to, and rows
+// that no id names are not touched; else it has dout's type, is 16-byte aligned, and is written whole.
 void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids64, void* dweight, bool accumulate, void* workspace,
                         long long T, long long V, int H, float scale, cudaStream_t stream);
 

@@ -330,7 +330,6 @@ Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, con
     contiguous_f32(dw, dout, V * H, "dweight");
   } else {
     dw = torch::empty({V, H}, dout.options());
-    embedding_zero(dw.data_ptr(), V * H * dw.element_size(), stream_of(dout));
   }
   Tensor workspace = torch::empty({embedding_gradient_workspace(T, (int)H, type)}, dout.options().dtype(torch::kUInt8));
   embedding_gradient(dout.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, dw.data_ptr(), dweight.has_value(), workspace.data_ptr(), T, V, (int)H, (float)scale,
@@ -430,8 +429,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     const cudaStream_t stream = stream_of(xc);
     Tensor dx, dw, dxc, partials;
     if (need_dx) {
-      dx = torch::empty({T, H}, xc.options());
-      if (map.numel() > 0) embedding_zero(dx.data_ptr(), T * H * 2, stream);  // rows that take no part
+      dx = map.numel() > 0 ? torch::zeros({T, H}, xc.options()) : torch::empty({T, H}, xc.options());  // rows that take no part: 0
       dxc = torch::empty({std::min(chunk, T), H}, xc.options());
       partials = empty_f32(streamk_partials(), xc);
     }
