@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(RUN / 2)
     return;
   }
   const long long base = (long long)blockIdx.x * RUN;
-  const int size = 2 * blockDim.x;  // power of two, >= 64
+  const int size = 2 * blockDim.x;  // a power of two above 64
   for (int i = threadIdx.x; i < size; i += blockDim.x) {
     const long long t = base + i;
     uint64_t key = kNoKey;
@@ -418,8 +418,7 @@ void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
   uint64_t* other = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(workspace) + key_bytes(T));
   float* partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 2 * key_bytes(T));
-  int threads = 32;
-  while (threads < RUN / 2 && 2 * threads < T) threads *= 2;
+  const int threads = T <= RUN / 2 ? RUN / 4 : RUN / 2;  // two keys each; not fewer, for the blocks that fill
   int kernels = 1;
   for (int log_length = LOG_RUN; (1LL << log_length) < T; log_length += LOG_FAN) ++kernels;
   // every kernel of the sort carries the same share of the zeros of a new gradient

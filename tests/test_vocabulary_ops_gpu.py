@@ -555,3 +555,58 @@ def test_outputs_may_be_changed_in_place_and_second_derivatives_are_refused():
     pair.loss.mul_(3.0)
     pair.chosen_rewards.add_(1.0)
     assert pair.loss.item() == pytest.approx(3 * math.log(2), rel=1e-6)
+
+
+def test_offsets_past_32_bits():
+    """2.6e9 logits and a table of 2.2e9 values: the last rows are those of a small call."""
+    tokens, vocab = 20011, 128256
+    logits = torch.zeros(tokens, vocab, device="cuda", dtype=torch.bfloat16)
+    gen = torch.Generator("cuda").manual_seed(0)
+    logits[-3:] = torch.randn(3, vocab, generator=gen, device="cuda")
+    labels = torch.full((tokens,), -100, device="cuda")
+    labels[-3:] = torch.tensor([0, vocab - 1, 77], device="cuda")
+    logits.requires_grad_(True)
+    lp = ops.token_log_probs(logits, labels)
+    (grad,) = torch.autograd.grad(lp.sum(), logits)
+    one = torch.ones(3, device="cuda", dtype=torch.float64)
+    _check_log_probs(logits.detach()[-3:].double(), labels[-3:], -100, one, 0 * one, lp[-3:], None, grad[-3:], 1.0, torch.bfloat16)
+    assert (lp[:-3] == 0).all() and grad[:-3].abs().max() == 0
+    del logits, grad
+    w = torch.zeros(550_000, 4096, device="cuda", dtype=torch.bfloat16)
+    w[-1] = torch.randn(4096, generator=gen, device="cuda")
+    w.requires_grad_(True)
+    ids = torch.tensor([549_999, 3, 549_999], device="cuda", dtype=torch.int32)
+    out = ops.embedding(w, ids, sorted_gradient=True)
+    assert torch.equal(out[0], w.detach()[-1]) and torch.equal(out[2], out[0]) and (out[1] == 0).all()
+    (grad,) = torch.autograd.grad(out, w, torch.ones_like(out))
+    assert (grad[-1] == 2).all() and (grad[3] == 1).all() and grad.sum(dtype=torch.float64).item() == 3 * 4096
+
+
+def test_on_a_stream_of_its_own_and_twice_at_once():
+    """Two streams run the same step on their own inputs at the same time; both give what the default stream gives."""
+    def step(seed):
+        x, w, labels, g, h = _linear_case(400, 128, 3000, seed)
+        labels[::5] = -100
+        x.requires_grad_(True)
+        w.requires_grad_(True)
+        ids = labels.clamp_min(0)
+        lp = ops.fused_linear_token_log_probs(x, w, labels)
+        cu = torch.tensor([0, 100, 150, 350, 400], device="cuda", dtype=torch.int32)
+        pref = ops.preference_loss(lp, lp.detach() - 0.1 * g, cu)
+        pol = ops.policy_loss(lp, lp.detach() + 0.3 * h, g, cu_seqlens=cu)
+        emb = ops.embedding(w, ids, 0.5, sorted_gradient=True)
+        grads = torch.autograd.grad(pref.loss + pol.loss + (emb * x.detach()).sum(), (x, w))
+        return [t.detach() for t in (lp, pref.loss, pol.loss, emb, *grads)]
+
+    want = [step(s) for s in (1, 2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [None, None]
+    for _ in range(3):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = step(i + 1)
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for s, t in zip(a, b):
+            assert torch.equal(s, t)
