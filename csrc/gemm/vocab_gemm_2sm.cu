@@ -18,6 +18,12 @@
 // scheduler and each instruction waiting for the one before, the epilogue of a tile with entropy took about 20000 cycles and
 // bounded the kernel up to K = 2048 (16384 cycles of MMAs a tile).
 //
+// The tensor cores' fp32 accumulator is truncated at every step of 16 products, an error that grows with K and always points the same way.
+// So K is taken in parts of 1024: the epilogue threads add the parts up in registers, 128 columns a thread, rounding to nearest, while
+// the tensor cores work on the next part (about 700 cycles against 8192). Log-probabilities at K = 4096 against 64 bits, relative:
+// 1.5e-6 in one part, 3.5e-7 in parts of 1024 (at every larger K), 1.8e-7 in parts of 512. 4096 x 4096 x 128256 takes the same time either way;
+// 777 x 2048 x 49152, whose last epilogue is not covered, 145 us in one part, 153 in parts of 1024, 158 in parts of 512.
+//
 // Rows whose label does not count are left out of all products: the batch is compacted to its live rows beforehand, whose number only
 // the device knows (LiveRows), so the kernel takes its row count from memory and the grid is sized for the whole batch.
 #include <cuda.h>
@@ -38,6 +44,7 @@ constexpr int BN = 256;       // columns per pair
 constexpr int SLICES = BN / kVocabSlice;
 constexpr int BN_HALF = 128;  // W rows staged per CTA
 constexpr int BK = 64;
+constexpr int PART = 16;      // k-blocks whose products stay in the tensor cores' accumulator
 constexpr int STAGES = 6;
 constexpr int A_STAGE_BYTES = BM * BK * 2;
 constexpr int B_STAGE_BYTES = BN_HALF * BK * 2;
@@ -63,13 +70,23 @@ struct RowArgs {
   long long ignore_index;
 };
 
+// 16 columns of this warp's 32 lanes (with 32 at a time the accumulators of a thread no longer fit its registers).
+__device__ __forceinline__ void tmem_load_16(uint32_t (&v)[16], uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]),
+        "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(addr)
+      : "memory");
+}
+
 enum class Mode : int { kStats, kStatsKeep, kGrad };
 
-// v[i] of 32 registers for a lane's own i: halved five times, so that the array stays in registers.
-__device__ __forceinline__ uint32_t select32_bits(const uint32_t (&v)[32], int i) {
-  uint32_t t[16];
+// x[i] of 32 registers for a lane's own i: halved five times, so that the array stays in registers.
+__device__ __forceinline__ float select32(const float (&x)[32], int i) {
+  float t[16];
 #pragma unroll
-  for (int k = 0; k < 16; ++k) t[k] = (i & 16) ? v[k + 16] : v[k];
+  for (int k = 0; k < 16; ++k) t[k] = (i & 16) ? x[k + 16] : x[k];
 #pragma unroll
   for (int k = 0; k < 8; ++k) t[k] = (i & 8) ? t[k + 8] : t[k];
 #pragma unroll
@@ -171,39 +188,43 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint32_t idesc = umma_idesc_bf16(2 * BM, BN, 0, 0);
       uint32_t it = 0, tcount = 0;
       bool ok = true;
-      for (int tile = pair; tile < total && ok; tile += num_pairs, ++tcount) {
-        const uint32_t buf = tcount & 1;
-        const uint32_t aph = (tcount >> 1) & 1;
-        if (!mbar_wait(&acc_empty[buf], aph ^ 1, abort_flag)) {
-          raise_status(status, kStatusWaitTimeoutMma, abort_flag);
-          break;
-        }
-        tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + buf * BN;
-        for (int kb = 0; kb < k_blocks; ++kb, ++it) {
-          const uint32_t s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          if (!mbar_wait(&full[s], ph, abort_flag)) {
+      for (int tile = pair; tile < total && ok; tile += num_pairs) {
+        for (int part = 0; part < k_blocks && ok; part += PART, ++tcount) {
+          const uint32_t buf = tcount & 1;
+          const uint32_t aph = (tcount >> 1) & 1;
+          if (!mbar_wait(&acc_empty[buf], aph ^ 1, abort_flag)) {
             raise_status(status, kStatusWaitTimeoutMma, abort_flag);
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t a_base = smem_u32(sA + s * A_STAGE_BYTES);
-          const uint32_t b_base = smem_u32(sB + s * B_STAGE_BYTES);
+          const uint32_t d_tmem = tmem_base + buf * BN;
+          const int part_end = min(k_blocks, part + PART);
+          for (int kb = part; kb < part_end; ++kb, ++it) {
+            const uint32_t s = it % STAGES;
+            const uint32_t ph = (it / STAGES) & 1;
+            if (!mbar_wait(&full[s], ph, abort_flag)) {
+              raise_status(status, kStatusWaitTimeoutMma, abort_flag);
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t a_base = smem_u32(sA + s * A_STAGE_BYTES);
+            const uint32_t b_base = smem_u32(sB + s * B_STAGE_BYTES);
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k) {
-            umma_f16_ss_2sm(d_tmem, umma_smem_desc_sw128(a_base + k * 32, 16, 1024), umma_smem_desc_sw128(b_base + k * 32, 16, 1024),
-                            idesc, (kb != 0 || k != 0) ? 1u : 0u);
+            for (int k = 0; k < BK / 16; ++k) {
+              umma_f16_ss_2sm(d_tmem, umma_smem_desc_sw128(a_base + k * 32, 16, 1024), umma_smem_desc_sw128(b_base + k * 32, 16, 1024),
+                              idesc, (kb != part || k != 0) ? 1u : 0u);
+            }
+            const uint32_t e_local = smem_u32(&empty[s]);  // release the stage in both CTAs
+            umma_commit_2sm(map_to_cta(e_local, 0));
+            umma_commit_2sm(map_to_cta(e_local, 1));
           }
-          const uint32_t e_local = smem_u32(&empty[s]);  // release the stage in both CTAs
-          umma_commit_2sm(map_to_cta(e_local, 0));
-          umma_commit_2sm(map_to_cta(e_local, 1));
-        }
-        if (ok) {
-          const uint32_t f_local = smem_u32(&acc_full[buf]);
-          umma_commit_2sm(map_to_cta(f_local, 0));
-          umma_commit_2sm(map_to_cta(f_local, 1));
+          if (ok) {
+            const uint32_t f_local = smem_u32(&acc_full[buf]);
+            umma_commit_2sm(map_to_cta(f_local, 0));
+            umma_commit_2sm(map_to_cta(f_local, 1));
+          }
         }
       }
     }
@@ -215,17 +236,16 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint8_t* box = sStage + (warp - 2) * BOX_BYTES;
     const float scale2 = rows.logit_scale * kLog2e;
     uint32_t tcount = 0;
-    for (int tile = pair; tile < total; tile += num_pairs, ++tcount) {
+    bool ok = true;
+    for (int tile = pair; tile < total && ok; tile += num_pairs) {
       const TileCoord tc = tile_coord(tile, m_tiles, n_tiles, group);
-      const uint32_t buf = tcount & 1;
-      const uint32_t aph = (tcount >> 1) & 1;
       const int row0 = tc.mi * (2 * BM) + (int)cta_rank * BM + q * 32;
       const int row = row0 + lane;
       const int slice_col0 = tc.ni * BN + half * kVocabSlice;
       // the label's column relative to the slice; -1: not here
       int label = -1;
       bool ignored = true;
-      long long t = 0;  // the row's place in the batch
+      int t = 0;  // the row's place in the batch
       if (row < live) {
         t = rows.live.index != nullptr ? rows.live.index[rows.live.base + row] : rows.live.base + row;
         const long long l = load_label(rows.labels, rows.labels64, t);
@@ -237,46 +257,57 @@ __global__ void __launch_bounds__(THREADS, 1)
       bool zero = true;
       if (MODE == Mode::kGrad && !ignored) {
         L = rows.lse[t];
-        gs = rows.d_log_probs[t * rows.d_log_probs_stride] * rows.logit_scale;
+        gs = rows.d_log_probs[(long long)t * rows.d_log_probs_stride] * rows.logit_scale;
         if (ENTROPY) {
-          hs = rows.d_entropy[t * rows.d_entropy_stride] * rows.logit_scale;
+          hs = rows.d_entropy[(long long)t * rows.d_entropy_stride] * rows.logit_scale;
           H = rows.entropy[t];
         }
         zero = gs == 0.f && hs == 0.f;
       }
-      if (!mbar_wait(&acc_full[buf], aph, abort_flag)) {
-        raise_status(status, kStatusWaitTimeoutEpilogue, abort_flag);
-        break;
-      }
-      tc_fence_after_sync();
-      const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + half * kVocabSlice;
-      if (slice_col0 >= N) {  // nothing of the vocabulary here: the accumulator is handed back unread
+      // the parts of K, added up
+      float acc[kVocabSlice];
+#pragma unroll
+      for (int e = 0; e < kVocabSlice; ++e) acc[e] = 0.f;
+#pragma unroll 1
+      for (int part = 0; part < k_blocks; part += PART, ++tcount) {
+        const uint32_t buf = tcount & 1;
+        const uint32_t aph = (tcount >> 1) & 1;
+        if (!mbar_wait(&acc_full[buf], aph, abort_flag)) {
+          raise_status(status, kStatusWaitTimeoutEpilogue, abort_flag);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t t_row = tmem_base + (uint32_t(q * 32) << 16) + buf * BN + half * kVocabSlice;
+#pragma unroll
+        for (int c = 0; c < kVocabSlice / 16; ++c) {
+          uint32_t v[16];
+          tmem_load_16(v, t_row + c * 16);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[c * 16 + e] += __uint_as_float(v[e]);
+        }
+        // hand the TMEM buffer back
+        tc_fence_before_sync();
         __syncwarp();
         if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
-        continue;
       }
+      if (!ok || slice_col0 >= N) continue;  // nothing of the vocabulary here
 
       if (MODE != Mode::kGrad) {
         Stats st = empty_stats();
         float x_label = 0.f;
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < kVocabSlice / 32; ++c) {
           const int col0 = slice_col0 + c * 32;
           if (col0 >= N) break;
-          uint32_t v[32];
-          B200_TMEM_LD_32(v, t_row + c * 32);
-          tmem_ld_wait();
-          if (c == kVocabSlice / 32 - 1 || col0 + 32 >= N) {
-            // last read of this accumulator: hand the TMEM buffer back before the arithmetic
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
-          }
+          float(&x)[32] = *reinterpret_cast<float(*)[32]>(acc + c * 32);
           if (MODE == Mode::kStatsKeep) {
             if (lane == 0) tma_store_wait_read<0>();  // the store that used the box before has read it
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j) box_write(box, lane, j, make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+            for (int j = 0; j < 8; ++j)
+              box_write(box, lane, j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])));
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && row0 < live) {
@@ -287,21 +318,21 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (col0 + 32 > N) {
 #pragma unroll
             for (int e = 0; e < 32; ++e)
-              if (col0 + e >= N) v[e] = __float_as_uint(-INFINITY);
+              if (col0 + e >= N) x[e] = -INFINITY;
           }
-          if ((label >> 5) == c) x_label = __uint_as_float(select32_bits(v, label & 31));
-          float top = __uint_as_float(v[0]);
+          if ((label >> 5) == c) x_label = select32(x, label & 31);
+          float top = x[0];
           F2 f[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            top = fmaxf(top, fmaxf(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])));
-            f[e] = pack2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1]));
+            top = fmaxf(top, fmaxf(x[2 * e], x[2 * e + 1]));
+            f[e] = pack2(x[2 * e], x[2 * e + 1]);
           }
           accumulate<ENTROPY, 32>(st, f, top, scale2);
         }
         if (row < live) rows.stats[(long long)(tc.ni * SLICES + half) * rows.live.rows + row] = make_float4(st.m, st.s, st.u, x_label);
       } else {
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < kVocabSlice / 64; ++c) {
           const int col0 = slice_col0 + c * 64;
           if (col0 >= N) break;
@@ -309,30 +340,23 @@ __global__ void __launch_bounds__(THREADS, 1)
           __syncwarp();
 #pragma unroll
           for (int part = 0; part < 2; ++part) {
-            uint32_t v[32];
-            B200_TMEM_LD_32(v, t_row + c * 64 + part * 32);
-            tmem_ld_wait();
+            const float(&x)[32] = *reinterpret_cast<const float(*)[32]>(acc + c * 64 + part * 32);
             uint32_t w[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-              const float a = score_gradient<ENTROPY>(log2_prob(__uint_as_float(v[2 * e]), L, scale2), gs, hs, H);
-              const float b = score_gradient<ENTROPY>(log2_prob(__uint_as_float(v[2 * e + 1]), L, scale2), gs, hs, H);
+              const float a = score_gradient<ENTROPY>(log2_prob(x[2 * e], L, scale2), gs, hs, H);
+              const float b = score_gradient<ENTROPY>(log2_prob(x[2 * e + 1], L, scale2), gs, hs, H);
               w[e] = zero ? 0u : pack_bf16x2(a, b);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) box_write(box, lane, part * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
             if ((label >> 5) == 2 * c + part && !zero) {
               // the label's own gradient, over the element of the row just written
-              const float d = log2_prob(__uint_as_float(select32_bits(v, label & 31)), L, scale2);
+              const float d = log2_prob(select32(x, label & 31), L, scale2);
               const int e = label & 63;
               *reinterpret_cast<__nv_bfloat16*>(box + lane * 128 + (((e >> 3) ^ (lane & 7)) << 4) + (e & 7) * 2) =
                   __float2bfloat16(gs + score_gradient<ENTROPY>(d, gs, hs, H));
             }
-          }
-          if (c == kVocabSlice / 64 - 1 || col0 + 64 >= N) {
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&acc_empty[buf]), 0));
           }
           fence_proxy_async_smem();
           __syncwarp();
