@@ -2,7 +2,7 @@
 //   dW[v] = scale * sum over t with id_t = v, in ascending t, of dout[t]
 //
 // The gradient sorts the pairs (id, t) as 64-bit keys, which are distinct, so the order is unique and every sum is taken in
-// the same order on every run; nothing is added atomically. Sorting: runs of 512 keys in shared memory (bitonic), then
+// the same order on every run; nothing is added atomically. Sorting: runs of 1024 keys in shared memory (bitonic), then
 // levels that merge 16 runs at a time by rank: a key's place is its place in its own run plus the number of smaller keys in
 // each of the 15 others (independent binary searches, 16 loads in flight). Summing: a block takes 8 to 128 consecutive sorted
 // tokens (a chunk) and a slab of columns and reads each dout row once; a run of equal ids inside of the chunk goes straight to its row of
@@ -20,7 +20,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int LOG_RUN = 9, RUN = 1 << LOG_RUN;  // keys sorted by one block
+constexpr int LOG_RUN = 10, RUN = 1 << LOG_RUN;  // keys sorted by one block
 constexpr int LOG_FAN = 4, FAN = 1 << LOG_FAN;  // runs merged per level
 constexpr int MAX_CHUNK = 128;   // sorted tokens summed by one block, at most
 constexpr int SUM_THREADS = 128;
@@ -418,7 +418,8 @@ void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
   uint64_t* other = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(workspace) + key_bytes(T));
   float* partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 2 * key_bytes(T));
-  const int threads = T <= RUN / 2 ? RUN / 4 : RUN / 2;  // two keys each; not fewer, for the blocks that fill
+  // two keys each; not fewer than 128, for the blocks that fill
+  const int threads = T <= RUN / 4 ? RUN / 8 : T <= RUN / 2 ? RUN / 4 : RUN / 2;
   int kernels = 1;
   for (int log_length = LOG_RUN; (1LL << log_length) < T; log_length += LOG_FAN) ++kernels;
   // every kernel of the sort carries the same share of the zeros of a new gradient
