@@ -317,11 +317,17 @@ __global__ void __launch_bounds__(JOIN_THREADS)
 #pragma unroll
       for (int e = 0; e < N; ++e) acc[e] = element<float, N>(v, e);
     }
-#pragma unroll 8
-    for (int k = lane; k < parts; k += JOIN_LANES) {
-      const Pack<float, N> v = load_pack<float, N>(partials + 2LL * (chunk + 1 + k) * H + c);
+    constexpr int BATCH = 8;
+    for (int k0 = lane; k0 < parts; k0 += BATCH * JOIN_LANES) {
+      Pack<float, N> v[BATCH];
 #pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] += element<float, N>(v, e);
+      for (int b = 0; b < BATCH; ++b) v[b] = load_pack<float, N>(partials + 2LL * (chunk + 1 + min(k0 + b * JOIN_LANES, parts - 1)) * H + c);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        if (k0 + b * JOIN_LANES >= parts) break;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += element<float, N>(v[b], e);
+      }
     }
   }
 #pragma unroll
