@@ -93,4 +93,31 @@ __device__ __forceinline__ void box_write(uint8_t* box, int lane, int chunk, uin
   *reinterpret_cast<uint4*>(box + lane * 128 + ((chunk ^ (lane & 7)) << 4)) = v;
 }
 
+// Rows of the K-major A operand that the two CTAs of a pair fetch per k-block. A batch of at most one tile fetches the rows that it has
+// (a multiple of eight): rows of a box that lie outside of the matrix are zeros, but they are asked for all the same, all at
+// one address, and with a single row the pairs queued up there (scores of 1 x 4096 x 128256: 262 to 300 us, depending on where the
+// row lay; XXX with boxes of eight rows).
+struct RowBoxes {
+  int rows0, rows1;
+
+  explicit RowBoxes(int rows) : rows0(128), rows1(128) {
+    if (rows <= 128) {
+      rows0 = (rows + 7) / 8 * 8;
+      rows1 = 0;
+    } else if (rows <= 256) {
+      rows1 = (rows - 128 + 7) / 8 * 8;
+    }
+  }
+};
+
+// Zeros in the rows of each stage that no copy fills (whole block; 128 rows of 128 bytes per stage).
+__device__ __forceinline__ void clear_rows(uint8_t* stages, int count, int stage_bytes, int filled) {
+  const int words = (128 - filled) * 8;
+  for (int i = threadIdx.x; i < count * words; i += blockDim.x) {
+    const int s = i / words;
+    *reinterpret_cast<uint4*>(stages + s * stage_bytes + filled * 128 + (i - s * words) * 16) = make_uint4(0, 0, 0, 0);
+  }
+  if (words > 0) fence_proxy_async_smem();  // the tensor cores read them through the async proxy
+}
+
 }  // namespace b200

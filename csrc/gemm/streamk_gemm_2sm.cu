@@ -98,8 +98,8 @@ __device__ __forceinline__ int live_count(const LiveRows& live) {
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-    streamk_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-                            const __grid_constant__ CUtensorMap tmP, int N, int K, LiveRows live, int* status) {
+    streamk_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+                            const __grid_constant__ CUtensorMap tmP, int N, int K, RowBoxes rows, LiveRows live, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -133,6 +133,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
+  clear_rows(sA, STAGES, A_STAGE_BYTES, cta_rank == 0 ? rows.rows0 : rows.rows1);
   __syncthreads();
   if (warp == 1) {
     tmem_alloc_2sm(tmem_slot, TMEM_COLS);
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
-      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(leader ? &tmA : &tmA1);
       tma_prefetch_desc(&tmB);
       uint32_t it = 0;
       bool ok = true;
@@ -165,9 +166,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             break;
           }
           const uint32_t full_leader = map_to_cta(smem_u32(&full[s]), 0);
-          if (leader) mbar_arrive_expect_tx(&full[s], 2 * (A_STAGE_BYTES + B_STAGE_BYTES));
+          if (leader) mbar_arrive_expect_tx(&full[s], (rows.rows0 + rows.rows1) * (BK * 2) + 2 * B_STAGE_BYTES);
           uint8_t* b_dst = sB + s * B_STAGE_BYTES;
-          tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA, full_leader, kb * BK, m0);
+          if (leader) tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA, full_leader, kb * BK, m0);
+          else if (rows.rows1 > 0) tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA1, full_leader, kb * BK, m0);
 #pragma unroll
           for (int j = 0; j < BN_HALF / 64; ++j) tma_load_2d_pair(b_dst + j * (BK * 128), &tmB, full_leader, n0 + j * 64, kb * BK);
         }
@@ -344,7 +346,9 @@ long long streamk_partials() { return 2LL * grid_pairs() * (2 * BM) * BN; }
 
 void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
-  const CUtensorMap tmA = make_tensor_map_2d_b16(A, K, live.rows, lda, BK, BM);
+  const RowBoxes rows(live.rows);
+  const CUtensorMap tmA = make_tensor_map_2d_b16(A, K, live.rows, lda, BK, rows.rows0);
+  const CUtensorMap tmA1 = make_tensor_map_2d_b16(A, K, live.rows, lda, BK, rows.rows1 > 0 ? rows.rows1 : rows.rows0);
   const CUtensorMap tmB = make_tensor_map_2d_b16(B, N, K, ldb, 64, BK);
   const CUtensorMap tmC = make_tensor_map_2d_b16(C, N, live.rows, N, 64, 32);
   const CUtensorMap tmP = make_tensor_map_2d_f32(partials, BN, 2LL * grid_pairs() * (2 * BM), BN, 32, 32);
@@ -361,7 +365,7 @@ void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRo
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, streamk_gemm_2sm_kernel, tmA, tmB, tmC, tmP, N, K, live, status), "stream-k gemm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, streamk_gemm_2sm_kernel, tmA, tmA1, tmB, tmC, tmP, N, K, rows, live, status), "stream-k gemm launch");
   count_launch();
 }
 

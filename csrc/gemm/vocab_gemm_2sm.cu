@@ -98,8 +98,8 @@ __device__ __forceinline__ float select32(const float (&x)[32], int i) {
 
 template <Mode MODE, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 1)
-    vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                          const __grid_constant__ CUtensorMap tmOut, int N, int K, int* status, RowArgs rows) {
+    vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB,
+                          const __grid_constant__ CUtensorMap tmOut, int N, int K, RowBoxes box, int* status, RowArgs rows) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -141,6 +141,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     *abort_flag = 0;
     fence_barrier_init();
   }
+  clear_rows(sA, STAGES, A_STAGE_BYTES, cta_rank == 0 ? box.rows0 : box.rows1);
   __syncthreads();
   if (warp == 1) {
     tmem_alloc_2sm(tmem_slot, TMEM_COLS);
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (warp == 0) {
     // ------------------------------------------------------------------ TMA producer (both CTAs)
     if (lane == 0) {
-      tma_prefetch_desc(&tmA);
+      tma_prefetch_desc(leader ? &tmA : &tmA1);
       tma_prefetch_desc(&tmB);
       uint32_t it = 0;
       bool ok = true;
@@ -172,8 +173,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             break;
           }
           const uint32_t full_leader = map_to_cta(smem_u32(&full[s]), 0);
-          if (leader) mbar_arrive_expect_tx(&full[s], 2 * (A_STAGE_BYTES + B_STAGE_BYTES));
-          tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA, full_leader, kb * BK, m0);
+          if (leader) mbar_arrive_expect_tx(&full[s], (box.rows0 + box.rows1) * (BK * 2) + 2 * B_STAGE_BYTES);
+          if (leader) tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA, full_leader, kb * BK, m0);
+          else if (box.rows1 > 0) tma_load_2d_pair(sA + s * A_STAGE_BYTES, &tmA1, full_leader, kb * BK, m0);
           tma_load_2d_pair(sB + s * B_STAGE_BYTES, &tmB, full_leader, kb * BK, n0);
         }
       }
@@ -233,7 +235,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // ------------------------------------------------------------------ epilogue: 32 rows x 128 columns of this CTA's 128 x 256 half
     const int q = warp & 3;             // the quarter of the lanes that this warp can read
     const int half = (warp - 2) >> 2;   // its half of the columns
-    uint8_t* box = sStage + (warp - 2) * BOX_BYTES;
+    uint8_t* store_box = sStage + (warp - 2) * BOX_BYTES;
     const float scale2 = rows.logit_scale * kLog2e;
     uint32_t tcount = 0;
     bool ok = true;
@@ -307,11 +309,11 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              box_write(box, lane, j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])));
+              box_write(store_box, lane, j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])));
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && row0 < live) {
-              tma_store_2d(&tmOut, box, col0, row0);
+              tma_store_2d(&tmOut, store_box, col0, row0);
               tma_store_commit();
             }
           }
@@ -349,19 +351,19 @@ __global__ void __launch_bounds__(THREADS, 1)
               w[e] = zero ? 0u : pack_bf16x2(a, b);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) box_write(box, lane, part * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
+            for (int j = 0; j < 4; ++j) box_write(store_box, lane, part * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
             if ((label >> 5) == 2 * c + part && !zero) {
               // the label's own gradient, over the element of the row just written
               const float d = log2_prob(select32(x, label & 31), L, scale2);
               const int e = label & 63;
-              *reinterpret_cast<__nv_bfloat16*>(box + lane * 128 + (((e >> 3) ^ (lane & 7)) << 4) + (e & 7) * 2) =
+              *reinterpret_cast<__nv_bfloat16*>(store_box + lane * 128 + (((e >> 3) ^ (lane & 7)) << 4) + (e & 7) * 2) =
                   __float2bfloat16(gs + score_gradient<ENTROPY>(d, gs, hs, H));
             }
           }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0 && row0 < rows.live.rows) {
-            tma_store_2d(&tmOut, box, col0, row0);
+            tma_store_2d(&tmOut, store_box, col0, row0);
             tma_store_commit();
           }
         }
@@ -385,9 +387,13 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 template <Mode MODE, bool ENTROPY>
-void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmOut, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
+void launch(const void* x, long long ldx, const CUtensorMap& tmB, const CUtensorMap* out, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
   auto kernel = vocab_gemm_2sm_kernel<MODE, ENTROPY>;
   check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "vocab gemm smem attr");
+  const RowBoxes box(rows.live.rows);
+  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, rows.live.rows, ldx, BK, box.rows0);
+  const CUtensorMap tmA1 = make_tensor_map_2d_b16(x, K, rows.live.rows, ldx, BK, box.rows1 > 0 ? box.rows1 : box.rows0);
+  const CUtensorMap& tmOut = out != nullptr ? *out : tmA;
   const int m_tiles = (rows.live.rows + 2 * BM - 1) / (2 * BM), n_tiles = (N + BN - 1) / BN;
   int pairs = sm_count() / 2;
   if ((long long)m_tiles * n_tiles < pairs) pairs = m_tiles * n_tiles;
@@ -403,7 +409,7 @@ void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& t
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmB, tmOut, N, K, status, rows), "vocab gemm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, kernel, tmA, tmA1, tmB, tmOut, N, K, box, status, rows), "vocab gemm launch");
   count_launch();
 }
 
@@ -412,7 +418,6 @@ void launch(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& t
 void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl, bool entropy, LiveRows live, int N,
                       int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
-  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, live.rows, ldx, BK, BM);
   const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
   RowArgs rows = {};
   rows.live = live;
@@ -423,12 +428,12 @@ void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool lab
   rows.ignore_index = -1;  // every label outside of [0, N) counts as none here
   if (logits != nullptr) {
     const CUtensorMap tmL = make_tensor_map_2d_f32(logits, N, live.rows, ldl, 32, 32);
-    if (entropy) launch<Mode::kStatsKeep, true>(tmA, tmB, tmL, N, K, status, rows, stream);
-    else launch<Mode::kStatsKeep, false>(tmA, tmB, tmL, N, K, status, rows, stream);
+    if (entropy) launch<Mode::kStatsKeep, true>(x, ldx, tmB, &tmL, N, K, status, rows, stream);
+    else launch<Mode::kStatsKeep, false>(x, ldx, tmB, &tmL, N, K, status, rows, stream);
   } else if (entropy) {
-    launch<Mode::kStats, true>(tmA, tmB, tmA, N, K, status, rows, stream);
+    launch<Mode::kStats, true>(x, ldx, tmB, nullptr, N, K, status, rows, stream);
   } else {
-    launch<Mode::kStats, false>(tmA, tmB, tmA, N, K, status, rows, stream);
+    launch<Mode::kStats, false>(x, ldx, tmB, nullptr, N, K, status, rows, stream);
   }
 }
 
@@ -437,7 +442,6 @@ void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labe
                      void* grad, LiveRows live, int N, int K, long long ldx, long long ldw, long long ldg, float logit_scale,
                      long long ignore_index, int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
-  const CUtensorMap tmA = make_tensor_map_2d_b16(x, K, live.rows, ldx, BK, BM);
   const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
   const CUtensorMap tmG = make_tensor_map_2d_b16(grad, N, live.rows, ldg, 64, 32);
   RowArgs rows = {};
@@ -452,8 +456,8 @@ void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labe
   rows.d_entropy_stride = d_entropy_stride;
   rows.logit_scale = logit_scale;
   rows.ignore_index = ignore_index;
-  if (d_entropy != nullptr) launch<Mode::kGrad, true>(tmA, tmB, tmG, N, K, status, rows, stream);
-  else launch<Mode::kGrad, false>(tmA, tmB, tmG, N, K, status, rows, stream);
+  if (d_entropy != nullptr) launch<Mode::kGrad, true>(x, ldx, tmB, &tmG, N, K, status, rows, stream);
+  else launch<Mode::kGrad, false>(x, ldx, tmB, &tmG, N, K, status, rows, stream);
 }
 
 }  // namespace b200
