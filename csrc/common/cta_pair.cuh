@@ -96,7 +96,7 @@ __device__ __forceinline__ void box_write(uint8_t* box, int lane, int chunk, uin
 // Rows of the K-major A operand that the two CTAs of a pair fetch per k-block. A batch of at most one tile fetches the rows that it has
 // (a multiple of eight): rows of a box that lie outside of the matrix are zeros, but they are asked for all the same, all at
 // one address, and with a single row the pairs queued up there (scores of 1 x 4096 x 128256: 262 to 300 us, depending on where the
-// row lay; XXX with boxes of eight rows).
+// row lay; 204 with boxes of eight rows).
 struct RowBoxes {
   int rows0, rows1;
 

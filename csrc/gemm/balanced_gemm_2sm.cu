@@ -2,11 +2,11 @@
 // vocabulary. bf16 operands (A K-major, B row-major), fp32 accumulation, bf16 result.
 //
 // A 256 x 256 output tile on a CTA pair takes K / 64 steps, and M N / 65536 tiles seldom divide by the 74 pairs: 14 x 16 tiles take
-// four rounds where 3.03 would do, 1 x 16 tiles leave 58 pairs idle. So the rounds that occupy every pair are worked on tile by tile (the
-// pairs walk K together and share their operands in L2), and when at most half of the pairs would have a tile in the last round, the
+// four waves where 3.03 would do, 1 x 16 tiles leave 58 pairs idle. So the waves that occupy every pair are worked on tile by tile (the
+// pairs walk K together and share their operands in L2), and when at most half of the pairs would have a tile in the last wave, the
 // steps of its tiles, tile after tile, are cut into equal ranges, one per pair. A tile that lies in one range is stored as bf16; of a
 // tile that is cut, every pair that worked on it leaves an fp32 partial tile (at most two per pair: the tile its range begins in and the
-// one it ends in), and streamk_rows adds them in the order of the pairs, so the result does not depend on the order of execution.
+// one it ends in), and balanced_rows adds them in the order of the pairs, so the result does not depend on the order of execution.
 // The number of rows may be known on the device only (LiveRows): the cut is computed there, the same way by both kernels.
 //
 // Staging and synchronisation are those of the pair GEMM of gemm_bf16_2sm.cu. 3584 live rows x 4096 x 128256: 3.23 ms with whole
@@ -98,7 +98,7 @@ __device__ __forceinline__ int live_count(const LiveRows& live) {
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-    streamk_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
+    balanced_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
                             const __grid_constant__ CUtensorMap tmP, int N, int K, RowBoxes rows, LiveRows live, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 // The product's live rows at their places in the batch: out[t] (bf16, N columns, a multiple of 8) is the row of C where the tile was
 // computed whole, and the sum of its partial tiles in the order of the pairs where it was cut. One block per row.
 __global__ void __launch_bounds__(128)
-    streamk_rows_kernel(const __nv_bfloat16* __restrict__ C, const float* __restrict__ partials, LiveRows live, __nv_bfloat16* __restrict__ out, int N, int K, int pairs) {
+    balanced_rows_kernel(const __nv_bfloat16* __restrict__ C, const float* __restrict__ partials, LiveRows live, __nv_bfloat16* __restrict__ out, int N, int K, int pairs) {
   const int r = blockIdx.x, rows = live_count(live);
   if (r >= rows) return;
   const long long t = live.index != nullptr ? live.index[live.base + r] : live.base + r;
@@ -342,9 +342,9 @@ int grid_pairs() { return sm_count() / 2; }
 
 }  // namespace
 
-long long streamk_partials() { return 2LL * grid_pairs() * (2 * BM) * BN; }
+long long balanced_partials() { return 2LL * grid_pairs() * (2 * BM) * BN; }
 
-void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream) {
+void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
   const RowBoxes rows(live.rows);
   const CUtensorMap tmA = make_tensor_map_2d_b16(A, K, live.rows, lda, BK, rows.rows0);
@@ -352,7 +352,7 @@ void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRo
   const CUtensorMap tmB = make_tensor_map_2d_b16(B, N, K, ldb, 64, BK);
   const CUtensorMap tmC = make_tensor_map_2d_b16(C, N, live.rows, N, 64, 32);
   const CUtensorMap tmP = make_tensor_map_2d_f32(partials, BN, 2LL * grid_pairs() * (2 * BM), BN, 32, 32);
-  check_cuda(cudaFuncSetAttribute(streamk_gemm_2sm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "stream-k gemm smem attr");
+  check_cuda(cudaFuncSetAttribute(balanced_gemm_2sm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "balanced gemm smem attr");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * grid_pairs(), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
@@ -365,15 +365,15 @@ void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRo
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, streamk_gemm_2sm_kernel, tmA, tmA1, tmB, tmC, tmP, N, K, rows, live, status), "stream-k gemm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, balanced_gemm_2sm_kernel, tmA, tmA1, tmB, tmC, tmP, N, K, rows, live, status), "balanced gemm launch");
   count_launch();
 }
 
-void streamk_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream) {
+void balanced_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream) {
   if (live.rows <= 0) return;
-  streamk_rows_kernel<<<live.rows, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(C), partials, live, reinterpret_cast<__nv_bfloat16*>(out), N, K, grid_pairs());
+  balanced_rows_kernel<<<live.rows, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(C), partials, live, reinterpret_cast<__nv_bfloat16*>(out), N, K, grid_pairs());
   count_launch();
-  check_cuda(cudaGetLastError(), "stream-k rows launch");
+  check_cuda(cudaGetLastError(), "balanced rows launch");
 }
 
 }  // namespace b200

@@ -61,12 +61,12 @@ void token_log_probs_grad_rows(const float* logits, long long ldl, const void* l
                                long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long ldg, LiveRows live, int N, float logit_scale,
                                long long ignore_index, cudaStream_t stream);
 
-// ---- gemm/streamk_gemm_2sm.cu: C [live.rows, N] = A [live.rows, K] B [K, N], bf16, for few tiles and a long K. Tiles that several CTA
-// pairs share leave fp32 partial tiles in `partials` (streamk_partials() words); streamk_rows puts the result together and writes live
+// ---- gemm/balanced_gemm_2sm.cu: C [live.rows, N] = A [live.rows, K] B [K, N], bf16, for few tiles and a long K. Tiles that several CTA
+// pairs share leave fp32 partial tiles in `partials` (balanced_partials() words); balanced_rows puts the result together and writes live
 // row r to row t of `out`, its place in the batch. lda, ldb and N: multiples of 8; C and out: rows of N.
-long long streamk_partials();
-void streamk_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream);
-void streamk_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream);
+long long balanced_partials();
+void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream);
+void balanced_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream);
 
 // ---- gemm/gemm_bf16_2sm.cu: C [M, N] (+)= A [K, M]^T B [K, N] on CTA pairs, where the K rows are those of a compacted batch: the
 // contraction ends at max(1, *count - base). Rows from there to the next multiple of 64 must be 0 in both operands.

@@ -431,7 +431,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     if (need_dx) {
       dx = map.numel() > 0 ? torch::zeros({T, H}, xc.options()) : torch::empty({T, H}, xc.options());  // rows that take no part: 0
       dxc = torch::empty({std::min(chunk, T), H}, xc.options());
-      partials = empty_f32(streamk_partials(), xc);
+      partials = empty_f32(balanced_partials(), xc);
     }
     OptTensor target;
     if (need_dw) {
@@ -457,8 +457,8 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
         vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0),
                         dl.stride(0), logit_scale, ignore_index, st, stream);
       if (need_dx) {
-        streamk_gemm(dl.data_ptr(), w.data_ptr(), dxc.data_ptr(), partials.data_ptr<float>(), live, (int)H, (int)V, dl.stride(0), w.stride(0), st, stream);
-        streamk_rows(dxc.data_ptr(), partials.data_ptr<float>(), live, dx.data_ptr(), (int)H, (int)V, stream);
+        balanced_gemm(dl.data_ptr(), w.data_ptr(), dxc.data_ptr(), partials.data_ptr<float>(), live, (int)H, (int)V, dl.stride(0), w.stride(0), st, stream);
+        balanced_rows(dxc.data_ptr(), partials.data_ptr<float>(), live, dx.data_ptr(), (int)H, (int)V, stream);
       }
       if (need_dw) {
         const bool f32 = dw.scalar_type() == torch::kFloat32;
