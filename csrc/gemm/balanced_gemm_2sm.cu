@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 // The product's live rows at their places in the batch: out[t] (bf16, N columns, a multiple of 8) is the row of C where the tile was
-// computed whole, and the sum of its partial tiles in the order of the pairs where it was cut. One block per row.
+// computed whole, and the sum of its partial tiles in the order of the pairs where it was cut. One block per row and 1024 columns.
 __global__ void __launch_bounds__(128)
     balanced_rows_kernel(const __nv_bfloat16* __restrict__ C, const float* __restrict__ partials, LiveRows live, __nv_bfloat16* __restrict__ out, int N, int K, int pairs) {
   const int r = blockIdx.x, rows = live_count(live);
@@ -310,7 +310,8 @@ __global__ void __launch_bounds__(128)
   const int group = min(cut.m_tiles, 8);
   const int mi = r / (2 * BM), row = r % (2 * BM);
   const int panel = mi / group, panel_rows = min(cut.m_tiles - panel * group, group);
-  for (int c = threadIdx.x * 8; c < N; c += 128 * 8) {
+  const int c = (blockIdx.y * 128 + threadIdx.x) * 8;
+  if (c < N) {
     const int ni = c / BN, col = c % BN;
     const int tile = panel * group * cut.n_tiles + ni * panel_rows + (mi - panel * group);  // inverse of tile_coord
     uint4 v;
@@ -371,7 +372,8 @@ void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveR
 
 void balanced_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream) {
   if (live.rows <= 0) return;
-  balanced_rows_kernel<<<live.rows, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(C), partials, live, reinterpret_cast<__nv_bfloat16*>(out), N, K, grid_pairs());
+  const dim3 grid((unsigned)live.rows, (unsigned)((N + 1023) / 1024));
+  balanced_rows_kernel<<<grid, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(C), partials, live, reinterpret_cast<__nv_bfloat16*>(out), N, K, grid_pairs());
   count_launch();
   check_cuda(cudaGetLastError(), "balanced rows launch");
 }

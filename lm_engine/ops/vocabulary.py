@@ -86,17 +86,17 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: 
 
 # ----------------------------------------------------------------------------- from hidden states
 def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0,
-                                 ignore_index: int = -100, return_entropy: bool = False):
+                                 ignore_index: int = -100, return_entropy: bool = False, keep_logits: bool | None = None):
     """:func:`token_log_probs` of ``logits = x @ weight.T`` without the logits: ``x [..., H]``, ``weight [V, H]``, ``labels [...]``.
 
     The logits are formed in fp32 on the tensor cores and reduced where they are. Without gradients they never reach memory; with gradients they
-    are kept in fp32 until the backward pass where that takes at most 4 GiB, and formed a second time otherwise.
+    are kept in fp32 until the backward pass (``keep_logits``; by default where that takes at most 4 GiB) or formed a second time in it.
     The backward pass needs a transient bf16 buffer of at most about 2.2 GB. Rows whose label is ignored take no part in any product. bf16 operands with
     ``H`` a multiple of 8 run on the kernels. Gradients of ``weight`` go to its ``main_grad`` when the engine provides one."""
     if x.is_cuda and x.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0:
         with site("loss.lm_head.log_probs"):
             out = native().linear_token_log_probs(x, weight, labels, logit_scale, ignore_index, return_entropy, _flce_chunk_rows(labels.numel(), weight.shape[0]),
-                                                  _KEEP_LOGITS_BYTES, status_word(x.device))
+                                                  _KEEP_LOGITS_BYTES if keep_logits is None else (1 << 62) * bool(keep_logits), status_word(x.device))
         return tuple(out) if return_entropy else out[0]
     logit_scale = _check_logit_scale(logit_scale)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0 or weight.shape[1] == 0:

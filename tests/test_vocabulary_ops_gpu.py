@@ -219,17 +219,14 @@ def test_fused_linear_token_log_probs_in_chunks_and_into_main_grad(monkeypatch):
 
 @pytest.mark.parametrize("tokens,hidden,vocab", [(1, 8, 1), (130, 72, 257), (300, 256, 1003), (1000, 64, 5000)])
 @pytest.mark.parametrize("entropy", [False, True])
-def test_fused_linear_token_log_probs_kept_or_formed_twice_are_the_same(tokens, hidden, vocab, entropy, monkeypatch):
-    import lm_engine.ops.vocabulary as vocabulary
-
+def test_fused_linear_token_log_probs_kept_or_formed_twice_are_the_same(tokens, hidden, vocab, entropy):
     x, w, labels, g, h = _linear_case(tokens, hidden, vocab, tokens)
     labels[::3] = -100
     x.requires_grad_(True)
     w.requires_grad_(True)
     results = []
-    for keep in (0, 1 << 30):
-        monkeypatch.setattr(vocabulary, "_KEEP_LOGITS_BYTES", keep)
-        out = ops.fused_linear_token_log_probs(x, w, labels, logit_scale=1.25, return_entropy=entropy)
+    for keep in (False, True):
+        out = ops.fused_linear_token_log_probs(x, w, labels, logit_scale=1.25, return_entropy=entropy, keep_logits=keep)
         outs = out if entropy else (out,)
         results.append((*outs, *torch.autograd.grad(outs, (x, w), [g, h][: len(outs)])))
     for i, (a, b) in enumerate(zip(*results)):
