@@ -11,7 +11,6 @@
 #include <algorithm>
 #include <cmath>
 
-#include "ops.h"
 #include "vocabulary.h"
 
 namespace b200 {
@@ -150,7 +149,8 @@ int64_t stats_rows(int64_t rows, int64_t slices) {
   return std::min(rows, std::min<int64_t>(most, 1 << 20));
 }
 
-// A batch of more rows than one tile is compacted to its live rows first: a tile is computed whole, so a smaller batch gains nothing.
+// A batch of more rows than one tile is compacted to its live rows first, and so is every batch that will be differentiated: what an
+// ignored row holds must not reach the weight's gradient as 0 * NaN. A smaller batch without gradients gains nothing (a tile is computed whole).
 constexpr int64_t kCompactAbove = 256;
 
 // map: int32 [T + 1] = index [T], count, or empty where the batch is not compacted
@@ -167,7 +167,7 @@ void* row_ptr(const Tensor& t, int64_t row) { return reinterpret_cast<char*>(t.d
 
 // (log_probs, entropy, lse, the rows that were multiplied, row map, their logits if they are kept)
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
-                                                                        bool want_entropy, bool keep_logits, const Tensor& status) {
+                                                                        bool want_entropy, bool differentiated, bool keep_logits, const Tensor& status) {
   check_linear(x, w, labels);
   int* st = status_of(status, x);
   const c10::cuda::CUDAGuard guard(x.device());
@@ -176,7 +176,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(
   const cudaStream_t stream = stream_of(x);
   Tensor log_probs = empty_f32(rows, x), lse = empty_pairs(rows, x), entropy = want_entropy ? empty_f32(rows, x) : Tensor();
   float* ent = want_entropy ? entropy.data_ptr<float>() : nullptr;
-  const bool compact = rows > kCompactAbove;
+  const bool compact = differentiated || rows > kCompactAbove;
   Tensor map = torch::empty({compact ? rows + 1 : 0}, x.options().dtype(torch::kInt32)), xc = x;
   Tensor logits;
   if (keep_logits) logits = empty_f32(rows * ((V + 3) / 4 * 4), x).view({rows, (V + 3) / 4 * 4});
@@ -398,12 +398,12 @@ OptTensor main_grad(const Tensor& weight) {
 
 // Forward reduces the logits to 16 bytes per row and 128 columns. Backward needs them again: kept in fp32 where `keep_logits` says so, else
 // formed a second time; either way they become, chunk of rows by chunk, their bf16 gradient, which is multiplied with the weight and
-// the hidden states. Both ways see the same fp32 logits. Batches of more than 256 rows are compacted to the
-// rows whose label counts, and all products end there.
+// the hidden states. Both ways see the same fp32 logits. The batch is compacted to the rows whose label counts, and all products end
+// there.
 struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy, int64_t chunk,
-                               bool keep_logits, const Tensor& status) {
-    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy, keep_logits, status);
+                               bool differentiated, bool keep_logits, const Tensor& status) {
+    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy, differentiated, keep_logits, status);
     ctx->save_for_backward({xc, w, labels, lse, entropy, map, status, logits});
     ctx->saved_data["logit_scale"] = logit_scale;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -416,7 +416,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5], &logits = saved[7];
     const bool has_h = grads.size() > 1 && grads[1].defined();
-    if (!grads[0].defined() && !has_h) return variable_list(9);
+    if (!grads[0].defined() && !has_h) return variable_list(10);
     const int64_t T = xc.size(0), H = xc.size(1), V = w.size(0);
     const int64_t chunk = std::max<int64_t>(std::min(ctx->saved_data["chunk"].toInt(), T), 1);
     const bool need_dx = ctx->needs_input_grad(0), need_dw = ctx->needs_input_grad(1);
@@ -429,7 +429,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     const cudaStream_t stream = stream_of(xc);
     Tensor dx, dw, dxc, partials;
     if (need_dx) {
-      dx = map.numel() > 0 ? torch::zeros({T, H}, xc.options()) : torch::empty({T, H}, xc.options());  // rows that take no part: 0
+      dx = torch::zeros({T, H}, xc.options());  // rows that take no part
       dxc = torch::empty({std::min(chunk, T), H}, xc.options());
       partials = empty_f32(balanced_partials(), xc);
     }
@@ -461,15 +461,10 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
         balanced_rows(dxc.data_ptr(), partials.data_ptr<float>(), live, dx.data_ptr(), (int)H, (int)V, stream);
       }
       if (need_dw) {
-        const bool f32 = dw.scalar_type() == torch::kFloat32;
-        if (live.count != nullptr)
-          gemm_bf16_2sm_live(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0), dw.stride(0), f32, live, st, stream);
-        else
-          (V >= 256 ? gemm_bf16_2sm : gemm_bf16)(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0), dw.stride(0), true, true, f32 ? 2 : 0, 1.f,
-                                                 st, 0, stream);
+        gemm_bf16_2sm_live(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0), dw.stride(0), dw.scalar_type() == torch::kFloat32, live, st, stream);
       }
     }
-    variable_list out(9);
+    variable_list out(10);
     if (need_dx) out[0] = once(dx, "fused_linear_token_log_probs");
     if (need_dw && !target.has_value()) out[1] = once(dw.to(w.scalar_type()), "fused_linear_token_log_probs");
     return out;
@@ -508,9 +503,10 @@ variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Ten
                     text(x.device()), " and ", text(w.scalar_type()), " on ", text(w.device()));
   const auto shape = x.sizes().slice(0, x.dim() - 1);
   check_label_shape(labels, shape, x);
-  const bool keep = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()) && 4.0 * (double)labels.numel() * (double)w.size(0) <= (double)keep_bytes;
+  const bool differentiated = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
+  const bool keep = differentiated && 4.0 * (double)labels.numel() * (double)w.size(0) <= (double)keep_bytes;
   variable_list out = LinearTokenLogProbs::apply(mapped_rows(x.reshape({labels.numel(), x.size(-1)})), mapped_rows(w), labels.reshape({labels.numel()}).contiguous(), logit_scale, ignore_index,
-                                                 return_entropy, chunk, keep, status);
+                                                 return_entropy, chunk, differentiated, keep, status);
   if (x.dim() != 2)
     for (auto& t : out) t = t.view(shape);
   return out;

@@ -238,14 +238,14 @@ def test_fused_linear_token_log_probs_kept_or_formed_twice_are_the_same(tokens, 
 
 @pytest.mark.parametrize("keep", [0, 4 << 30])
 @pytest.mark.parametrize("kept", [0.0, 0.01, 0.5])
-@pytest.mark.parametrize("chunk", [128, 384, 4096])
-def test_fused_linear_token_log_probs_leaves_ignored_rows_out(kept, chunk, keep, monkeypatch):
+@pytest.mark.parametrize("chunk,tokens", [(128, 1000), (384, 1000), (4096, 1000), (4096, 100), (4096, 3)])
+def test_fused_linear_token_log_probs_leaves_ignored_rows_out(kept, chunk, tokens, keep, monkeypatch):
     import lm_engine.ops.vocabulary as vocabulary
 
     monkeypatch.setattr(vocabulary, "_KEEP_LOGITS_BYTES", keep)
     monkeypatch.setattr(vocabulary, "_flce_chunk_rows", lambda T, V: min(T, chunk))
-    x, w, labels, g, h = _linear_case(1000, 64, 333, 8)
-    labels[torch.rand(1000, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) >= kept] = -100
+    x, w, labels, g, h = _linear_case(tokens, 64, 333, 8)
+    labels[torch.rand(tokens, device="cuda", generator=torch.Generator("cuda").manual_seed(1)) >= kept] = -100
     x[labels == -100] = math.nan  # not looked at
     junk = torch.full((64 << 20,), math.nan, device="cuda")  # what the allocator hands out next holds NaN
     del junk
