@@ -71,7 +71,8 @@ struct Walk {
   int tile, kb0, kb1, slot;
   bool complete;  // the tile is computed whole
 
-  __device__ Walk(const Cut& c, int p) : cut(c), pair(p), next_tile(p), u(c.begin(p)), first(c.begin(p)), last(c.begin(p + 1)), tile(0), kb0(0), kb1(0), slot(0), complete(true) {}
+  __device__ Walk(const Cut& c, int p) : cut(c), pair(p), next_tile(p), u(c.begin(p)), first(c.begin(p)), last(c.begin(p + 1)), tile(0),
+      kb0(0), kb1(0), slot(0), complete(true) {}
   __device__ bool next() {
     if (next_tile < cut.whole) {
       tile = next_tile;
@@ -98,8 +99,9 @@ __device__ __forceinline__ int live_count(const LiveRows& live) {
 }
 
 __global__ void __launch_bounds__(THREADS, 1)
-    balanced_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC,
-                            const __grid_constant__ CUtensorMap tmP, int N, int K, RowBoxes rows, LiveRows live, int* status) {
+    balanced_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1,
+        const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmP,
+        int N, int K, RowBoxes rows, LiveRows live, int* status) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -208,8 +210,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           const uint32_t b_base = smem_u32(sB + s * B_STAGE_BYTES);
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k) {
-            umma_f16_ss_2sm(d_tmem, umma_smem_desc_sw128(a_base + k * 32, 16, 1024), umma_smem_desc_sw128(b_base + k * 16 * 128, BK * 128, 1024), idesc,
-                            (kb != walk.kb0 || k != 0) ? 1u : 0u);
+            umma_f16_ss_2sm(d_tmem, umma_smem_desc_sw128(a_base + k * 32, 16, 1024),
+                umma_smem_desc_sw128(b_base + k * 16 * 128, BK * 128, 1024), idesc, (kb != walk.kb0 || k != 0) ? 1u : 0u);
           }
           const uint32_t e_local = smem_u32(&empty[s]);  // release the stage in both CTAs
           umma_commit_2sm(map_to_cta(e_local, 0));
@@ -257,9 +259,10 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              box_write(box, lane, half * 4 + j,
-                        make_uint4(pack_bf16x2(__uint_as_float(v[8 * j]), __uint_as_float(v[8 * j + 1])), pack_bf16x2(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3])),
-                                   pack_bf16x2(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5])), pack_bf16x2(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7]))));
+              box_write(box, lane, half * 4 + j, make_uint4(pack_bf16x2(__uint_as_float(v[8 * j]), __uint_as_float(v[8 * j + 1])),
+                  pack_bf16x2(__uint_as_float(v[8 * j + 2]), __uint_as_float(v[8 * j + 3])),
+                  pack_bf16x2(__uint_as_float(v[8 * j + 4]), __uint_as_float(v[8 * j + 5])),
+                  pack_bf16x2(__uint_as_float(v[8 * j + 6]), __uint_as_float(v[8 * j + 7]))));
             }
           }
         } else {
@@ -302,7 +305,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 // The product's live rows at their places in the batch: out[t] (bf16, N columns, a multiple of 8) is the row of C where the tile was
 // computed whole, and the sum of its partial tiles in the order of the pairs where it was cut. One block per row and 1024 columns.
 __global__ void __launch_bounds__(128)
-    balanced_rows_kernel(const __nv_bfloat16* __restrict__ C, const float* __restrict__ partials, LiveRows live, __nv_bfloat16* __restrict__ out, int N, int K, int pairs) {
+    balanced_rows_kernel(const __nv_bfloat16* __restrict__ C, const float* __restrict__ partials, LiveRows live,
+        __nv_bfloat16* __restrict__ out, int N, int K, int pairs) {
   const int r = blockIdx.x, rows = live_count(live);
   if (r >= rows) return;
   const long long t = live.index != nullptr ? live.index[live.base + r] : live.base + r;
@@ -345,7 +349,8 @@ int grid_pairs() { return sm_count() / 2; }
 
 long long balanced_partials() { return 2LL * grid_pairs() * (2 * BM) * BN; }
 
-void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream) {
+void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb,
+    int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
   const RowBoxes rows(live.rows);
   const CUtensorMap tmA = make_tensor_map_2d_b16(A, K, live.rows, lda, BK, rows.rows0);
@@ -353,7 +358,8 @@ void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveR
   const CUtensorMap tmB = make_tensor_map_2d_b16(B, N, K, ldb, 64, BK);
   const CUtensorMap tmC = make_tensor_map_2d_b16(C, N, live.rows, N, 64, 32);
   const CUtensorMap tmP = make_tensor_map_2d_f32(partials, BN, 2LL * grid_pairs() * (2 * BM), BN, 32, 32);
-  check_cuda(cudaFuncSetAttribute(balanced_gemm_2sm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "balanced gemm smem attr");
+  check_cuda(cudaFuncSetAttribute(balanced_gemm_2sm_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES),
+      "balanced gemm smem attr");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * grid_pairs(), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
@@ -366,14 +372,16 @@ void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveR
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  check_cuda(cudaLaunchKernelEx(&cfg, balanced_gemm_2sm_kernel, tmA, tmA1, tmB, tmC, tmP, N, K, rows, live, status), "balanced gemm launch");
+  check_cuda(cudaLaunchKernelEx(&cfg, balanced_gemm_2sm_kernel, tmA, tmA1, tmB, tmC, tmP, N, K, rows, live, status),
+      "balanced gemm launch");
   count_launch();
 }
 
 void balanced_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream) {
   if (live.rows <= 0) return;
   const dim3 grid((unsigned)live.rows, (unsigned)((N + 1023) / 1024));
-  balanced_rows_kernel<<<grid, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(C), partials, live, reinterpret_cast<__nv_bfloat16*>(out), N, K, grid_pairs());
+  balanced_rows_kernel<<<grid, 128, 0, stream>>>(reinterpret_cast<const __nv_bfloat16*>(C), partials, live,
+      reinterpret_cast<__nv_bfloat16*>(out), N, K, grid_pairs());
   count_launch();
   check_cuda(cudaGetLastError(), "balanced rows launch");
 }

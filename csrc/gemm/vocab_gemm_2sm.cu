@@ -98,8 +98,9 @@ __device__ __forceinline__ float select32(const float (&x)[32], int i) {
 
 template <Mode MODE, bool ENTROPY>
 __global__ void __launch_bounds__(THREADS, 1)
-    vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1, const __grid_constant__ CUtensorMap tmB,
-                          const __grid_constant__ CUtensorMap tmOut, int N, int K, RowBoxes box, int* status, RowArgs rows) {
+    vocab_gemm_2sm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA1,
+        const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmOut, int N, int K, RowBoxes box, int* status,
+        RowArgs rows) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -309,7 +310,8 @@ __global__ void __launch_bounds__(THREADS, 1)
             __syncwarp();
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              box_write(store_box, lane, j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]), __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])));
+              box_write(store_box, lane, j, make_uint4(__float_as_uint(x[4 * j]), __float_as_uint(x[4 * j + 1]),
+                  __float_as_uint(x[4 * j + 2]), __float_as_uint(x[4 * j + 3])));
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0 && row0 < live) {
@@ -351,7 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1)
               w[e] = zero ? 0u : pack_bf16x2(a, b);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) box_write(store_box, lane, part * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
+            for (int j = 0; j < 4; ++j)
+              box_write(store_box, lane, part * 4 + j, make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]));
             if ((label >> 5) == 2 * c + part && !zero) {
               // the label's own gradient, over the element of the row just written
               const float d = log2_prob(select32(x, label & 31), L, scale2);
@@ -387,7 +390,8 @@ __global__ void __launch_bounds__(THREADS, 1)
 }
 
 template <Mode MODE, bool ENTROPY>
-void launch(const void* x, long long ldx, const CUtensorMap& tmB, const CUtensorMap* out, int N, int K, int* status, const RowArgs& rows, cudaStream_t stream) {
+void launch(const void* x, long long ldx, const CUtensorMap& tmB, const CUtensorMap* out, int N, int K, int* status,
+    const RowArgs& rows, cudaStream_t stream) {
   auto kernel = vocab_gemm_2sm_kernel<MODE, ENTROPY>;
   check_cuda(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES), "vocab gemm smem attr");
   const RowBoxes box(rows.live.rows);
@@ -415,8 +419,8 @@ void launch(const void* x, long long ldx, const CUtensorMap& tmB, const CUtensor
 
 }  // namespace
 
-void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl, bool entropy, LiveRows live, int N,
-                      int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream) {
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl,
+    bool entropy, LiveRows live, int N, int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream) {
   if (live.rows <= 0) return;
   const CUtensorMap tmB = make_tensor_map_2d_b16(w, K, N, ldw, BK, BN_HALF);
   RowArgs rows = {};

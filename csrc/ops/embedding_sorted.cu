@@ -176,7 +176,8 @@ __global__ void __launch_bounds__(RUN / 2)
 }
 
 // One level: groups of FAN sorted runs of `length` keys (a power of two; the last run may be short) become one sorted run each.
-__global__ void __launch_bounds__(128) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int T, int log_length, int blocks, Fill fill) {
+__global__ void __launch_bounds__(128) merge_runs_kernel(const uint64_t* __restrict__ in, uint64_t* __restrict__ out, int T,
+    int log_length, int blocks, Fill fill) {
   if (blockIdx.x >= blocks) {
     fill_zero(fill, blockIdx.x - blocks);
     return;
@@ -287,11 +288,13 @@ constexpr int JOIN_THREADS = JOIN_LANES * JOIN_COLUMNS;
 
 template <typename D, int N, bool ACC>
 __global__ void __launch_bounds__(JOIN_THREADS)
-    join_runs_kernel(const uint64_t* __restrict__ keys, D* __restrict__ dweight, const float* __restrict__ partials, int tokens, int chunk_tokens, int H, float scale) {
+    join_runs_kernel(const uint64_t* __restrict__ keys, D* __restrict__ dweight, const float* __restrict__ partials, int tokens,
+        int chunk_tokens, int H, float scale) {
   __shared__ Pack<float, N> s[JOIN_LANES][JOIN_COLUMNS];
   const int chunks = (tokens + chunk_tokens - 1) / chunk_tokens, chunk = blockIdx.x;
   const int first = chunk * chunk_tokens, next = first + chunk_tokens;  // next < tokens: the last chunk has no block
-  const uint32_t id = key_id(keys[next - 1]), after = key_id(keys[next]), here = key_id(keys[first]), before = first > 0 ? key_id(keys[first - 1]) : ~0u;
+  const uint32_t id = key_id(keys[next - 1]), after = key_id(keys[next]), here = key_id(keys[first]),
+      before = first > 0 ? key_id(keys[first - 1]) : ~0u;
   if (id == kNoId || after != id) return;          // no run crosses this border
   if (here == id && before == id) return;          // it began in an earlier chunk
   // chunks behind this one that the run fills to their last token, and one more in which it ends
@@ -321,7 +324,10 @@ __global__ void __launch_bounds__(JOIN_THREADS)
     for (int k0 = lane; k0 < parts; k0 += BATCH * JOIN_LANES) {
       Pack<float, N> v[BATCH];
 #pragma unroll
-      for (int b = 0; b < BATCH; ++b) v[b] = load_pack<float, N>(partials + 2LL * (chunk + 1 + min(k0 + b * JOIN_LANES, parts - 1)) * H + c);
+      for (int b = 0; b < BATCH; ++b) {
+        const int k = min(k0 + b * JOIN_LANES, parts - 1);
+        v[b] = load_pack<float, N>(partials + 2LL * (chunk + 1 + k) * H + c);
+      }
 #pragma unroll
       for (int b = 0; b < BATCH; ++b) {
         if (k0 + b * JOIN_LANES >= parts) break;
@@ -348,15 +354,18 @@ bool wide_rows(int H, const void* a, const void* b) {
 }
 
 template <typename T>
-void lookup(const void* weight, const void* ids, bool ids64, void* out, long long tokens, long long V, int H, float scale, int* status, cudaStream_t stream) {
+void lookup(const void* weight, const void* ids, bool ids64, void* out, long long tokens, long long V, int H, float scale, int* status,
+    cudaStream_t stream) {
   constexpr int N = 16 / sizeof(T);
   const bool wide = wide_rows<T>(H, weight, out);
   const int per_block = LOOKUP_THREADS * (wide ? N : 1);
   const dim3 grid((unsigned)((tokens + LOOKUP_ROWS - 1) / LOOKUP_ROWS), (unsigned)((H + per_block - 1) / per_block));
   if (wide)
-    embedding_lookup_kernel<T, N><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64, reinterpret_cast<T*>(out), tokens, V, H, scale, status);
+    embedding_lookup_kernel<T, N><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64,
+        reinterpret_cast<T*>(out), tokens, V, H, scale, status);
   else
-    embedding_lookup_kernel<T, 1><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64, reinterpret_cast<T*>(out), tokens, V, H, scale, status);
+    embedding_lookup_kernel<T, 1><<<grid, LOOKUP_THREADS, 0, stream>>>(reinterpret_cast<const T*>(weight), ids, ids64,
+        reinterpret_cast<T*>(out), tokens, V, H, scale, status);
 }
 
 // Tokens of one chunk: as many as leave about four blocks per SM, at most 128 (fewer and longer chunks mean fewer partial sums; with
@@ -369,11 +378,13 @@ int chunk_tokens(long long T, int H, int columns) {
 }
 
 template <typename T, typename D, int N, bool ACC>
-void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials, long long tokens, int H, float scale, cudaStream_t stream) {
+void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials, long long tokens, int H, float scale,
+    cudaStream_t stream) {
   const int columns = SUM_THREADS * N, n = chunk_tokens(tokens, H, columns);
   const long long chunks = (tokens + n - 1) / n;
   const dim3 grid((unsigned)chunks, (unsigned)((H + columns - 1) / columns));
-  sum_tokens_kernel<T, D, N, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys, reinterpret_cast<D*>(dweight), partials, tokens, n, H, scale);
+  sum_tokens_kernel<T, D, N, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys,
+      reinterpret_cast<D*>(dweight), partials, tokens, n, H, scale);
   count_launch();
   check_cuda(cudaGetLastError(), "embedding gradient sum launch");
   if (chunks > 1) {
@@ -386,7 +397,8 @@ void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials
 }
 
 template <typename T>
-void gradient(const void* dout, const uint64_t* keys, void* dweight, bool accumulate, float* partials, long long tokens, int H, float scale, cudaStream_t stream) {
+void gradient(const void* dout, const uint64_t* keys, void* dweight, bool accumulate, float* partials, long long tokens, int H,
+    float scale, cudaStream_t stream) {
   constexpr int N = 16 / sizeof(T);
   const bool wide = wide_rows<T>(H, dout, dweight);
   if (accumulate) {
@@ -434,7 +446,10 @@ void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids
     const long long begin = words * k / kernels, end = words * (k + 1) / kernels;
     return Fill{reinterpret_cast<uint4*>(dweight) + begin, end - begin, k + 1 == kernels ? (int)(bytes % 16) : 0};
   };
-  auto fill_blocks = [](const Fill& f, int block) { return (unsigned)((f.n + FILL_WORDS * block - 1) / (FILL_WORDS * block) + (f.n == 0 && f.tail > 0 ? 1 : 0)); };
+  auto fill_blocks = [](const Fill& f, int block) {
+    const int words = FILL_WORDS * block;
+    return (unsigned)((f.n + words - 1) / words + (f.n == 0 && f.tail > 0 ? 1 : 0));
+  };
   const unsigned runs = (unsigned)((T + RUN - 1) / RUN), blocks = (unsigned)((T + 127) / 128);
   Fill fill = share(0);
   sort_runs_kernel<<<runs + fill_blocks(fill, threads), threads, 0, stream>>>(ids, ids64, keys, T, V, (int)runs, fill);

@@ -115,7 +115,8 @@ struct Chunk {
   long long base;
   int count;  // tokens below T
 
-  __device__ __forceinline__ Chunk(const PackedTokens& p, long long chunk) : base(chunk * (32 * K)), count((int)min((long long)(32 * K), p.T - chunk * (32 * K))) {}
+  __device__ __forceinline__ Chunk(const PackedTokens& p, long long chunk)
+      : base(chunk * (32 * K)), count((int)min((long long)(32 * K), p.T - base)) {}
   __device__ __forceinline__ int at(int k) const { return (threadIdx.x & 31) + 32 * k; }
   template <typename V>
   __device__ __forceinline__ void load(const V* p, V (&v)[K]) const {
@@ -275,7 +276,8 @@ __device__ __forceinline__ void preference_pairs(const PackedTokens& p, const Pr
 
 template <int K, bool ONE_LAUNCH>
 __global__ void __launch_bounds__(CLUSTER_THREADS)
-    preference_cluster_kernel(PreferenceIn in, PackedTokens p, PreferenceArgs args, float* partials, float* loss, float* chosen, float* rejected, float* slope) {
+    preference_cluster_kernel(PreferenceIn in, PackedTokens p, PreferenceArgs args, float* partials, float* loss, float* chosen,
+        float* rejected, float* slope) {
   __shared__ SumSpace<1> space;
   if (ONE_LAUNCH) {
     for (long long c = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5); c < chunk_count<K>(p); c += CLUSTER * (CLUSTER_THREADS / 32))
@@ -294,7 +296,8 @@ __global__ void __launch_bounds__(WARPS_A * 32) preference_chunks_kernel(Prefere
 
 template <int K>
 __global__ void __launch_bounds__(WARPS_A * 32)
-    preference_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ d_loss, long long d_loss_stride, PackedTokens p, float* __restrict__ grad) {
+    preference_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ d_loss, long long d_loss_stride, PackedTokens p,
+        float* __restrict__ grad) {
   const long long chunk = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
   if (chunk >= chunk_count<K>(p)) return;
   const Chunk<K> c(p, chunk);
@@ -373,7 +376,8 @@ __device__ __forceinline__ TokenLoss policy_token(float lp, float old, float ref
 // Partial (loss, kl, clipped, tokens) of the warp's chunk: per sequence into slot (chunk + sequence) for the mean over
 // sequences, else all together into slot `chunk`. Writes the tokens' slopes.
 template <int K>
-__device__ __forceinline__ void policy_chunk(const PolicyIn& in, const PackedTokens& p, const PolicyArgs& a, long long chunk, float* partials, float* slope) {
+__device__ __forceinline__ void policy_chunk(const PolicyIn& in, const PackedTokens& p, const PolicyArgs& a, long long chunk,
+    float* partials, float* slope) {
   const Chunk<K> c(p, chunk);
   const int lane = threadIdx.x & 31;
   float lp[K], old[K], ref[K], adv[K];
@@ -391,7 +395,8 @@ __device__ __forceinline__ void policy_chunk(const PolicyIn& in, const PackedTok
   for (int k = 0; k < K; ++k) {
     v[k] = {0.f, 0.f, 0.f, 0};
     if (seq[k] < 0) continue;
-    v[k] = policy_token(lp[k], old[k], in.reference != nullptr ? ref[k] : 0.f, in.reference != nullptr, a.per_token_advantage ? adv[k] : in.advantages[seq[k]], a);
+    v[k] = policy_token(lp[k], old[k], in.reference != nullptr ? ref[k] : 0.f, in.reference != nullptr,
+        a.per_token_advantage ? adv[k] : in.advantages[seq[k]], a);
   }
   if (slope != nullptr) {
     float s[K];
@@ -416,12 +421,15 @@ __device__ __forceinline__ void policy_chunk(const PolicyIn& in, const PackedTok
     kl = warp_sum(kl);
     clipped = __reduce_add_sync(0xffffffffu, clipped);
     count = __reduce_add_sync(0xffffffffu, count);
-    if (lane == 0) *reinterpret_cast<float4*>(partials + (chunk + (by_sequence ? i : 0)) * WORDS) = make_float4(loss, kl, (float)clipped, (float)count);
+    if (lane == 0)
+      *reinterpret_cast<float4*>(partials + (chunk + (by_sequence ? i : 0)) * WORDS) =
+          make_float4(loss, kl, (float)clipped, (float)count);
   }
 }
 
 template <int K>
-__device__ __forceinline__ void policy_totals(const PackedTokens& p, const PolicyArgs& a, const float* partials, const PolicyOut& out, float* weight, SumSpace<5>& space) {
+__device__ __forceinline__ void policy_totals(const PackedTokens& p, const PolicyArgs& a, const float* partials, const PolicyOut& out,
+    float* weight, SumSpace<5>& space) {
   const int lane = threadIdx.x & 31;
   const int warp = cluster_ctarank() * (CLUSTER_THREADS / 32) + (threadIdx.x >> 5);
   constexpr int kWarps = CLUSTER * (CLUSTER_THREADS / 32);
@@ -486,15 +494,16 @@ __global__ void __launch_bounds__(CLUSTER_THREADS)
 }
 
 template <int K>
-__global__ void __launch_bounds__(WARPS_A * 32) policy_chunks_kernel(PolicyIn in, PackedTokens p, PolicyArgs args, float* partials, float* slope) {
+__global__ void __launch_bounds__(WARPS_A * 32) policy_chunks_kernel(PolicyIn in, PackedTokens p, PolicyArgs args, float* partials,
+    float* slope) {
   const long long c = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
   if (c < chunk_count<K>(p)) policy_chunk<K>(in, p, args, c, partials, slope);
 }
 
 template <int K>
 __global__ void __launch_bounds__(WARPS_A * 32)
-    policy_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ factor, const float* __restrict__ weight, const float* __restrict__ d_loss, PackedTokens p, int reduction,
-                      float* __restrict__ grad) {
+    policy_bwd_kernel(const float* __restrict__ slope, const float* __restrict__ factor, const float* __restrict__ weight,
+        const float* __restrict__ d_loss, PackedTokens p, int reduction, float* __restrict__ grad) {
   const long long chunk = (long long)blockIdx.x * WARPS_A + (threadIdx.x >> 5);
   if (chunk >= chunk_count<K>(p)) return;
   const Chunk<K> c(p, chunk);
@@ -553,16 +562,18 @@ void preference_loss_fwd(const float* log_probs, const float* reference, PackedT
   launch_cluster(preference_cluster_kernel<WIDE, false>, stream, in, tokens, args, partials, loss, chosen, rejected, slope);
 }
 
-void preference_loss_bwd(const float* slope, const float* d_loss, long long d_loss_stride, PackedTokens tokens, float* grad, cudaStream_t stream) {
+void preference_loss_bwd(const float* slope, const float* d_loss, long long d_loss_stride, PackedTokens tokens, float* grad,
+    cudaStream_t stream) {
   if (tokens.T == 0) return;
-  if (tokens.T <= kOneLaunch) preference_bwd_kernel<NARROW><<<chunk_blocks<NARROW>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, d_loss, d_loss_stride, tokens, grad);
+  if (tokens.T <= kOneLaunch)
+    preference_bwd_kernel<NARROW><<<chunk_blocks<NARROW>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, d_loss, d_loss_stride, tokens, grad);
   else preference_bwd_kernel<WIDE><<<chunk_blocks<WIDE>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, d_loss, d_loss_stride, tokens, grad);
   count_launch();
   check_cuda(cudaGetLastError(), "preference_loss backward launch");
 }
 
 void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const float* reference, const float* advantages,
-                     PackedTokens tokens, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight, cudaStream_t stream) {
+    PackedTokens tokens, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight, cudaStream_t stream) {
   const PolicyIn in = {log_probs, old_log_probs, reference, advantages};
   if (tokens.T <= kOneLaunch) {
     launch_cluster(policy_cluster_kernel<NARROW, true>, stream, in, tokens, args, partials, out, slope, weight);
@@ -577,8 +588,12 @@ void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const f
 void policy_loss_bwd(const float* slope, const float* factor, const float* weight, const float* d_loss, PackedTokens tokens, int reduction,
                      float* grad, cudaStream_t stream) {
   if (tokens.T == 0) return;
-  if (tokens.T <= kOneLaunch) policy_bwd_kernel<NARROW><<<chunk_blocks<NARROW>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, factor, weight, d_loss, tokens, reduction, grad);
-  else policy_bwd_kernel<WIDE><<<chunk_blocks<WIDE>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, factor, weight, d_loss, tokens, reduction, grad);
+  if (tokens.T <= kOneLaunch)
+    policy_bwd_kernel<NARROW><<<chunk_blocks<NARROW>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, factor, weight, d_loss, tokens,
+        reduction, grad);
+  else
+    policy_bwd_kernel<WIDE><<<chunk_blocks<WIDE>(tokens.T), WARPS_A * 32, 0, stream>>>(slope, factor, weight, d_loss, tokens, reduction,
+        grad);
   count_launch();
   check_cuda(cudaGetLastError(), "policy_loss backward launch");
 }

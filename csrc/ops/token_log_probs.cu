@@ -88,7 +88,9 @@ struct Vec<float> {
     f[0] = pack2(__uint_as_float(v.x), __uint_as_float(v.y));
     f[1] = pack2(__uint_as_float(v.z), __uint_as_float(v.w));
   }
-  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }
   static __device__ __forceinline__ float top(uint32_t w) { return __uint_as_float(w); }
   static __device__ __forceinline__ float load(const float* p) { return *p; }
   static __device__ __forceinline__ void store(float* p, float f) { *p = f; }
@@ -363,9 +365,9 @@ __global__ void __launch_bounds__(BWD_THREADS)
 // and its lanes join the 32 warps' statistics pairwise.
 template <bool ENTROPY>
 __global__ void __launch_bounds__(1024)
-    token_log_probs_join_kernel(const float4* __restrict__ stats, int slices, int slice_width, const void* __restrict__ labels, bool labels64,
-                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, LiveRows live, int V,
-                                float scale2, long long ignore_index) {
+    token_log_probs_join_kernel(const float4* __restrict__ stats, int slices, int slice_width, const void* __restrict__ labels,
+        bool labels64, float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, LiveRows live, int V,
+        float scale2, long long ignore_index) {
   __shared__ Stats red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = live.count == nullptr ? live.rows : min(live.rows, *live.count - live.base);
@@ -426,7 +428,8 @@ void fwd(const void* logits, const void* labels, bool labels64, float* log_probs
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    check_cuda(cudaLaunchKernelEx(&cfg, kernel, x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index), "token_log_probs forward launch");
+    check_cuda(cudaLaunchKernelEx(&cfg, kernel, x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index),
+        "token_log_probs forward launch");
   };
   // Blocks per row: more than one only while all of them run at once, four per SM, and each has a vector per thread. Few long rows
   // gain (32 x 49152 bf16: 7.8 us with one block of 1024 threads, 6.6 with eight of 256); with more blocks than run at a time the
@@ -453,11 +456,13 @@ void bwd(const void* logits, const void* labels, bool labels64, const float2* ls
   const unsigned grid = (unsigned)rows * chunks;
   const float scale2 = logit_scale * kLog2e;
   if (d_entropy != nullptr)
-    token_log_probs_bwd_kernel<T, true><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
-                                                                          reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index, chunks);
+    token_log_probs_bwd_kernel<T, true><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs,
+        d_log_probs_stride, d_entropy, d_entropy_stride, reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2,
+        ignore_index, chunks);
   else
-    token_log_probs_bwd_kernel<T, false><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
-                                                                           reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2, ignore_index, chunks);
+    token_log_probs_bwd_kernel<T, false><<<grid, BWD_THREADS, 0, stream>>>(x, labels, labels64, lse, entropy, d_log_probs,
+        d_log_probs_stride, d_entropy, d_entropy_stride, reinterpret_cast<T*>(grad), V, map, grad_stride, logit_scale, scale2,
+        ignore_index, chunks);
 }
 
 }  // namespace
@@ -484,14 +489,16 @@ void token_log_probs_bwd(const void* logits, Scalar type, const void* labels, bo
 }
 
 void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
-                          float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream) {
+    float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream) {
   if (live.rows <= 0) return;
   const unsigned blocks = (unsigned)((live.rows + 31) / 32);
   const float4* st = reinterpret_cast<const float4*>(stats);
   if (entropy != nullptr)
-    token_log_probs_join_kernel<true><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, live, V, logit_scale * kLog2e, ignore_index);
+    token_log_probs_join_kernel<true><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse,
+        live, V, logit_scale * kLog2e, ignore_index);
   else
-    token_log_probs_join_kernel<false><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse, live, V, logit_scale * kLog2e, ignore_index);
+    token_log_probs_join_kernel<false><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse,
+        live, V, logit_scale * kLog2e, ignore_index);
   count_launch();
   check_cuda(cudaGetLastError(), "token_log_probs join launch");
 }
@@ -506,9 +513,10 @@ constexpr int GRAD_UNROLL = 4;  // vectors of eight columns per thread: 32 KB of
 // behind are left alone.
 template <bool ENTROPY>
 __global__ void __launch_bounds__(GRAD_THREADS)
-    grad_rows_kernel(const float* __restrict__ logits, long long ldl, const void* __restrict__ labels, bool labels64, const float2* __restrict__ lse, const float* __restrict__ entropy,
-                     const float* __restrict__ d_log_probs, long long d_log_probs_stride, const float* __restrict__ d_entropy, long long d_entropy_stride,
-                     __nv_bfloat16* __restrict__ grad, long long ldg, LiveRows live, int V, float logit_scale, float scale2, long long ignore_index, unsigned chunks) {
+    grad_rows_kernel(const float* __restrict__ logits, long long ldl, const void* __restrict__ labels, bool labels64,
+        const float2* __restrict__ lse, const float* __restrict__ entropy, const float* __restrict__ d_log_probs,
+        long long d_log_probs_stride, const float* __restrict__ d_entropy, long long d_entropy_stride, __nv_bfloat16* __restrict__ grad,
+        long long ldg, LiveRows live, int V, float logit_scale, float scale2, long long ignore_index, unsigned chunks) {
   const unsigned chunk = blockIdx.x % chunks;
   const int r = blockIdx.x / chunks;
   const int rows = live.count == nullptr ? live.rows : max(0, min(live.rows, *live.count - live.base));
@@ -571,7 +579,8 @@ __global__ void __launch_bounds__(GRAD_THREADS)
       const float2 d = unpack2(product ? fma2(f[j], c2, off2) : fma2(add2(f[j], off2), c2, log2_s));
       const F2 p = pack2(fast_exp2(d.x), fast_exp2(d.y));
       float2 y;
-      if (ENTROPY) y = unpack2(mul2(p, pack2(-fmaf(hs, fmaf(fmaxf(d.x, kFloor2), kLn2, H), gs), -fmaf(hs, fmaf(fmaxf(d.y, kFloor2), kLn2, H), gs))));
+      if (ENTROPY) y = unpack2(mul2(p, pack2(-fmaf(hs, fmaf(fmaxf(d.x, kFloor2), kLn2, H), gs),
+          -fmaf(hs, fmaf(fmaxf(d.y, kFloor2), kLn2, H), gs))));
       else y = unpack2(mul2(p, gs2));
       w[j] = zero ? 0u : pack_bf16x2(y.x, y.y);
     }
@@ -589,15 +598,16 @@ __global__ void __launch_bounds__(GRAD_THREADS)
 
 }  // namespace
 
-void token_log_probs_grad_rows(const float* logits, long long ldl, const void* labels, bool labels64, const float2* lse, const float* entropy, const float* d_log_probs,
-                               long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long ldg, LiveRows live, int N, float logit_scale,
-                               long long ignore_index, cudaStream_t stream) {
+void token_log_probs_grad_rows(const float* logits, long long ldl, const void* labels, bool labels64, const float2* lse,
+    const float* entropy, const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
+    void* grad, long long ldg, LiveRows live, int N, float logit_scale, long long ignore_index, cudaStream_t stream) {
   if (live.rows <= 0) return;
   constexpr int kColumns = GRAD_THREADS * GRAD_UNROLL * 8;
   const unsigned chunks = (unsigned)((N + kColumns - 1) / kColumns);
   auto kernel = d_entropy != nullptr ? grad_rows_kernel<true> : grad_rows_kernel<false>;
-  kernel<<<(unsigned)live.rows * chunks, GRAD_THREADS, 0, stream>>>(logits, ldl, labels, labels64, lse, entropy, d_log_probs, d_log_probs_stride, d_entropy, d_entropy_stride,
-                                                                    reinterpret_cast<__nv_bfloat16*>(grad), ldg, live, N, logit_scale, logit_scale * kLog2e, ignore_index, chunks);
+  kernel<<<(unsigned)live.rows * chunks, GRAD_THREADS, 0, stream>>>(logits, ldl, labels, labels64, lse, entropy, d_log_probs,
+      d_log_probs_stride, d_entropy, d_entropy_stride, reinterpret_cast<__nv_bfloat16*>(grad), ldg, live, N, logit_scale,
+      logit_scale * kLog2e, ignore_index, chunks);
   count_launch();
   check_cuda(cudaGetLastError(), "kept logits gradient launch");
 }
@@ -611,9 +621,9 @@ namespace {
 constexpr int COMPACT_THREADS = 256;
 
 __global__ void __launch_bounds__(COMPACT_THREADS)
-    compact_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V, const __nv_bfloat16* __restrict__ x, long long ldx, int H, int share,
-                        int* __restrict__ index, int* __restrict__ count, __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs,
-                        float* __restrict__ entropy, float2* __restrict__ lse) {
+    compact_rows_kernel(const void* __restrict__ labels, bool labels64, long long ignore_index, int T, int V,
+        const __nv_bfloat16* __restrict__ x, long long ldx, int H, int share, int* __restrict__ index, int* __restrict__ count,
+        __nv_bfloat16* __restrict__ compact, float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse) {
   __shared__ int warp_count[COMPACT_THREADS / 32], place[32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int first = blockIdx.x * share, end = min(T, first + share);
@@ -667,13 +677,14 @@ __global__ void __launch_bounds__(COMPACT_THREADS)
 
 }  // namespace
 
-void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* count, void* compact,
-                        float* log_probs, float* entropy, float2* lse, cudaStream_t stream) {
+void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H,
+    int* index, int* count, void* compact, float* log_probs, float* entropy, float2* lse, cudaStream_t stream) {
   // a row per warp as long as that makes at most 1024 blocks (each of them reads all labels before its rows)
   int share = 8;
   while ((T + share - 1) / share > 1024) share *= 2;
-  compact_rows_kernel<<<(T + share - 1) / share, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V, reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, share, index, count,
-                                                                               reinterpret_cast<__nv_bfloat16*>(compact), log_probs, entropy, lse);
+  compact_rows_kernel<<<(T + share - 1) / share, COMPACT_THREADS, 0, stream>>>(labels, labels64, ignore_index, T, V,
+      reinterpret_cast<const __nv_bfloat16*>(x), ldx, H, share, index, count, reinterpret_cast<__nv_bfloat16*>(compact), log_probs,
+      entropy, lse);
   count_launch();
   check_cuda(cudaGetLastError(), "compact rows launch");
 }

@@ -35,20 +35,20 @@ struct LiveRows {
 };
 // index[0 .. *count) <- rows with a label in [0, V) other than ignore_index, in order; compact[r] <-
 // x[index[r]] (bf16 rows of H, a multiple of 8 elements), zeros from *count on; outputs of the rows that do not count <- 0.
-void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H, int* index, int* count, void* compact,
-                        float* log_probs, float* entropy, float2* lse, cudaStream_t stream);
+void vocab_compact_rows(const void* labels, bool labels64, long long ignore_index, int T, int V, const void* x, long long ldx, int H,
+    int* index, int* count, void* compact, float* log_probs, float* entropy, float2* lse, cudaStream_t stream);
 // Joins the statistics of `slices` column slices of the rows: stats[slice][live.rows] = (m, s, u, the label's logit if it lies in the
 // slice), see softmax_stats.cuh. Ignored rows give 0.
 void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
-                          float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream);
+    float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream);
 
 // ---- gemm/vocab_gemm_2sm.cu: logits = x [M, K] w [N, K]^T, bf16 operands with row strides that are multiples of 8 elements;
 // the logits stay in tensor memory.
 // x holds the rows of this launch; labels, lse and gradients are those of the whole batch.
 constexpr int kVocabSlice = 128;  // columns per slice of the statistics
 // logits: null, or fp32 [live.rows, N] with a row stride ldl that is a multiple of 4, which keeps the live rows' logits.
-void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl, bool entropy, LiveRows live, int N,
-                      int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream);
+void vocab_gemm_stats(const void* x, const void* w, const void* labels, bool labels64, float* stats, float* logits, long long ldl,
+    bool entropy, LiveRows live, int N, int K, long long ldx, long long ldw, float logit_scale, int* status, cudaStream_t stream);
 // grad[live.rows, N] (bf16, row stride ldg, a multiple of 8): gradient of the logits, as token_log_probs_bwd defines it; rows behind
 // the live ones are 0 up to the next multiple of 256.
 void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labels64, const float2* lse, const float* entropy,
@@ -57,21 +57,22 @@ void vocab_gemm_grad(const void* x, const void* w, const void* labels, bool labe
                      long long ignore_index, int* status, cudaStream_t stream);
 
 // The same from kept logits (fp32, row stride ldl), without a product.
-void token_log_probs_grad_rows(const float* logits, long long ldl, const void* labels, bool labels64, const float2* lse, const float* entropy, const float* d_log_probs,
-                               long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride, void* grad, long long ldg, LiveRows live, int N, float logit_scale,
-                               long long ignore_index, cudaStream_t stream);
+void token_log_probs_grad_rows(const float* logits, long long ldl, const void* labels, bool labels64, const float2* lse,
+    const float* entropy, const float* d_log_probs, long long d_log_probs_stride, const float* d_entropy, long long d_entropy_stride,
+    void* grad, long long ldg, LiveRows live, int N, float logit_scale, long long ignore_index, cudaStream_t stream);
 
 // ---- gemm/balanced_gemm_2sm.cu: C [live.rows, N] = A [live.rows, K] B [K, N], bf16, for few tiles and a long K. Tiles that several CTA
 // pairs share leave fp32 partial tiles in `partials` (balanced_partials() words); balanced_rows puts the result together and writes live
 // row r to row t of `out`, its place in the batch. lda, ldb and N: multiples of 8; C and out: rows of N.
 long long balanced_partials();
-void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb, int* status, cudaStream_t stream);
+void balanced_gemm(const void* A, const void* B, void* C, float* partials, LiveRows live, int N, int K, long long lda, long long ldb,
+    int* status, cudaStream_t stream);
 void balanced_rows(const void* C, const float* partials, LiveRows live, void* out, int N, int K, cudaStream_t stream);
 
 // ---- gemm/gemm_bf16_2sm.cu: C [M, N] (+)= A [K, M]^T B [K, N] on CTA pairs, where the K rows are those of a compacted batch: the
 // contraction ends at max(1, *count - base). Rows from there to the next multiple of 64 must be 0 in both operands.
-void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc, bool f32_accumulate, LiveRows live, int* status,
-                        cudaStream_t stream);
+void gemm_bf16_2sm_live(const void* A, const void* B, void* C, int M, int N, int K, long long lda, long long ldb, long long ldc,
+    bool f32_accumulate, LiveRows live, int* status, cudaStream_t stream);
 
 // ---- ops/preference.cu
 // A packed batch of `sequences` sequences of per-token values: sequence i is tokens [cu[i], cu[i + 1]), or, without cu,
@@ -115,10 +116,10 @@ struct PolicyOut {
 // kl: mean KL estimate, clipped: share of tokens whose gradient is clipped; slope (or null): [T] d(token's loss) /
 // d(log-prob); weight: [sequences] 1 / tokens of the sequence (reduction 2 only).
 void policy_loss_fwd(const float* log_probs, const float* old_log_probs, const float* reference, const float* advantages,
-                     PackedTokens tokens, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight, cudaStream_t stream);
+    PackedTokens tokens, PolicyArgs args, float* partials, PolicyOut out, float* slope, float* weight, cudaStream_t stream);
 // grad[t] = slope[t] * factor (* weight[sequence of t]) * d_loss, 0 for tokens that take no part.
-void policy_loss_bwd(const float* slope, const float* factor, const float* weight, const float* d_loss, PackedTokens tokens, int reduction, float* grad,
-                     cudaStream_t stream);
+void policy_loss_bwd(const float* slope, const float* factor, const float* weight, const float* d_loss, PackedTokens tokens,
+    int reduction, float* grad, cudaStream_t stream);
 
 // ---- ops/embedding_sorted.cu
 constexpr int kStatusBadTokenId = 7;  // an id outside of [0, V): its output row is 0, it takes no part in the gradient

@@ -50,7 +50,8 @@ void check_device(const Tensor& t, const Tensor& like, const char* name) {
 
 void check_indices(const Tensor& t, const Tensor& like, const char* name) {
   check_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32, name, " must be int64 or int32, got ", text(t.scalar_type()));
+  TORCH_CHECK(t.scalar_type() == torch::kInt64 || t.scalar_type() == torch::kInt32, name, " must be int64 or int32, got ",
+      text(t.scalar_type()));
   TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
 }
 
@@ -64,7 +65,8 @@ const float* row_values(const Tensor& t, const Tensor& like, int64_t rows, const
 
 const float* contiguous_f32(const Tensor& t, const Tensor& like, int64_t count, const char* name) {
   check_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.numel() == count, name, " must be contiguous fp32 with ", text(count), " elements");
+  TORCH_CHECK(t.scalar_type() == torch::kFloat32 && t.is_contiguous() && t.numel() == count, name, " must be contiguous fp32 with ",
+      text(count), " elements");
   return t.data_ptr<float>();
 }
 
@@ -85,7 +87,8 @@ RowMap row_map(const Tensor& logits) {
   return {std::max<int64_t>(logits.size(1), 1), logits.stride(0), logits.stride(1)};
 }
 
-std::tuple<Tensor, Tensor, Tensor> log_probs_fwd(const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy) {
+std::tuple<Tensor, Tensor, Tensor> log_probs_fwd(const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index,
+    bool want_entropy) {
   TORCH_CHECK(logits.is_cuda(), "logits must be a CUDA tensor");
   const Scalar type = scalar_of(logits, "logits");
   const RowMap map = row_map(logits);
@@ -95,7 +98,8 @@ std::tuple<Tensor, Tensor, Tensor> log_probs_fwd(const Tensor& logits, const Ten
   const c10::cuda::CUDAGuard guard(logits.device());
   // outputs are tensors of their own, not views: a caller may change them in place
   const auto f32 = logits.options().dtype(torch::kFloat32);
-  Tensor log_probs = torch::empty(labels.sizes(), f32), lse = empty_pairs(rows, logits), entropy = want_entropy ? torch::empty(labels.sizes(), f32) : Tensor();
+  Tensor log_probs = torch::empty(labels.sizes(), f32), lse = empty_pairs(rows, logits),
+      entropy = want_entropy ? torch::empty(labels.sizes(), f32) : Tensor();
   token_log_probs_fwd(logits.data_ptr(), type, labels.data_ptr(), labels.scalar_type() == torch::kInt64, log_probs.data_ptr<float>(),
                       want_entropy ? entropy.data_ptr<float>() : nullptr, pairs(lse), rows, (int)logits.size(2), map, (float)logit_scale,
                       ignore_index, stream_of(logits));
@@ -119,19 +123,22 @@ Tensor log_probs_bwd(const Tensor& logits, const Tensor& labels, const Tensor& l
   const int64_t per_16 = 16 / logits.element_size();
   const int64_t pitch = (V + per_16 - 1) / per_16 * per_16;
   Tensor grad = torch::empty({outer, inner, pitch}, logits.options()).narrow(2, 0, V);
-  token_log_probs_bwd(logits.data_ptr(), type, labels.data_ptr(), labels.scalar_type() == torch::kInt64, checked_pairs(lse, logits, rows),
-                      h != nullptr ? contiguous_f32(*entropy, logits, rows, "entropy") : nullptr, g, g_stride, h, h_stride, grad.data_ptr(), rows, (int)V,
-                      map, pitch, (float)logit_scale, ignore_index, stream_of(logits));
+  token_log_probs_bwd(logits.data_ptr(), type, labels.data_ptr(), labels.scalar_type() == torch::kInt64,
+      checked_pairs(lse, logits, rows), h != nullptr ? contiguous_f32(*entropy, logits, rows, "entropy") : nullptr, g, g_stride, h,
+      h_stride, grad.data_ptr(), rows, (int)V, map, pitch, (float)logit_scale, ignore_index, stream_of(logits));
   return grad;
 }
 
 void check_linear(const Tensor& x, const Tensor& w, const Tensor& labels) {
-  TORCH_CHECK(x.is_cuda() && x.scalar_type() == torch::kBFloat16 && w.scalar_type() == torch::kBFloat16, "hidden states and weight must be bf16 CUDA tensors");
+  TORCH_CHECK(x.is_cuda() && x.scalar_type() == torch::kBFloat16 && w.scalar_type() == torch::kBFloat16,
+      "hidden states and weight must be bf16 CUDA tensors");
   check_device(w, x, "weight");
   TORCH_CHECK(x.dim() == 2 && w.dim() == 2 && x.size(1) == w.size(1), "hidden states must be [T, H] and the weight [V, H]");
   TORCH_CHECK(x.stride(1) == 1 && w.stride(1) == 1, "hidden states and weight must have a unit inner stride");
-  TORCH_CHECK(x.size(1) > 0 && x.size(1) % 8 == 0 && x.stride(0) % 8 == 0 && w.stride(0) % 8 == 0, "H and the row strides must be multiples of 8");
-  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(w.data_ptr())) % 16 == 0, "hidden states and weight must be 16-byte aligned");
+  TORCH_CHECK(x.size(1) > 0 && x.size(1) % 8 == 0 && x.stride(0) % 8 == 0 && w.stride(0) % 8 == 0,
+      "H and the row strides must be multiples of 8");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(x.data_ptr()) | reinterpret_cast<uintptr_t>(w.data_ptr())) % 16 == 0,
+      "hidden states and weight must be 16-byte aligned");
   TORCH_CHECK(w.size(0) > 0 && w.size(0) <= (1 << 29) && x.size(1) < (1 << 30) && x.size(0) < (1LL << 31), "sizes out of range");
   check_indices(labels, x, "labels");
   TORCH_CHECK(labels.numel() == x.size(0), "labels must have one entry per row of hidden states");
@@ -157,7 +164,8 @@ constexpr int64_t kCompactAbove = 256;
 LiveRows live_rows(const Tensor& map, int64_t T, int64_t base, int64_t rows) {
   LiveRows live = {nullptr, nullptr, (int)base, (int)rows};
   if (map.numel() == 0) return live;
-  TORCH_CHECK(map.is_cuda() && map.scalar_type() == torch::kInt32 && map.is_contiguous() && map.numel() == T + 1, "the row map must be int32 [T + 1]");
+  TORCH_CHECK(map.is_cuda() && map.scalar_type() == torch::kInt32 && map.is_contiguous() && map.numel() == T + 1,
+      "the row map must be int32 [T + 1]");
   live.index = map.data_ptr<int>();
   live.count = map.data_ptr<int>() + T;
   return live;
@@ -166,8 +174,8 @@ LiveRows live_rows(const Tensor& map, int64_t T, int64_t base, int64_t rows) {
 void* row_ptr(const Tensor& t, int64_t row) { return reinterpret_cast<char*>(t.data_ptr()) + row * t.stride(0) * t.element_size(); }
 
 // (log_probs, entropy, lse, the rows that were multiplied, row map, their logits if they are kept)
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
-                                                                        bool want_entropy, bool differentiated, bool keep_logits, const Tensor& status) {
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels,
+    double logit_scale, int64_t ignore_index, bool want_entropy, bool differentiated, bool keep_logits, const Tensor& status) {
   check_linear(x, w, labels);
   int* st = status_of(status, x);
   const c10::cuda::CUDAGuard guard(x.device());
@@ -184,18 +192,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(
   if (compact) {
     int* m = map.data_ptr<int>();
     xc = torch::empty({rows, H}, x.options());
-    vocab_compact_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, x.data_ptr(), x.stride(0), (int)H, m, m + rows, xc.data_ptr(),
-                       log_probs.data_ptr<float>(), ent, pairs(lse), stream);
+    vocab_compact_rows(labels.data_ptr(), labels64, ignore_index, (int)rows, (int)V, x.data_ptr(), x.stride(0), (int)H, m, m + rows,
+        xc.data_ptr(), log_probs.data_ptr<float>(), ent, pairs(lse), stream);
   }
   const int64_t most = stats_rows(rows, slices);
   Tensor stats = empty_f32(most * slices * 4, x);
   for (int64_t r = 0; r < rows; r += most) {
     const LiveRows live = live_rows(map, rows, r, std::min(most, rows - r));
-    vocab_gemm_stats(row_ptr(xc, r), w.data_ptr(), labels.data_ptr(), labels64, stats.data_ptr<float>(), keep_logits ? reinterpret_cast<float*>(row_ptr(logits, r)) : nullptr,
-                     keep_logits ? logits.stride(0) : 0, want_entropy, live, (int)V, (int)H, xc.stride(0), w.stride(0),
-                     (float)logit_scale, st, stream);
-    token_log_probs_join(stats.data_ptr<float>(), (int)slices, kVocabSlice, labels.data_ptr(), labels64, log_probs.data_ptr<float>(), ent, pairs(lse), live, (int)V,
-                         (float)logit_scale, ignore_index, stream);
+    vocab_gemm_stats(row_ptr(xc, r), w.data_ptr(), labels.data_ptr(), labels64, stats.data_ptr<float>(),
+        keep_logits ? reinterpret_cast<float*>(row_ptr(logits, r)) : nullptr, keep_logits ? logits.stride(0) : 0, want_entropy, live,
+        (int)V, (int)H, xc.stride(0), w.stride(0), (float)logit_scale, st, stream);
+    token_log_probs_join(stats.data_ptr<float>(), (int)slices, kVocabSlice, labels.data_ptr(), labels64, log_probs.data_ptr<float>(),
+        ent, pairs(lse), live, (int)V, (float)logit_scale, ignore_index, stream);
   }
   return {log_probs, entropy, lse, xc, map, logits};
 }
@@ -209,7 +217,8 @@ PackedTokens packed_tokens(const Tensor& values, const OptTensor& cu, int64_t le
   p.sequences = (int)sequences;
   if (cu.has_value()) {
     check_device(*cu, values, "cu_seqlens");
-    TORCH_CHECK(cu->scalar_type() == torch::kInt32 && cu->is_contiguous() && cu->numel() == sequences + 1, "cu_seqlens must be contiguous int32 [sequences + 1]");
+    TORCH_CHECK(cu->scalar_type() == torch::kInt32 && cu->is_contiguous() && cu->numel() == sequences + 1,
+        "cu_seqlens must be contiguous int32 [sequences + 1]");
     p.cu = cu->data_ptr<int>();
   } else {
     TORCH_CHECK(length * sequences == p.T, "sequences of one length must cover all tokens");
@@ -224,8 +233,9 @@ PackedTokens packed_tokens(const Tensor& values, const OptTensor& cu, int64_t le
 }
 
 // (loss, chosen rewards, rejected rewards, slope [2 * pairs])
-std::tuple<Tensor, Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu, int64_t length, int64_t sequences,
-                                                  const OptTensor& mask, int64_t kind, double beta, double label_smoothing, bool average, int64_t reduction) {
+std::tuple<Tensor, Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu,
+    int64_t length, int64_t sequences, const OptTensor& mask, int64_t kind, double beta, double label_smoothing, bool average,
+    int64_t reduction) {
   TORCH_CHECK(log_probs.is_cuda(), "log_probs must be a CUDA tensor");
   TORCH_CHECK(sequences > 0 && sequences % 2 == 0, "an even number of sequences is needed: chosen, then rejected");
   TORCH_CHECK(kind >= 0 && kind <= 2 && reduction >= 0 && reduction <= 2, "unknown loss type or reduction");
@@ -234,13 +244,16 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_prob
   const float* ref = reference.has_value() ? contiguous_f32(*reference, log_probs, p.T, "reference_log_probs") : nullptr;
   const c10::cuda::CUDAGuard guard(log_probs.device());
   Tensor loss = reduction == 0 ? empty_f32(sequences / 2, log_probs) : torch::empty({}, log_probs.options());
-  Tensor chosen = empty_f32(sequences / 2, log_probs), rejected = empty_f32(sequences / 2, log_probs), slope = empty_f32(sequences, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
+  Tensor chosen = empty_f32(sequences / 2, log_probs), rejected = empty_f32(sequences / 2, log_probs),
+      slope = empty_f32(sequences, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
   const PreferenceArgs args = {(PreferenceKind)kind, (float)beta, (float)label_smoothing, average, (int)reduction};
-  preference_loss_fwd(lp, ref, p, args, partials.data_ptr<float>(), loss.data_ptr<float>(), chosen.data_ptr<float>(), rejected.data_ptr<float>(), slope.data_ptr<float>(), stream_of(log_probs));
+  preference_loss_fwd(lp, ref, p, args, partials.data_ptr<float>(), loss.data_ptr<float>(), chosen.data_ptr<float>(),
+      rejected.data_ptr<float>(), slope.data_ptr<float>(), stream_of(log_probs));
   return {loss, chosen, rejected, slope};
 }
 
-Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& log_probs, const OptTensor& cu, int64_t length, const OptTensor& mask) {
+Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& log_probs, const OptTensor& cu, int64_t length,
+    const OptTensor& mask) {
   const int64_t sequences = slope.numel();
   const PackedTokens p = packed_tokens(log_probs, cu, length, sequences, mask);
   contiguous_f32(slope, log_probs, sequences, "slope");
@@ -258,9 +271,9 @@ Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& l
 }
 
 // (loss, kl, clipped share, factor [1], slope [T] or undefined, weight [sequences])
-std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Tensor& old_log_probs, const OptTensor& reference, const Tensor& advantages, bool per_token,
-                                              const OptTensor& cu, int64_t length, int64_t sequences, const OptTensor& mask, double clip_low, double clip_high,
-                                              double dual_clip, double kl_coef, int64_t reduction, bool want_slope) {
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_fwd(const Tensor& log_probs, const Tensor& old_log_probs,
+    const OptTensor& reference, const Tensor& advantages, bool per_token, const OptTensor& cu, int64_t length, int64_t sequences,
+    const OptTensor& mask, double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t reduction, bool want_slope) {
   TORCH_CHECK(log_probs.is_cuda(), "log_probs must be a CUDA tensor");
   TORCH_CHECK(reduction >= 0 && reduction <= 2, "unknown reduction");
   const PackedTokens p = packed_tokens(log_probs, cu, length, sequences, mask);
@@ -269,7 +282,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_fwd(const Tens
   const float* ref = reference.has_value() ? contiguous_f32(*reference, log_probs, p.T, "reference_log_probs") : nullptr;
   const float* adv = contiguous_f32(advantages, log_probs, per_token ? p.T : sequences, "advantages");
   const c10::cuda::CUDAGuard guard(log_probs.device());
-  Tensor loss = torch::empty({}, log_probs.options()), kl = torch::empty_like(loss), clipped = torch::empty_like(loss), factor = empty_f32(1, log_probs), slope = want_slope ? empty_f32(p.T, log_probs) : Tensor();
+  Tensor loss = torch::empty({}, log_probs.options()), kl = torch::empty_like(loss), clipped = torch::empty_like(loss),
+      factor = empty_f32(1, log_probs), slope = want_slope ? empty_f32(p.T, log_probs) : Tensor();
   Tensor weight = empty_f32(reduction == 2 ? sequences : 0, log_probs), partials = empty_f32(packed_partials(p.T, p.sequences), log_probs);
   PolicyArgs args = {};
   args.log_low = std::log1p(-clip_low);
@@ -280,13 +294,14 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> policy_fwd(const Tens
   args.kl_coef = (float)kl_coef;
   args.per_token_advantage = per_token;
   args.reduction = (int)reduction;
-  policy_loss_fwd(lp, old, ref, adv, p, args, partials.data_ptr<float>(), {loss.data_ptr<float>(), kl.data_ptr<float>(), clipped.data_ptr<float>(), factor.data_ptr<float>()}, want_slope ? slope.data_ptr<float>() : nullptr, weight.data_ptr<float>(),
-                  stream_of(log_probs));
+  policy_loss_fwd(lp, old, ref, adv, p, args, partials.data_ptr<float>(), {loss.data_ptr<float>(), kl.data_ptr<float>(),
+      clipped.data_ptr<float>(), factor.data_ptr<float>()}, want_slope ? slope.data_ptr<float>() : nullptr, weight.data_ptr<float>(),
+      stream_of(log_probs));
   return {loss, kl, clipped, factor, slope, weight};
 }
 
-Tensor policy_bwd(const Tensor& slope, const Tensor& factor, const Tensor& weight, const Tensor& d_loss, at::IntArrayRef shape, const OptTensor& cu, int64_t length,
-                  int64_t sequences, const OptTensor& mask, int64_t reduction) {
+Tensor policy_bwd(const Tensor& slope, const Tensor& factor, const Tensor& weight, const Tensor& d_loss, at::IntArrayRef shape,
+    const OptTensor& cu, int64_t length, int64_t sequences, const OptTensor& mask, int64_t reduction) {
   const PackedTokens p = packed_tokens(slope, cu, length, sequences, mask);
   contiguous_f32(slope, slope, p.T, "slope");
   contiguous_f32(factor, slope, 1, "factor");
@@ -295,8 +310,8 @@ Tensor policy_bwd(const Tensor& slope, const Tensor& factor, const Tensor& weigh
   const c10::cuda::CUDAGuard guard(slope.device());
   Tensor grad = torch::empty(shape, slope.options());
   TORCH_CHECK(grad.numel() == p.T, "shape mismatch");
-  policy_loss_bwd(slope.data_ptr<float>(), factor.data_ptr<float>(), weight.data_ptr<float>(), d_loss.data_ptr<float>(), p, (int)reduction, grad.data_ptr<float>(),
-                  stream_of(slope));
+  policy_loss_bwd(slope.data_ptr<float>(), factor.data_ptr<float>(), weight.data_ptr<float>(), d_loss.data_ptr<float>(), p,
+      (int)reduction, grad.data_ptr<float>(), stream_of(slope));
   return grad;
 }
 
@@ -311,8 +326,8 @@ Tensor embedding_lookup_(const Tensor& weight, const Tensor& ids, double scale, 
   auto shape = ids.sizes().vec();
   shape.push_back(weight.size(1));
   Tensor out = torch::empty(shape, weight.options());
-  embedding_lookup(weight.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, out.data_ptr(), ids.numel(), weight.size(0), (int)weight.size(1), (float)scale, st,
-                   stream_of(weight));
+  embedding_lookup(weight.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, out.data_ptr(), ids.numel(),
+      weight.size(0), (int)weight.size(1), (float)scale, st, stream_of(weight));
   return out;
 }
 
@@ -322,7 +337,8 @@ Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, con
   const Scalar type = scalar_of(dout, "dout");
   check_indices(ids, dout, "ids");
   const int64_t T = ids.numel(), H = dout.size(-1);
-  TORCH_CHECK(dout.numel() == T * H && T <= (1LL << 30) && H < (1 << 30) && V >= 0 && V < (1LL << 31) - 1, "dout must be [T, H] for T ids; at most 2^30 tokens and 2^31 - 2 rows");
+  TORCH_CHECK(dout.numel() == T * H && T <= (1LL << 30) && H < (1 << 30) && V >= 0 && V < (1LL << 31) - 1,
+      "dout must be [T, H] for T ids; at most 2^30 tokens and 2^31 - 2 rows");
   const c10::cuda::CUDAGuard guard(dout.device());
   Tensor dw;
   if (dweight.has_value()) {
@@ -332,8 +348,8 @@ Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, con
     dw = torch::empty({V, H}, dout.options());
   }
   Tensor workspace = torch::empty({embedding_gradient_workspace(T, (int)H, type)}, dout.options().dtype(torch::kUInt8));
-  embedding_gradient(dout.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, dw.data_ptr(), dweight.has_value(), workspace.data_ptr(), T, V, (int)H, (float)scale,
-                     stream_of(dout));
+  embedding_gradient(dout.data_ptr(), type, ids.data_ptr(), ids.scalar_type() == torch::kInt64, dw.data_ptr(), dweight.has_value(),
+      workspace.data_ptr(), T, V, (int)H, (float)scale, stream_of(dout));
   return dw;
 }
 
@@ -363,7 +379,8 @@ Tensor rows3(const Tensor& logits) {
 }
 
 struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy) {
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& labels, double logit_scale,
+      int64_t ignore_index, bool want_entropy) {
     auto [log_probs, entropy, lse] = log_probs_fwd(rows3(logits), labels.contiguous(), logit_scale, ignore_index, want_entropy);
     ctx->save_for_backward({logits, labels, lse, entropy});
     ctx->saved_data["logit_scale"] = logit_scale;
@@ -378,9 +395,9 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     const bool has_h = grads.size() > 1 && grads[1].defined();
     if (!grads[0].defined() && !has_h) return variable_list(5);
     const int64_t rows = labels.numel();
-    Tensor grad = log_probs_bwd(rows3(logits), labels.contiguous(), lse, entropy.defined() ? OptTensor(entropy) : OptTensor(), row_gradient(grads[0], rows, lse),
-                                has_h ? OptTensor(row_gradient(grads[1], rows, lse)) : OptTensor(), ctx->saved_data["logit_scale"].toDouble(),
-                                ctx->saved_data["ignore_index"].toInt());
+    Tensor grad = log_probs_bwd(rows3(logits), labels.contiguous(), lse, entropy.defined() ? OptTensor(entropy) : OptTensor(),
+        row_gradient(grads[0], rows, lse), has_h ? OptTensor(row_gradient(grads[1], rows, lse)) : OptTensor(),
+        ctx->saved_data["logit_scale"].toDouble(), ctx->saved_data["ignore_index"].toInt());
     return {once(grad.view(logits.sizes()), "token_log_probs"), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
@@ -392,7 +409,8 @@ OptTensor main_grad(const Tensor& weight) {
   const py::object target = py::getattr(p, "main_grad", py::none());
   if (target.is_none()) return OptTensor();
   Tensor t = py::cast<Tensor>(target).view(weight.sizes());
-  TORCH_CHECK(t.is_cuda() && t.device() == weight.device() && t.scalar_type() == torch::kFloat32 && t.is_contiguous(), "main_grad must be a contiguous fp32 tensor on the weight's device");
+  TORCH_CHECK(t.is_cuda() && t.device() == weight.device() && t.scalar_type() == torch::kFloat32 && t.is_contiguous(),
+      "main_grad must be a contiguous fp32 tensor on the weight's device");
   return t;
 }
 
@@ -401,9 +419,10 @@ OptTensor main_grad(const Tensor& weight) {
 // the hidden states. Both ways see the same fp32 logits. The batch is compacted to the rows whose label counts, and all products end
 // there.
 struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool want_entropy, int64_t chunk,
-                               bool differentiated, bool keep_logits, const Tensor& status) {
-    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy, differentiated, keep_logits, status);
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale,
+      int64_t ignore_index, bool want_entropy, int64_t chunk, bool differentiated, bool keep_logits, const Tensor& status) {
+    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy,
+        differentiated, keep_logits, status);
     ctx->save_for_backward({xc, w, labels, lse, entropy, map, status, logits});
     ctx->saved_data["logit_scale"] = logit_scale;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -414,7 +433,8 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5], &logits = saved[7];
+    const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5],
+        &logits = saved[7];
     const bool has_h = grads.size() > 1 && grads[1].defined();
     if (!grads[0].defined() && !has_h) return variable_list(10);
     const int64_t T = xc.size(0), H = xc.size(1), V = w.size(0);
@@ -451,17 +471,19 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
       const int64_t ignore_index = ctx->saved_data["ignore_index"].toInt();
       const float* ent = has_h ? entropy.data_ptr<float>() : nullptr;
       if (logits.defined())
-        token_log_probs_grad_rows(reinterpret_cast<const float*>(row_ptr(logits, r)), logits.stride(0), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(),
-                                  dl.stride(0), live, (int)V, logit_scale, ignore_index, stream);
+        token_log_probs_grad_rows(reinterpret_cast<const float*>(row_ptr(logits, r)), logits.stride(0), labels.data_ptr(), labels64,
+            pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), dl.stride(0), live, (int)V, logit_scale, ignore_index, stream);
       else
-        vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0),
-                        dl.stride(0), logit_scale, ignore_index, st, stream);
+        vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride,
+            dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0), dl.stride(0), logit_scale, ignore_index, st, stream);
       if (need_dx) {
-        balanced_gemm(dl.data_ptr(), w.data_ptr(), dxc.data_ptr(), partials.data_ptr<float>(), live, (int)H, (int)V, dl.stride(0), w.stride(0), st, stream);
+        balanced_gemm(dl.data_ptr(), w.data_ptr(), dxc.data_ptr(), partials.data_ptr<float>(), live, (int)H, (int)V, dl.stride(0),
+            w.stride(0), st, stream);
         balanced_rows(dxc.data_ptr(), partials.data_ptr<float>(), live, dx.data_ptr(), (int)H, (int)V, stream);
       }
       if (need_dw) {
-        gemm_bf16_2sm_live(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0), dw.stride(0), dw.scalar_type() == torch::kFloat32, live, st, stream);
+        gemm_bf16_2sm_live(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0),
+            dw.stride(0), dw.scalar_type() == torch::kFloat32, live, st, stream);
       }
     }
     variable_list out(10);
@@ -476,14 +498,16 @@ void check_logit_scale(double logit_scale) {
 }
 
 void check_label_shape(const Tensor& labels, at::IntArrayRef shape, const Tensor& like) {
-  TORCH_CHECK_VALUE(labels.scalar_type() == torch::kInt64 || labels.scalar_type() == torch::kInt32, "labels must be int64 or int32, got ", text(labels.scalar_type()));
+  TORCH_CHECK_VALUE(labels.scalar_type() == torch::kInt64 || labels.scalar_type() == torch::kInt32,
+      "labels must be int64 or int32, got ", text(labels.scalar_type()));
   TORCH_CHECK_VALUE(labels.sizes() == shape, "labels must have the shape ", text(shape), ", got ", text(labels.sizes()));
   TORCH_CHECK_VALUE(labels.device() == like.device(), "labels must be on ", text(like.device()), ", got ", text(labels.device()));
 }
 
 variable_list token_log_probs(const Tensor& logits, const Tensor& labels, double logit_scale, int64_t ignore_index, bool return_entropy) {
   check_logit_scale(logit_scale);
-  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must have a last dimension of at least 1, got ", text(logits.sizes()));
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) > 0, "logits must have a last dimension of at least 1, got ",
+      text(logits.sizes()));
   check_label_shape(labels, logits.sizes().slice(0, logits.dim() - 1), logits);
   return TokenLogProbs::apply(logits, labels, logit_scale, ignore_index, return_entropy);
 }
@@ -494,19 +518,20 @@ Tensor mapped_rows(const Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
-variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index, bool return_entropy, int64_t chunk, int64_t keep_bytes,
-                                     const Tensor& status) {
+variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
+    bool return_entropy, int64_t chunk, int64_t keep_bytes, const Tensor& status) {
   check_logit_scale(logit_scale);
-  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(0) > 0 && w.size(1) > 0, "hidden states [..., H] and a weight [V, H] are needed, got ", text(x.sizes()), " and ",
-                    text(w.sizes()));
-  TORCH_CHECK_VALUE(x.device() == w.device() && x.scalar_type() == w.scalar_type(), "hidden states and weight must be of one type on one device, got ", text(x.scalar_type()), " on ",
-                    text(x.device()), " and ", text(w.scalar_type()), " on ", text(w.device()));
+  TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1) && w.size(0) > 0 && w.size(1) > 0,
+      "hidden states [..., H] and a weight [V, H] are needed, got ", text(x.sizes()), " and ", text(w.sizes()));
+  TORCH_CHECK_VALUE(x.device() == w.device() && x.scalar_type() == w.scalar_type(),
+      "hidden states and weight must be of one type on one device, got ", text(x.scalar_type()), " on ", text(x.device()), " and ",
+      text(w.scalar_type()), " on ", text(w.device()));
   const auto shape = x.sizes().slice(0, x.dim() - 1);
   check_label_shape(labels, shape, x);
   const bool differentiated = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
   const bool keep = differentiated && 4.0 * (double)labels.numel() * (double)w.size(0) <= (double)keep_bytes;
-  variable_list out = LinearTokenLogProbs::apply(mapped_rows(x.reshape({labels.numel(), x.size(-1)})), mapped_rows(w), labels.reshape({labels.numel()}).contiguous(), logit_scale, ignore_index,
-                                                 return_entropy, chunk, differentiated, keep, status);
+  variable_list out = LinearTokenLogProbs::apply(mapped_rows(x.reshape({labels.numel(), x.size(-1)})), mapped_rows(w),
+      labels.reshape({labels.numel()}).contiguous(), logit_scale, ignore_index, return_entropy, chunk, differentiated, keep, status);
   if (x.dim() != 2)
     for (auto& t : out) t = t.view(shape);
   return out;
@@ -522,12 +547,14 @@ Sequences check_sequences(const Tensor& log_probs, const OptTensor& cu_seqlens, 
   Sequences s = {};
   TORCH_CHECK_VALUE(log_probs.is_floating_point(), "log_probs must be floating point, got ", text(log_probs.scalar_type()));
   if (mask.has_value()) {
-    TORCH_CHECK_VALUE(mask->sizes() == log_probs.sizes() && mask->device() == log_probs.device() && !mask->is_floating_point(), "mask must be boolean or integer, shaped ",
-                      text(log_probs.sizes()), " on ", text(log_probs.device()), ", got ", text(mask->scalar_type()), " ", text(mask->sizes()), " on ", text(mask->device()));
+    TORCH_CHECK_VALUE(mask->sizes() == log_probs.sizes() && mask->device() == log_probs.device() && !mask->is_floating_point(),
+        "mask must be boolean or integer, shaped ", text(log_probs.sizes()), " on ", text(log_probs.device()), ", got ",
+        text(mask->scalar_type()), " ", text(mask->sizes()), " on ", text(mask->device()));
     s.mask = (mask->scalar_type() == torch::kBool ? *mask : mask->ne(0)).contiguous();
   }
   if (!cu_seqlens.has_value()) {
-    TORCH_CHECK_VALUE(log_probs.dim() == 2, "log_probs must be [sequences, length], or [tokens] with cu_seqlens, got ", text(log_probs.sizes()));
+    TORCH_CHECK_VALUE(log_probs.dim() == 2, "log_probs must be [sequences, length], or [tokens] with cu_seqlens, got ",
+        text(log_probs.sizes()));
     s.count = log_probs.size(0);
     s.length = log_probs.size(1);
     return s;
@@ -542,18 +569,22 @@ Sequences check_sequences(const Tensor& log_probs, const OptTensor& cu_seqlens, 
 }
 
 Tensor check_values(const Tensor& t, at::IntArrayRef shape, const Tensor& like, const char* name) {
-  TORCH_CHECK_VALUE(t.sizes() == shape && t.device() == like.device() && t.is_floating_point(), name, " must be floating point, shaped ", text(shape), " on ", text(like.device()), ", got ",
-                    text(t.scalar_type()), " ", text(t.sizes()), " on ", text(t.device()));
-  TORCH_CHECK_VALUE(!t.requires_grad(), name, " must not require a gradient (detach it): the loss is differentiated with respect to log_probs alone");
+  TORCH_CHECK_VALUE(t.sizes() == shape && t.device() == like.device() && t.is_floating_point(), name,
+      " must be floating point, shaped ", text(shape), " on ", text(like.device()), ", got ", text(t.scalar_type()), " ",
+      text(t.sizes()), " on ", text(t.device()));
+  TORCH_CHECK_VALUE(!t.requires_grad(), name,
+      " must not require a gradient (detach it): the loss is differentiated with respect to log_probs alone");
   return t.to(torch::kFloat32).contiguous();
 }
 
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu, const OptTensor& mask, int64_t length,
-                               int64_t sequences, int64_t kind, double beta, double label_smoothing, bool average, int64_t reduction) {
-    auto [loss, chosen, rejected, slope] = preference_fwd(log_probs, reference, cu, length, sequences, mask, kind, beta, label_smoothing, average, reduction);
+  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu,
+      const OptTensor& mask, int64_t length, int64_t sequences, int64_t kind, double beta, double label_smoothing, bool average,
+      int64_t reduction) {
+    auto [loss, chosen, rejected, slope] = preference_fwd(log_probs, reference, cu, length, sequences, mask, kind, beta,
+        label_smoothing, average, reduction);
     ctx->save_for_backward({slope, log_probs, cu.value_or(Tensor()), mask.value_or(Tensor())});
     ctx->saved_data["length"] = length;
     ctx->mark_non_differentiable({chosen, rejected});
@@ -564,13 +595,15 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(11);
     if (!grads[0].defined()) return out;
-    out[0] = once(preference_bwd(saved[0], grads[0], saved[1], optional(saved[2]), ctx->saved_data["length"].toInt(), optional(saved[3])), "preference_loss");
+    out[0] = once(preference_bwd(saved[0], grads[0], saved[1], optional(saved[2]), ctx->saved_data["length"].toInt(),
+                                 optional(saved[3])),
+                  "preference_loss");
     return out;
   }
 };
 
-variable_list preference_loss(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu_seqlens, const OptTensor& mask, int64_t kind, double beta,
-                              double label_smoothing, bool average, int64_t reduction) {
+variable_list preference_loss(const Tensor& log_probs, const OptTensor& reference, const OptTensor& cu_seqlens, const OptTensor& mask,
+    int64_t kind, double beta, double label_smoothing, bool average, int64_t reduction) {
   const Sequences s = check_sequences(log_probs, cu_seqlens, mask);
   TORCH_CHECK_VALUE(s.count > 0 && s.count % 2 == 0, "an even number of answers is needed (chosen, then rejected), got ", text(s.count));
   TORCH_CHECK_VALUE(std::isfinite(beta) && beta > 0, "beta must be positive and finite, got ", text(beta));
@@ -578,14 +611,16 @@ variable_list preference_loss(const Tensor& log_probs, const OptTensor& referenc
                     "label_smoothing must be in [0, 0.5) and goes with loss_type='sigmoid', got ", text(label_smoothing));
   OptTensor ref;
   if (reference.has_value()) ref = check_values(*reference, log_probs.sizes(), log_probs, "reference_log_probs");
-  return PreferenceLoss::apply(log_probs.to(torch::kFloat32).contiguous(), ref, s.cu, s.mask, s.length, s.count, kind, beta, label_smoothing, average, reduction);
+  return PreferenceLoss::apply(log_probs.to(torch::kFloat32).contiguous(), ref, s.cu, s.mask, s.length, s.count, kind, beta,
+      label_smoothing, average, reduction);
 }
 
 struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const Tensor& old, const OptTensor& reference, const Tensor& advantages, bool per_token,
-                               const OptTensor& cu, const OptTensor& mask, int64_t length, int64_t sequences, double clip_low, double clip_high, double dual_clip, double kl_coef,
-                               int64_t reduction, bool want_slope) {
-    auto [loss, kl, clipped, factor, slope, weight] = policy_fwd(log_probs, old, reference, advantages, per_token, cu, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction, want_slope);
+  static variable_list forward(AutogradContext* ctx, const Tensor& log_probs, const Tensor& old, const OptTensor& reference,
+      const Tensor& advantages, bool per_token, const OptTensor& cu, const OptTensor& mask, int64_t length, int64_t sequences,
+      double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t reduction, bool want_slope) {
+    auto [loss, kl, clipped, factor, slope, weight] = policy_fwd(log_probs, old, reference, advantages, per_token, cu, length,
+        sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction, want_slope);
     ctx->save_for_backward({slope, factor, weight, cu.value_or(Tensor()), mask.value_or(Tensor())});
     ctx->saved_data["shape"] = log_probs.sizes().vec();
     ctx->saved_data["length"] = length;
@@ -599,29 +634,34 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(15);
     if (!grads[0].defined()) return out;
-    out[0] = once(policy_bwd(saved[0], saved[1], saved[2], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[3]), ctx->saved_data["length"].toInt(),
-                             ctx->saved_data["sequences"].toInt(), optional(saved[4]), ctx->saved_data["reduction"].toInt()),
-                  "policy_loss");
+    out[0] = once(policy_bwd(saved[0], saved[1], saved[2], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[3]),
+        ctx->saved_data["length"].toInt(), ctx->saved_data["sequences"].toInt(), optional(saved[4]),
+        ctx->saved_data["reduction"].toInt()), "policy_loss");
     return out;
   }
 };
 
-variable_list policy_loss(const Tensor& log_probs, const Tensor& old, const Tensor& advantages, const OptTensor& reference, const OptTensor& cu_seqlens, const OptTensor& mask,
-                          double clip_low, double clip_high, double dual_clip, double kl_coef, int64_t reduction) {
+variable_list policy_loss(const Tensor& log_probs, const Tensor& old, const Tensor& advantages, const OptTensor& reference,
+    const OptTensor& cu_seqlens, const OptTensor& mask, double clip_low, double clip_high, double dual_clip, double kl_coef,
+    int64_t reduction) {
   const Sequences s = check_sequences(log_probs, cu_seqlens, mask);
   const Tensor o = check_values(old, log_probs.sizes(), log_probs, "old_log_probs");
   OptTensor ref;
   if (reference.has_value()) ref = check_values(*reference, log_probs.sizes(), log_probs, "reference_log_probs");
   const bool per_sequence = advantages.dim() == 1 && advantages.size(0) == s.count;  // also where there are as many tokens
   const bool per_token = !per_sequence && advantages.sizes() == log_probs.sizes();
-  const Tensor a = per_token ? check_values(advantages, log_probs.sizes(), log_probs, "advantages") : check_values(advantages, {s.count}, log_probs, "advantages");
-  TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low must be in [0, 1] and clip_high at least 0, got ", text(clip_low), " and ", text(clip_high));
+  const Tensor a = per_token ? check_values(advantages, log_probs.sizes(), log_probs, "advantages")
+                             : check_values(advantages, {s.count}, log_probs, "advantages");
+  TORCH_CHECK_VALUE(clip_low >= 0 && clip_low <= 1 && clip_high >= 0, "clip_low must be in [0, 1] and clip_high at least 0, got ",
+      text(clip_low), " and ", text(clip_high));
   TORCH_CHECK_VALUE(std::isfinite(kl_coef) && kl_coef >= 0, "kl_coef must be finite and at least 0, got ", text(kl_coef));
   TORCH_CHECK_VALUE(kl_coef == 0 || reference.has_value(), "kl_coef needs reference_log_probs");
-  TORCH_CHECK_VALUE(dual_clip == 0 || (std::isfinite(dual_clip) && dual_clip > 1), "dual_clip must be finite and above 1, got ", text(dual_clip));
+  TORCH_CHECK_VALUE(dual_clip == 0 || (std::isfinite(dual_clip) && dual_clip > 1), "dual_clip must be finite and above 1, got ",
+      text(dual_clip));
   const Tensor lp = log_probs.to(torch::kFloat32).contiguous();
   const bool want_slope = at::GradMode::is_enabled() && lp.requires_grad();
-  return PolicyLoss::apply(lp, o, ref, a, per_token, s.cu, s.mask, s.length, s.count, clip_low, clip_high, dual_clip, kl_coef, reduction, want_slope);
+  return PolicyLoss::apply(lp, o, ref, a, per_token, s.cu, s.mask, s.length, s.count, clip_low, clip_high, dual_clip, kl_coef,
+      reduction, want_slope);
 }
 
 struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
@@ -644,7 +684,8 @@ struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
 
 Tensor embedding_sorted(const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
   TORCH_CHECK_VALUE(weight.dim() == 2, "the embedding table must be [V, H], got ", text(weight.sizes()));
-  TORCH_CHECK_VALUE(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "ids must be int64 or int32, got ", text(ids.scalar_type()));
+  TORCH_CHECK_VALUE(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "ids must be int64 or int32, got ",
+      text(ids.scalar_type()));
   TORCH_CHECK_VALUE(ids.device() == weight.device(), "ids must be on ", text(weight.device()), ", got ", text(ids.device()));
   return EmbeddingSorted::apply(weight.contiguous(), ids.contiguous(), scale, status);
 }
