@@ -402,7 +402,10 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   }
 };
 
-// The engine's fp32 gradient buffer of a parameter (its Python attribute main_grad), if it has one.
+// The engine's fp32 gradient buffer of a parameter (its Python attribute main_grad), if it has one. It is looked up in the backward
+// pass, on the tensor that forward was given: a variable that was saved may come back as another one (recomputed, or moved away and
+// back) without the attribute. So the functions keep weights in `saved_data`, which hands back what it was given, and so they do with
+// the status word, whose value takes no part in a gradient.
 OptTensor main_grad(const Tensor& weight) {
   const py::gil_scoped_acquire gil;
   const py::object p = py::cast(weight);
@@ -423,7 +426,9 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
       int64_t ignore_index, bool want_entropy, int64_t chunk, bool differentiated, bool keep_logits, const Tensor& status) {
     auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy,
         differentiated, keep_logits, status);
-    ctx->save_for_backward({xc, w, labels, lse, entropy, map, status, logits});
+    ctx->save_for_backward({xc, w, labels, lse, entropy, map, logits});
+    ctx->saved_data["weight"] = w;
+    ctx->saved_data["status"] = status;
     ctx->saved_data["logit_scale"] = logit_scale;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["chunk"] = chunk;
@@ -434,7 +439,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &xc = saved[0], &w = saved[1], &labels = saved[2], &lse = saved[3], &entropy = saved[4], &map = saved[5],
-        &logits = saved[7];
+        &logits = saved[6];
     const bool has_h = grads.size() > 1 && grads[1].defined();
     if (!grads[0].defined() && !has_h) return variable_list(10);
     const int64_t T = xc.size(0), H = xc.size(1), V = w.size(0);
@@ -444,7 +449,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     long long g_stride = 0, h_stride = 0;
     const float* gp = row_values(g, xc, T, "d_log_probs", &g_stride);
     const float* hp = has_h ? row_values(h, xc, T, "d_entropy", &h_stride) : nullptr;
-    int* st = status_of(saved[6], xc);
+    int* st = status_of(ctx->saved_data["status"].toTensor(), xc);
     const c10::cuda::CUDAGuard guard(xc.device());
     const cudaStream_t stream = stream_of(xc);
     Tensor dx, dw, dxc, partials;
@@ -455,7 +460,7 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
     }
     OptTensor target;
     if (need_dw) {
-      target = main_grad(w);
+      target = main_grad(ctx->saved_data["weight"].toTensor());
       // one chunk writes the weight's gradient in its own type; several add up in fp32
       if (target.has_value()) dw = *target;
       else if (chunk == T) dw = torch::empty({V, H}, w.options());
@@ -667,17 +672,18 @@ variable_list policy_loss(const Tensor& log_probs, const Tensor& old, const Tens
 struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
     Tensor out = embedding_lookup_(weight, ids, scale, status);
-    ctx->save_for_backward({weight, ids});
+    ctx->save_for_backward({ids});
+    ctx->saved_data["weight"] = weight;
     ctx->saved_data["scale"] = scale;
     ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor& weight = saved[0];
     if (!grads[0].defined()) return variable_list(4);
+    const Tensor weight = ctx->saved_data["weight"].toTensor();
     const OptTensor target = main_grad(weight);
-    Tensor dw = embedding_gradient_(grads[0].contiguous(), saved[1], weight.size(0), target, ctx->saved_data["scale"].toDouble());
+    Tensor dw = embedding_gradient_(grads[0].contiguous(), saved[0], weight.size(0), target, ctx->saved_data["scale"].toDouble());
     return {target.has_value() ? Tensor() : once(dw, "embedding_sorted"), Tensor(), Tensor(), Tensor()};
   }
 };

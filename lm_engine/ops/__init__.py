@@ -47,7 +47,8 @@ def status_word(device: torch.device | None = None) -> torch.Tensor:
     """Per-device int32 word that kernels raise when a bounded wait runs out (0 = healthy)."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     if index not in _STATUS:
-        _STATUS[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        with torch.inference_mode(False):  # it outlives the call, and is written to outside of inference mode as well
+            _STATUS[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
     return _STATUS[index]
 
 

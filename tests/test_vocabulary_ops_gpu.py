@@ -607,3 +607,53 @@ def test_on_a_stream_of_its_own_and_twice_at_once():
     for a, b in zip(want, got):
         for s, t in zip(a, b):
             assert torch.equal(s, t)
+
+
+def test_training_after_inference_mode_and_after_a_raised_status(monkeypatch):
+    """The status word is made by the first call, here one under inference mode, and is cleared between a forward pass and its backward pass."""
+    monkeypatch.setattr(ops, "_STATUS", {})
+    gen = torch.Generator("cuda").manual_seed(0)
+    x = torch.randn(5, 64, device="cuda", generator=gen, dtype=torch.bfloat16)
+    w = torch.randn(100, 64, device="cuda", generator=gen, dtype=torch.bfloat16)
+    labels = torch.tensor([1, 99, -100, 4, 0], device="cuda")
+    with torch.inference_mode():
+        scored = ops.fused_linear_token_log_probs(x, w, labels)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    lp = ops.fused_linear_token_log_probs(x, w, labels)
+    assert torch.equal(lp.detach(), scored)
+    rows = ops.embedding_sorted(w, labels)  # -100 is not in the table
+    with pytest.raises(RuntimeError, match="outside of its table"):
+        ops.check_status()
+    (lp.sum() + rows.sum()).backward()
+    again = torch.autograd.grad(ops.fused_linear_token_log_probs(x, w, labels).sum(), x)[0]
+    assert torch.equal(x.grad, again)
+
+
+def test_main_grad_of_a_recomputed_block_and_a_table_changed_in_place():
+    from torch.utils.checkpoint import checkpoint
+
+    gen = torch.Generator("cuda").manual_seed(0)
+    ids = torch.randint(0, 100, (7,), device="cuda", generator=gen)
+
+    def block(w):
+        return ops.fused_linear_token_log_probs(ops.embedding_sorted(w, ids), w, ids)
+
+    grads = []
+    for recompute in (False, True):
+        gen.manual_seed(1)
+        w = torch.randn(100, 64, device="cuda", generator=gen, dtype=torch.bfloat16).requires_grad_(True)
+        w.main_grad = torch.zeros(100, 64, device="cuda")
+        lp = checkpoint(block, w, use_reentrant=False) if recompute else block(w)
+        lp.sum().backward()
+        assert w.grad is None
+        grads.append(w.main_grad)
+    assert grads[0].abs().sum() > 0 and torch.equal(*grads)
+
+    # the gradient of a lookup does not depend on the table's values
+    table = torch.zeros(100, 64, device="cuda", requires_grad=True)
+    rows = ops.embedding_sorted(table, ids)
+    with torch.no_grad():
+        table.add_(1.0)
+    rows.sum().backward()
+    assert torch.equal(table.grad, torch.bincount(ids, minlength=100).float()[:, None].expand(100, 64))
