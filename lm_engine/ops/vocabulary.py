@@ -51,12 +51,12 @@ _KEEP_LOGITS_BYTES = 4 << 30
 
 # ----------------------------------------------------------------------------- token log-probabilities
 def _token_log_probs_torch(logits: torch.Tensor, labels: torch.Tensor, logit_scale: float, ignore_index: int, return_entropy: bool):
-    vocab = logits.shape[-1]
+    vocab, labels = logits.shape[-1], labels.long()  # an ignore_index beyond 32 bits would wrap around next to int32 labels
     kept = (labels != ignore_index) & (labels >= 0) & (labels < vocab)
     z = logits if logits.dtype == torch.float64 else logits.float()
     z = torch.where(kept[..., None], z, 0.0) * logit_scale  # whatever an ignored row holds, it has no part and no gradient
     logp = z.log_softmax(-1)
-    picked = logp.gather(-1, torch.where(kept, labels, 0).long()[..., None]).squeeze(-1)
+    picked = logp.gather(-1, torch.where(kept, labels, 0)[..., None]).squeeze(-1)
     picked = torch.where(kept, picked, 0.0)
     if not return_entropy:
         return picked
@@ -93,7 +93,7 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
     are kept in fp32 until the backward pass (``keep_logits``; by default where that takes at most 4 GiB) or formed a second time in it.
     The backward pass needs a transient bf16 buffer of at most about 2.2 GB. Rows whose label is ignored take no part in any product. bf16 operands with
     ``H`` a multiple of 8 run on the kernels. Gradients of ``weight`` go to its ``main_grad`` when the engine provides one."""
-    if x.is_cuda and x.dtype == torch.bfloat16 and x.shape[-1] % 8 == 0:
+    if x.is_cuda and x.dtype == torch.bfloat16 and x.dim() > 0 and weight.dim() == 2 and x.shape[-1] % 8 == 0:
         with site("loss.lm_head.log_probs"):
             out = native().linear_token_log_probs(x, weight, labels, logit_scale, ignore_index, return_entropy, _flce_chunk_rows(labels.numel(), weight.shape[0]),
                                                   _KEEP_LOGITS_BYTES if keep_logits is None else (1 << 62) * bool(keep_logits), status_word(x.device))

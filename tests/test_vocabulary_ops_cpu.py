@@ -283,3 +283,10 @@ def test_the_extension_refuses_the_same_calls(call):
     """Its checks come before anything that needs a device, so their errors (numbers in them included) are raised here as they are on a GPU."""
     with pytest.raises(ValueError):
         call(ops.native())
+
+
+def test_an_ignored_label_beyond_32_bits_is_no_int32_label():
+    z = torch.randn(4, 5, generator=torch.Generator().manual_seed(0))
+    labels = torch.tensor([0, 1, 2, 0])
+    got = ops.token_log_probs(z, labels.int(), ignore_index=-(1 << 40))
+    assert torch.equal(got, ops.token_log_probs(z, labels))

@@ -657,3 +657,12 @@ def test_main_grad_of_a_recomputed_block_and_a_table_changed_in_place():
         table.add_(1.0)
     rows.sum().backward()
     assert torch.equal(table.grad, torch.bincount(ids, minlength=100).float()[:, None].expand(100, 64))
+
+
+def test_operands_without_dimensions_are_refused():
+    one = torch.tensor(1.0, device="cuda", dtype=torch.bfloat16)
+    rows = torch.zeros(3, 8, device="cuda", dtype=torch.bfloat16)
+    label = torch.tensor(1, device="cuda")
+    for x, w, labels in ((one, rows, label), (rows, one, label.expand(3))):
+        with pytest.raises(ValueError):
+            ops.fused_linear_token_log_probs(x, w, labels)
