@@ -24,8 +24,8 @@ _LOGIT_TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 # CUDA tensors of the kernels' types go straight to the extension, which makes the same checks (as ValueErrors) as the Python
-# code makes for the other path: one call of the smallest cases costs a few microseconds there, tens of them here. `native()` raises where
-# the extension cannot be loaded.
+# code makes for the other path: one call of the smallest cases costs a few microseconds there, tens of them here. `native()`
+# raises where the extension cannot be loaded.
 
 
 def _check_labels(labels: torch.Tensor, rows: torch.Size, device: torch.device, name: str = "labels") -> None:
@@ -44,8 +44,8 @@ def _check_logit_scale(logit_scale: float) -> float:
     return logit_scale
 
 
-# Fused linear form: fp32 logits up to this size are kept between the passes instead of being formed twice. 4096 x 4096 x 128256 (2.1 GB) both
-# directions: 10.2 ms kept, 12.5 ms formed twice.
+# Fused linear form: fp32 logits up to this size are kept between the passes instead of being formed twice.
+# 4096 x 4096 x 128256 (2.1 GB) both directions: 10.2 ms kept, 12.5 ms formed twice.
 _KEEP_LOGITS_BYTES = 4 << 30
 
 
@@ -89,20 +89,23 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
                                  ignore_index: int = -100, return_entropy: bool = False, keep_logits: bool | None = None):
     """:func:`token_log_probs` of ``logits = x @ weight.T`` without the logits: ``x [..., H]``, ``weight [V, H]``, ``labels [...]``.
 
-    The logits are formed in fp32 on the tensor cores and reduced where they are. Without gradients they never reach memory; with gradients they
-    are kept in fp32 until the backward pass (``keep_logits``; by default where that takes at most 4 GiB) or formed a second time in it.
-    The backward pass needs a transient bf16 buffer of at most about 2.2 GB. Rows whose label is ignored take no part in any product. bf16 operands with
-    ``H`` a multiple of 8 run on the kernels. Gradients of ``weight`` go to its ``main_grad`` when the engine provides one."""
+    The logits are formed in fp32 on the tensor cores and reduced where they are. Without gradients they never reach memory;
+    with gradients they are kept in fp32 until the backward pass (``keep_logits``; by default where that takes at most 4 GiB) or
+    formed a second time in it. The backward pass needs a transient bf16 buffer of at most about 2.2 GB. Rows whose label is
+    ignored take no part in any product. bf16 operands with ``H`` a multiple of 8 run on the kernels. Gradients of ``weight`` go
+    to its ``main_grad`` when the engine provides one."""
     if x.is_cuda and x.dtype == torch.bfloat16 and x.dim() > 0 and weight.dim() == 2 and x.shape[-1] % 8 == 0:
         with site("loss.lm_head.log_probs"):
-            out = native().linear_token_log_probs(x, weight, labels, logit_scale, ignore_index, return_entropy, _flce_chunk_rows(labels.numel(), weight.shape[0]),
-                                                  _KEEP_LOGITS_BYTES if keep_logits is None else (1 << 62) * bool(keep_logits), status_word(x.device))
+            out = native().linear_token_log_probs(
+                x, weight, labels, logit_scale, ignore_index, return_entropy, _flce_chunk_rows(labels.numel(), weight.shape[0]),
+                _KEEP_LOGITS_BYTES if keep_logits is None else (1 << 62) * bool(keep_logits), status_word(x.device))
         return tuple(out) if return_entropy else out[0]
     logit_scale = _check_logit_scale(logit_scale)
     if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"hidden states [..., H] and a weight [V, H] are needed, got {tuple(x.shape)} and {tuple(weight.shape)}")
     if x.device != weight.device or x.dtype != weight.dtype or not x.is_floating_point():
-        raise ValueError(f"hidden states and weight must be floating point of one type on one device, got {x.dtype} on {x.device} and {weight.dtype} on {weight.device}")
+        raise ValueError(f"hidden states and weight must be floating point of one type on one device, got {x.dtype} on {x.device} "
+                         f"and {weight.dtype} on {weight.device}")
     _check_labels(labels, x.shape[:-1], x.device)
     note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
     return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
@@ -128,7 +131,8 @@ _POLICY_REDUCTIONS = {"sum": 0, "token_mean": 1, "sequence_mean": 2}
 
 def _check_like(t: torch.Tensor, like: torch.Tensor, name: str) -> torch.Tensor:
     if t.shape != like.shape or t.device != like.device or not t.is_floating_point():
-        raise ValueError(f"{name} must be floating point, shaped {tuple(like.shape)} on {like.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        raise ValueError(f"{name} must be floating point, shaped {tuple(like.shape)} on {like.device}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
     if t.requires_grad:
         raise ValueError(f"{name} must not require a gradient (detach it): the loss is differentiated with respect to log_probs alone")
     return t
@@ -139,15 +143,18 @@ def _check_sequences(log_probs: torch.Tensor, cu_seqlens: torch.Tensor | None, m
     if not log_probs.is_floating_point():
         raise ValueError(f"log_probs must be floating point, got {log_probs.dtype}")
     if mask is not None and (mask.shape != log_probs.shape or mask.device != log_probs.device or mask.is_floating_point()):
-        raise ValueError(f"mask must be boolean or integer, shaped {tuple(log_probs.shape)} on {log_probs.device}, got {mask.dtype} {tuple(mask.shape)} on {mask.device}")
+        raise ValueError(f"mask must be boolean or integer, shaped {tuple(log_probs.shape)} on {log_probs.device}, got {mask.dtype} "
+                         f"{tuple(mask.shape)} on {mask.device}")
     if cu_seqlens is None:
         if log_probs.dim() != 2:
             raise ValueError(f"log_probs must be [sequences, length], or [tokens] with cu_seqlens, got {tuple(log_probs.shape)}")
         return log_probs.shape[0], log_probs.shape[1]
     if log_probs.dim() != 1:
         raise ValueError(f"with cu_seqlens log_probs must be [tokens], got {tuple(log_probs.shape)}")
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.dtype not in (torch.int32, torch.int64) or cu_seqlens.device != log_probs.device:
-        raise ValueError(f"cu_seqlens must be int32 or int64 [sequences + 1] on {log_probs.device}, got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)} on {cu_seqlens.device}")
+    integers = cu_seqlens.dtype in (torch.int32, torch.int64)
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or not integers or cu_seqlens.device != log_probs.device:
+        raise ValueError(f"cu_seqlens must be int32 or int64 [sequences + 1] on {log_probs.device}, got {cu_seqlens.dtype} "
+                         f"{tuple(cu_seqlens.shape)} on {cu_seqlens.device}")
     return cu_seqlens.numel() - 1, 0
 
 
@@ -188,9 +195,10 @@ def preference_loss(log_probs: torch.Tensor, reference_log_probs: torch.Tensor |
     """Loss over pairs of answers from per-token log-probabilities of the policy and of a frozen reference.
 
     ``log_probs`` is packed ``[tokens]`` with ``cu_seqlens [2 * pairs + 1]`` or padded ``[2 * pairs, length]``: the chosen answers first,
-    then the rejected ones in the same order. With ``s`` an answer's sum (``average_log_probs``: mean) of ``log_probs - reference`` over the tokens
-    that ``mask`` keeps and ``D = s_chosen - s_rejected``: ``sigmoid`` is ``(1 - e) softplus(-beta D) + e softplus(beta D)`` with
-    ``e = label_smoothing``, ``hinge`` is ``max(0, 1 - beta D)``, ``ipo`` is ``(D - 1 / (2 beta))^2``. ``reference_log_probs=None`` leaves the reference out.
+    then the rejected ones in the same order. With ``s`` an answer's sum (``average_log_probs``: mean) of ``log_probs - reference``
+    over the tokens that ``mask`` keeps and ``D = s_chosen - s_rejected``: ``sigmoid`` is ``(1 - e) softplus(-beta D) + e softplus(beta D)``
+    with ``e = label_smoothing``, ``hinge`` is ``max(0, 1 - beta D)``, ``ipo`` is ``(D - 1 / (2 beta))^2``.
+    ``reference_log_probs=None`` leaves the reference out.
 
     Returns the loss (reduced over pairs, or one per pair with ``reduction="none"``) and ``beta * s`` of the chosen and the rejected answers
     (no gradient). An answer without tokens has ``s = 0``. Masked tokens, and tokens outside of all sequences, are not looked at and get a
@@ -199,8 +207,9 @@ def preference_loss(log_probs: torch.Tensor, reference_log_probs: torch.Tensor |
         raise ValueError(f"unexpected loss_type ({loss_type}) or reduction ({reduction})")
     if log_probs.is_cuda and log_probs.dtype in _LOGIT_TYPES:
         with site("preference_loss"):
-            return PreferenceLossOutput(*native().preference_loss(log_probs, reference_log_probs, cu_seqlens, mask, _PREFERENCE_KINDS[loss_type], beta, label_smoothing,
-                                                                  average_log_probs, _PREFERENCE_REDUCTIONS[reduction]))
+            return PreferenceLossOutput(*native().preference_loss(
+                log_probs, reference_log_probs, cu_seqlens, mask, _PREFERENCE_KINDS[loss_type], beta, label_smoothing, average_log_probs,
+                _PREFERENCE_REDUCTIONS[reduction]))
     sequences, length = _check_sequences(log_probs, cu_seqlens, mask)
     if sequences == 0 or sequences % 2:
         raise ValueError(f"an even number of answers is needed (chosen, then rejected), got {sequences}")
@@ -213,12 +222,14 @@ def preference_loss(log_probs: torch.Tensor, reference_log_probs: torch.Tensor |
         _check_like(reference_log_probs, log_probs, "reference_log_probs")
     args = (_PREFERENCE_KINDS[loss_type], beta, label_smoothing, bool(average_log_probs), _PREFERENCE_REDUCTIONS[reduction])
     wide = log_probs if log_probs.dtype == torch.float64 else log_probs.float()
-    loss, rewards = _preference_loss_torch(wide, None if reference_log_probs is None else reference_log_probs.to(wide.dtype), cu_seqlens, length, sequences, mask, *args)
+    reference = None if reference_log_probs is None else reference_log_probs.to(wide.dtype)
+    loss, rewards = _preference_loss_torch(wide, reference, cu_seqlens, length, sequences, mask, *args)
     pairs = sequences // 2
     return PreferenceLossOutput(loss, rewards[:pairs], rewards[pairs:])
 
 
-def _policy_loss_torch(log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high, dual_clip, kl_coef, reduction):
+def _policy_loss_torch(log_probs, old, reference, advantages, per_token, cu_seqlens, length, sequences, mask, clip_low, clip_high,
+                       dual_clip, kl_coef, reduction):
     lp = log_probs.reshape(-1)
     ids = _sequence_ids(sequences, length, cu_seqlens, lp)
     kept = ids < sequences if mask is None else (ids < sequences) & (mask.reshape(-1) != 0)
@@ -227,7 +238,8 @@ def _policy_loss_torch(log_probs, old, reference, advantages, per_token, cu_seql
     adv = advantages.reshape(-1) if per_token else torch.cat([advantages, advantages.new_zeros(1)])[ids]
     adv = torch.where(kept, adv, 0.0)
     delta = own.double() - old.double()
-    clipped = ((adv > 0) & (delta > math.log1p(clip_high))) | ((adv < 0) & (delta < (math.log1p(-clip_low) if clip_low < 1 else -math.inf)))
+    log_low, log_high = math.log1p(-clip_low) if clip_low < 1 else -math.inf, math.log1p(clip_high)
+    clipped = ((adv > 0) & (delta > log_high)) | ((adv < 0) & (delta < log_low))
     ratio = torch.where(clipped | (adv == 0), 0.0, delta).exp().to(own.dtype)
     value = torch.where(clipped, -adv * torch.where(adv > 0, torch.full_like(adv, 1 + clip_high), 1 - clip_low), -adv * ratio)
     if dual_clip:
@@ -250,27 +262,31 @@ def _policy_loss_torch(log_probs, old, reference, advantages, per_token, cu_seql
     return loss, (kl.sum() / n).detach(), clipped.sum().to(value.dtype) / n
 
 
-def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor, *, reference_log_probs: torch.Tensor | None = None,
-                cu_seqlens: torch.Tensor | None = None, mask: torch.Tensor | None = None, clip_low: float = 0.2, clip_high: float = 0.2,
-                dual_clip: float | None = None, kl_coef: float = 0.0, reduction: str = "token_mean") -> PolicyLossOutput:
+def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages: torch.Tensor, *,
+                reference_log_probs: torch.Tensor | None = None, cu_seqlens: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                clip_low: float = 0.2, clip_high: float = 0.2, dual_clip: float | None = None, kl_coef: float = 0.0,
+                reduction: str = "token_mean") -> PolicyLossOutput:
     """Clipped policy-gradient loss with a KL term, from per-token log-probabilities of sampled answers.
 
     ``log_probs`` is packed ``[tokens]`` with ``cu_seqlens [sequences + 1]`` or padded ``[sequences, length]``; ``advantages`` is
-    ``[sequences]``, one value per answer, or else has the shape of ``log_probs``. A token's loss is ``max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high))`` with
-    ``r = exp(log_probs - old_log_probs)``, bounded by ``-dual_clip A`` where ``A < 0``, plus ``kl_coef (exp(k) - 1 - k)`` with ``k = reference - log_probs``.
-    ``token_mean`` divides the sum by the number of tokens that ``mask`` keeps, ``sequence_mean`` averages the answers' token means over the answers
-    that keep a token, ``sum`` does neither.
+    ``[sequences]``, one value per answer, or else has the shape of ``log_probs``. A token's loss is
+    ``max(-A r, -A clip(r, 1 - clip_low, 1 + clip_high))`` with ``r = exp(log_probs - old_log_probs)``, bounded by ``-dual_clip A``
+    where ``A < 0``, plus ``kl_coef (exp(k) - 1 - k)`` with ``k = reference - log_probs``. ``token_mean`` divides the sum by the
+    number of tokens that ``mask`` keeps, ``sequence_mean`` averages the answers' token means over the answers that keep a token,
+    ``sum`` does neither.
 
-    Returns the loss, and over the kept tokens the mean of ``exp(k) - 1 - k`` (0 without a reference) and the share whose gradient was clipped (neither has
-    a gradient). Masked tokens, and tokens outside of all sequences, are not looked at and get a gradient of 0; nothing kept gives 0."""
+    Returns the loss, and over the kept tokens the mean of ``exp(k) - 1 - k`` (0 without a reference) and the share whose gradient
+    was clipped (neither has a gradient). Masked tokens, and tokens outside of all sequences, are not looked at and get a gradient
+    of 0; nothing kept gives 0."""
     if reduction not in _POLICY_REDUCTIONS:
         raise ValueError(f"unexpected reduction ({reduction})")
     if dual_clip is not None and not (math.isfinite(dual_clip) and dual_clip > 1):
         raise ValueError(f"dual_clip must be finite and above 1, got {dual_clip}")
     if log_probs.is_cuda and log_probs.dtype in _LOGIT_TYPES:
         with site("policy_loss"):
-            return PolicyLossOutput(*native().policy_loss(log_probs, old_log_probs, advantages, reference_log_probs, cu_seqlens, mask, clip_low, clip_high, dual_clip or 0.0,
-                                                          kl_coef, _POLICY_REDUCTIONS[reduction]))
+            return PolicyLossOutput(*native().policy_loss(
+                log_probs, old_log_probs, advantages, reference_log_probs, cu_seqlens, mask, clip_low, clip_high, dual_clip or 0.0, kl_coef,
+                _POLICY_REDUCTIONS[reduction]))
     sequences, length = _check_sequences(log_probs, cu_seqlens, mask)
     _check_like(old_log_probs, log_probs, "old_log_probs")
     if reference_log_probs is not None:
@@ -292,10 +308,12 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
 
 # ----------------------------------------------------------------------------- embedding
 def embedding_sorted(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-    """``scale * weight[ids]`` whose weight gradient adds the rows of a token in ascending position: the same bits on every run, one rounding, no fp32
-    copy of the whole table (``ops.embedding(sorted_gradient=True)``). bf16, fp16 and fp32 tables of any width run on the kernels.
+    """``scale * weight[ids]`` whose weight gradient adds the rows of a token in an order fixed by their positions: the same bits on
+    every run, one rounding, no fp32 copy of the whole table (``ops.embedding(sorted_gradient=True)``). bf16, fp16 and fp32 tables
+    of any width run on the kernels.
 
-    On the GPU an id outside of the table gives a row of zeros, takes no part in the gradient and raises the status word (``ops.check_status()``)."""
+    On the GPU an id outside of the table gives a row of zeros, takes no part in the gradient and raises the status word
+    (``ops.check_status()``)."""
     if weight.is_cuda and weight.dtype in _LOGIT_TYPES:
         with site("embedding"):
             return native().embedding_sorted(weight, ids, scale, status_word(weight.device))
