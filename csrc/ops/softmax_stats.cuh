@@ -115,7 +115,11 @@ __device__ __forceinline__ void accumulate(Stats& a, const F2 (&f)[N / 2], float
   }
 }
 
-// Log-probability in base 2 of logit x under a row's (m, log2 s).
+// Log-probability (natural) of logit x under a row's (m, log2 s). Not formed in base 2: next to a mask of the type's lowest value the factor
+// log2 e would overflow before ln 2 takes it back.
+__device__ __forceinline__ float log_prob(float x, float2 lse, float logit_scale) { return fmaf(x - lse.x, logit_scale, -lse.y * kLn2); }
+
+// The same in base 2, as the exponent of a probability (where -inf is as good as any number below -150).
 __device__ __forceinline__ float log2_prob(float x, float2 lse, float c) { return fmaf(x - lse.x, c, -lse.y); }
 
 // d(score) / d(z_j) times logit_scale, from the log-probability d in base 2: gs, hs = upstream gradients times logit_scale, H = entropy. The

@@ -204,7 +204,7 @@ template <typename T, bool ENTROPY, int CLUSTER>
 __global__ void __launch_bounds__(FWD_THREADS, FWD_BLOCKS)
     token_log_probs_fwd_kernel(const T* __restrict__ logits, const void* __restrict__ labels, bool labels64,
                                float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, int V,
-                               RowMap map, float scale2, long long ignore_index) {
+                               RowMap map, float logit_scale, float scale2, long long ignore_index) {
   __shared__ Stats red[FWD_THREADS / 32];
   __shared__ Stats block_stats;
   const long long row = blockIdx.x / CLUSTER;
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(FWD_THREADS, FWD_BLOCKS)
   if (threadIdx.x == 0 && rank == 0) {
     const float log2_s = log2f(st.s);
     lse[row] = make_float2(st.m, log2_s);
-    log_probs[row] = log2_prob(Vec<T>::load(r.p + label), make_float2(st.m, log2_s), scale2) * kLn2;
+    log_probs[row] = log_prob(Vec<T>::load(r.p + label), make_float2(st.m, log2_s), logit_scale);
     if (ENTROPY) entropy[row] = (log2_s - st.u / st.s) * kLn2;
   }
 }
@@ -367,7 +367,7 @@ template <bool ENTROPY>
 __global__ void __launch_bounds__(1024)
     token_log_probs_join_kernel(const float4* __restrict__ stats, int slices, int slice_width, const void* __restrict__ labels,
         bool labels64, float* __restrict__ log_probs, float* __restrict__ entropy, float2* __restrict__ lse, LiveRows live, int V,
-        float scale2, long long ignore_index) {
+        float logit_scale, float scale2, long long ignore_index) {
   __shared__ Stats red[32][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int rows = live.count == nullptr ? live.rows : min(live.rows, *live.count - live.base);
@@ -408,13 +408,13 @@ __global__ void __launch_bounds__(1024)
   }
   const float log2_s = log2f(st.s), x = stats[(long long)(label / slice_width) * live.rows + r].w;
   lse[row] = make_float2(st.m, log2_s);
-  log_probs[row] = log2_prob(x, make_float2(st.m, log2_s), scale2) * kLn2;
+  log_probs[row] = log_prob(x, make_float2(st.m, log2_s), logit_scale);
   if (ENTROPY) entropy[row] = (log2_s - st.u / st.s) * kLn2;
 }
 
 template <typename T>
 void fwd(const void* logits, const void* labels, bool labels64, float* log_probs, float* entropy, float2* lse, long long rows,
-         int V, RowMap map, float scale2, long long ignore_index, cudaStream_t stream) {
+         int V, RowMap map, float logit_scale, long long ignore_index, cudaStream_t stream) {
   const T* x = reinterpret_cast<const T*>(logits);
   auto launch = [&](auto kernel, int cluster) {
     cudaLaunchConfig_t cfg = {};
@@ -428,8 +428,8 @@ void fwd(const void* logits, const void* labels, bool labels64, float* log_probs
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = cluster > 1 ? 1 : 0;
-    check_cuda(cudaLaunchKernelEx(&cfg, kernel, x, labels, labels64, log_probs, entropy, lse, V, map, scale2, ignore_index),
-        "token_log_probs forward launch");
+    check_cuda(cudaLaunchKernelEx(&cfg, kernel, x, labels, labels64, log_probs, entropy, lse, V, map, logit_scale,
+        logit_scale * kLog2e, ignore_index), "token_log_probs forward launch");
   };
   // Blocks per row: more than one only while all of them run at once, four per SM, and each has a vector per thread. Few long rows
   // gain (32 x 49152 bf16: 7.8 us with one block of 1024 threads, 6.6 with eight of 256); with more blocks than run at a time the
@@ -471,7 +471,7 @@ void token_log_probs_fwd(const void* logits, Scalar type, const void* labels, bo
                          float2* lse, long long T, int V, RowMap map, float logit_scale, long long ignore_index, cudaStream_t stream) {
   if (T == 0) return;
   auto launch = type == Scalar::kBf16 ? fwd<__nv_bfloat16> : type == Scalar::kF16 ? fwd<__half> : fwd<float>;
-  launch(logits, labels, labels64, log_probs, entropy, lse, T, V, map, logit_scale * kLog2e, ignore_index, stream);
+  launch(logits, labels, labels64, log_probs, entropy, lse, T, V, map, logit_scale, ignore_index, stream);
   count_launch();
   check_cuda(cudaGetLastError(), "token_log_probs forward launch");
 }
@@ -495,10 +495,10 @@ void token_log_probs_join(const float* stats, int slices, int slice_width, const
   const float4* st = reinterpret_cast<const float4*>(stats);
   if (entropy != nullptr)
     token_log_probs_join_kernel<true><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse,
-        live, V, logit_scale * kLog2e, ignore_index);
+        live, V, logit_scale, logit_scale * kLog2e, ignore_index);
   else
     token_log_probs_join_kernel<false><<<blocks, 1024, 0, stream>>>(st, slices, slice_width, labels, labels64, log_probs, entropy, lse,
-        live, V, logit_scale * kLog2e, ignore_index);
+        live, V, logit_scale, logit_scale * kLog2e, ignore_index);
   count_launch();
   check_cuda(cudaGetLastError(), "token_log_probs join launch");
 }
