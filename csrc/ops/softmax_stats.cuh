@@ -75,16 +75,13 @@ __device__ __forceinline__ F2 mul2(F2 a, F2 b) {
   return r;
 }
 
-// Up to here the product m c can stand in for m: d = x c - m c is one FMA. Beyond (masks of the type's lowest value as the largest
-// logit, infinities) the difference is formed first. In the FMA form the rounding of m c is common to all elements of a row and cancels
-// between a logit and the sum.
-constexpr float kProductLimit = 1e30f;
-
-// N logits (an even number, in pairs) whose maximum is `top` enter the statistics.
+// N logits (an even number, in pairs) whose maximum is `top` enter the statistics. The difference x - m is formed before it is scaled:
+// d = x c - m c in one FMA would carry the rounding of m c into the sums, which grows with the row's distance from zero (5e-3 in a
+// log-probability at logits around 1e5) and differs between the parts of a row, whose maxima differ, so that nothing takes it back.
 template <bool ENTROPY, int N>
 __device__ __forceinline__ void accumulate(Stats& a, const F2 (&f)[N / 2], float top, float c) {
   if (top > a.m) rescale<ENTROPY>(a, top, c);
-  const float m = a.m == -INFINITY ? 0.f : a.m, mc = m * c;
+  const float m = a.m == -INFINITY ? 0.f : a.m;
   F2 s0 = pack2(0.f, 0.f), s1 = s0, u0 = s0, u1 = s0;
   const F2 c2 = pack2(c, c);
   auto add = [&](F2 d2, int i) {
@@ -98,15 +95,9 @@ __device__ __forceinline__ void accumulate(Stats& a, const F2 (&f)[N / 2], float
       else u0 = fma2(x, e, u0);
     }
   };
-  if (fabsf(mc) < kProductLimit) {
-    const F2 off = pack2(-mc, -mc);
+  const F2 off = pack2(-m, -m);
 #pragma unroll
-    for (int i = 0; i < N / 2; ++i) add(fma2(f[i], c2, off), i);
-  } else {
-    const F2 off = pack2(-m, -m);
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) add(mul2(add2(f[i], off), c2), i);
-  }
+  for (int i = 0; i < N / 2; ++i) add(mul2(add2(f[i], off), c2), i);
   const float2 s = unpack2(add2(s0, s1));
   a.s += s.x + s.y;
   if (ENTROPY) {

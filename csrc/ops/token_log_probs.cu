@@ -316,10 +316,7 @@ __global__ void __launch_bounds__(BWD_THREADS)
       if (i < r.vectors) v[k] = r.load(i);
     }
   }
-  const float mc = L.x * scale2;
-  const bool product = fabsf(mc) < kProductLimit;
-  const float off = product ? -mc - L.y : -L.x;
-  const F2 c2 = pack2(scale2, scale2), off2 = pack2(off, off), log2_s = pack2(-L.y, -L.y), gs2 = pack2(-gs, -gs);
+  const F2 c2 = pack2(scale2, scale2), off2 = pack2(-L.x, -L.x), log2_s = pack2(-L.y, -L.y), gs2 = pack2(-gs, -gs);
   const int label_vector = zero ? -1 : (int)(label / N);
 #pragma unroll
   for (int k = 0; k < BWD_UNROLL; ++k) {
@@ -333,7 +330,7 @@ __global__ void __launch_bounds__(BWD_THREADS)
         f[j] = pack2(0.f, 0.f);
         continue;
       }
-      const float2 d = unpack2(product ? fma2(f[j], c2, off2) : fma2(add2(f[j], off2), c2, log2_s));
+      const float2 d = unpack2(fma2(add2(f[j], off2), c2, log2_s));
       const F2 p = pack2(fast_exp2(d.x), fast_exp2(d.y));
       if (ENTROPY) {
         const F2 w = pack2(-fmaf(hs, fmaf(fmaxf(d.x, kFloor2), kLn2, H), gs), -fmaf(hs, fmaf(fmaxf(d.y, kFloor2), kLn2, H), gs));
@@ -354,8 +351,7 @@ __global__ void __launch_bounds__(BWD_THREADS)
     }
     // the label's own gradient, over the vector just written by this thread
     if (i == label_vector) {
-      const float x = Vec<T>::load(r.p + label);
-      const float d = product ? fmaf(x, scale2, off) : log2_prob(x, L, scale2);
+      const float d = log2_prob(Vec<T>::load(r.p + label), L, scale2);
       Vec<T>::store(out + label, gs + score_gradient<ENTROPY>(d, gs, hs, H));
     }
   }
@@ -562,10 +558,7 @@ __global__ void __launch_bounds__(GRAD_THREADS)
       v[k][1] = make_uint4(w[4], w[5], w[6], w[7]);
     }
   }
-  const float mc = L.x * scale2;
-  const bool product = fabsf(mc) < kProductLimit;
-  const float off = product ? -mc - L.y : -L.x;
-  const F2 c2 = pack2(scale2, scale2), off2 = pack2(off, off), log2_s = pack2(-L.y, -L.y), gs2 = pack2(-gs, -gs);
+  const F2 c2 = pack2(scale2, scale2), off2 = pack2(-L.x, -L.x), log2_s = pack2(-L.y, -L.y), gs2 = pack2(-gs, -gs);
 #pragma unroll
   for (int k = 0; k < GRAD_UNROLL; ++k) {
     const int i = i0 + k * GRAD_THREADS;
@@ -576,7 +569,7 @@ __global__ void __launch_bounds__(GRAD_THREADS)
     uint32_t w[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float2 d = unpack2(product ? fma2(f[j], c2, off2) : fma2(add2(f[j], off2), c2, log2_s));
+      const float2 d = unpack2(fma2(add2(f[j], off2), c2, log2_s));
       const F2 p = pack2(fast_exp2(d.x), fast_exp2(d.y));
       float2 y;
       if (ENTROPY) y = unpack2(mul2(p, pack2(-fmaf(hs, fmaf(fmaxf(d.x, kFloor2), kLn2, H), gs),

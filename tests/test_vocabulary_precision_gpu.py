@@ -55,3 +55,81 @@ def test_a_label_of_the_lowest_value_from_hidden_states(keep):
     if keep is not None:
         (dx,) = torch.autograd.grad(lp.sum(), x)
         assert torch.isfinite(dx[:, 1:]).all()
+
+# ----------------------------------------------------------------------------- rows far from zero, tokens all but certain
+def _grid(tokens, vocab, seed):
+    """Scores on a grid of 1/16 below 4 in size: exact in every type, and next to a shift too where it is a multiple of 32 below 2^17 (fp32)."""
+    gen = torch.Generator("cuda").manual_seed(seed)
+    base = torch.randint(-63, 64, (tokens, vocab), generator=gen, device="cuda") / 16
+    labels = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    g, h = torch.randn(tokens, generator=gen, device="cuda"), torch.randn(tokens, generator=gen, device="cuda")
+    return base, labels, g, h
+
+
+@pytest.mark.parametrize("dtype,shift", [(torch.float32, 96.0), (torch.float32, 1024.0), (torch.float32, -10240.0), (torch.float16, 64.0)])
+@pytest.mark.parametrize("tokens,vocab", [(5, 1003), (40, 50000)])
+@pytest.mark.parametrize("scale", [1.0, 0.7])
+def test_log_probs_do_not_depend_on_where_a_row_lies(dtype, shift, tokens, vocab, scale):
+    """A softmax depends on differences alone. Those are exact here, so every later value has to be the same, bit for bit."""
+    base, labels, g, h = _grid(tokens, vocab, vocab)
+    results = []
+    for z in (base, base + shift):
+        z = z.to(dtype).requires_grad_(True)
+        outs = ops.token_log_probs(z, labels, logit_scale=scale, return_entropy=True)
+        results.append((*outs, *torch.autograd.grad(outs, z, (g, h)), *torch.autograd.grad(ops.token_log_probs(z, labels, logit_scale=scale), z, g)))
+    for a, b in zip(*results):
+        assert torch.equal(a, b), (a.double() - b.double()).abs().max().item()
+
+
+@pytest.mark.parametrize("shift", [96.0, 1024.0, -10240.0])
+@pytest.mark.parametrize("keep", [True, False])
+def test_fused_linear_log_probs_do_not_depend_on_where_a_row_lies(shift, keep):
+    """Logits on the grid: row t of x takes column 1 + t of the weight, and column 0 adds the shift to all of them. All products and their sums are exact."""
+    tokens, hidden, vocab = 63, 64, 5003
+    base, labels, g, h = _grid(tokens, vocab, 3)
+    x = torch.zeros(tokens, hidden, device="cuda", dtype=torch.bfloat16)
+    x[:, 0] = 1.0
+    x[torch.arange(tokens), 1 + torch.arange(tokens)] = 1.0
+    results = []
+    for s in (0.0, shift):
+        w = torch.zeros(vocab, hidden, device="cuda", dtype=torch.bfloat16)
+        w[:, 0], w[:, 1:] = s, base.t()
+        x.requires_grad_(True), w.requires_grad_(True)
+        outs = ops.fused_linear_token_log_probs(x, w, labels, return_entropy=True, keep_logits=keep)
+        dx, dw = torch.autograd.grad(outs, (x, w), (g, h))
+        results.append((*outs, dx[:, 1:], dw))
+    for a, b in zip(*results):
+        assert torch.equal(a, b), (a.double() - b.double()).abs().max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("top", [20.0, 40.0, 100.0])
+def test_no_log_probability_is_above_zero(dtype, top):
+    gen = torch.Generator("cuda").manual_seed(int(top))
+    tokens, vocab = 600, 4001
+    logits = (2.5 * torch.randn(tokens, vocab, generator=gen, device="cuda")).to(dtype)
+    labels = torch.randint(0, vocab, (tokens,), generator=gen, device="cuda")
+    logits[torch.arange(tokens), labels] += top
+    lp, entropy = ops.token_log_probs(logits, labels, return_entropy=True)
+    want = logits.double().log_softmax(-1).gather(1, labels[:, None])[:, 0]
+    assert (lp <= 0).all() and (entropy >= 0).all()
+    # the sum is 1 + r with r < 1 in all but a few rows: its additions and the logarithm round by half a step of it (2^-24) in each of the
+    # (at most 4001 / 256 / 4 + 24 additions and 24 merges) steps that still move it; terms of r are good to 2^-20
+    assert ((lp.double() - want).abs() <= 52 * 2.0**-24 + 2.0**-20 * want.abs()).all()
+    if top >= 40:
+        assert lp.abs().max() <= 2.0**-23  # what is left of the sum next to 1
+
+
+@pytest.mark.parametrize("top", [24.0, 40.0, 96.0])
+def test_no_log_probability_from_hidden_states_is_above_zero(top):
+    tokens, hidden, vocab = 63, 64, 4001
+    base, labels, _, _ = _grid(tokens, vocab, 5)
+    x = torch.zeros(tokens, hidden, device="cuda", dtype=torch.bfloat16)
+    x[torch.arange(tokens), 1 + torch.arange(tokens)] = 1.0
+    base[torch.arange(tokens), labels] = top
+    w = torch.zeros(vocab, hidden, device="cuda", dtype=torch.bfloat16)
+    w[:, 1:] = base.t()
+    lp, entropy = ops.fused_linear_token_log_probs(x, w, labels, return_entropy=True)
+    want = base.double().log_softmax(-1).gather(1, labels[:, None])[:, 0]
+    assert (lp <= 0).all() and (entropy >= 0).all()
+    assert ((lp.double() - want).abs() <= 52 * 2.0**-24 + 2.0**-20 * want.abs()).all()
