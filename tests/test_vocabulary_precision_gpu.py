@@ -133,3 +133,27 @@ def test_no_log_probability_from_hidden_states_is_above_zero(top):
     want = base.double().log_softmax(-1).gather(1, labels[:, None])[:, 0]
     assert (lp <= 0).all() and (entropy >= 0).all()
     assert ((lp.double() - want).abs() <= 52 * 2.0**-24 + 2.0**-20 * want.abs()).all()
+
+# ----------------------------------------------------------------------------- long sums of the embedding's gradient
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("tokens,hidden", [(100, 64), (1000, 64), (200001, 16), (30000, 3)])
+@pytest.mark.parametrize("into_buffer", [False, True])
+def test_the_gradient_of_a_frequent_token_is_a_sum_of_few_roundings(dtype, tokens, hidden, into_buffer):
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    w = torch.zeros(7, hidden, device="cuda", dtype=dtype, requires_grad=True)
+    ids = torch.full((tokens,), 3, device="cuda")
+    ids[::97] = 5
+    dout = (1 + torch.rand(tokens, hidden, generator=gen, device="cuda")).to(dtype) / 64
+    exact = torch.zeros(7, hidden, device="cuda", dtype=torch.float64).index_add_(0, ids, dout.double())
+    if into_buffer:
+        w.main_grad = torch.zeros(7, hidden, device="cuda")
+    out = ops.embedding(w, ids, sorted_gradient=True)
+    if into_buffer:
+        out.backward(dout)
+        grad = w.main_grad
+    else:
+        (grad,) = torch.autograd.grad(out, w, dout)
+    # fp32 rows: a chunk's sum is rounded once, their total once, all values have one sign. 16-bit rows hold at most 11 bits, and sums of
+    # up to 128 of them in one binade below 2^18 steps are exact.
+    half = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-24 if into_buffer else 2.0**-8, torch.float16: 2.0**-24 if into_buffer else 2.0**-11}[dtype]
+    assert ((grad.double() - exact).abs() <= (half + 2.0**-24) * (1 + 2.0**-20) * exact).all()
