@@ -1,8 +1,9 @@
 // Embedding lookup, out[t] = scale * W[id_t], and its gradient summed in sorted token order:
-//   dW[v] = scale * sum over t with id_t = v, in ascending t, of dout[t]
+//   dW[v] = scale * sum over t with id_t = v of dout[t]
 //
-// The gradient sorts the pairs (id, t) as 64-bit keys, which are distinct, so the order is unique and every sum is taken in
-// the same order on every run; nothing is added atomically. Sorting: runs of 1024 keys in shared memory (bitonic), then
+// The gradient sorts the pairs (id, t) as 64-bit keys, which are distinct, so their order is unique and every sum is taken in
+// the same order on every run, one fixed by the ids and the sizes: ascending t inside of a chunk, and the chunks' parts by every fourth on four
+// lanes, lane after lane; nothing is added atomically. Sorting: runs of 1024 keys in shared memory (bitonic), then
 // levels that merge 16 runs at a time by rank: a key's place is its place in its own run plus the number of smaller keys in
 // each of the 15 others (independent binary searches, 16 loads in flight). Summing: a block takes 8 to 128 consecutive sorted
 // tokens (a chunk) and a slab of columns and reads each dout row once; a run of equal ids inside of the chunk goes straight to its row of
@@ -381,8 +382,11 @@ void lookup(const void* weight, const void* ids, bool ids64, void* out, long lon
 }
 
 // Tokens of one chunk: as many as leave about four blocks per SM, at most 128 (fewer and longer chunks mean fewer partial sums; with
-// fewer blocks the chains of loads of a chunk are not covered). A rule on the sizes alone, so the order of additions is, too.
-int chunk_tokens(long long T, int H, int columns) {
+// fewer blocks the chains of loads of a chunk are not covered). A rule on the sizes and the type alone, not on the addresses that decide how
+// wide the loads are, so that the order of additions does not depend on them either.
+template <typename E>
+int chunk_tokens(long long T, int H) {
+  constexpr int columns = SUM_THREADS * 16 / (int)sizeof(E);
   const long long slabs = (H + columns - 1) / columns;
   int n = 8;
   while (n < MAX_CHUNK && (T + 2 * n - 1) / (2 * n) * slabs >= 592) n *= 2;
@@ -392,7 +396,7 @@ int chunk_tokens(long long T, int H, int columns) {
 template <typename T, typename D, int N, bool ACC>
 void sums(const void* dout, const uint64_t* keys, void* dweight, float* partials, long long tokens, int H, float scale,
     cudaStream_t stream) {
-  const int columns = SUM_THREADS * N, n = chunk_tokens(tokens, H, columns);
+  const int columns = SUM_THREADS * N, n = chunk_tokens<T>(tokens, H);
   const long long chunks = (tokens + n - 1) / n;
   const dim3 grid((unsigned)chunks, (unsigned)((H + columns - 1) / columns));
   sum_tokens_kernel<T, D, N, ACC><<<grid, SUM_THREADS, 0, stream>>>(reinterpret_cast<const T*>(dout), keys,
@@ -436,8 +440,7 @@ void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids
 }
 
 long long embedding_gradient_workspace(long long T, int H, Scalar type) {
-  const int columns = SUM_THREADS * (type == Scalar::kF32 ? 4 : 8);  // narrower slabs never make more chunks
-  const int n = chunk_tokens(T, H, columns);
+  const int n = type == Scalar::kF32 ? chunk_tokens<float>(T, H) : chunk_tokens<__nv_bfloat16>(T, H);
   const long long chunks = (T + n - 1) / n;
   return 2 * key_bytes(T) + (chunks > 1 ? 2 * chunks * H * 4 : 0);
 }

@@ -128,7 +128,7 @@ void embedding_lookup(const void* weight, Scalar type, const void* ids, bool ids
                       float scale, int* status, cudaStream_t stream);
 // Bytes of the workspace of the gradient (256-byte aligned).
 long long embedding_gradient_workspace(long long T, int H, Scalar type);
-// dweight[v] = scale * sum of dout[t] over the tokens with id v, in the order of t. accumulate: dweight is fp32, is added to, and rows
+// dweight[v] = scale * sum of dout[t] over the tokens with id v, in an order that the ids and sizes fix. accumulate: dweight is fp32, is added to, and rows
 // that no id names are not touched; else it has dout's type, is 16-byte aligned, and is written whole.
 void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids64, void* dweight, bool accumulate, void* workspace,
                         long long T, long long V, int H, float scale, cudaStream_t stream);

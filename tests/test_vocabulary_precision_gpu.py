@@ -157,3 +157,24 @@ def test_the_gradient_of_a_frequent_token_is_a_sum_of_few_roundings(dtype, token
     # up to 128 of them in one binade below 2^18 steps are exact.
     half = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-24 if into_buffer else 2.0**-8, torch.float16: 2.0**-24 if into_buffer else 2.0**-11}[dtype]
     assert ((grad.double() - exact).abs() <= (half + 2.0**-24) * (1 + 2.0**-20) * exact).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,hidden", [(8192, 1024), (4099, 64)])
+def test_the_order_of_the_embeddings_sums_does_not_depend_on_addresses(dtype, tokens, hidden):
+    """Upstream gradients and buffers that start at an odd element are read and written narrowly, and give the same bits."""
+    gen = torch.Generator("cuda").manual_seed(hidden)
+    ids = torch.randint(0, 30, (tokens,), generator=gen, device="cuda")
+    dout = torch.randn(tokens, hidden, generator=gen, device="cuda").to(dtype)
+    shifted = torch.empty(tokens * hidden + 1, device="cuda", dtype=dtype)[1:].view(tokens, hidden).copy_(dout)
+    buffer = torch.zeros(30 * hidden + 1, device="cuda")[1:].view(30, hidden)
+    grads = []
+    for up, main_grad in ((dout, torch.zeros(30, hidden, device="cuda")), (shifted, torch.zeros(30, hidden, device="cuda")), (dout, buffer)):
+        w = torch.zeros(30, hidden, device="cuda", dtype=dtype, requires_grad=True)
+        out = ops.embedding(w, ids, 0.3, sorted_gradient=True)
+        (grad,) = torch.autograd.grad(out, w, up)
+        w.main_grad = main_grad
+        ops.embedding(w, ids, 0.3, sorted_gradient=True).backward(up)
+        grads.append((grad, main_grad))
+    for grad, main_grad in grads[1:]:
+        assert torch.equal(grad, grads[0][0]) and torch.equal(main_grad, grads[0][1])
