@@ -447,7 +447,7 @@ long long embedding_gradient_workspace(long long T, int H, Scalar type) {
 
 void embedding_gradient(const void* dout, Scalar type, const void* ids, bool ids64, void* dweight, bool accumulate, void* workspace,
                         long long T, long long V, int H, float scale, cudaStream_t stream) {
-  if (H == 0 || (T == 0 && accumulate)) return;
+  if (H == 0 || (T == 0 && (accumulate || V == 0))) return;  // nothing to add and nothing to clear
   uint64_t* keys = reinterpret_cast<uint64_t*>(workspace);
   uint64_t* other = reinterpret_cast<uint64_t*>(reinterpret_cast<char*>(workspace) + key_bytes(T));
   float* partials = reinterpret_cast<float*>(reinterpret_cast<char*>(workspace) + 2 * key_bytes(T));
