@@ -173,6 +173,13 @@ LiveRows live_rows(const Tensor& map, int64_t T, int64_t base, int64_t rows) {
 
 void* row_ptr(const Tensor& t, int64_t row) { return reinterpret_cast<char*>(t.data_ptr()) + row * t.stride(0) * t.element_size(); }
 
+// Rows that a tensor map can describe: unit inner stride, row stride and base multiples of 16 bytes. Others are copied, also where they
+// count as contiguous (at an odd address, or a single row of an odd stride).
+Tensor mapped_rows(const Tensor& t) {
+  const bool ok = t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
 // (log_probs, entropy, lse, the rows that were multiplied, row map, their logits if they are kept)
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> linear_log_probs_fwd(const Tensor& x, const Tensor& w, const Tensor& labels,
     double logit_scale, int64_t ignore_index, bool want_entropy, bool differentiated, bool keep_logits, const Tensor& status) {
@@ -422,12 +429,13 @@ OptTensor main_grad(const Tensor& weight) {
 // the hidden states. Both ways see the same fp32 logits. The batch is compacted to the rows whose label counts, and all products end
 // there.
 struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale,
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Tensor& labels, double logit_scale,
       int64_t ignore_index, bool want_entropy, int64_t chunk, bool differentiated, bool keep_logits, const Tensor& status) {
-    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(x, w, labels, logit_scale, ignore_index, want_entropy,
+    const Tensor w = mapped_rows(weight);
+    auto [log_probs, entropy, lse, xc, map, logits] = linear_log_probs_fwd(mapped_rows(x), w, labels, logit_scale, ignore_index, want_entropy,
         differentiated, keep_logits, status);
     ctx->save_for_backward({xc, w, labels, lse, entropy, map, logits});
-    ctx->saved_data["weight"] = w;
+    ctx->saved_data["weight"] = weight;
     ctx->saved_data["status"] = status;
     ctx->saved_data["logit_scale"] = logit_scale;
     ctx->saved_data["ignore_index"] = ignore_index;
@@ -517,12 +525,6 @@ variable_list token_log_probs(const Tensor& logits, const Tensor& labels, double
   return TokenLogProbs::apply(logits, labels, logit_scale, ignore_index, return_entropy);
 }
 
-// Rows that a tensor map can describe: unit inner stride, row stride and base multiples of 16 bytes.
-Tensor mapped_rows(const Tensor& t) {
-  const bool ok = t.stride(1) == 1 && t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  return ok ? t : t.contiguous();
-}
-
 variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Tensor& labels, double logit_scale, int64_t ignore_index,
     bool return_entropy, int64_t chunk, int64_t keep_bytes, const Tensor& status) {
   check_logit_scale(logit_scale);
@@ -535,7 +537,7 @@ variable_list linear_token_log_probs(const Tensor& x, const Tensor& w, const Ten
   check_label_shape(labels, shape, x);
   const bool differentiated = at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad());
   const bool keep = differentiated && 4.0 * (double)labels.numel() * (double)w.size(0) <= (double)keep_bytes;
-  variable_list out = LinearTokenLogProbs::apply(mapped_rows(x.reshape({labels.numel(), x.size(-1)})), mapped_rows(w),
+  variable_list out = LinearTokenLogProbs::apply(x.reshape({labels.numel(), x.size(-1)}), w,
       labels.reshape({labels.numel()}).contiguous(), logit_scale, ignore_index, return_entropy, chunk, differentiated, keep, status);
   if (x.dim() != 2)
     for (auto& t : out) t = t.view(shape);
@@ -671,7 +673,7 @@ variable_list policy_loss(const Tensor& log_probs, const Tensor& old, const Tens
 
 struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
   static Tensor forward(AutogradContext* ctx, const Tensor& weight, const Tensor& ids, double scale, const Tensor& status) {
-    Tensor out = embedding_lookup_(weight, ids, scale, status);
+    Tensor out = embedding_lookup_(weight.contiguous(), ids, scale, status);
     ctx->save_for_backward({ids});
     ctx->saved_data["weight"] = weight;
     ctx->saved_data["scale"] = scale;
@@ -693,7 +695,7 @@ Tensor embedding_sorted(const Tensor& weight, const Tensor& ids, double scale, c
   TORCH_CHECK_VALUE(ids.scalar_type() == torch::kInt64 || ids.scalar_type() == torch::kInt32, "ids must be int64 or int32, got ",
       text(ids.scalar_type()));
   TORCH_CHECK_VALUE(ids.device() == weight.device(), "ids must be on ", text(weight.device()), ", got ", text(ids.device()));
-  return EmbeddingSorted::apply(weight.contiguous(), ids.contiguous(), scale, status);
+  return EmbeddingSorted::apply(weight, ids.contiguous(), scale, status);
 }
 
 }  // namespace

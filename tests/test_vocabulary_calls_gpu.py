@@ -27,3 +27,60 @@ def test_embedding_of_nothing(dtype, vocab, tokens, hidden):
     w.main_grad = torch.ones(vocab, hidden, device="cuda")
     ops.embedding(w, torch.zeros(tokens, device="cuda", dtype=torch.long), sorted_gradient=True).sum().backward()
     assert (w.main_grad == 1).all()
+
+
+# ----------------------------------------------------------------------------- operands that no tensor map can describe
+def _operands(tokens, hidden=64, vocab=300):
+    gen = torch.Generator("cuda").manual_seed(tokens)
+    x = torch.randn(tokens, hidden, generator=gen, device="cuda").bfloat16()
+    w = (torch.randn(vocab, hidden, generator=gen, device="cuda") / 8).bfloat16()
+    return x, w, torch.randint(0, vocab, (tokens,), generator=gen, device="cuda"), torch.randn(tokens, generator=gen, device="cuda")
+
+
+def _at_an_odd_address(t):
+    return torch.empty(t.numel() + 1, device=t.device, dtype=t.dtype)[1:].view(t.shape).copy_(t)
+
+
+def _in_odd_rows(t):
+    return torch.zeros(t.shape[0], t.shape[1] + 3, device=t.device, dtype=t.dtype)[:, : t.shape[1]].copy_(t)
+
+
+def _of_one_column_stride(t):
+    return t.t().contiguous().t()
+
+
+@pytest.mark.parametrize("place", [_at_an_odd_address, _in_odd_rows, _of_one_column_stride])
+@pytest.mark.parametrize("tokens,vocab", [(1, 300), (1, 1), (20, 300)])
+@pytest.mark.parametrize("into_buffer", [False, True])
+def test_fused_linear_log_probs_of_operands_that_lie_oddly(place, tokens, vocab, into_buffer):
+    x, w, labels, g = _operands(tokens, vocab=vocab)
+    results = []
+    for a, b in ((x, w), (place(x), w), (x, place(w)), (place(x), place(w))):
+        a, b = a.detach().requires_grad_(True), b.detach().requires_grad_(True)
+        if into_buffer:
+            b.main_grad = torch.zeros(vocab, 64, device="cuda")
+        lp = ops.fused_linear_token_log_probs(a, b, labels)
+        lp.backward(g)
+        assert (b.grad is None) == into_buffer
+        with torch.no_grad():
+            assert torch.equal(ops.fused_linear_token_log_probs(a, b, labels), lp)
+        results.append((lp.detach(), a.grad, b.main_grad if into_buffer else b.grad))
+    for result in results[1:]:
+        for got, want in zip(result, results[0]):
+            assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("place", [_at_an_odd_address, _in_odd_rows, _of_one_column_stride])
+def test_a_table_that_lies_oddly_finds_its_main_grad(place):
+    _, w, ids, _ = _operands(20)
+    dout = torch.randn(20, 64, device="cuda").bfloat16()
+    buffers = []
+    for table in (w, place(w)):
+        table = table.detach().requires_grad_(True)
+        table.main_grad = torch.zeros(300, 64, device="cuda")
+        out = ops.embedding(table, ids, sorted_gradient=True)
+        assert torch.equal(out, w[ids])
+        out.backward(dout)
+        assert table.grad is None
+        buffers.append(table.main_grad)
+    assert buffers[0].abs().max() > 0 and torch.equal(*buffers)
