@@ -50,9 +50,13 @@ _KEEP_LOGITS_BYTES = 4 << 30
 
 
 # ----------------------------------------------------------------------------- token log-probabilities
+def _kept(labels: torch.Tensor, ignore_index: int, vocab: int) -> torch.Tensor:
+    return (labels != ignore_index) & (labels >= 0) & (labels < vocab)
+
+
 def _token_log_probs_torch(logits: torch.Tensor, labels: torch.Tensor, logit_scale: float, ignore_index: int, return_entropy: bool):
     vocab, labels = logits.shape[-1], labels.long()  # an ignore_index beyond 32 bits would wrap around next to int32 labels
-    kept = (labels != ignore_index) & (labels >= 0) & (labels < vocab)
+    kept = _kept(labels, ignore_index, vocab)
     z = logits if logits.dtype == torch.float64 else logits.float()
     z = torch.where(kept[..., None], z, 0.0) * logit_scale  # whatever an ignored row holds, it has no part and no gradient
     logp = z.log_softmax(-1)
@@ -108,6 +112,8 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
                          f"and {weight.dtype} on {weight.device}")
     _check_labels(labels, x.shape[:-1], x.device)
     note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
+    # rows that do not count are left out of the products: their values would reach the weight's gradient as 0 * NaN
+    x = torch.where(_kept(labels.long(), ignore_index, weight.shape[0])[..., None], x, 0.0)
     return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
 
 
