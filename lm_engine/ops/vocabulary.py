@@ -96,8 +96,9 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
     The logits are formed in fp32 on the tensor cores and reduced where they are. Without gradients they never reach memory;
     with gradients they are kept in fp32 until the backward pass (``keep_logits``; by default where that takes at most 4 GiB) or
     formed a second time in it. The backward pass needs a transient bf16 buffer of at most about 2.2 GB. Rows whose label is
-    ignored take no part in any product. bf16 operands with ``H`` a multiple of 8 run on the kernels. Gradients of ``weight`` go
-    to its ``main_grad`` when the engine provides one."""
+    ignored take no part in any product. bf16 operands with ``H`` a multiple of 8 run on the kernels, which add the gradient of
+    ``weight`` into its ``main_grad`` when the engine provides one; other types and sizes run as PyTorch operations in fp32 (fp64 operands
+    in fp64), with the logits kept."""
     if x.is_cuda and x.dtype == torch.bfloat16 and x.dim() > 0 and weight.dim() == 2 and x.shape[-1] % 8 == 0:
         with site("loss.lm_head.log_probs"):
             out = native().linear_token_log_probs(
@@ -112,9 +113,11 @@ def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: 
                          f"and {weight.dtype} on {weight.device}")
     _check_labels(labels, x.shape[:-1], x.device)
     note_fallback("fused_linear_token_log_probs", "the hidden size is not a multiple of 8", x, weight)
-    # rows that do not count are left out of the products: their values would reach the weight's gradient as 0 * NaN
+    # logits of fp32 as on the kernels, and rows that do not count are left out of the products: their values would reach the
+    # weight's gradient as 0 * NaN
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
     x = torch.where(_kept(labels.long(), ignore_index, weight.shape[0])[..., None], x, 0.0)
-    return _token_log_probs_torch(F.linear(x, weight), labels, logit_scale, ignore_index, return_entropy)
+    return _token_log_probs_torch(F.linear(x.to(wide), weight.to(wide)), labels, logit_scale, ignore_index, return_entropy)
 
 
 # ----------------------------------------------------------------------------- losses over packed answers

@@ -24,3 +24,28 @@ def test_ignored_rows_are_in_no_product_of_the_fused_linear_log_probs(dtype):
         for got, want in zip(result, results[0]):
             assert torch.isfinite(got).all() and torch.equal(got, want)
     assert (results[0][2][ignored] == 0).all() and results[0][3].abs().max() > 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hidden", [12, 64])
+def test_fused_linear_log_probs_off_the_kernels_form_their_logits_in_32_bits(dtype, hidden):
+    gen = torch.Generator().manual_seed(hidden)
+    x, w = (torch.randn(n, hidden, generator=gen).to(dtype) for n in (20, 300))
+    labels = torch.randint(0, 300, (20,), generator=gen)
+    labels[5] = -100
+    x.requires_grad_(True), w.requires_grad_(True)
+    lp, entropy = ops.fused_linear_token_log_probs(x, w, labels, return_entropy=True)
+    dx, dw = torch.autograd.grad(lp.sum(), (x, w))
+    x64, w64 = x.detach().double(), w.detach().double()
+    logp = (x64 @ w64.t()).log_softmax(-1)
+    want = torch.where(labels < 0, 0.0, logp.gather(1, labels.clamp_min(0)[:, None])[:, 0])
+    # `hidden` products and additions and at most 300 terms of the softmax, each rounded to fp32, of logits below 64
+    bound = (hidden + 300 + 16) * 2.0**-24 * (1 + (x64.abs() @ w64.abs().t()).max())
+    assert lp.dtype == torch.float32 and ((lp.double() - want).abs() <= bound).all() and torch.isfinite(entropy).all()
+    dz = -logp.exp()
+    dz[torch.arange(20), labels.clamp_min(0)] += 1
+    dz[labels < 0] = 0
+    half = {torch.float32: 2.0**-24, torch.bfloat16: 2.0**-8, torch.float16: 2.0**-11}[dtype]
+    for got, exact, size in ((dx, dz @ w64, dz.abs() @ w64.abs()), (dw, dz.t() @ x64, dz.abs().t() @ x64.abs())):
+        assert got.dtype == dtype and ((got.double() - exact).abs() <= half * exact.abs() + 4 * bound * size + 2.0**-24).all()
+    assert (dx[5] == 0).all()
