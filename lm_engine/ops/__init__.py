@@ -336,8 +336,14 @@ class _EmbeddingFn(torch.autograd.Function):
 
 def embedding(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0, *, sorted_gradient: bool | None = None) -> torch.Tensor:
     """``scale * weight[ids]``. ``sorted_gradient`` sums the weight gradient in sorted token order instead of with atomics, whose
-    order differs from run to run (see :func:`embedding_sorted`); by default it follows ``torch.use_deterministic_algorithms``."""
-    if torch.are_deterministic_algorithms_enabled() if sorted_gradient is None else sorted_gradient:
+    order differs from run to run (see :func:`embedding_sorted`). By default it follows ``torch.use_deterministic_algorithms`` for the
+    tables whose gradient would be added up by atomics (bf16 on the GPU); other CUDA tables run ``F.embedding``, whose gradient is
+    summed in a fixed order and can be differentiated again, either way."""
+    if sorted_gradient is None and torch.are_deterministic_algorithms_enabled():
+        if use_native(weight) and weight.dtype == torch.bfloat16 and ids.is_cuda:
+            return embedding_sorted(weight, ids.long(), scale)
+        sorted_gradient = weight.device.type == "cpu"
+    if sorted_gradient:
         return embedding_sorted(weight, ids, scale)
     if use_native(weight) and weight.dtype == torch.bfloat16 and ids.is_cuda and weight.shape[1] % 8 == 0:
         return _EmbeddingFn.apply(weight, ids.long(), float(scale))

@@ -84,3 +84,37 @@ def test_a_table_that_lies_oddly_finds_its_main_grad(place):
         assert table.grad is None
         buffers.append(table.main_grad)
     assert buffers[0].abs().max() > 0 and torch.equal(*buffers)
+
+
+# ----------------------------------------------------------------------------- the deterministic switch
+@pytest.fixture
+def deterministic():
+    torch.use_deterministic_algorithms(True)
+    yield
+    torch.use_deterministic_algorithms(False)
+
+
+def test_fp32_tables_keep_their_embedding_under_deterministic_algorithms(deterministic, monkeypatch):
+    w = torch.randn(50, 8, device="cuda", requires_grad=True)
+    ids = torch.randint(0, 50, (40,), device="cuda")
+
+    def never():
+        raise AssertionError("the extension is not needed here")
+
+    monkeypatch.setattr(ops, "native", never)
+    out = ops.embedding(w, ids, 2.0)
+    (grad,) = torch.autograd.grad(out.square().sum(), w, create_graph=True)
+    (second,) = torch.autograd.grad(grad.sum(), w)  # out^2 = 4 w[ids]^2, twice differentiated: 8 for each time an id appears
+    assert torch.equal(second, 8.0 * torch.bincount(ids, minlength=50).float()[:, None].expand(50, 8))
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        assert (torch.autograd.forward_ad.unpack_dual(ops.embedding(dual, ids, 2.0)).tangent == 2).all()
+
+
+@pytest.mark.parametrize("kind", [torch.int16, torch.uint8, torch.int32])
+def test_bf16_tables_take_any_integer_ids_under_deterministic_algorithms(deterministic, kind):
+    w = torch.randn(50, 16, device="cuda").bfloat16().requires_grad_(True)
+    ids = torch.randint(0, 50, (3, 40), device="cuda")
+    (want,) = torch.autograd.grad(ops.embedding(w, ids, sorted_gradient=True).sum(), w)
+    out = ops.embedding(w, ids.to(kind))
+    assert torch.equal(out, w[ids]) and torch.equal(torch.autograd.grad(out.sum(), w)[0], want)
