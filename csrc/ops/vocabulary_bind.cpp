@@ -259,21 +259,21 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> preference_fwd(const Tensor& log_prob
   return {loss, chosen, rejected, slope};
 }
 
-Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, const Tensor& log_probs, const OptTensor& cu, int64_t length,
+Tensor preference_bwd(const Tensor& slope, const Tensor& d_loss, at::IntArrayRef shape, const OptTensor& cu, int64_t length,
     const OptTensor& mask) {
   const int64_t sequences = slope.numel();
-  const PackedTokens p = packed_tokens(log_probs, cu, length, sequences, mask);
-  contiguous_f32(slope, log_probs, sequences, "slope");
+  const c10::cuda::CUDAGuard guard(slope.device());
+  Tensor grad = torch::empty(shape, slope.options());
+  const PackedTokens p = packed_tokens(grad, cu, length, sequences, mask);
+  contiguous_f32(slope, slope, sequences, "slope");
   long long stride = 0;
   const float* d = nullptr;
   if (d_loss.dim() == 0) {
-    d = contiguous_f32(d_loss, log_probs, 1, "d_loss");
+    d = contiguous_f32(d_loss, slope, 1, "d_loss");
   } else {
-    d = row_values(d_loss, log_probs, sequences / 2, "d_loss", &stride);
+    d = row_values(d_loss, slope, sequences / 2, "d_loss", &stride);
   }
-  const c10::cuda::CUDAGuard guard(log_probs.device());
-  Tensor grad = torch::empty(log_probs.sizes(), log_probs.options());
-  preference_loss_bwd(slope.data_ptr<float>(), d, stride, p, grad.data_ptr<float>(), stream_of(log_probs));
+  preference_loss_bwd(slope.data_ptr<float>(), d, stride, p, grad.data_ptr<float>(), stream_of(slope));
   return grad;
 }
 
@@ -592,7 +592,8 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
       int64_t reduction) {
     auto [loss, chosen, rejected, slope] = preference_fwd(log_probs, reference, cu, length, sequences, mask, kind, beta,
         label_smoothing, average, reduction);
-    ctx->save_for_backward({slope, log_probs, cu.value_or(Tensor()), mask.value_or(Tensor())});
+    ctx->save_for_backward({slope, cu.value_or(Tensor()), mask.value_or(Tensor())});
+    ctx->saved_data["shape"] = log_probs.sizes().vec();
     ctx->saved_data["length"] = length;
     ctx->mark_non_differentiable({chosen, rejected});
     ctx->set_materialize_grads(false);
@@ -602,9 +603,8 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(11);
     if (!grads[0].defined()) return out;
-    out[0] = once(preference_bwd(saved[0], grads[0], saved[1], optional(saved[2]), ctx->saved_data["length"].toInt(),
-                                 optional(saved[3])),
-                  "preference_loss");
+    out[0] = once(preference_bwd(saved[0], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[1]),
+        ctx->saved_data["length"].toInt(), optional(saved[2])), "preference_loss");
     return out;
   }
 };

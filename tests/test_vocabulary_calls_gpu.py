@@ -118,3 +118,22 @@ def test_bf16_tables_take_any_integer_ids_under_deterministic_algorithms(determi
     (want,) = torch.autograd.grad(ops.embedding(w, ids, sorted_gradient=True).sum(), w)
     out = ops.embedding(w, ids.to(kind))
     assert torch.equal(out, w[ids]) and torch.equal(torch.autograd.grad(out.sum(), w)[0], want)
+
+
+# ----------------------------------------------------------------------------- values changed between the passes
+@pytest.mark.parametrize("padded", [False, True])
+def test_log_probs_may_be_changed_between_the_passes_of_the_losses(padded):
+    """Neither loss needs them again: what their gradients take is formed in the forward pass."""
+    shape = (4, 25) if padded else (100,)
+    cu = None if padded else torch.tensor([0, 10, 10, 70, 100], device="cuda", dtype=torch.int32)
+    values, old = torch.randn(shape, device="cuda") / 10, torch.randn(shape, device="cuda") / 10
+    for loss in (lambda lp: ops.preference_loss(lp, old, cu).loss, lambda lp: ops.policy_loss(lp, old, torch.ones(4, device="cuda"), cu_seqlens=cu).loss):
+        grads = []
+        for change in (False, True):
+            lp = values.clone().requires_grad_(True)
+            out = loss(lp)
+            if change:
+                with torch.no_grad():
+                    lp.zero_()
+            grads.append(torch.autograd.grad(out, lp)[0])
+        assert grads[0].abs().max() > 0 and torch.equal(*grads)
