@@ -9,7 +9,9 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <memory>
 
 #include "vocabulary.h"
 
@@ -360,6 +362,53 @@ Tensor embedding_gradient_(const Tensor& dout, const Tensor& ids, int64_t V, con
   return dw;
 }
 
+// ------------------------------------------------------------------------- launch sites of the backward passes
+// The function of lm_engine/ops/timeline.py that opens a site by name, while sites are on. Kept for the process's life and touched with the
+// interpreter's lock held; the flag alone is read without it, so that a pass pays nothing while they are off.
+std::atomic<bool> sites_on{false};
+py::object& site_function() {
+  static py::object* f = new py::object(py::none());
+  return *f;
+}
+
+void set_site(const py::object& function) {
+  site_function() = function;
+  sites_on = !function.is_none();
+}
+
+class Site {
+ public:
+  explicit Site(const char* name) {
+    if (!sites_on.load(std::memory_order_relaxed)) return;
+    const py::gil_scoped_acquire gil;
+    if (site_function().is_none()) return;
+    std::string error;
+    try {
+      auto context = std::make_unique<py::object>(site_function()(name));
+      context->attr("__enter__")();
+      context_ = context.release();
+    } catch (py::error_already_set& e) {  // the engine's threads know the library's errors only
+      error = e.what();
+    }
+    TORCH_CHECK(error.empty(), "launch site ", name, ": ", error);
+  }
+  ~Site() {
+    if (context_ == nullptr) return;
+    const py::gil_scoped_acquire gil;
+    try {
+      context_->attr("__exit__")(py::none(), py::none(), py::none());
+    } catch (py::error_already_set& e) {
+      e.discard_as_unraisable("launch site");
+    }
+    delete context_;
+  }
+  Site(const Site&) = delete;
+  Site& operator=(const Site&) = delete;
+
+ private:
+  py::object* context_ = nullptr;
+};
+
 // ------------------------------------------------------------------------- differentiable functions
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
@@ -402,6 +451,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
     const bool has_h = grads.size() > 1 && grads[1].defined();
     if (!grads[0].defined() && !has_h) return variable_list(5);
     const int64_t rows = labels.numel();
+    const Site site("token_log_probs.bwd");
     Tensor grad = log_probs_bwd(rows3(logits), labels.contiguous(), lse, entropy.defined() ? OptTensor(entropy) : OptTensor(),
         row_gradient(grads[0], rows, lse), has_h ? OptTensor(row_gradient(grads[1], rows, lse)) : OptTensor(),
         ctx->saved_data["logit_scale"].toDouble(), ctx->saved_data["ignore_index"].toInt());
@@ -483,18 +533,23 @@ struct LinearTokenLogProbs : torch::autograd::Function<LinearTokenLogProbs> {
       const float logit_scale = (float)ctx->saved_data["logit_scale"].toDouble();
       const int64_t ignore_index = ctx->saved_data["ignore_index"].toInt();
       const float* ent = has_h ? entropy.data_ptr<float>() : nullptr;
-      if (logits.defined())
-        token_log_probs_grad_rows(reinterpret_cast<const float*>(row_ptr(logits, r)), logits.stride(0), labels.data_ptr(), labels64,
-            pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), dl.stride(0), live, (int)V, logit_scale, ignore_index, stream);
-      else
-        vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride,
-            dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0), dl.stride(0), logit_scale, ignore_index, st, stream);
+      {
+        const Site site("loss.lm_head.dlogits");
+        if (logits.defined())
+          token_log_probs_grad_rows(reinterpret_cast<const float*>(row_ptr(logits, r)), logits.stride(0), labels.data_ptr(), labels64,
+              pairs(lse), ent, gp, g_stride, hp, h_stride, dl.data_ptr(), dl.stride(0), live, (int)V, logit_scale, ignore_index, stream);
+        else
+          vocab_gemm_grad(xr.data_ptr(), w.data_ptr(), labels.data_ptr(), labels64, pairs(lse), ent, gp, g_stride, hp, h_stride,
+              dl.data_ptr(), live, (int)V, (int)H, xc.stride(0), w.stride(0), dl.stride(0), logit_scale, ignore_index, st, stream);
+      }
       if (need_dx) {
+        const Site site("loss.lm_head.dgrad");
         balanced_gemm(dl.data_ptr(), w.data_ptr(), dxc.data_ptr(), partials.data_ptr<float>(), live, (int)H, (int)V, dl.stride(0),
             w.stride(0), st, stream);
         balanced_rows(dxc.data_ptr(), partials.data_ptr<float>(), live, dx.data_ptr(), (int)H, (int)V, stream);
       }
       if (need_dw) {
+        const Site site("loss.lm_head.wgrad");
         gemm_bf16_2sm_live(dl.data_ptr(), xr.data_ptr(), dw.data_ptr(), (int)V, (int)H, (int)n, dl.stride(0), xr.stride(0),
             dw.stride(0), dw.scalar_type() == torch::kFloat32, live, st, stream);
       }
@@ -603,6 +658,7 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(11);
     if (!grads[0].defined()) return out;
+    const Site site("preference_loss.bwd");
     out[0] = once(preference_bwd(saved[0], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[1]),
         ctx->saved_data["length"].toInt(), optional(saved[2])), "preference_loss");
     return out;
@@ -641,6 +697,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
     const auto saved = ctx->get_saved_variables();
     variable_list out(15);
     if (!grads[0].defined()) return out;
+    const Site site("policy_loss.bwd");
     out[0] = once(policy_bwd(saved[0], saved[1], saved[2], grads[0], ctx->saved_data["shape"].toIntVector(), optional(saved[3]),
         ctx->saved_data["length"].toInt(), ctx->saved_data["sequences"].toInt(), optional(saved[4]),
         ctx->saved_data["reduction"].toInt()), "policy_loss");
@@ -685,6 +742,7 @@ struct EmbeddingSorted : torch::autograd::Function<EmbeddingSorted> {
     if (!grads[0].defined()) return variable_list(4);
     const Tensor weight = ctx->saved_data["weight"].toTensor();
     const OptTensor target = main_grad(weight);
+    const Site site("embedding.bwd");
     Tensor dw = embedding_gradient_(grads[0].contiguous(), saved[0], weight.size(0), target, ctx->saved_data["scale"].toDouble());
     return {target.has_value() ? Tensor() : once(dw, "embedding_sorted"), Tensor(), Tensor(), Tensor()};
   }
@@ -705,6 +763,7 @@ void register_vocabulary(pybind11::module_& m) {
   m.def("linear_token_log_probs", &linear_token_log_probs, "the same from hidden states and the output weight");
   m.def("preference_loss", &preference_loss, "loss over pairs of answers: (loss, chosen rewards, rejected rewards)");
   m.def("policy_loss", &policy_loss, "clipped policy loss with a KL term: (loss, KL estimate, clipped share)");
+  m.def("set_site", &set_site, "opens the launch sites of backward passes: a function of the name, or None");
   m.def("embedding_sorted", &embedding_sorted, "embedding whose gradient is summed in sorted token order");
 }
 

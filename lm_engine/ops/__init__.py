@@ -11,6 +11,7 @@ from __future__ import annotations
 import torch
 import torch.nn.functional as F
 
+from . import timeline
 from .build import is_extension_built, load_extension
 from .timeline import site
 
@@ -23,6 +24,7 @@ def native() :
     global _C
     if _C is None:
         _C = load_extension()
+        timeline.follow(_C.set_site)
     return _C
 
 

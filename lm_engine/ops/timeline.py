@@ -8,7 +8,8 @@
 * ``enable_nvtx()`` (or ``LM_ENGINE_NVTX=1`` in the environment) pushes an NVTX range per site, so that a timeline
   tool shows the schedule with names instead of anonymous kernels.
 
-Both are process-wide switches read at every site, so they can be flipped between steps.
+Both are process-wide switches read at every site, so they can be flipped between steps. The backward passes that live in the
+extension are told by ``follow()`` and open the same sites.
 """
 
 from __future__ import annotations
@@ -21,6 +22,7 @@ import torch
 _TIMING = False
 _NVTX = os.environ.get("LM_ENGINE_NVTX", "0") == "1"
 _EVENTS: dict[str, list[tuple[torch.cuda.Event, torch.cuda.Event]]] = defaultdict(list)
+_FOLLOWERS: list = []
 
 
 class _Null:
@@ -66,9 +68,21 @@ def site(name: str):
     return _Site(name)
 
 
+def follow(tell) -> None:
+    """Calls ``tell(site)`` while timing or ranges are on and ``tell(None)`` while they are off: now, and whenever one is switched."""
+    _FOLLOWERS.append(tell)
+    tell(site if _TIMING or _NVTX else None)
+
+
+def _tell() -> None:
+    for tell in _FOLLOWERS:
+        tell(site if _TIMING or _NVTX else None)
+
+
 def enable_timing(on: bool = True) -> None:
     global _TIMING
     _TIMING = on and torch.cuda.is_available()
+    _tell()
     if on:
         _EVENTS.clear()
 
@@ -76,6 +90,7 @@ def enable_timing(on: bool = True) -> None:
 def enable_nvtx(on: bool = True) -> None:
     global _NVTX
     _NVTX = on and torch.cuda.is_available()
+    _tell()
 
 
 def report() -> dict[str, dict[str, float]]:

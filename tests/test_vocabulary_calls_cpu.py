@@ -49,3 +49,22 @@ def test_fused_linear_log_probs_off_the_kernels_form_their_logits_in_32_bits(dty
     for got, exact, size in ((dx, dz @ w64, dz.abs() @ w64.abs()), (dw, dz.t() @ x64, dz.abs().t() @ x64.abs())):
         assert got.dtype == dtype and ((got.double() - exact).abs() <= half * exact.abs() + 4 * bound * size + 2.0**-24).all()
     assert (dx[5] == 0).all()
+
+
+def test_followers_of_the_timeline_are_told_of_its_switches(monkeypatch):
+    from lm_engine.ops import timeline
+
+    monkeypatch.setattr(timeline, "_FOLLOWERS", [])
+    monkeypatch.setattr(timeline, "_TIMING", False)
+    monkeypatch.setattr(timeline, "_NVTX", False)
+    told = []
+    timeline.follow(told.append)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    timeline.enable_timing()
+    timeline.enable_nvtx()
+    timeline.enable_timing(False)
+    timeline.enable_nvtx(False)
+    assert told == [None, timeline.site, timeline.site, timeline.site, None]
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    timeline.enable_timing()  # nothing to time here
+    assert told[-1] is None

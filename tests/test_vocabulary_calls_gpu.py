@@ -137,3 +137,54 @@ def test_log_probs_may_be_changed_between_the_passes_of_the_losses(padded):
                     lp.zero_()
             grads.append(torch.autograd.grad(out, lp)[0])
         assert grads[0].abs().max() > 0 and torch.equal(*grads)
+
+
+# ----------------------------------------------------------------------------- launch sites
+def test_backward_passes_open_their_sites():
+    from lm_engine.ops import timeline
+
+    x, w, labels, g = _operands(40)
+    x, w = x.requires_grad_(True), w.requires_grad_(True)
+    cu = torch.tensor([0, 10, 20, 30, 40], device="cuda", dtype=torch.int32)
+
+    def step():
+        rows = ops.embedding(w, labels, sorted_gradient=True)
+        lp = ops.fused_linear_token_log_probs(rows + x, w, labels, keep_logits=False)
+        lp = lp + ops.token_log_probs(x @ w.t(), labels)
+        loss = ops.preference_loss(lp, None, cu).loss + ops.policy_loss(lp, lp.detach(), torch.ones(4, device="cuda"), cu_seqlens=cu).loss
+        return torch.autograd.grad(loss, (x, w))
+
+    plain = step()
+    both = {"token_log_probs": ["token_log_probs.bwd"], "preference_loss": ["preference_loss.bwd"], "policy_loss": ["policy_loss.bwd"],
+            "embedding": ["embedding.bwd"], "loss.lm_head.log_probs": ["loss.lm_head.dlogits", "loss.lm_head.dgrad", "loss.lm_head.wgrad"]}
+    timeline.enable_timing()
+    try:
+        timed = step()
+        sites = timeline.report()
+    finally:
+        timeline.enable_timing(False)
+    for forward, backward in both.items():
+        for name in (forward, *backward):
+            assert sites[name]["calls"] == 1 and sites[name]["ms"] > 0, name
+    step()
+    assert timeline.report().keys() == sites.keys() and all(timeline.report()[n]["calls"] == sites[n]["calls"] for n in sites)
+    for a, b in zip(plain, timed):
+        assert torch.equal(a, b)
+
+
+def test_an_error_of_a_site_reaches_the_caller():
+    _, w, ids, _ = _operands(5)
+    w.requires_grad_(True)
+    out = ops.embedding(w, ids, sorted_gradient=True).sum()
+
+    def refuse(name):
+        raise KeyError(name)
+
+    ops.native().set_site(refuse)
+    try:
+        with pytest.raises(RuntimeError, match="launch site embedding.bwd: KeyError"):
+            out.backward(retain_graph=True)
+    finally:
+        ops.native().set_site(None)
+    out.backward()
+    assert w.grad.abs().max() == torch.bincount(ids).max()
