@@ -135,7 +135,8 @@ def get_token_log_probs(
     """Per-token log-probabilities of the labels, the input of ``ops.preference_loss`` and ``ops.policy_loss``, with the conventions of
     :func:`get_autoregressive_language_modeling_loss` (ignored label = -100; ``lm_logits``, or ``hidden_states`` and ``vocab_weight`` for the
     fused path). The result (fp32, with ``return_entropy`` also the entropies) is shaped like ``labels``: when labels are shifted, position ``t``
-    holds the log-probability of token ``t + 1`` and the last position of every document or row holds 0."""
+    holds the log-probability of token ``t + 1`` and the last position of every document or row holds 0. A mask of tokens that goes into a loss
+    with them has to be shifted alike: on at ``t`` where token ``t + 1`` counts, off at last positions, whose 0 would count as a token."""
     fused = lm_logits is None
     if tensor_parallel_enabled:
         raise ValueError("token log-probabilities need the whole vocabulary on one rank; they cannot be combined with tensor parallelism")

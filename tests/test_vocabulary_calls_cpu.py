@@ -68,3 +68,45 @@ def test_followers_of_the_timeline_are_told_of_its_switches(monkeypatch):
     monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
     timeline.enable_timing()  # nothing to time here
     assert told[-1] is None
+
+
+@pytest.mark.parametrize("packed", [True, False])
+def test_masks_are_shifted_like_the_log_probs_of_a_model(packed):
+    """The documented use: position t holds token t + 1, so a mask of answer tokens moves one position to the left and is off at last positions."""
+    from lm_engine.hf_models import get_token_log_probs
+
+    gen = torch.Generator().manual_seed(0)
+    lengths, vocab = [5, 5, 5, 5], 11
+    logits = torch.randn(20, vocab, generator=gen, dtype=torch.float64)
+    tokens = torch.randint(0, vocab, (20,), generator=gen)
+    answer_tokens = torch.tensor([0, 0, 1, 1, 1] + [0, 1, 1, 0, 0] + [1, 0, 0, 1, 1] + [0, 0, 0, 0, 1]).bool()
+    cu = torch.tensor([0, 5, 10, 15, 20])
+    if packed:
+        lp = get_token_log_probs(logits, tokens, cu_seqlens=cu, use_padding_free_transformer=True)
+        mask = answer_tokens.roll(-1)
+        mask[cu[1:].long() - 1] = False
+    else:
+        logits, tokens, answer_tokens, cu = logits.view(4, 5, vocab), tokens.view(4, 5), answer_tokens.view(4, 5), None
+        lp = get_token_log_probs(logits, tokens)
+        mask = answer_tokens.roll(-1, 1)
+        mask[:, -1] = False
+    old, reference = lp - 0.1 * torch.randn(lp.shape, generator=gen), lp + 0.1 * torch.randn(lp.shape, generator=gen)
+    advantages = torch.tensor([1.0, -0.5, 2.0, -1.5], dtype=torch.float64)
+
+    logp = logits.reshape(4, 5, vocab).log_softmax(-1)
+    old4, ref4, answer4, token4 = old.view(4, 5), reference.view(4, 5), answer_tokens.view(4, 5), tokens.view(4, 5)
+    values, sums = [], []
+    for i in range(4):
+        # a token is predicted one position earlier; the first token of a document is predicted by nothing
+        own = [(logp[i, t - 1, token4[i, t]], old4[i, t - 1], ref4[i, t - 1]) for t in range(1, 5) if answer4[i, t]]
+        values.append([max(-advantages[i] * (a - b).exp(), -advantages[i] * (a - b).exp().clamp(0.8, 1.2)).item() for a, b, _ in own])
+        sums.append(sum((a - r).item() for a, _, r in own) / len(own))
+    token_mean = sum(map(sum, values)) / sum(map(len, values))
+    sequence_mean = sum(sum(v) / len(v) for v in values) / 4
+    for reduction, want in (("token_mean", token_mean), ("sequence_mean", sequence_mean)):
+        got = ops.policy_loss(lp, old, advantages, cu_seqlens=cu, mask=mask, reduction=reduction).loss.item()
+        assert got == pytest.approx(want, rel=1e-12)
+        unshifted = ops.policy_loss(lp, old, advantages, cu_seqlens=cu, mask=answer_tokens, reduction=reduction).loss.item()
+        assert abs(unshifted - want) > 1e-3
+    got = ops.preference_loss(lp, reference, cu, beta=0.5, average_log_probs=True, mask=mask).loss.item()
+    assert got == pytest.approx(sum(math.log1p(math.exp(-0.5 * (sums[i] - sums[i + 2]))) for i in range(2)) / 2, rel=1e-12)
