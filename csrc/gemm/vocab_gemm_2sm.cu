@@ -1,12 +1,12 @@
 // Output projection fused with the softmax that follows it: logits = x [M, K] W [N, K]^T are formed on CTA pairs in 256 x 256
-// tiles (tcgen05 cta_group::2) and never leave tensor memory.
+// tiles (tcgen05 cta_group::2) and are reduced, or turned into their gradient, on the way out of tensor memory.
 //
 //   statistics: the epilogue reduces each row of a tile to (m, s, u, x[label]): largest logit, sums of softmax_stats.cuh
 //               relative to it, and the label's logit if it lies in the tile's columns; 16 bytes per row and tile go to
 //               stats[slice][row] for every 128 columns instead of 256 bytes of logits. token_log_probs_join combines them.
 //   statistics, logits kept: the same, and the fp32 logits leave through shared memory and bulk tensor stores, for a backward
-//               pass that has the memory for them: 2.1 GB of stores hide under 2.6 ms of MMAs (4096 x 4096 x 128256), and what
-//               the gradient mode would take, 2.7 ms, becomes a pass over memory.
+//               pass that has the memory for them: 2.1 GB of stores hide under 2.7 ms of MMAs (4096 x 4096 x 128256), and what
+//               the gradient mode would take, 2.7 ms, becomes a pass over memory (0.42 ms).
 //   gradient:   the logits are formed again, and the epilogue writes d(logits) in bf16, the operand type of the two products
 //               that follow (d(x) = d(logits) W, dW = d(logits)^T x); the factor 1[label] - p is formed in fp32 from the fp32
 //               logits, so the one rounding is that of the stored operand.

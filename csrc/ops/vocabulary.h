@@ -42,8 +42,7 @@ void vocab_compact_rows(const void* labels, bool labels64, long long ignore_inde
 void token_log_probs_join(const float* stats, int slices, int slice_width, const void* labels, bool labels64, float* log_probs,
     float* entropy, float2* lse, LiveRows live, int V, float logit_scale, long long ignore_index, cudaStream_t stream);
 
-// ---- gemm/vocab_gemm_2sm.cu: logits = x [M, K] w [N, K]^T, bf16 operands with row strides that are multiples of 8 elements;
-// the logits stay in tensor memory.
+// ---- gemm/vocab_gemm_2sm.cu: logits = x [M, K] w [N, K]^T, bf16 operands with row strides that are multiples of 8 elements.
 // x holds the rows of this launch; labels, lse and gradients are those of the whole batch.
 constexpr int kVocabSlice = 128;  // columns per slice of the statistics
 // logits: null, or fp32 [live.rows, N] with a row stride ldl that is a multiple of 4, which keeps the live rows' logits.

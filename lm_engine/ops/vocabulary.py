@@ -1,7 +1,7 @@
 """Operators over the vocabulary for preference and reward tuning.
 
 * :func:`token_log_probs`: log-probabilities (and entropies) of given tokens under rows of logits
-* :func:`fused_linear_token_log_probs`: the same from hidden states and the output weight, logits never in memory
+* :func:`fused_linear_token_log_probs`: the same from hidden states and the output weight
 * :func:`preference_loss`: loss over pairs of answers from their summed log-probability ratios
 * :func:`policy_loss`: clipped policy-gradient loss with a KL term
 * :func:`embedding_sorted`: embedding whose gradient is summed in sorted token order (``ops.embedding(sorted_gradient=True)``)
@@ -91,11 +91,13 @@ def token_log_probs(logits: torch.Tensor, labels: torch.Tensor, *, logit_scale: 
 # ----------------------------------------------------------------------------- from hidden states
 def fused_linear_token_log_probs(x: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, *, logit_scale: float = 1.0,
                                  ignore_index: int = -100, return_entropy: bool = False, keep_logits: bool | None = None):
-    """:func:`token_log_probs` of ``logits = x @ weight.T`` without the logits: ``x [..., H]``, ``weight [V, H]``, ``labels [...]``.
+    """:func:`token_log_probs` of ``logits = x @ weight.T`` from the operands: ``x [..., H]``, ``weight [V, H]``, ``labels [...]``.
 
     The logits are formed in fp32 on the tensor cores and reduced where they are. Without gradients they never reach memory;
     with gradients they are kept in fp32 until the backward pass (``keep_logits``; by default where that takes at most 4 GiB) or
-    formed a second time in it. The backward pass needs a transient bf16 buffer of at most about 2.2 GB. Rows whose label is
+    formed a second time in it. The backward pass needs a transient buffer of at most about 2.2 GB, which holds the gradient of the logits
+    in bf16, the operand type of the two products that follow: their results are off by one rounding more (relative error against 64 bits
+    2.3e-3; rounding the result alone gives 1.7e-3). Rows whose label is
     ignored take no part in any product. bf16 operands with ``H`` a multiple of 8 run on the kernels, which add the gradient of
     ``weight`` into its ``main_grad`` when the engine provides one; other types and sizes run as PyTorch operations in fp32 (fp64 operands
     in fp64), with the logits kept."""
@@ -317,9 +319,10 @@ def policy_loss(log_probs: torch.Tensor, old_log_probs: torch.Tensor, advantages
 
 # ----------------------------------------------------------------------------- embedding
 def embedding_sorted(weight: torch.Tensor, ids: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
-    """``scale * weight[ids]`` whose weight gradient adds the rows of a token in an order fixed by their positions: the same bits on
-    every run, one rounding, no fp32 copy of the whole table (``ops.embedding(sorted_gradient=True)``). bf16, fp16 and fp32 tables
-    of any width run on the kernels.
+    """``scale * weight[ids]`` whose weight gradient adds the rows of a token in an order fixed by the ids and the sizes: the same bits on
+    every run, no fp32 copy of the whole table (``ops.embedding(sorted_gradient=True)``). Sums are fp32 for up to 128 rows of a 16-bit
+    token and 64-bit otherwise. bf16, fp16 and fp32 tables of any width run on the kernels. The gradient has no derivative, and forward-mode
+    differentiation is not available there.
 
     On the GPU an id outside of the table gives a row of zeros, takes no part in the gradient and raises the status word
     (``ops.check_status()``)."""
